@@ -8,6 +8,7 @@ gdn/tests/test_correctness.py:221-223), cu_seqlens int32 or int64.
 """
 from __future__ import annotations
 
+import contextlib
 import math
 
 import torch
@@ -69,6 +70,14 @@ def check_heads(HQ: int, HV: int, D: int) -> None:
         raise ValueError(f"head_size must be {HEAD_DIM}, got {D}")
     if HQ <= 0 or HV % HQ != 0:
         raise ValueError(f"num_v_heads ({HV}) must be a positive multiple of num_q_heads ({HQ})")
+
+
+_SAME = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context in which `device` is current; free where it is already (the usual call)."""
+    return _SAME if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def stream_handle(device: torch.device) -> int:

@@ -66,6 +66,26 @@ SIGNATURES = {
          _p, _int, _p, _int, _p, _int, _p, _int,
          _p, _int, _f32, _p, _p, _i64, _i64, _i32, _i32, _i32, _p],
     ),
+    "gdn_conv_prefill_fwd": (
+        _int,
+        [_p, _i64, _p, _int, _p, _int, _p, _p, _int,  # x stride weight bias state cu (+dtype)
+         _int, _i32, _p, _p, _f32, _p, _p, _i64, _i64, _i32, _i32, _p, _p],
+    ),
+    "gdn_conv_decode_fwd": (
+        _int,
+        [_p, _i64, _p, _int, _p, _int, _p,
+         _int, _i32, _p, _p, _f32, _p, _p, _i64, _i32, _i32, _p],
+    ),
+    "gdn_ssm_decode_fwd": (
+        _int,
+        [_p, _p, _int, _p, _int, _p, _p, _p, _int, _p, _int,  # x dt A_log B C D dt_bias
+         _p, _int, _p, _p, _i64, _i32, _i32, _i32, _i32, _p],
+    ),
+    "gdn_ssm_prefill_recurrent_fwd": (
+        _int,
+        [_p, _p, _int, _p, _int, _p, _p, _p, _int, _p, _int,
+         _p, _p, _int, _p, _p, _i64, _i64, _i32, _i32, _i32, _i32, _p, _p],
+    ),
     "gdn_selftest_umma": (_int, [_p, _p, _p, _int, _int, _p, _p]),
     "gdn_selftest_wait_timeout": (_int, [_p, _p, _p]),
     "gdn_selftest_umma_ts": (_int, [_p, _p, _p, _p, _p]),

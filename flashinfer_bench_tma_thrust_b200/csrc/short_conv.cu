@@ -1,0 +1,381 @@
+// short_conv.cu — short causal depthwise convolution over packed prompts and for one new
+// token per sequence, with silu, split outputs and the L2 norm of 128-channel heads fused
+// into the store.
+//
+// With W taps (2 to 4) and u the inputs of a sequence, its W-1 earlier rows (the state, or
+// zeros) in front:
+//     c_t[ch] = bias[ch] + sum_k weight[ch][k] u_{t-W+1+k}[ch],   y = silu(c)
+// and in a normed section every head of 128 channels is divided by sqrt(sum y^2 + eps).
+// 2 W flop stand against 4 bytes of traffic per element, so HBM bounds it: each input is
+// read once, a run of tokens per thread keeps the last W-1 rows in registers, and the
+// outputs leave in 16-byte stores, each section to its own dense tensor (what the operators
+// behind it take) with no pass of its own for split, silu or norm.
+//
+// A thread owns 8 adjacent channels (16 bytes of a row), so a head is 16 lanes of a warp and
+// its norm four shuffles. Sums are fp32; silu takes ex2.approx and an approximate division
+// (a few fp32 ulp, far below the bf16 rounding of the output, the only other one).
+#include "gdn_b200.h"
+#include "gdn_common.cuh"
+#include "ssm_launch.h"
+
+namespace gdn {
+namespace {
+
+constexpr int kVec = 8;         // channels per thread
+constexpr int kThreads = 128;   // 1024 channels per block
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Eight channels of one row as stored.
+struct Row {
+  uint4 w;
+};
+
+__device__ __forceinline__ void unpack(const Row& r, float (&v)[kVec]) {
+  const uint32_t u[4] = {r.w.x, r.w.y, r.w.z, r.w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(u[i] << 16);
+    v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+  }
+}
+
+__device__ __forceinline__ Row pack(const float (&v)[kVec]) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
+  return Row{make_uint4(u[0], u[1], u[2], u[3])};
+}
+
+// Channels [c, c + 8) of a row; with kWide one 16-byte access (the launcher has checked
+// alignment and that 8 divides every section), else one access per channel below C.
+template <bool kWide>
+__device__ __forceinline__ Row load_row(const __nv_bfloat16* row, int c, int C) {
+  if (kWide) return Row{*reinterpret_cast<const uint4*>(row + c)};
+  const unsigned short* p = reinterpret_cast<const unsigned short*>(row);
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = c + 2 * i < C ? p[c + 2 * i] : 0u;
+    const uint32_t hi = c + 2 * i + 1 < C ? p[c + 2 * i + 1] : 0u;
+    u[i] = lo | (hi << 16);
+  }
+  return Row{make_uint4(u[0], u[1], u[2], u[3])};
+}
+
+template <bool kWide>
+__device__ __forceinline__ void store_row(__nv_bfloat16* row, int c, int C, const Row& r) {
+  if (kWide) {
+    *reinterpret_cast<uint4*>(row + c) = r.w;
+    return;
+  }
+  unsigned short* p = reinterpret_cast<unsigned short*>(row);
+  const uint32_t u[4] = {r.w.x, r.w.y, r.w.z, r.w.w};
+#pragma unroll
+  for (int i = 0; i < kVec; ++i)
+    if (c + i < C) p[c + i] = static_cast<unsigned short>(u[i >> 1] >> ((i & 1) * 16));
+}
+
+// What a thread knows of its channels.
+template <int W>
+struct Taps {
+  float w[W][kVec];
+  float bias[kVec];
+};
+
+template <int W, bool kWide>
+__device__ __forceinline__ Taps<W> load_taps(const ConvParams& p, int c) {
+  Taps<W> t;
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    const int ch = c + i;
+    const bool in = kWide || ch < p.C;
+    t.bias[i] = p.bias && in ? load_scalar(p.bias, p.bias_dtype, ch) : 0.f;
+#pragma unroll
+    for (int k = 0; k < W; ++k)
+      t.w[k][i] = in ? load_scalar(p.weight, p.weight_dtype, static_cast<int64_t>(ch) * W + k) : 0.f;
+  }
+  return t;
+}
+
+// Where a thread's channels go: its section (kWide: all 8 channels lie in one).
+struct Place {
+  __nv_bfloat16* out;
+  int width, at, normed;
+};
+__device__ __forceinline__ Place place_of(const ConvParams& p, int c) {
+  int s = 0;
+#pragma unroll 1
+  while (s + 1 < p.sections && c >= p.begin[s + 1]) ++s;
+  return Place{p.out[s], p.begin[s + 1] - p.begin[s], c - p.begin[s], p.normed[s]};
+}
+
+__device__ __forceinline__ float silu(float v) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-kLog2e * v));
+  return __fdividef(v, 1.f + e);
+}
+
+// One output row: activation, norm of the head (16 lanes), store. All lanes of the warp call
+// it; `live` says whether this thread's channels exist.
+template <bool kWide>
+__device__ __forceinline__ void finish(const ConvParams& p, const Place& pl, int c, int64_t row,
+                                       float (&v)[kVec], bool live) {
+  if (p.silu) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) v[i] = silu(v[i]);
+  }
+  if (pl.normed) {  // the same for all 16 lanes of a head
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) q = fmaf(v[i], v[i], q);
+    const uint32_t lanes = 0xffffu << (threadIdx.x & 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) q += __shfl_xor_sync(lanes, q, o);
+    const float r = rsqrtf(q + p.eps);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) v[i] *= r;
+  }
+  if (!live) return;
+  const Row r = pack(v);
+  if (kWide) {
+    *reinterpret_cast<uint4*>(pl.out + row * pl.width + pl.at) = r.w;
+  } else {
+    const uint32_t u[4] = {r.w.x, r.w.y, r.w.z, r.w.w};
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      if (c + i >= p.C) break;
+      const Place q = place_of(p, c + i);
+      reinterpret_cast<unsigned short*>(q.out)[row * q.width + q.at] =
+          static_cast<unsigned short>(u[i >> 1] >> ((i & 1) * 16));
+    }
+  }
+}
+
+// How many i in [1, N] have cu[i] <= t: the sequence that token t lies in (N: none). A
+// 32-way search by the whole warp: one round for up to 32 sequences, two up to 1024.
+__device__ __forceinline__ int64_t find_sequence(const void* cu, int dtype, int64_t N, int64_t t) {
+  const int lane = threadIdx.x & 31;
+  int64_t lo = 0, hi = N;
+  while (hi > lo) {
+    const int64_t step = (hi - lo + 31) / 32;
+    const int64_t i = lo + (lane + 1) * step - 1;
+    const bool le = i < hi && load_index(cu, dtype, i + 1) <= t;
+    lo += __popc(__ballot_sync(0xffffffffu, le)) * step;
+    hi = min(hi, lo + step - 1);
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int64_t bound(const ConvParams& p, int64_t i) {
+  const int64_t v = load_index(p.cu_seqlens, p.cu_dtype, i);
+  return v < 0 ? 0 : (v > p.T ? p.T : v);
+}
+
+// Prompts. Blocks [0, tiles) of grid.y take `run` tokens each; the N behind them write one
+// sequence's new state (its last W-1 inputs, from the state where it is shorter).
+constexpr int kAhead = 8;  // rows loaded before the first is used
+
+template <int W, bool kWide>
+__global__ void __launch_bounds__(kThreads) conv_prefill_kernel(const __grid_constant__ ConvParams p,
+                                                               int64_t tiles, int run) {
+  const int c = (blockIdx.x * kThreads + threadIdx.x) * kVec;
+  const bool live = c < p.C;
+  const int64_t by = blockIdx.y + static_cast<int64_t>(blockIdx.z) * gridDim.y;
+  if (by >= tiles + p.N) return;
+  if (by >= tiles) {
+    const int64_t n = by - tiles;
+    const int64_t start = bound(p, n), end = bound(p, n + 1);
+    const int64_t len = end > start ? end - start : 0;
+    if (c == 0) {
+      const int64_t lo = load_index(p.cu_seqlens, p.cu_dtype, n);
+      const int64_t hi = load_index(p.cu_seqlens, p.cu_dtype, n + 1);
+      if (lo < 0 || hi > p.T || hi < lo) report_bad_bounds(p.status);
+    }
+    if (!live) return;
+#pragma unroll
+    for (int r = 0; r < W - 1; ++r) {
+      Row v{make_uint4(0u, 0u, 0u, 0u)};
+      const int64_t at = len + r;  // row of [state; inputs]
+      if (at >= W - 1) {
+        v = load_row<kWide>(p.x + (start + at - (W - 1)) * p.x_stride, c, p.C);
+      } else if (p.state) {
+        v = load_row<kWide>(p.state + (n * (W - 1) + at) * p.C, c, p.C);
+      }
+      store_row<kWide>(p.new_state + (n * (W - 1) + r) * p.C, c, p.C, v);
+    }
+    return;
+  }
+  const int64_t t0 = by * run;
+  const int64_t t1 = min(t0 + run, p.T);
+  int64_t n = find_sequence(p.cu_seqlens, p.cu_dtype, p.N, t0);
+  int64_t start = p.T, end = p.T;  // of sequence n; none left: nothing is written
+  if (n < p.N) {
+    start = bound(p, n);
+    end = bound(p, n + 1);
+  }
+  const int cl = live ? c : 0;
+  const Taps<W> taps = load_taps<W, kWide>(p, cl);
+  Place pl = place_of(p, cl);
+  if (!live) pl.normed = 0;  // no lane waits in the head's shuffles for one without channels
+  float win[W - 1][kVec];  // the W-1 rows before the token
+#pragma unroll
+  for (int r = 0; r < W - 1; ++r) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) win[r][i] = 0.f;
+  }
+  if (n < p.N && start < t0) {  // the tile begins inside a sequence
+#pragma unroll
+    for (int r = 0; r < W - 1; ++r) {
+      const int64_t u = t0 - (W - 1) + r;
+      if (u >= start) {
+        unpack(load_row<kWide>(p.x + u * p.x_stride, cl, p.C), win[r]);
+      } else if (p.state) {
+        unpack(load_row<kWide>(p.state + (n * (W - 1) + (u - start) + (W - 1)) * p.C, cl, p.C), win[r]);
+      }
+    }
+  }
+  for (int64_t tb = t0; tb < t1; tb += kAhead) {
+    Row rows[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a)
+      rows[a] = load_row<kWide>(p.x + min(tb + a, p.T - 1) * p.x_stride, cl, p.C);
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const int64_t t = tb + a;
+      if (t >= t1) break;
+      while (t >= end && n < p.N) {  // into the next sequence that has tokens
+        ++n;
+        start = end = p.T;
+        if (n < p.N) {
+          start = bound(p, n);
+          end = bound(p, n + 1);
+        }
+      }
+      if (n >= p.N || t < start) continue;  // a token of no sequence
+      if (t == start) {
+#pragma unroll
+        for (int r = 0; r < W - 1; ++r) {
+          Row v{make_uint4(0u, 0u, 0u, 0u)};
+          if (p.state) v = load_row<kWide>(p.state + (n * (W - 1) + r) * p.C, cl, p.C);
+          unpack(v, win[r]);
+        }
+      }
+      float cur[kVec], y[kVec];
+      unpack(rows[a], cur);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        float s = taps.bias[i];
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) s = fmaf(taps.w[k][i], win[k][i], s);
+        y[i] = fmaf(taps.w[W - 1][i], cur[i], s);
+      }
+#pragma unroll
+      for (int r = 0; r + 1 < W - 1; ++r) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) win[r][i] = win[r + 1][i];
+      }
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) win[W - 2][i] = cur[i];
+      finish<kWide>(p, pl, cl, t, y, live);
+    }
+  }
+}
+
+// One token per sequence: each thread reads its 8 channels of the W-1 state rows and of x,
+// and writes the rows moved up by one, so the new state may be the old one's memory.
+template <int W, bool kWide>
+__global__ void __launch_bounds__(kThreads) conv_decode_kernel(const __grid_constant__ ConvParams p) {
+  const int c = (blockIdx.x * kThreads + threadIdx.x) * kVec;
+  const bool live = c < p.C;
+  const int64_t n = blockIdx.y + static_cast<int64_t>(blockIdx.z) * gridDim.y;
+  if (n >= p.N) return;
+  const int cl = live ? c : 0;
+  Row rows[W];
+#pragma unroll
+  for (int r = 0; r < W - 1; ++r)
+    rows[r] = p.state ? load_row<kWide>(p.state + (n * (W - 1) + r) * p.C, cl, p.C)
+                      : Row{make_uint4(0u, 0u, 0u, 0u)};
+  rows[W - 1] = load_row<kWide>(p.x + n * p.x_stride, cl, p.C);
+  const Taps<W> taps = load_taps<W, kWide>(p, cl);
+  Place pl = place_of(p, cl);
+  if (!live) pl.normed = 0;
+  float y[kVec];
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) y[i] = taps.bias[i];
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+    float v[kVec];
+    unpack(rows[k], v);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) y[i] = fmaf(taps.w[k][i], v[i], y[i]);
+  }
+  if (live) {
+#pragma unroll
+    for (int r = 0; r < W - 1; ++r)
+      store_row<kWide>(p.new_state + (n * (W - 1) + r) * p.C, c, p.C, rows[r + 1]);
+  }
+  finish<kWide>(p, pl, cl, n, y, live);
+}
+
+bool wide_ok(const ConvParams& p) {
+  auto al = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; };
+  if (!al(p.x) || p.x_stride % kVec || p.C % kVec || !al(p.new_state) || (p.state && !al(p.state)))
+    return false;
+  for (int s = 0; s < p.sections; ++s)
+    if (p.begin[s + 1] % kVec || !al(p.out[s])) return false;
+  return true;
+}
+
+// grid.y holds at most 65535 rows; more go to grid.z.
+dim3 rows_grid(unsigned bx, int64_t rows) {
+  const int64_t y = rows < 32768 ? rows : 32768;
+  return dim3(bx, static_cast<unsigned>(y), static_cast<unsigned>((rows + y - 1) / y));
+}
+
+template <int W>
+int prefill_w(const ConvParams& p, cudaStream_t stream) {
+  const unsigned bx = (p.C + kThreads * kVec - 1) / (kThreads * kVec);
+  // A run of `run` tokens reads W-1 rows again; short runs fill the SMs for short prompts.
+  int run = 64;
+  while (run > kAhead && bx * ((p.T + run - 1) / run) < 148 * 8) run /= 2;
+  const int64_t tiles = (p.T + run - 1) / run;
+  const int64_t rows = tiles + p.N;
+  if (rows > (int64_t{1} << 30)) return GDN_ERR_UNSUPPORTED_SHAPE;
+  const dim3 grid = rows_grid(bx, rows);
+  if (wide_ok(p)) {
+    conv_prefill_kernel<W, true><<<grid, kThreads, 0, stream>>>(p, tiles, run);
+  } else {
+    conv_prefill_kernel<W, false><<<grid, kThreads, 0, stream>>>(p, tiles, run);
+  }
+  return cudaGetLastError() == cudaSuccess ? 0 : GDN_ERR_CUDA;
+}
+
+template <int W>
+int decode_w(const ConvParams& p, cudaStream_t stream) {
+  const unsigned bx = (p.C + kThreads * kVec - 1) / (kThreads * kVec);
+  if (p.N > (int64_t{1} << 30)) return GDN_ERR_UNSUPPORTED_SHAPE;
+  const dim3 grid = rows_grid(bx, p.N);
+  if (wide_ok(p)) {
+    conv_decode_kernel<W, true><<<grid, kThreads, 0, stream>>>(p);
+  } else {
+    conv_decode_kernel<W, false><<<grid, kThreads, 0, stream>>>(p);
+  }
+  return cudaGetLastError() == cudaSuccess ? 0 : GDN_ERR_CUDA;
+}
+
+}  // namespace
+
+int launch_conv_prefill(const ConvParams& p, cudaStream_t stream) {
+  if (p.W == 2) return prefill_w<2>(p, stream);
+  if (p.W == 3) return prefill_w<3>(p, stream);
+  return prefill_w<4>(p, stream);
+}
+
+int launch_conv_decode(const ConvParams& p, cudaStream_t stream) {
+  if (p.W == 2) return decode_w<2>(p, stream);
+  if (p.W == 3) return decode_w<3>(p, stream);
+  return decode_w<4>(p, stream);
+}
+
+}  // namespace gdn

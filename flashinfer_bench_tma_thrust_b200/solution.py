@@ -26,8 +26,8 @@ SOLUTIONS = {
 }
 AUTHOR = "gdn-b200"
 ENTRY = "kernel.py::kernel"
-HOST_MODULES = ("__init__.py", "_lib.py", "_checks.py", "build.py", "decode.py", "prefill.py",
-                "partition.py", "workloads.py")
+HOST_MODULES = ("__init__.py", "_lib.py", "_checks.py", "_status.py", "build.py", "decode.py",
+                "prefill.py", "short_conv.py", "ssm.py", "partition.py", "workloads.py")
 
 ENTRY_TEMPLATE = '''"""Entry point of the {name} solution (generated by {pkg}.solution)."""
 import os

@@ -235,6 +235,82 @@ GDN_API int gdn_prefill_chunked_fwd_noalloc(const void* q, const void* k, const 
                                             int32_t HV, int32_t D, void* stream);
 
 /*
+ * Short causal depthwise convolution (W = 2, 3 or 4 taps) over cu_seqlens-packed prompts.
+ *
+ *   u: the inputs of a sequence behind its W-1 earlier rows (`state`, or zeros)
+ *   c_t = bias + sum_k weight[:, k] u_{t-W+1+k};   y = activation ? c * sigmoid(c) : c
+ *
+ *   x           bf16 [T, C], rows x_row_stride elements apart
+ *   weight      [C, W] contiguous (F32 or BF16);  bias [C] (F32 or BF16) or NULL
+ *   state       bf16 [N, W-1, C] or NULL;  new_state bf16 [N, W-1, C]: each sequence's last
+ *               W-1 inputs (an empty sequence keeps its rows); must not alias state or x
+ *   sections    1 to 8: the channels are split into sections of widths[i] (host array,
+ *               summing to C); section i is written densely to outs[i], bf16 [T, widths[i]]
+ *               (outs: host array of device pointers)
+ *   normed      host array: where non-zero, each head of 128 channels of the section is
+ *               divided by sqrt(sum of squares + eps); the section's begin and width must
+ *               then be multiples of 128
+ *   status      two int32 words (device or mapped host memory) or NULL: [1] becomes 1 when
+ *               cu_seqlens has a bound outside [0, T] (used clamped) or a decreasing pair
+ *
+ * Outputs of tokens that no sequence covers are left as they were. One launch.
+ */
+GDN_API int gdn_conv_prefill_fwd(const void* x, int64_t x_row_stride, const void* weight,
+                                 int weight_dtype, const void* bias, int bias_dtype,
+                                 const void* state, const void* cu_seqlens, int cu_dtype,
+                                 int activation, int32_t sections, const int32_t* widths,
+                                 const int32_t* normed, float eps, void* const* outs,
+                                 void* new_state, int64_t T, int64_t N, int32_t C, int32_t W,
+                                 int32_t* status, void* stream);
+
+/* The same for one new token of each of B sequences: x bf16 [B, C], state bf16
+ * [B, W-1, C] or NULL. new_state may alias state (in place). One launch. */
+GDN_API int gdn_conv_decode_fwd(const void* x, int64_t x_row_stride, const void* weight,
+                                int weight_dtype, const void* bias, int bias_dtype,
+                                const void* state, int activation, int32_t sections,
+                                const int32_t* widths, const int32_t* normed, float eps,
+                                void* const* outs, void* new_state, int64_t B, int32_t C,
+                                int32_t W, void* stream);
+
+/*
+ * Selective state space scan, one new token of each of `batch` sequences.
+ *
+ *   d = softplus(dt + dt_bias);  g = exp(-exp(A_log) d)
+ *   S <- g S + d x (outer) B;    y = S C + D x            per head, S [P, Ns]
+ *
+ *   x        bf16 [batch, H, P];  B, C bf16 [batch, G, Ns] (head h reads group h / (H / G))
+ *   dt       [batch, H];  A_log, dt_bias [H];  D [H] or NULL (each F32 or BF16)
+ *   state    [batch, H, P, Ns] of type state_dtype (F32; BF16: the math is fp32, the new
+ *            state is rounded) or NULL (zeros); new_state the same, may alias state
+ *   out      bf16 [batch, H, P]
+ *
+ * P: 1 to 256; Ns: 16, 32, 64, 128 or 256; H a multiple of G. B, C and the states 16-byte
+ * aligned. One launch.
+ */
+GDN_API int gdn_ssm_decode_fwd(const void* x, const void* dt, int dt_dtype, const void* A_log,
+                               int A_log_dtype, const void* B, const void* C, const void* D,
+                               int D_dtype, const void* dt_bias, int dt_bias_dtype,
+                               const void* state, int state_dtype, void* out, void* new_state,
+                               int64_t batch, int32_t H, int32_t G, int32_t P, int32_t Ns,
+                               void* stream);
+
+/*
+ * The scan over cu_seqlens-packed prompts, token by token (x bf16 [T, H, P], B, C bf16
+ * [T, G, Ns], dt [T, H], state fp32 [N, H, P, Ns] or NULL, out bf16 [T, H, P]); sizes as
+ * for single tokens. An empty sequence passes its state through; outputs of tokens that no
+ * sequence covers are left as they were; new_state must not alias state. status as for
+ * gdn_conv_prefill_fwd. One launch.
+ */
+GDN_API int gdn_ssm_prefill_recurrent_fwd(const void* x, const void* dt, int dt_dtype,
+                                          const void* A_log, int A_log_dtype, const void* B,
+                                          const void* C, const void* D, int D_dtype,
+                                          const void* dt_bias, int dt_bias_dtype,
+                                          const float* state, const void* cu_seqlens,
+                                          int cu_dtype, void* out, float* new_state, int64_t T,
+                                          int64_t N, int32_t H, int32_t G, int32_t P, int32_t Ns,
+                                          int32_t* status, void* stream);
+
+/*
  * Diagnostics. Known-answer check of the tensor-core path the chunked prefill
  * is built on (no counterpart in the reference): D[128x64] fp32 = A[128x128] x
  * B[128x64], bf16 row-major inputs, staged in shared memory in the K-major

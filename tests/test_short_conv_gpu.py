@@ -1,0 +1,242 @@
+"""The short convolution on the GPU against its definition in fp64."""
+import pytest
+import torch
+
+from flashinfer_bench_tma_thrust_b200 import GDNError, prefill, short_conv
+from oracle import gdn_oracle
+from oracle.ssm_oracle import BF16, assert_within, conv
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def clean_status():
+    short_conv.reset_device_status()
+    yield
+    short_conv.reset_device_status()
+
+
+def make(lengths, C, W, state=True, bias=True, wdtype=torch.bfloat16, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    T, N = sum(lengths), len(lengths)
+    x = torch.randn(T, C, generator=g).bfloat16()
+    w = (torch.randn(C, W, generator=g) * W ** -0.5).to(wdtype)
+    b = torch.randn(C, generator=g).to(wdtype) if bias else None
+    s = torch.randn(N, W - 1, C, generator=g).bfloat16() if state else None
+    cu = torch.tensor([0] + lengths).cumsum(0).to(torch.int32)
+    return x, w, b, s, cu
+
+
+def dev(*ts):
+    return [t.cuda() if isinstance(t, torch.Tensor) else t for t in ts]
+
+
+def check(got, new_state, x, w, b, s, bounds, activation="silu", split=None, norm=None, eps=1e-6):
+    split = split or (x.shape[1],)
+    norm = norm or (False,) * len(split)
+    want, states = conv(x, w, b, s, bounds, activation, split, norm, eps)
+    got = got if isinstance(got, tuple) else (got,)
+    for i, (o, (v, e)) in enumerate(zip(got, want)):
+        assert o.dtype == torch.bfloat16 and o.is_contiguous()
+        assert_within(o, v, e, f"section {i}", rounding=BF16)
+    assert torch.equal(new_state.cpu().double(), states)
+
+
+LENGTHS = [[1], [2], [3], [5, 0, 1, 2, 3, 4, 0, 7], [64, 1, 65], [200], [0, 0], [7, 130, 9, 33]]
+
+
+@pytest.mark.parametrize("lengths", LENGTHS)
+@pytest.mark.parametrize("W", [2, 3, 4])
+@pytest.mark.parametrize("state", [True, False])
+def test_prompt(lengths, W, state):
+    x, w, b, s, cu = make(lengths, 264, W, state)
+    got, ns = short_conv.prefill(*dev(x, w, b, s, cu), check=True)
+    check(got, ns, x, w, b, s, cu.tolist())
+
+
+@pytest.mark.parametrize("C,split,norm", [
+    (512, (128, 128, 256), (True, True, False)),
+    (512, (128, 384), (False, True)),
+    (1160, (128, 1024, 8), (True, True, False)),
+    (357, (128, 229), (True, False)),            # odd channels: no vector access
+    (333, (100, 33, 200), (False, False, False)),
+    (1, (1,), (False,)),
+    (2304, (1024, 1024, 256), (True, False, True)),
+])
+@pytest.mark.parametrize("wdtype", [torch.bfloat16, torch.float32])
+def test_sections_and_norms(C, split, norm, wdtype):
+    x, w, b, s, cu = make([3, 70, 1], C, 4, wdtype=wdtype, seed=C)
+    got, ns = short_conv.prefill(*dev(x, w, b, s, cu), split=split, l2norm=norm)
+    check(got, ns, x, w, b, s, cu.tolist(), split=split, norm=norm)
+    xt = x[:9, None]
+    st = torch.randn(9, 3, C, generator=torch.Generator().manual_seed(1)).bfloat16()
+    got, ns = short_conv.decode(*dev(xt, w, b, st), split=split, l2norm=norm)
+    assert got[0].shape == (9, 1, split[0])
+    check(got, ns, x[:9], w, b, st, list(range(10)), split=split, norm=norm)
+
+
+def test_zero_head_norm_and_eps():
+    """A head of zeros stays zero; eps enters under the root."""
+    x, w, _, _, cu = make([5], 256, 4, bias=False, seed=3)
+    x[:, :128] = 0
+    got, ns = short_conv.prefill(*dev(x, w), None, None, cu.cuda(), l2norm=True, eps=0.25)
+    check(got, ns, x, w, None, None, cu.tolist(), norm=(True,), eps=0.25)
+    assert (got[:, :128] == 0).all()
+
+
+@pytest.mark.parametrize("activation", ["silu", None])
+def test_no_bias_no_activation_3d_weight_int64(activation):
+    x, w, _, s, cu = make([4, 9], 64, 4, seed=4)
+    got, ns = short_conv.prefill(x.cuda(), w[:, None].cuda(), None, s.cuda(), cu.long().cuda(),
+                                 activation=activation)
+    check(got, ns, x, w, None, s, cu.tolist(), activation=activation)
+
+
+@pytest.mark.parametrize("offset,width", [(0, 800), (8, 800), (3, 777)])
+def test_strided_rows(offset, width):
+    """x as a slice of wider rows: its own stride and start (aligned or not)."""
+    x, w, b, s, cu = make([20, 21], 256, 4, seed=5)
+    wide = torch.full((41, width), float("nan"), dtype=torch.bfloat16)
+    wide[:, offset:offset + 256] = x
+    view = wide.cuda()[:, offset:offset + 256]
+    got, ns = short_conv.prefill(view, *dev(w, b, s, cu))
+    check(got, ns, x, w, b, s, cu.tolist())
+    got, ns = short_conv.decode(view[:2, None], *dev(w, b, s))
+    check(got, ns, x[:2], w, b, s, [0, 1, 2])
+    t = x.cuda().t().contiguous().t()            # channels not adjacent
+    got, ns = short_conv.prefill(t, *dev(w, b, s, cu))
+    check(got, ns, x, w, b, s, cu.tolist())
+
+
+def test_prompt_in_pieces_then_tokens_equals_one_prompt():
+    """A prompt cut in two with the state carried, then single tokens in place, gives the bits
+    of the whole prompt."""
+    x, w, b, s, cu = make([40], 512, 4, seed=6)
+    x, w, b, s, cu = dev(x, w, b, s, cu)
+    kw = dict(split=(128, 128, 256), l2norm=(True, True, False))
+    whole, end = short_conv.prefill(x, w, b, s, cu, **kw)
+    parts, st = [], s
+    for lo, hi in ((0, 2), (2, 3), (3, 30)):
+        o, st = short_conv.prefill(x[lo:hi], w, b, st, torch.tensor([0, hi - lo]).cuda(), **kw)
+        parts.append(o)
+    for t in range(30, 40):
+        o, st2 = short_conv.decode_inplace(x[t:t + 1, None], w, b, st, **kw)
+        assert st2 is st
+        parts.append(tuple(v[:, 0] for v in o))
+    for i in range(3):
+        assert torch.equal(torch.cat([p[i] for p in parts]), whole[i])
+    assert torch.equal(st, end)
+
+
+def test_decode_without_state_and_inputs_unchanged():
+    x, w, b, s, _ = make([1] * 5, 256, 4, seed=7)
+    xd, wd, bd, sd = dev(x, w, b, s)
+    got, ns = short_conv.decode(xd[:, None], wd, bd)
+    check(got, ns, x, w, b, None, list(range(6)))
+    got, ns = short_conv.decode(xd[:, None], wd, bd, sd)
+    assert torch.equal(sd.cpu(), s) and torch.equal(xd.cpu(), x)
+    got2, ns2 = short_conv.decode_inplace(xd[:, None], wd, bd, sd)
+    assert torch.equal(got, got2) and torch.equal(ns, ns2) and ns2 is sd
+
+
+def test_uncovered_rows_and_neighbours():
+    """Tokens in front of and behind the sequences are not written and not read; a NaN stays in
+    its own sequence, channel and the W - 1 tokens behind it."""
+    x, w, b, s, _ = make([30], 256, 4, seed=8)
+    x[0:3] = float("nan")
+    x[25:] = float("nan")
+    x[10, 7] = float("nan")
+    cu = torch.tensor([3, 12, 12, 25], dtype=torch.int32)
+    s3 = torch.randn(3, 3, 256, generator=torch.Generator().manual_seed(9)).bfloat16()
+    xd, wd, bd, sd, cud = dev(x, w, b, s3, cu)
+    # the allocator hands the freed block out again: its values show what is not written
+    fill = torch.full((30, 256), 7.0, dtype=torch.bfloat16, device="cuda")
+    at = fill.data_ptr()
+    del fill
+    got, ns = short_conv.prefill(xd, wd, bd, sd, cud, check=True)
+    want, states = conv(x, w, b, s3, cu.tolist(), True, (256,), (False,), 1e-6)
+    assert_within(got, want[0][0], want[0][1], "covered", rounding=BF16)
+    nan = torch.isnan(got.cpu())
+    expect = torch.isnan(want[0][0])
+    assert torch.equal(nan[3:25], expect[3:25])
+    if got.data_ptr() == at:
+        assert (got[:3] == 7).all() and (got[25:] == 7).all()
+    assert torch.equal(torch.isnan(ns.cpu()), torch.isnan(states))
+
+
+@pytest.mark.parametrize("cu", [[0, 5, 99], [-3, 4, 10], [0, 7, 2, 10]])
+def test_bad_cu_seqlens_is_reported(cu):
+    x, w, b, _, _ = make([10], 256, 4, seed=10)
+    args = (*dev(x, w, b), None, torch.tensor(cu, dtype=torch.int64).cuda())
+    with pytest.raises(GDNError, match="cu_seqlens"):
+        short_conv.prefill(*args, check=True)
+    with pytest.raises(GDNError, match="cu_seqlens"):   # sticky until cleared
+        short_conv.prefill(*args)
+    short_conv.reset_device_status()
+    good = torch.tensor([0, 10]).cuda()
+    short_conv.prefill(*dev(x, w, b), None, good, check=True)
+
+
+def test_many_sequences():
+    lengths = [(i * 7) % 5 for i in range(3000)]
+    x, w, b, s, cu = make(lengths, 64, 4, seed=11)
+    got, ns = short_conv.prefill(*dev(x, w, b, s, cu), check=True)
+    check(got, ns, x, w, b, s, cu.tolist())
+
+
+def test_empty_calls():
+    x, w, b, s, _ = make([0, 0], 256, 4, seed=12)
+    got, ns = short_conv.prefill(*dev(x, w, b, s), torch.zeros(3, dtype=torch.int32).cuda())
+    assert got.shape == (0, 256) and torch.equal(ns.cpu(), s)
+    got, ns = short_conv.prefill(*dev(x, w, b), None, torch.zeros(1, dtype=torch.int32).cuda())
+    assert got.shape == (0, 256) and ns.shape == (0, 3, 256)
+    got, ns = short_conv.decode(torch.empty(0, 1, 256, dtype=torch.bfloat16, device="cuda"),
+                                *dev(w, b))
+    assert got.shape == (0, 1, 256) and ns.shape == (0, 3, 256)
+
+
+def test_graph_and_other_stream():
+    """A captured call replayed on new inputs, and a call on a side stream, give the eager
+    call's bits."""
+    x, w, b, s, cu = dev(*make([33, 8], 512, 4, seed=13))
+    x2 = torch.randn_like(x)
+    kw = dict(split=(128, 128, 256), l2norm=(True, True, False))
+    want = short_conv.prefill(x2, w, b, s, cu, **kw)
+    wantd = short_conv.decode(x2[:2, None], w, b, s, **kw)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = short_conv.prefill(x2, w, b, s, cu, **kw)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = short_conv.prefill(x, w, b, s, cu, **kw)
+        gotd = short_conv.decode(x[:2, None], w, b, s, **kw)
+    x.copy_(x2)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, c in ((want, other), (want, got), (wantd, gotd)):
+        assert all(torch.equal(u, v) for u, v in zip(a[0], c[0])) and torch.equal(a[1], c[1])
+
+
+def test_feeds_gdn_prefill():
+    """Convolution, split, silu and norms in front of the GDN prefill, as a layer runs them."""
+    HQ, HV = 2, 4
+    lengths = [70, 0, 9]
+    C = (2 * HQ + HV) * 128
+    x, w, b, s, cu = make(lengths, C, 4, seed=14)
+    g = torch.Generator().manual_seed(15)
+    T = sum(lengths)
+    A_log = torch.log(torch.rand(HV, generator=g) * 15 + 1)
+    dtb = torch.rand(HV, generator=g) * 2 - 1
+    a, bb = torch.randn(T, HV, generator=g).bfloat16(), torch.randn(T, HV, generator=g).bfloat16()
+    split, norm = (HQ * 128, HQ * 128, HV * 128), (True, True, False)
+    (q, k, v), ns = short_conv.prefill(*dev(x, w, b, s, cu), split=split, l2norm=norm)
+    out, state = prefill.kernel(q.view(T, HQ, 128), k.view(T, HQ, 128), v.view(T, HV, 128), None,
+                                *dev(A_log, a, dtb, bb, cu), None, check=True)
+    want, wstate = gdn_oracle.prefill(q.cpu().view(T, HQ, 128), k.cpu().view(T, HQ, 128),
+                                      v.cpu().view(T, HV, 128), None, A_log, a, dtb, bb, cu)
+    check((q, k, v), ns, x, w, b, s, cu.tolist(), split=split, norm=norm)
+    assert ((out.float().cpu() - want.float()).abs() <= 1e-2 + 1e-2 * want.float().abs()).all()
+    assert ((state.cpu() - wstate).norm() / wstate.norm()) < 1e-3

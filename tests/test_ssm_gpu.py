@@ -1,0 +1,236 @@
+"""The state space scan on the GPU against its definition in fp64."""
+import pytest
+import torch
+
+from flashinfer_bench_tma_thrust_b200 import GDNError, short_conv, ssm
+from oracle.ssm_oracle import BF16, assert_within, scan
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def clean_status():
+    ssm.reset_device_status()
+    yield
+    ssm.reset_device_status()
+
+
+def make(lengths, H=4, G=2, P=64, Ns=64, state=True, skip=True, gdtype=torch.float32, gates="slow",
+         seed=0):
+    g = torch.Generator().manual_seed(seed)
+    T, N = sum(lengths), len(lengths)
+    silu = torch.nn.functional.silu
+    x = silu(torch.randn(T, H, P, generator=g)).bfloat16()
+    B = silu(torch.randn(T, G, Ns, generator=g)).bfloat16()
+    C = silu(torch.randn(T, G, Ns, generator=g)).bfloat16()
+    if gates == "slow":    # softplus from 0.001 to 0.1: the state lives for many tokens
+        dt = (torch.randn(T, H, generator=g) * 0.5).to(gdtype)
+        d = torch.exp(torch.rand(H, generator=g) * 4.6 - 6.9)
+        dtb = d + torch.log(-torch.expm1(-d))
+        A_log = torch.log(torch.rand(H, generator=g) * 15 + 1)
+    else:                  # "fast": decays to nothing within a few tokens, also below fp32
+        dt = (torch.randn(T, H, generator=g) * 3).to(gdtype)
+        dtb = torch.rand(H, generator=g) * 30 - 5
+        A_log = torch.log(torch.rand(H, generator=g) * 15 + 1)
+    D = torch.randn(H, generator=g) if skip else None
+    s = torch.randn(N, H, P, Ns, generator=g) if state else None
+    cu = torch.tensor([0] + lengths).cumsum(0).to(torch.int32)
+    return [x, dt, A_log, B, C, D, dtb, s, cu]
+
+
+def dev(ts):
+    return [t.cuda() if isinstance(t, torch.Tensor) else t for t in ts]
+
+
+def check_prompt(got, a, chunked, bounds=None):
+    out, ns = got
+    assert out.dtype == torch.bfloat16 and ns.dtype == torch.float32
+    y, ye, fin, fe = scan(*a[:8], bounds or a[8].tolist(), chunk_products=chunked)
+    assert_within(out, y, ye, "output", rounding=BF16)
+    assert_within(ns, fin, fe, "state")
+
+
+LENGTHS = [[1], [2, 0, 5], [127, 1], [128], [129], [300, 0, 0, 64, 3], [0]]
+
+
+@pytest.mark.parametrize("lengths", LENGTHS)
+@pytest.mark.parametrize("gates", ["slow", "fast"])
+def test_recurrent_prompt(lengths, gates):
+    a = make(lengths, gates=gates, seed=len(lengths))
+    check_prompt(ssm.prefill_recurrent(*dev(a), check=True), a, False)
+
+
+SIZES = [(1, 16), (8, 16), (40, 32), (64, 64), (80, 128), (128, 128), (100, 256), (256, 256), (3, 64)]
+
+
+@pytest.mark.parametrize("P,Ns", SIZES)
+def test_recurrent_sizes(P, Ns):
+    a = make([9, 4], H=6, G=2, P=P, Ns=Ns, seed=P + Ns)
+    check_prompt(ssm.prefill_recurrent(*dev(a)), a, False)
+
+
+@pytest.mark.parametrize("P,Ns", SIZES)
+@pytest.mark.parametrize("batch", [1, 5])
+@pytest.mark.parametrize("sdtype", [torch.float32, torch.bfloat16])
+def test_token(P, Ns, batch, sdtype):
+    a = make([1] * batch, H=6, G=3, P=P, Ns=Ns, seed=P + Ns)
+    a[7] = a[7].to(sdtype)
+    tok = [a[0][:, None], a[1][:, None], a[2], a[3][:, None], a[4][:, None], a[5], a[6], a[7]]
+    out, ns = ssm.decode(*dev(tok))
+    assert out.shape == (batch, 1, 6, P) and ns.dtype == sdtype and ns.shape == a[7].shape
+    y, ye, fin, fe = scan(*a[:8], list(range(batch + 1)))
+    assert_within(out, y, ye, "output", rounding=BF16)
+    assert_within(ns, fin, fe, "state", rounding=BF16 if sdtype == torch.bfloat16 else 0.0)
+
+
+@pytest.mark.parametrize("gates", ["slow", "fast"])
+@pytest.mark.parametrize("H,G", [(1, 1), (3, 1), (5, 5), (8, 2)])
+def test_token_heads_and_gates(H, G, gates):
+    a = make([1] * 3, H=H, G=G, gates=gates, gdtype=torch.bfloat16, skip=False, seed=H)
+    tok = [a[0][:, None], a[1][:, None], a[2], a[3][:, None], a[4][:, None], None, a[6], a[7]]
+    out, ns = ssm.decode(*dev(tok))
+    y, ye, fin, fe = scan(*a[:8], [0, 1, 2, 3])
+    assert_within(out, y, ye, "output", rounding=BF16)
+    assert_within(ns, fin, fe, "state")
+    tok[7] = None
+    out, ns = ssm.decode(*dev(tok))
+    y, ye, fin, fe = scan(*a[:7], None, [0, 1, 2, 3])
+    assert_within(out, y, ye, "output, no state", rounding=BF16)
+    assert_within(ns, fin, fe, "state, no state")
+
+
+@pytest.mark.parametrize("sdtype", [torch.float32, torch.bfloat16])
+def test_token_in_place_and_inputs_unchanged(sdtype):
+    a = make([1] * 4, seed=21)
+    a[7] = a[7].to(sdtype)
+    tok = dev([a[0][:, None], a[1][:, None], a[2], a[3][:, None], a[4][:, None], a[5], a[6], a[7]])
+    before = [t.clone() for t in tok]
+    out, ns = ssm.decode(*tok)
+    assert all(torch.equal(u, v) for u, v in zip(tok, before))
+    out2, ns2 = ssm.decode_inplace(*tok)
+    assert ns2 is tok[7] and torch.equal(out, out2) and torch.equal(ns, ns2)
+
+
+def test_strided_and_unaligned_inputs():
+    """x, B and C as slices of one wide row, at starts that 16 bytes do not divide."""
+    a = make([37, 12], seed=22)
+    T = 49
+    wide = torch.full((T, 1 + 4 * 64 + 3 + 2 * 64 + 2 * 64 + 5), float("nan"), dtype=torch.bfloat16)
+    at = [1, 1 + 256 + 3, 1 + 256 + 3 + 128]
+    for i, o, w in ((0, at[0], 256), (3, at[1], 128), (4, at[2], 128)):
+        wide[:, o:o + w] = a[i].reshape(T, w)
+    wd = wide.cuda()
+    d = dev(a)
+    want = ssm.prefill(*d)
+    d[0] = wd[:, at[0]:at[0] + 256].unflatten(1, (4, 64))
+    d[3] = wd[:, at[1]:at[1] + 128].unflatten(1, (2, 64))
+    d[4] = wd[:, at[2]:at[2] + 128].unflatten(1, (2, 64))
+    got = ssm.prefill(*d)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    tok = [d[0][:5, None], d[1][:5, None], d[2], d[3][:5, None], d[4][:5, None], d[5], d[6], None]
+    same = [t.contiguous() if isinstance(t, torch.Tensor) else t for t in tok]
+    for u, v in zip(ssm.decode(*tok), ssm.decode(*same)):
+        assert torch.equal(u, v)
+
+
+@pytest.mark.parametrize("cu", [[0, 5, 99], [-3, 4, 10], [0, 7, 2, 10]])
+def test_bad_cu_seqlens_is_reported(cu):
+    a = make([10], state=False, seed=23)
+    a[8] = torch.tensor(cu, dtype=torch.int64)
+    for fn in (ssm.prefill, ssm.prefill_recurrent):
+        with pytest.raises(GDNError, match="cu_seqlens"):
+            fn(*dev(a), check=True)
+        with pytest.raises(GDNError, match="cu_seqlens"):
+            fn(*dev(a))
+        ssm.reset_device_status()
+
+
+def test_empty_calls():
+    a = make([0, 0], seed=24)
+    for fn in (ssm.prefill, ssm.prefill_recurrent):
+        out, ns = fn(*dev(a))
+        assert out.shape == (0, 4, 64) and torch.equal(ns.cpu(), a[7])
+        out, ns = fn(*dev(a[:7]), None, torch.zeros(1, dtype=torch.int32).cuda())
+        assert ns.shape == (0, 4, 64, 64)
+    tok = dev([a[0][:, None], a[1][:, None], a[2], a[3][:, None], a[4][:, None], a[5], a[6],
+               a[7][:0]])
+    out, ns = ssm.decode(*tok)
+    assert out.shape == (0, 1, 4, 64) and ns.shape == (0, 4, 64, 64)
+
+
+def test_large_offsets():
+    """A state past 2^31 elements: the last sequences of a large batch."""
+    n, H, P, Ns = 2300, 64, 128, 128
+    s = torch.zeros(n, H, P, Ns, device="cuda")
+    assert s.numel() > 2 ** 31
+    s[-1] = torch.randn(H, P, Ns, device="cuda")
+    x = torch.randn(n, 1, H, P, device="cuda").bfloat16()
+    B, C = (torch.randn(n, 1, 1, Ns, device="cuda").bfloat16() for _ in range(2))
+    dt, A_log, dtb = torch.randn(n, 1, H).cuda(), torch.zeros(H).cuda(), torch.zeros(H).cuda()
+    out, ns = ssm.decode_inplace(x, dt, A_log, B, C, None, dtb, s.clone())
+    for i in (0, n - 1):
+        y, ye, fin, fe = scan(x[i], dt[i], A_log, B[i], C[i], None, dtb, s[i:i + 1], [0, 1])
+        assert_within(out[i], y, ye, "output", rounding=BF16)
+        assert_within(ns[i:i + 1], fin, fe, "state")
+
+
+def test_layer_prompt_then_tokens():
+    """The run of a layer: convolution with split, scan, then single tokens in place for both,
+    against the whole text as one prompt through the definition."""
+    H, G, P, Ns, W = 6, 2, 64, 64, 4
+    split = (H * P, G * Ns, G * Ns)
+    ch = sum(split)
+    g = torch.Generator().manual_seed(25)
+    total, cut = [150, 40], [140, 30]
+    u = torch.randn(sum(total), ch, generator=g).bfloat16().cuda()
+    w, b = (torch.randn(ch, W, generator=g) / 2).cuda(), torch.zeros(ch).cuda()
+    dt = (torch.randn(sum(total), H, generator=g) * 0.5 - 3).cuda()
+    A_log, D, dtb = (torch.randn(H, generator=g).cuda() for _ in range(3))
+    starts = [0, total[0]]
+    idx = torch.cat([torch.arange(s, s + c) for s, c in zip(starts, cut)]).cuda()
+    cu = torch.tensor([0, cut[0], sum(cut)], dtype=torch.int32).cuda()
+
+    (x, B, C), cs = short_conv.prefill(u[idx], w, b, None, cu, split=split)
+    view = lambda x, B, C, lead: (x.view(*lead, H, P), B.view(*lead, G, Ns), C.view(*lead, G, Ns))  # noqa: E731
+    xv, Bv, Cv = view(x, B, C, (sum(cut),))
+    outs, xs = [], [(xv, Bv, Cv)]
+    y, st = ssm.prefill(xv, dt[idx], A_log, Bv, Cv, D, dtb, None, cu, check=True)
+    outs.append(y)
+    for k in range(10):
+        t = torch.tensor([s + c + k for s, c in zip(starts, cut)]).cuda()
+        parts, _ = short_conv.decode_inplace(u[t][:, None], w, b, cs, split=split)
+        xt, Bt, Ct = view(*parts, (2, 1))
+        y, _ = ssm.decode_inplace(xt, dt[t][:, None], A_log, Bt, Ct, D, dtb, st)
+        outs.append(y[:, 0])
+        xs.append((xt[:, 0], Bt[:, 0], Ct[:, 0]))
+
+    for n in range(2):
+        lo, hi = (0, cut[0]) if n == 0 else (cut[0], sum(cut))
+        seq = lambda parts: torch.cat([parts[0][lo:hi]] + [p[n:n + 1] for p in parts[1:]])  # noqa: E731
+        xa, Ba, Ca = (seq([p[i] for p in xs]) for i in range(3))
+        rows = slice(starts[n], starts[n] + total[n])
+        y, ye, fin, fe = scan(xa, dt[rows], A_log, Ba, Ca, D, dtb, None, [0, total[n]],
+                              chunk_products=True)
+        assert_within(seq(outs), y, ye, f"sequence {n}", rounding=BF16)
+        assert_within(st[n:n + 1], fin, fe, f"state {n}")
+
+
+def test_graph_and_other_stream():
+    a = dev(make([150, 8], seed=26))
+    x2 = torch.randn_like(a[0])
+    tok = lambda x: [x[:2, None], a[1][:2, None], a[2], a[3][:2, None], a[4][:2, None], a[5], a[6], a[7]]  # noqa: E731
+    want, wantd = ssm.prefill(x2, *a[1:]), ssm.decode(*tok(x2))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = ssm.prefill(x2, *a[1:])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, gotd = ssm.prefill(*a), ssm.decode(*tok(a[0]))
+    a[0].copy_(x2)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    for u, v in ((want, other), (want, got), (wantd, gotd)):
+        assert torch.equal(u[0], v[0]) and torch.equal(u[1], v[1])
