@@ -81,6 +81,12 @@ SIGNATURES = {
         [_p, _p, _int, _p, _int, _p, _p, _p, _int, _p, _int,  # x dt A_log B C D dt_bias
          _p, _int, _p, _p, _i64, _i32, _i32, _i32, _i32, _p],
     ),
+    "gdn_ssm_prefill_workspace_size": (_size, [_i64, _i64, _i32, _i32, _i32, _i32]),
+    "gdn_ssm_prefill_fwd": (
+        _int,
+        [_p, _p, _int, _p, _int, _p, _p, _p, _int, _p, _int,
+         _p, _p, _int, _p, _p, _i64, _i64, _i32, _i32, _i32, _i32, _p, _size, _p, _p],
+    ),
     "gdn_ssm_prefill_recurrent_fwd": (
         _int,
         [_p, _p, _int, _p, _int, _p, _p, _p, _int, _p, _int,

@@ -167,4 +167,37 @@ int gdn_ssm_prefill_recurrent_fwd(const void* x, const void* dt, int dt_dtype, c
   return gdn::launch_ssm_recurrent(p, static_cast<cudaStream_t>(stream));
 }
 
+size_t gdn_ssm_prefill_workspace_size(int64_t T, int64_t N, int32_t H, int32_t G, int32_t P,
+                                      int32_t Ns) {
+  if (T < 0 || N < 0 || H <= 0 || G <= 0 || H % G || !gdn::ssm_chunked_takes(P, Ns)) return 0;
+  return gdn::ssm_chunked_workspace(T, N, H, G, P, Ns);
+}
+
+int gdn_ssm_prefill_fwd(const void* x, const void* dt, int dt_dtype, const void* A_log,
+                        int A_log_dtype, const void* B, const void* C, const void* D,
+                        int D_dtype, const void* dt_bias, int dt_bias_dtype, const float* state,
+                        const void* cu_seqlens, int cu_dtype, void* out, float* new_state,
+                        int64_t T, int64_t N, int32_t H, int32_t G, int32_t P, int32_t Ns,
+                        void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  gdn::SsmParams p;
+  const int rc = fill_ssm(&p, x, dt, dt_dtype, A_log, A_log_dtype, B, C, D, D_dtype, dt_bias,
+                          dt_bias_dtype, state, out, new_state, T, N, H, G, P, Ns);
+  if (rc != GDN_OK) return rc;
+  if (!index_ok(cu_dtype)) return GDN_ERR_UNSUPPORTED_DTYPE;
+  if (N == 0) return GDN_OK;
+  if (!cu_seqlens) return GDN_ERR_INVALID_ARG;
+  p.cu_seqlens = cu_seqlens;
+  p.cu_dtype = cu_dtype;
+  p.status = status;
+  if (!gdn::ssm_chunked_takes(P, Ns))
+    return gdn::launch_ssm_recurrent(p, static_cast<cudaStream_t>(stream));
+  // bulk copies read x and write out; token coordinates are 32-bit
+  if (!aligned16(x) || !aligned16(out) || !aligned16(workspace)) return GDN_ERR_INVALID_ARG;
+  if (T > 0x7fffff00LL) return GDN_ERR_UNSUPPORTED_SHAPE;
+  const size_t need = gdn::ssm_chunked_workspace(T, N, H, G, P, Ns);
+  if (need && (!workspace || workspace_bytes < need)) return GDN_ERR_WORKSPACE;
+  p.workspace = static_cast<float*>(workspace);
+  return gdn::launch_ssm_chunked(p, static_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"

@@ -1,0 +1,863 @@
+// ssm_prefill_chunked.cu — the state space scan over packed prompts on the tensor cores
+// (head sizes and state sizes of 64 and 128).
+//
+// Chunks of L = 128 tokens. With G_t the in-chunk cumulative log decay (log2 units), d_t the
+// step and S the state entering the chunk, per head
+//     y_i   = e^{G_i} (C_i S^T) + sum_{j <= i} (C_i . B_j) e^{G_i - G_j} d_j x_j + D x_i
+//     S'    = e^{G_L} S + sum_j (e^{G_L - G_j} d_j x_j) (outer) B_j
+// What a chunk adds to the state does not depend on S, so the chunks of a sequence are
+// chained by one multiply-add of the state only, and everything else overlaps.
+//
+// One block per (column block, segment): 128 columns of x, that is one head of 128 or two
+// heads of 64 of one group (they share C B^T), over the chunks of one segment of a sequence.
+// Four products per chunk on tcgen05, accumulators in TMEM (512 columns):
+//     CB  [token i, token j]   = C B^T            operands as TMA brings them
+//     Y   [token, column]      = C S^T            S rounded to bf16, written to shared memory
+//     dS  [column, n]          = (f x)^T B        f x transposed into TMEM as bf16 hi + lo
+//     Y                       += M x              M = CB masked and decayed, bf16 in TMEM
+// Between the second and the fourth the block multiplies Y by e^{G_i} in TMEM. The state stays
+// in fp32 registers (thread = column, a quarter of n) for the whole segment.
+//
+// Roundings: x, B and C are exact bf16 operands. f x is a hi + lo pair (each term of the state
+// is off by 2^-16 at most, measured 6e-7 over all: the state is an fp32 result). S and M are
+// rounded once to bf16 as operands: they reach only y, which is rounded to bf16 itself.
+//
+// Segments. With few (sequence, column block) chains the sequences are cut into segments of a
+// multiple of 128 tokens. A first kernel (the same code, third product only) computes what
+// each segment adds to the state and what it leaves of it; each block of the second kernel
+// then folds those of the segments before its own into its first state.
+//
+// Warps: 0-15 compute, 16 issues the products, 17 all bulk copies, 18 and 19 the gates (one
+// head each, one chunk ahead). Every wait is bounded; a block that gives up reports it and
+// runs on without waiting, so no barrier is left short of its threads.
+#include "gdn_b200.h"
+#include "gdn_chunk_common.cuh"
+#include "ssm_launch.h"
+
+namespace gdn {
+namespace {
+
+using namespace sm100;
+using chunk::kLog2e;
+using chunk::named_bar_sync;
+
+constexpr int kL = 128;             // tokens per chunk
+constexpr int kBlock = 16384;       // a [128 rows x 64 columns] bf16 tile
+constexpr int kComputeWarps = 16;
+constexpr int kThreads = 20 * 32;
+
+// TMEM columns
+constexpr uint32_t kTG = 0;         // C B^T, then M (64 columns per head)
+constexpr uint32_t kTY = 128;
+constexpr uint32_t kTD = 256;       // dS
+constexpr uint32_t kTF = 384;       // f x: hi 64 columns, lo 64 columns
+
+struct Gates {                      // of one head and chunk
+  float cum[kL];                    // G from the start of the token's block of 32
+  float dec[kL];                    // e^G
+  float u[kL];                      // d_j e^{G_r - G_j}, r the end of j's block of 32
+  float f[kL];                      // d_j e^{G_L - G_j}
+  float d[kL];
+  float tot[4];                     // G over each block of 32
+};
+
+struct Maps {
+  CUtensorMap x, b, c, out;         // {64, T, columns / 64}, box {64, 128, blocks}
+};
+
+struct Segments {
+  int64_t slots;                    // grid: slots x column blocks
+  int len;                          // tokens per segment; 0: one per sequence
+  float* add;                       // [slots, H, P, Ns]
+  float* left;                      // [slots, H]
+};
+
+template <int P, int NS, bool kStates>
+struct Cfg {
+  static constexpr int kHeads = 128 / P;
+  static constexpr int kNB = NS / 64;
+  static constexpr int kStages = kStates ? 3 : 2;
+  static constexpr uint32_t kXBytes = 2 * kBlock, kBBytes = kNB * kBlock;
+  static constexpr uint32_t kX = 0;
+  static constexpr uint32_t kB = kX + kStages * kXBytes;
+  static constexpr uint32_t kC = kB + kStages * kBBytes;
+  static constexpr uint32_t kS = kC + (kStates ? 0 : kBBytes);
+  static constexpr uint32_t kGates = kS + (kStates ? 0 : kBBytes);
+  static constexpr uint32_t kBars = kGates + 2 * kHeads * sizeof(Gates);
+  static constexpr uint32_t kBytes = kBars + 256 + 1024;  // and the alignment
+};
+
+enum Bar {
+  kFullX = 0,       // [3], [2] and so on: one per stage
+  kFullB = 3,       // [3]
+  kFullC = 6,
+  kGatesFull = 7,   // [2]
+  kGatesFree = 9,   // [2]
+  kCB = 11,         // products done: C B^T
+  kYS = 12,         //   C S^T
+  kDS = 13,         //   dS [3]
+  kYM = 16,         //   M x
+  kFx = 17,         // operands written: f x [2] (the output kernel: one)
+  kMy = 19,         //   M and the scaled Y
+  kState = 20,      //   S
+  kYFree = 21,      // Y read out
+  kStaged = 22,     // y in shared memory [2]
+  kZeroed = 24,
+};
+
+// Waits that stop waiting after the first that gave up.
+struct Waiter {
+  bool ok = true;
+  __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t parity) {
+    if (ok) ok = mbar_wait(bar, parity);
+  }
+  __device__ __forceinline__ void spin(uint64_t* bar, uint32_t parity) {
+    if (ok) ok = mbar_wait_spin(bar, parity);
+  }
+};
+
+__device__ __forceinline__ int64_t clamp_bound(const SsmParams& p, int64_t i) {
+  const int64_t v = load_index(p.cu_seqlens, p.cu_dtype, i);
+  return v < 0 ? 0 : (v > p.T ? p.T : v);
+}
+
+// Segment `slot` in the order of the sequences: (sequence, segment of it). Whole warp.
+__device__ __forceinline__ void find_segment(const SsmParams& p, const Segments& sg, int64_t slot,
+                                             int64_t& n, int64_t& seg) {
+  const int lane = threadIdx.x & 31;
+  seg = 0;
+  if (sg.len == 0) {
+    // One segment per sequence; up to 32 sequences go longest first, so that the longest do
+    // not start last.
+    n = slot;
+    if (p.N > 32) return;
+    int64_t len = -1;
+    if (lane < p.N) len = max(clamp_bound(p, lane + 1) - clamp_bound(p, lane), int64_t{0});
+    int rank = 0;
+    for (int k = 0; k < static_cast<int>(p.N); ++k) {
+      const int64_t other = __shfl_sync(0xffffffffu, len, k);
+      rank += other > len || (other == len && k < lane);
+    }
+    n = __ffs(__ballot_sync(0xffffffffu, lane < p.N && rank == slot)) - 1;
+    return;
+  }
+  int64_t before = 0;
+  for (int64_t n0 = 0; n0 < p.N; n0 += 32) {
+    int64_t cnt = 0;
+    if (n0 + lane < p.N) {
+      const int64_t len = clamp_bound(p, n0 + lane + 1) - clamp_bound(p, n0 + lane);
+      cnt = len > sg.len ? (len + sg.len - 1) / sg.len : 1;
+    }
+    int64_t incl = cnt;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, before + incl > slot);
+    if (past) {
+      const int src = __ffs(past) - 1;
+      n = n0 + src;
+      seg = slot - before - __shfl_sync(0xffffffffu, incl - cnt, src);
+      return;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  n = p.N;
+}
+
+// Gates of a chunk's first `valid` tokens (the others: d = 0, no decay) of one head, four per
+// lane. All sums run over terms of one sign, so none of them cancels.
+__device__ __forceinline__ void write_gates(Gates* g, const float (&raw)[4], float neg_a,
+                                            float dtb, int valid, int lane) {
+  float d[4], lg[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const bool in = lane * 4 + k < valid;
+    d[k] = in ? softplus_ref(raw[k] + dtb) : 0.f;
+    const float l = in ? neg_a * d[k] * kLog2e : 0.f;
+    // 2^-127 is zero to ex2: a stronger decay changes nothing, and the sums stay small. A NaN
+    // stays one.
+    lg[k] = l < -127.f ? -127.f : l;
+  }
+  // sums over the block of 32 tokens (8 lanes) up to and from this lane
+  float pre = (lg[0] + lg[1]) + (lg[2] + lg[3]), suf = pre;
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    const float a = __shfl_up_sync(0xffffffffu, pre, o, 8);
+    const float b = __shfl_down_sync(0xffffffffu, suf, o, 8);
+    if ((lane & 7) >= o) pre += a;
+    if ((lane & 7) + o < 8) suf += b;
+  }
+  float before = __shfl_up_sync(0xffffffffu, pre, 1, 8);
+  float behind = __shfl_down_sync(0xffffffffu, suf, 1, 8);
+  if ((lane & 7) == 0) before = 0.f;
+  if ((lane & 7) == 7) behind = 0.f;
+  const float b0 = __shfl_sync(0xffffffffu, pre, 7), b1 = __shfl_sync(0xffffffffu, pre, 15);
+  const float b2 = __shfl_sync(0xffffffffu, pre, 23), b3 = __shfl_sync(0xffffffffu, pre, 31);
+  const int blk = lane >> 3;
+  const float head = blk == 0 ? 0.f : (blk == 1 ? b0 : (blk == 2 ? b0 + b1 : b0 + b1 + b2));
+  const float tail = blk == 3 ? 0.f : (blk == 2 ? b3 : (blk == 1 ? b2 + b3 : b1 + b2 + b3));
+  float c[4], w[4];  // from the block's start, inclusive; to its end, exclusive
+  c[0] = before + lg[0];
+  c[1] = c[0] + lg[1];
+  c[2] = c[1] + lg[2];
+  c[3] = c[2] + lg[3];
+  w[3] = behind;
+  w[2] = w[3] + lg[3];
+  w[1] = w[2] + lg[2];
+  w[0] = w[1] + lg[1];
+  const int at = lane * 4;
+  *reinterpret_cast<float4*>(g->cum + at) = make_float4(c[0], c[1], c[2], c[3]);
+  *reinterpret_cast<float4*>(g->dec + at) =
+      make_float4(ex2(head + c[0]), ex2(head + c[1]), ex2(head + c[2]), ex2(head + c[3]));
+  *reinterpret_cast<float4*>(g->u + at) =
+      make_float4(d[0] * ex2(w[0]), d[1] * ex2(w[1]), d[2] * ex2(w[2]), d[3] * ex2(w[3]));
+  *reinterpret_cast<float4*>(g->f + at) =
+      make_float4(d[0] * ex2(w[0] + tail), d[1] * ex2(w[1] + tail), d[2] * ex2(w[2] + tail),
+                  d[3] * ex2(w[3] + tail));
+  *reinterpret_cast<float4*>(g->d + at) = make_float4(d[0], d[1], d[2], d[3]);
+  if ((lane & 7) == 7) g->tot[blk] = pre;
+}
+
+template <int P, int NS, bool kStates>
+__global__ void __launch_bounds__(kThreads, 1)
+ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Maps maps,
+                 const __grid_constant__ Segments sg, int col_blocks) {
+  using K = Cfg<P, NS, kStates>;
+  constexpr int kHeads = K::kHeads;
+  constexpr int kNC = NS / 4;      // state columns per thread
+  extern __shared__ uint8_t raw_smem[];
+  uint8_t* const sm = align_smem<1024>(raw_smem);
+  __shared__ int64_t s_where[2];
+  __shared__ uint32_t s_tmem;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  const int64_t slot = blockIdx.x / col_blocks;
+  const int cb = static_cast<int>(blockIdx.x - slot * col_blocks);
+  if (warp == 0) {
+    int64_t n, seg;
+    find_segment(p, sg, slot, n, seg);
+    if (lane == 0) {
+      s_where[0] = n;
+      s_where[1] = seg;
+    }
+  }
+  __syncthreads();
+  const int64_t n = s_where[0], seg = s_where[1];
+  if (n >= p.N) return;
+
+  const int rep = p.H / p.G;                                  // heads of a group
+  const int per_group = (rep + kHeads - 1) / kHeads;
+  const int grp = cb / per_group;
+  const int h0 = grp * rep + (cb - grp * per_group) * kHeads;  // first head of the block
+  const int heads = min(kHeads, (grp + 1) * rep - h0);
+  const int64_t s_begin = clamp_bound(p, n);
+  const int64_t s_end = max(clamp_bound(p, n + 1), s_begin);
+  if (cb == 0 && seg == 0 && threadIdx.x == 0) {
+    const int64_t lo = load_index(p.cu_seqlens, p.cu_dtype, n);
+    const int64_t hi = load_index(p.cu_seqlens, p.cu_dtype, n + 1);
+    if (lo < 0 || hi > p.T || hi < lo) report_bad_bounds(p.status);
+  }
+  const int64_t t_begin = sg.len ? s_begin + seg * sg.len : s_begin;
+  const int64_t t_end = sg.len ? min(t_begin + sg.len, s_end) : s_end;
+  const bool last = t_end >= s_end;
+  if (kStates && last) return;  // the second kernel computes the sequence's last state
+  const int tokens = static_cast<int>(t_end - t_begin);
+  const int chunks = (tokens + kL - 1) / kL;
+  const int tail = tokens - (chunks - 1) * kL;                // of the last chunk
+  const int tok0 = static_cast<int>(t_begin);
+
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(sm + K::kBars);
+  Gates* const gates = reinterpret_cast<Gates*>(sm + K::kGates);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(bars + kFullX + i, 1);
+      mbar_init(bars + kFullB + i, 1);
+      mbar_init(bars + kDS + i, 1);
+    }
+    mbar_init(bars + kFullC, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bars + kGatesFull + i, kHeads);
+      mbar_init(bars + kGatesFree + i, kComputeWarps);
+      mbar_init(bars + kFx + i, kComputeWarps);
+      mbar_init(bars + kStaged + i, kComputeWarps);
+    }
+    mbar_init(bars + kCB, 1);
+    mbar_init(bars + kYS, 1);
+    mbar_init(bars + kYM, 1);
+    for (int i : {kMy, kState, kYFree, kZeroed}) mbar_init(bars + i, kComputeWarps);
+    fence_mbar_init();
+  }
+  if (warp == 16) tmem_alloc(&s_tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tm = s_tmem;
+  Waiter wait;
+
+  if (warp < kComputeWarps) {
+    const int q = warp & 3, cg = warp >> 2;
+    const uint32_t lanes = tm + (static_cast<uint32_t>(32 * q) << 16);
+    const int row = 32 * q + lane;               // token of a chunk / column of the block
+    const int row_head = kHeads == 2 ? q >> 1 : 0;   // head of column `row`
+    const int col_head = kHeads == 2 ? cg >> 1 : 0;  // head of columns 32 cg to 32 cg + 31
+    const int64_t st_off =
+        ((n * p.H + h0) * static_cast<int64_t>(P) + row) * NS + kNC * cg;
+    const bool mine = row_head < heads;
+    float S[kNC];
+#pragma unroll
+    for (int i = 0; i < kNC; ++i) S[i] = 0.f;
+    float left = 1.f;
+
+    if (!kStates) {
+      if (p.state && mine) {
+        const float* src = static_cast<const float*>(p.state) + st_off;
+#pragma unroll
+        for (int i = 0; i < kNC; i += 4)
+          *reinterpret_cast<float4*>(S + i) = *reinterpret_cast<const float4*>(src + i);
+      }
+      if (mine) {  // the segments of this sequence before this one
+        for (int64_t r = slot - seg; r < slot; ++r) {
+          const float g = sg.left[r * p.H + h0 + row_head];
+          const float* src =
+              sg.add + ((r * p.H + h0) * static_cast<int64_t>(P) + row) * NS + kNC * cg;
+#pragma unroll
+          for (int i = 0; i < kNC; i += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(src + i);
+            S[i] = fmaf(g, S[i], v.x);
+            S[i + 1] = fmaf(g, S[i + 1], v.y);
+            S[i + 2] = fmaf(g, S[i + 2], v.z);
+            S[i + 3] = fmaf(g, S[i + 3], v.w);
+          }
+        }
+      }
+    }
+
+    // The state as the operand of the next chunk's C S^T: row = column of the block, n
+    // contiguous (K-major).
+    auto write_state = [&]() {
+#pragma unroll
+      for (int k = 0; k < kNC / 8; ++k) {
+        const int nn = kNC * cg + 8 * k;
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = pack2_rn(S[8 * k + 2 * e], S[8 * k + 2 * e + 1]);
+        *reinterpret_cast<uint4*>(sm + K::kS + (nn >> 6) * kBlock +
+                                  sw128_chunk(row, (nn >> 3) & 7)) =
+            make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      fence_async_smem();
+    };
+    auto arrive = [&](int bar) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bars + bar);
+    };
+
+    // (f x)^T of chunk c into TMEM, tokens 32 cg to 32 cg + 31 of columns 32 q to 32 q + 31:
+    // transposed by ldmatrix, scaled, split and stored as the fragments come.
+    auto write_fx = [&](int c) {
+      const int st = c % K::kStages, par = (c / K::kStages) & 1, gs = c & 1;
+      uint8_t* const xt = sm + K::kX + st * K::kXBytes;
+      wait(bars + kFullX + st, par);
+      if (c == chunks - 1 && tail < kL) {
+        // Rows behind the sequence hold other tokens or nothing: zeros, so that neither they
+        // nor a NaN among them enters a product.
+        uint8_t* const bt = sm + K::kB + st * K::kBBytes;
+        wait(bars + kFullB + st, par);
+        for (int i = threadIdx.x; i < (kL - tail) * 8; i += kComputeWarps * 32) {
+          const uint32_t off = (tail + (i >> 3)) * 128 + (i & 7) * 16;
+          const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+          *reinterpret_cast<uint4*>(xt + off) = z;
+          *reinterpret_cast<uint4*>(xt + kBlock + off) = z;
+#pragma unroll
+          for (int b = 0; b < K::kNB; ++b) *reinterpret_cast<uint4*>(bt + b * kBlock + off) = z;
+        }
+        fence_async_smem();
+        named_bar_sync(5, kComputeWarps * 32);
+        arrive(kZeroed);
+      }
+      wait(bars + kGatesFull + gs, (c >> 1) & 1);
+      const float* f = gates[gs * kHeads + row_head].f + 32 * cg + 2 * (lane & 3);
+      float2 fv[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) fv[j] = *reinterpret_cast<const float2*>(f + 8 * j);
+      const uint32_t xb = smem_u32(xt + (q >> 1) * kBlock);
+      const uint32_t t_hi = lanes + (kStates && (c & 1) ? kTG : kTF) + 16 * cg;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+          uint32_t u[4];  // tokens 8 (2 jj): columns 0-7, 8-15; tokens 8 (2 jj + 1): the same
+          const int tok = 32 * cg + 8 * (2 * jj + (lane >> 4)) + (lane & 7);
+          const int ch = (q & 1) * 4 + half * 2 + ((lane >> 3) & 1);
+          ldmatrix_x4_trans(xb + sw128_chunk(tok, ch), u);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 s = fv[2 * jj + (k >> 1)];
+            const float2 v = mul2(make_float2(__uint_as_float(u[k] << 16),
+                                              __uint_as_float(u[k] & 0xffff0000u)),
+                                  s);
+            split2(v.x, v.y, hi[4 * jj + k], lo[4 * jj + k]);
+          }
+        }
+        tmem_st_frag(t_hi + (static_cast<uint32_t>(16 * half) << 16), hi);
+        tmem_st_frag(t_hi + 64 + (static_cast<uint32_t>(16 * half) << 16), lo);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      arrive(kFx + (kStates ? (c & 1) : 0));
+    };
+
+    // The state behind chunk c, from what the chunk adds.
+    auto update_state = [&](int c) {
+      const int gs = c & 1;
+      wait(bars + kDS + c % K::kStages, (c / K::kStages) & 1);
+      tc_fence_after();
+      const float g = gates[gs * kHeads + row_head].dec[kL - 1];
+      const uint32_t td = lanes + (kStates && (c & 1) ? kTY : kTD) + kNC * cg;
+      if constexpr (kNC == 32) {
+        float v[32];
+        tmem_ld32(td, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) S[i] = fmaf(g, S[i], v[i]);
+      } else {
+        float v[16];
+        tmem_ld16(td, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) S[i] = fmaf(g, S[i], v[i]);
+      }
+      if (kStates) left *= g;
+      tc_fence_before();
+    };
+
+    if (kStates) {
+      if (chunks > 0) write_fx(0);
+      for (int c = 0; c < chunks; ++c) {
+        // fx and dS alternate between two places, so the next operand is written while the
+        // product of this one runs
+        if (c + 1 < chunks) write_fx(c + 1);
+        update_state(c);
+        arrive(kGatesFree + (c & 1));
+      }
+    } else if (chunks > 0) {
+      write_state();
+      arrive(kState);
+      write_fx(0);
+      for (int c = 0; c < chunks; ++c) {
+        const int gs = c & 1;
+        const Gates* const ga = gates + gs * kHeads;
+        // ---- M, over C B^T (this warp: tokens 32 q + lane, 32 cg to 32 cg + 31)
+        wait(bars + kCB, c & 1);
+        tc_fence_after();
+        float g[32];
+        if (cg <= q) {
+          tmem_ld32(lanes + kTG + 32 * cg, g);
+          tmem_ld_wait();
+        }
+        tc_fence_before();
+        named_bar_sync(1 + q, 128);  // every warp of these lanes has read before M overwrites
+        tc_fence_after();
+#pragma unroll
+        for (int hh = 0; hh < kHeads; ++hh) {
+          uint32_t m[16];
+          if (cg > q) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) m[j] = 0u;
+          } else if (cg < q) {
+            // e^{G_i - G_j} d_j = e^{G_i - G_r} (e^{G_r - G_j} d_j), r between j and i: both
+            // exponents are at most 0, and one exponential per row is left
+            float ex = ga[hh].cum[row];
+            for (int b = cg + 1; b < q; ++b) ex += ga[hh].tot[b];
+            const float a = ex2(ex);
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              const float4 u = *reinterpret_cast<const float4*>(ga[hh].u + 32 * cg + j);
+              const float2 v0 = mul2(mul2(make_float2(u.x, u.y), make_float2(a, a)),
+                                     make_float2(g[j], g[j + 1]));
+              const float2 v1 = mul2(mul2(make_float2(u.z, u.w), make_float2(a, a)),
+                                     make_float2(g[j + 2], g[j + 3]));
+              m[j / 2] = pack2_rn(v0.x, v0.y);
+              m[j / 2 + 1] = pack2_rn(v1.x, v1.y);
+            }
+          } else {
+            const float ci = ga[hh].cum[row];
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              const float4 cj = *reinterpret_cast<const float4*>(ga[hh].cum + 32 * cg + j);
+              const float4 dj = *reinterpret_cast<const float4*>(ga[hh].d + 32 * cg + j);
+              const float v0 = j <= lane ? g[j] * (ex2(ci - cj.x) * dj.x) : 0.f;
+              const float v1 = j + 1 <= lane ? g[j + 1] * (ex2(ci - cj.y) * dj.y) : 0.f;
+              const float v2 = j + 2 <= lane ? g[j + 2] * (ex2(ci - cj.z) * dj.z) : 0.f;
+              const float v3 = j + 3 <= lane ? g[j + 3] * (ex2(ci - cj.w) * dj.w) : 0.f;
+              m[j / 2] = pack2_rn(v0, v1);
+              m[j / 2 + 1] = pack2_rn(v2, v3);
+            }
+          }
+          tmem_st16(lanes + kTG + 64 * hh + 16 * cg, m);
+        }
+        // ---- Y = e^{G_i} (C S^T), in place
+        wait(bars + kYS, c & 1);
+        tc_fence_after();
+        {
+          float y[32];
+          const uint32_t ty = lanes + kTY + 32 * cg;
+          tmem_ld32(ty, y);
+          const float e = ga[col_head].dec[row];
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) y[i] *= e;
+          tmem_st32(ty, y);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        arrive(kMy);
+        // ---- state
+        update_state(c);
+        arrive(kGatesFree + gs);
+        if (c + 1 < chunks) {
+          write_state();
+          arrive(kState);
+          write_fx(c + 1);
+        }
+        // ---- y: out of TMEM, D x added, over the chunk's x in shared memory
+        const int st = c % K::kStages;
+        uint8_t* const xrow = sm + K::kX + st * K::kXBytes + (cg >> 1) * kBlock;
+        wait(bars + kYM, c & 1);
+        tc_fence_after();
+        {
+          float y[32];
+          tmem_ld32(lanes + kTY + 32 * cg, y);
+          tmem_ld_wait();
+          tc_fence_before();
+          arrive(kYFree);
+          const float skip =
+              p.D && col_head < heads ? load_scalar(p.D, p.D_dtype, h0 + col_head) : 0.f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint4* const at =
+                reinterpret_cast<uint4*>(xrow + sw128_chunk(row, (cg & 1) * 4 + k));
+            if (p.D) {
+              const uint4 xv = *at;
+              const uint32_t u[4] = {xv.x, xv.y, xv.z, xv.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                y[8 * k + 2 * e] = fmaf(skip, __uint_as_float(u[e] << 16), y[8 * k + 2 * e]);
+                y[8 * k + 2 * e + 1] =
+                    fmaf(skip, __uint_as_float(u[e] & 0xffff0000u), y[8 * k + 2 * e + 1]);
+              }
+            }
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = pack2_rn(y[8 * k + 2 * e], y[8 * k + 2 * e + 1]);
+            *at = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        if (c < chunks - 1 || tail == kL) {
+          fence_async_smem();
+          arrive(kStaged + st);  // a bulk store takes the whole tile
+        } else {
+          // only the sequence's rows: 16 lanes write the 256 bytes of one
+          named_bar_sync(5, kComputeWarps * 32);
+          uint8_t* const xt = sm + K::kX + st * K::kXBytes;
+          const int l = lane & 15, blk = l >> 3;
+          const int64_t base = (static_cast<int64_t>(tok0) + c * kL) * p.H + h0;
+          if (kHeads == 1 || blk < heads) {
+            for (int r = warp * 2 + (lane >> 4); r < tail; r += kComputeWarps * 2) {
+              const uint4 v =
+                  *reinterpret_cast<const uint4*>(xt + blk * kBlock + sw128_chunk(r, l & 7));
+              *reinterpret_cast<uint4*>(p.out + (base + static_cast<int64_t>(r) * p.H) * P +
+                                        l * 8) = v;
+            }
+          }
+        }
+      }
+    }
+    if (mine) {
+      if (kStates) {
+        float* dst =
+            sg.add + ((slot * p.H + h0) * static_cast<int64_t>(P) + row) * NS + kNC * cg;
+#pragma unroll
+        for (int i = 0; i < kNC; i += 4)
+          *reinterpret_cast<float4*>(dst + i) = make_float4(S[i], S[i + 1], S[i + 2], S[i + 3]);
+        if (cg == 0 && row % P == 0) sg.left[slot * p.H + h0 + row_head] = left;
+      } else if (last) {
+        float* dst = static_cast<float*>(p.new_state) + st_off;
+#pragma unroll
+        for (int i = 0; i < kNC; i += 4)
+          *reinterpret_cast<float4*>(dst + i) = make_float4(S[i], S[i + 1], S[i + 2], S[i + 3]);
+      }
+    }
+  } else if (warp == 16) {
+    // ---------------------------------------------------------------- products
+    constexpr uint32_t kIdCB = idesc_bf16(128, 128, false, false);
+    constexpr uint32_t kIdDS = idesc_bf16(128, NS, false, true);
+    constexpr uint32_t kIdYM = idesc_bf16(128, P, false, true);
+    const uint64_t d_c = desc_kmajor(smem_u32(sm + K::kC));
+    const uint64_t d_s = desc_kmajor(smem_u32(sm + K::kS));
+    auto kstep = [](int s) { return static_cast<uint64_t>(((s >> 2) * kBlock + (s & 3) * 32) >> 4); };
+    for (int c = 0; c < chunks; ++c) {
+      const int st = c % K::kStages, par = (c / K::kStages) & 1;
+      const uint32_t xb = smem_u32(sm + K::kX + st * K::kXBytes);
+      const uint32_t bb = smem_u32(sm + K::kB + st * K::kBBytes);
+      const bool zeroed = c == chunks - 1 && tail < kL;
+      auto issue_ds = [&](uint32_t td, uint32_t tf) {
+        const uint64_t db = desc_mnmajor(bb, kBlock);
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+          mma_bf16_ts_w(td, tf + 8 * s, db + static_cast<uint64_t>((s * 2048) >> 4), kIdDS, s > 0);
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+          mma_bf16_ts_w(td, tf + 64 + 8 * s, db + static_cast<uint64_t>((s * 2048) >> 4), kIdDS, 1);
+      };
+      if (kStates) {
+        wait.spin(bars + kFullB + st, par);
+        wait.spin(bars + kFx + (c & 1), (c >> 1) & 1);
+        tc_fence_after();
+        issue_ds(tm + (c & 1 ? kTY : kTD), tm + (c & 1 ? kTG : kTF));
+        mma_commit_w(bars + kDS + st);
+        continue;
+      }
+      // C B^T: over the place of the last chunk's M
+      wait.spin(bars + kFullB + st, par);
+      wait.spin(bars + kFullC, c & 1);
+      if (zeroed) wait.spin(bars + kZeroed, 0);
+      if (c > 0) wait.spin(bars + kYM, (c - 1) & 1);
+      tc_fence_after();
+      const uint64_t d_b = desc_kmajor(bb);
+#pragma unroll
+      for (int s = 0; s < NS / 16; ++s)
+        mma_bf16_w(tm + kTG, d_c + kstep(s), d_b + kstep(s), kIdCB, s > 0);
+      mma_commit_w(bars + kCB);
+      // C S^T
+      wait.spin(bars + kState, c & 1);
+      if (c > 0) wait.spin(bars + kYFree, (c - 1) & 1);
+      tc_fence_after();
+#pragma unroll
+      for (int s = 0; s < NS / 16; ++s)
+        mma_bf16_w(tm + kTY, d_c + kstep(s), d_s + kstep(s), kIdCB, s > 0);
+      mma_commit_w(bars + kYS);
+      // (f x)^T B
+      wait.spin(bars + kFx, c & 1);
+      tc_fence_after();
+      issue_ds(tm + kTD, tm + kTF);
+      mma_commit_w(bars + kDS + st);
+      // M x
+      wait.spin(bars + kMy, c & 1);
+      tc_fence_after();
+#pragma unroll
+      for (int hh = 0; hh < kHeads; ++hh) {
+        const uint64_t dx = desc_mnmajor(xb + hh * kBlock, kBlock);
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+          mma_bf16_ts_w(tm + kTY + hh * 64, tm + kTG + hh * 64 + 8 * s,
+                        dx + static_cast<uint64_t>((s * 2048) >> 4), kIdYM, 1);
+      }
+      mma_commit_w(bars + kYM);
+    }
+    // the block's TMEM may go once the last product is done
+    if (chunks > 0) {
+      const int c = chunks - 1;
+      if (kStates) {
+        mbar_wait(bars + kDS + c % K::kStages, (c / K::kStages) & 1);
+      } else {
+        mbar_wait(bars + kYM, c & 1);
+      }
+    }
+  } else if (warp == 17) {
+    // ---------------------------------------------------------------- bulk copies
+    if (lane == 0) {
+      const int xc = (h0 * P) / 64, bc = grp * K::kNB;
+      auto load_x = [&](int c) {
+        const int st = c % K::kStages;
+        mbar_arrive_expect_tx(bars + kFullX + st, K::kXBytes);
+        tma_load_3d(sm + K::kX + st * K::kXBytes, &maps.x, bars + kFullX + st, 0, tok0 + c * kL, xc);
+      };
+      auto load_b = [&](int c) {
+        const int st = c % K::kStages;
+        mbar_arrive_expect_tx(bars + kFullB + st, K::kBBytes);
+        tma_load_3d(sm + K::kB + st * K::kBBytes, &maps.b, bars + kFullB + st, 0, tok0 + c * kL, bc);
+      };
+      auto load_c = [&](int c) {
+        mbar_arrive_expect_tx(bars + kFullC, K::kBBytes);
+        tma_load_3d(sm + K::kC, &maps.c, bars + kFullC, 0, tok0 + c * kL, bc);
+      };
+      if (chunks > 0) {
+        load_b(0);
+        if (!kStates) load_c(0);
+        load_x(0);
+      }
+      for (int c = 1; c < K::kStages && c < chunks; ++c) {
+        load_b(c);
+        load_x(c);
+      }
+      for (int c = 0; c < chunks; ++c) {
+        if (kStates) {
+          if (c + K::kStages < chunks) {
+            wait(bars + kDS + c % K::kStages, (c / K::kStages) & 1);  // x was read before it
+            load_b(c + K::kStages);
+            load_x(c + K::kStages);
+          }
+          continue;
+        }
+        if (c + 1 < chunks) {
+          wait(bars + kYS, c & 1);
+          load_c(c + 1);
+        }
+        if (c + K::kStages < chunks) {
+          wait(bars + kDS + c % K::kStages, (c / K::kStages) & 1);
+          load_b(c + K::kStages);
+        }
+        if (c < chunks - 1 || tail == kL) {
+          wait(bars + kStaged + c % K::kStages, (c / K::kStages) & 1);
+          const uint8_t* xt = sm + K::kX + (c % K::kStages) * K::kXBytes;
+          for (int b = 0; b < 2; ++b)
+            if (kHeads == 1 || b < heads)
+              tma_store_3d(&maps.out, xt + b * kBlock, 0, tok0 + c * kL, xc + b);
+          bulk_commit();
+          if (c + K::kStages < chunks) {
+            bulk_wait_read();
+            load_x(c + K::kStages);
+          }
+        }
+      }
+      if (!kStates) bulk_wait_all();
+      if (!wait.ok && chunks > 0) {
+        // copies still in flight land in this block's shared memory: let them
+        const int c = chunks - 1;
+        mbar_wait(bars + kFullX + c % K::kStages, (c / K::kStages) & 1);
+        mbar_wait(bars + kFullB + c % K::kStages, (c / K::kStages) & 1);
+        if (!kStates) mbar_wait(bars + kFullC, c & 1);
+      }
+    }
+    __syncwarp();
+  } else if (warp - 18 < kHeads) {
+    // ---------------------------------------------------------------- gates of one head
+    const int hh = warp - 18;
+    const bool present = hh < heads;
+    const int h = h0 + (present ? hh : 0);
+    const float neg_a = -expf(load_scalar(p.A_log, p.A_log_dtype, h));
+    const float dtb = load_scalar(p.dt_bias, p.dt_bias_dtype, h);
+    auto load = [&](int c, float (&raw)[4]) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int t = c * kL + lane * 4 + k;
+        raw[k] = t < tokens
+                     ? load_scalar(p.dt, p.dt_dtype, (static_cast<int64_t>(tok0) + t) * p.H + h)
+                     : 0.f;
+      }
+    };
+    float raw[4];
+    if (chunks > 0) load(0, raw);
+    for (int c = 0; c < chunks; ++c) {
+      const int gs = c & 1;
+      float next[4] = {0.f, 0.f, 0.f, 0.f};
+      if (c + 1 < chunks) load(c + 1, next);
+      if (c >= 2) wait(bars + kGatesFree + gs, ((c >> 1) - 1) & 1);
+      write_gates(gates + gs * kHeads + hh, raw, neg_a, dtb, present ? tokens - c * kL : 0, lane);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bars + kGatesFull + gs);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) raw[k] = next[k];
+    }
+  }
+  if (!wait.ok) report_wait(p.status);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 16) tmem_dealloc(tm, 512);
+}
+
+bool encode(CUtensorMap* map, const void* base, int64_t T, int64_t cols, uint32_t blocks) {
+  chunk::EncodeTiledFn enc = chunk::get_encode_fn();
+  if (!enc) return false;
+  const cuuint64_t dims[3] = {64, static_cast<cuuint64_t>(T), static_cast<cuuint64_t>(cols / 64)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(cols) * 2, 128};
+  const cuuint32_t box[3] = {64, kL, blocks};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
+             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int column_blocks(int H, int G, int P) {
+  const int heads = 128 / P;
+  return G * ((H / G + heads - 1) / heads);
+}
+
+// Tokens per segment (0: whole sequences) and the number of slots that covers any lengths.
+void plan(int64_t T, int64_t N, int H, int G, int P, int& len, int64_t& slots) {
+  constexpr int kSms = 148, kLeast = 8 * kL;
+  len = 0;
+  slots = N;
+  const int64_t fit = kSms / column_blocks(H, G, P);  // segments that run at the same time
+  if (fit < 2 * N || T < 2 * kLeast) return;
+  const int64_t want = (T + fit - N) / (fit - N + 1);
+  const int64_t l = want > kLeast ? (want + kL - 1) / kL * kL : kLeast;
+  len = static_cast<int>(l);
+  slots = T / l + N;
+}
+
+template <int P, int NS>
+int launch_as(const SsmParams& p, cudaStream_t stream) {
+  Segments sg{};
+  plan(p.T, p.N, p.H, p.G, p.P, sg.len, sg.slots);
+  const int cols = column_blocks(p.H, p.G, p.P);
+  if (sg.slots * cols > 0x7fffffffLL) return GDN_ERR_UNSUPPORTED_SHAPE;
+  Maps maps;
+  const int64_t hp = static_cast<int64_t>(p.H) * P, gn = static_cast<int64_t>(p.G) * NS;
+  // without tokens the maps are not read; any mapped memory will do
+  const int64_t T = p.T > 0 ? p.T : 1;
+  const bool any = p.T > 0;
+  if (!encode(&maps.x, any ? static_cast<const void*>(p.x) : p.new_state, T, hp, 2) ||
+      !encode(&maps.b, any ? static_cast<const void*>(p.B) : p.new_state, T, gn, NS / 64) ||
+      !encode(&maps.c, any ? static_cast<const void*>(p.C) : p.new_state, T, gn, NS / 64) ||
+      !encode(&maps.out, any ? static_cast<const void*>(p.out) : p.new_state, T, hp, 1))
+    return GDN_ERR_CUDA;
+  const unsigned grid = static_cast<unsigned>(sg.slots * cols);
+  if (sg.len) {
+    if (!p.workspace) return GDN_ERR_WORKSPACE;
+    sg.add = p.workspace;
+    sg.left = p.workspace + sg.slots * hp * NS;
+    using K = Cfg<P, NS, true>;
+    auto fn = ssm_chunk_kernel<P, NS, true>;
+    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, K::kBytes) !=
+        cudaSuccess)
+      return GDN_ERR_CUDA;
+    fn<<<grid, kThreads, K::kBytes, stream>>>(p, maps, sg, cols);
+    if (cudaGetLastError() != cudaSuccess) return GDN_ERR_CUDA;
+  }
+  using K = Cfg<P, NS, false>;
+  auto fn = ssm_chunk_kernel<P, NS, false>;
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, K::kBytes) !=
+      cudaSuccess)
+    return GDN_ERR_CUDA;
+  fn<<<grid, kThreads, K::kBytes, stream>>>(p, maps, sg, cols);
+  return cudaGetLastError() == cudaSuccess ? 0 : GDN_ERR_CUDA;
+}
+
+}  // namespace
+
+bool ssm_chunked_takes(int P, int Ns) {
+  return (P == 64 || P == 128) && (Ns == 64 || Ns == 128);
+}
+
+size_t ssm_chunked_workspace(int64_t T, int64_t N, int H, int G, int P, int Ns) {
+  int len;
+  int64_t slots;
+  plan(T, N, H, G, P, len, slots);
+  return len ? static_cast<size_t>(slots) * H * (static_cast<size_t>(P) * Ns + 1) * sizeof(float)
+             : 0;
+}
+
+int launch_ssm_chunked(const SsmParams& p, cudaStream_t stream) {
+  if (p.P == 64) {
+    return p.Ns == 64 ? launch_as<64, 64>(p, stream) : launch_as<64, 128>(p, stream);
+  }
+  return p.Ns == 64 ? launch_as<128, 64>(p, stream) : launch_as<128, 128>(p, stream);
+}
+
+}  // namespace gdn

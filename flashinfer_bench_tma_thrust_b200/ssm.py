@@ -118,7 +118,23 @@ def prefill(x, dt, A_log, B, C, D, dt_bias, state, cu_seqlens, *, check=False):
     A ``cu_seqlens`` that leaves [0, T] or decreases, or a bounded wait that gave up, raises
     GDNError at the next call on the device, or at this one with ``check=True`` (which
     synchronises)."""
-    return prefill_recurrent(x, dt, A_log, B, C, D, dt_bias, state, cu_seqlens, check=check)
+    a = _prefill_args(x, dt, A_log, B, C, D, dt_bias, state, cu_seqlens)
+    lib = _lib.load()
+    with K.on_device(a.dev):
+        status = _status.address(a.dev.index)
+        out = torch.empty(a.T, a.H, a.P, dtype=torch.bfloat16, device=a.dev)
+        new_state = torch.empty(a.N, a.H, a.P, a.Ns, dtype=torch.float32, device=a.dev)
+        nbytes = lib.gdn_ssm_prefill_workspace_size(a.T, a.N, a.H, a.G, a.P, a.Ns)
+        # of this call alone: calls on several streams and captured graphs share nothing
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=a.dev) if nbytes else None
+        rc = lib.gdn_ssm_prefill_fwd(
+            _aligned(a.x).data_ptr(), a.dt.data_ptr(), a.dt_t, a.A.data_ptr(), a.A_t,
+            a.B.data_ptr(), a.C.data_ptr(), K.ptr(a.D), a.D_t, a.dtb.data_ptr(), a.dtb_t,
+            K.ptr(a.state), a.cu.data_ptr(), a.cu_t, out.data_ptr(), new_state.data_ptr(), a.T,
+            a.N, a.H, a.G, a.P, a.Ns, K.ptr(ws), nbytes, status, K.stream_handle(a.dev))
+        _lib.check(rc, "gdn_ssm_prefill_fwd")
+        _status.finish(a.dev.index, check)
+    return out, new_state
 
 
 def _decode(x, dt, A_log, B, C, D, dt_bias, state, inplace):

@@ -311,6 +311,31 @@ GDN_API int gdn_ssm_prefill_recurrent_fwd(const void* x, const void* dt, int dt_
                                           int32_t* status, void* stream);
 
 /*
+ * The scan over packed prompts, the fast path: arguments as gdn_ssm_prefill_recurrent_fwd,
+ * plus
+ *
+ *   workspace   gdn_ssm_prefill_workspace_size(T, N, H, G, P, Ns) bytes of device memory,
+ *               16-byte aligned, of any content (often 0 bytes: NULL). Calls that overlap on
+ *               the GPU need one each.
+ *   status      [0] becomes 1 where a bounded wait gave up (that call's results are invalid)
+ *
+ * With P and Ns of 64 or 128 the chunked tensor-core kernels run (chunks of 128 tokens; one
+ * launch, two where few long sequences are cut into segments; x and out 16-byte aligned,
+ * T < 2^31 - 256); other sizes run the token-by-token kernel. In a chunk an infinity or NaN
+ * in x also reaches the outputs of up to 127 tokens before it, of the same channel.
+ */
+GDN_API size_t gdn_ssm_prefill_workspace_size(int64_t T, int64_t N, int32_t H, int32_t G,
+                                              int32_t P, int32_t Ns);
+
+GDN_API int gdn_ssm_prefill_fwd(const void* x, const void* dt, int dt_dtype, const void* A_log,
+                                int A_log_dtype, const void* B, const void* C, const void* D,
+                                int D_dtype, const void* dt_bias, int dt_bias_dtype,
+                                const float* state, const void* cu_seqlens, int cu_dtype,
+                                void* out, float* new_state, int64_t T, int64_t N, int32_t H,
+                                int32_t G, int32_t P, int32_t Ns, void* workspace,
+                                size_t workspace_bytes, int32_t* status, void* stream);
+
+/*
  * Diagnostics. Known-answer check of the tensor-core path the chunked prefill
  * is built on (no counterpart in the reference): D[128x64] fp32 = A[128x128] x
  * B[128x64], bf16 row-major inputs, staged in shared memory in the K-major

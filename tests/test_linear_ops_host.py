@@ -49,15 +49,19 @@ def test_conv_abi_refusals(cuda_lib, fn):
 
 
 def _ssm(lib, fn="decode", H=4, G=2, P=64, Ns=64, T=4, N=1, dt=(1, 0, 0, 0), sdt=0, cu_dt=2,
-         ptr=P16, B=P16, cu=P16):
+         ptr=P16, B=P16, cu=P16,
+         out=None, ws=None, wb=0):
     head = (ptr, ptr, dt[0], ptr, dt[1], B, ptr, ptr, dt[2], ptr, dt[3])
     if fn == "decode":
         return lib.gdn_ssm_decode_fwd(*head, None, sdt, ptr, ptr, T, H, G, P, Ns, None)
+    if fn == "chunked":
+        return lib.gdn_ssm_prefill_fwd(*head, None, cu, cu_dt, out or ptr, ptr, T, N, H, G, P, Ns,
+                                       ws, wb, None, None)
     return lib.gdn_ssm_prefill_recurrent_fwd(*head, None, cu, cu_dt, ptr, ptr, T, N, H, G, P, Ns,
                                              None, None)
 
 
-@pytest.mark.parametrize("fn", ["decode", "recurrent"])
+@pytest.mark.parametrize("fn", ["decode", "recurrent", "chunked"])
 def test_ssm_abi_refusals(cuda_lib, fn):
     lib = cuda_lib
     assert _ssm(lib, fn, T=-1) == -1
@@ -79,6 +83,25 @@ def test_ssm_abi_refusals(cuda_lib, fn):
         assert _ssm(lib, fn, cu_dt=1) == -3
         assert _ssm(lib, fn, cu=None) == -1
         assert _ssm(lib, fn, N=0) == 0
+
+
+def test_ssm_chunked_workspace_and_alignment(cuda_lib):
+    """The workspace covers every segment of any lengths; a missing, small or unaligned one and
+    unaligned x or out are refused."""
+    lib = cuda_lib
+    size = lib.gdn_ssm_prefill_workspace_size
+    assert size(100, 1, 32, 16, 128, 128) == 0             # short
+    assert size(32768, 8, 32, 16, 128, 128) == 0           # enough chains
+    assert size(5000, 1, 4, 2, 80, 64) == 0                # token by token
+    assert size(-1, 1, 4, 2, 64, 64) == 0 and size(5000, 1, 3, 2, 64, 64) == 0
+    need = size(2500, 1, 2, 1, 64, 128)
+    assert need == (2500 // 1024 + 1) * 2 * (64 * 128 + 1) * 4
+    call = dict(T=2500, N=1, H=2, G=1, P=64, Ns=128)
+    assert _ssm(lib, "chunked", **call) == -5
+    assert _ssm(lib, "chunked", ws=P16, wb=need - 1, **call) == -5
+    assert _ssm(lib, "chunked", ws=P16 + 4, wb=need, **call) == -1
+    assert _ssm(lib, "chunked", out=P16 + 2) == -1
+    assert _ssm(lib, "chunked", T=0x7fffff01) == -2
 
 
 def test_cpu_tensors_are_refused():

@@ -60,6 +60,74 @@ def test_recurrent_prompt(lengths, gates):
     check_prompt(ssm.prefill_recurrent(*dev(a), check=True), a, False)
 
 
+@pytest.mark.parametrize("lengths", LENGTHS + [[513, 40]])
+@pytest.mark.parametrize("P,Ns", [(64, 64), (64, 128), (128, 64), (128, 128)])
+@pytest.mark.parametrize("gates", ["slow", "fast"])
+def test_chunked_prompt(lengths, P, Ns, gates):
+    a = make(lengths, P=P, Ns=Ns, gates=gates, seed=len(lengths) + P)
+    check_prompt(ssm.prefill(*dev(a), check=True), a, True)
+
+
+@pytest.mark.parametrize("H,G", [(1, 1), (3, 1), (3, 3), (10, 2), (6, 2)])
+@pytest.mark.parametrize("P", [64, 128])
+def test_chunked_heads(H, G, P):
+    """Groups of odd size: a column block of two heads with one of them missing."""
+    a = make([200, 128], H=H, G=G, P=P, Ns=64, state=False, skip=False, gdtype=torch.bfloat16,
+             seed=H)
+    check_prompt(ssm.prefill(*dev(a), check=True), a, True)
+
+
+@pytest.mark.parametrize("lengths", [[2500], [1500, 0, 1100, 7], [1024, 1024], [2049]])
+@pytest.mark.parametrize("P,Ns", [(64, 128), (128, 64)])
+def test_chunked_segments(lengths, P, Ns):
+    """Few heads and long sequences: cut into segments (two launches)."""
+    a = make(lengths, H=2, G=1, P=P, Ns=Ns, seed=3)
+    T, N = sum(lengths), len(lengths)
+    from flashinfer_bench_tma_thrust_b200 import _lib
+    assert (_lib.load().gdn_ssm_prefill_workspace_size(T, N, 2, 1, P, Ns) > 0)
+    check_prompt(ssm.prefill(*dev(a), check=True), a, True)
+
+
+def test_chunked_uncovered_rows_and_neighbours():
+    """Rows in front of, between and behind the sequences hold NaN: they reach nothing, and
+    their outputs are not written."""
+    a = make([400], seed=31)
+    bounds = [5, 140, 140, 300]
+    for i in (0, 3, 4):
+        a[i][:5] = float("nan")
+        a[i][300:] = float("nan")
+    a[1][:5] = float("nan")
+    a[1][300:] = float("nan")
+    a[7] = torch.randn(3, 4, 64, 64, generator=torch.Generator().manual_seed(32))
+    a[8] = torch.tensor(bounds, dtype=torch.int32)
+    d = dev(a)
+    for fn, chunked in ((ssm.prefill, True), (ssm.prefill_recurrent, False)):
+        fill = torch.full((400, 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+        at = fill.data_ptr()
+        del fill
+        got = fn(*d, check=True)
+        check_prompt(got, a, chunked, bounds)
+        if got[0].data_ptr() == at:
+            assert (got[0][:5] == 7).all() and (got[0][300:] == 7).all()
+        assert not torch.isnan(got[0][5:300]).any() and not torch.isnan(got[1]).any()
+
+
+def test_chunked_many_sequences():
+    lengths = [(i * 37) % 140 for i in range(200)]
+    a = make(lengths, H=2, G=1, seed=33)
+    check_prompt(ssm.prefill(*dev(a), check=True), a, True)
+
+
+def test_chunked_matches_recurrent_on_long_prompts():
+    """The two kernels at sizes beyond the oracle: outputs within two bf16 roundings and the
+    chunked form's bf16 operands, states within its 2^-16 terms (relative to the whole)."""
+    a = dev(make([3000, 0, 5000, 129], H=32, G=16, P=128, Ns=128, seed=34))
+    o1, s1 = ssm.prefill(*a, check=True)
+    o2, s2 = ssm.prefill_recurrent(*a)
+    assert ((o1.double() - o2.double()).norm() / o2.double().norm()) < 2 ** -8
+    assert ((s1 - s2).norm() / s2.norm()) < 2 ** -16
+
+
 SIZES = [(1, 16), (8, 16), (40, 32), (64, 64), (80, 128), (128, 128), (100, 256), (256, 256), (3, 64)]
 
 
