@@ -27,8 +27,8 @@
 // each segment adds to the state and what it leaves of it; each block of the second kernel
 // then folds those of the segments before its own into its first state.
 //
-// Warps: 0-15 compute, 16 issues the products, 17 all bulk copies, 18 and 19 the gates (one
-// head each, one chunk ahead). Every wait is bounded; a block that gives up reports it and
+// Warps: 0-15 compute, 16 issues the products, 17 the bulk copies and the gates (up to two
+// chunks ahead). Every wait is bounded; a block that gives up reports it and
 // runs on without waiting, so no barrier is left short of its threads.
 #include "gdn_b200.h"
 #include "gdn_chunk_common.cuh"
@@ -44,10 +44,10 @@ using chunk::named_bar_sync;
 constexpr int kL = 128;             // tokens per chunk
 constexpr int kBlock = 16384;       // a [128 rows x 64 columns] bf16 tile
 constexpr int kComputeWarps = 16;
-constexpr int kThreads = 20 * 32;
+constexpr int kThreads = 18 * 32;
 
 // TMEM columns
-constexpr uint32_t kTG = 0;         // C B^T, then M (64 columns per head)
+constexpr uint32_t kTG = 0;         // C B^T; then M, 8 of every 16 columns per head
 constexpr uint32_t kTY = 128;
 constexpr uint32_t kTD = 256;       // dS
 constexpr uint32_t kTF = 384;       // f x: hi 64 columns, lo 64 columns
@@ -278,7 +278,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     }
     mbar_init(bars + kFullC, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bars + kGatesFull + i, kHeads);
+      mbar_init(bars + kGatesFull + i, 1);
       mbar_init(bars + kGatesFree + i, kComputeWarps);
       mbar_init(bars + kFx + i, kComputeWarps);
       mbar_init(bars + kStaged + i, kComputeWarps);
@@ -453,51 +453,56 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         // ---- M, over C B^T (this warp: tokens 32 q + lane, 32 cg to 32 cg + 31)
         wait(bars + kCB, c & 1);
         tc_fence_after();
-        float g[32];
-        if (cg <= q) {
-          tmem_ld32(lanes + kTG + 32 * cg, g);
-          tmem_ld_wait();
-        }
-        tc_fence_before();
-        named_bar_sync(1 + q, 128);  // every warp of these lanes has read before M overwrites
-        tc_fence_after();
-#pragma unroll
-        for (int hh = 0; hh < kHeads; ++hh) {
-          uint32_t m[16];
-          if (cg > q) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) m[j] = 0u;
-          } else if (cg < q) {
-            // e^{G_i - G_j} d_j = e^{G_i - G_r} (e^{G_r - G_j} d_j), r between j and i: both
-            // exponents are at most 0, and one exponential per row is left
-            float ex = ga[hh].cum[row];
-            for (int b = cg + 1; b < q; ++b) ex += ga[hh].tot[b];
-            const float a = ex2(ex);
-#pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 u = *reinterpret_cast<const float4*>(ga[hh].u + 32 * cg + j);
-              const float2 v0 = mul2(mul2(make_float2(u.x, u.y), make_float2(a, a)),
-                                     make_float2(g[j], g[j + 1]));
-              const float2 v1 = mul2(mul2(make_float2(u.z, u.w), make_float2(a, a)),
-                                     make_float2(g[j + 2], g[j + 3]));
-              m[j / 2] = pack2_rn(v0.x, v0.y);
-              m[j / 2 + 1] = pack2_rn(v1.x, v1.y);
-            }
-          } else {
-            const float ci = ga[hh].cum[row];
-#pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const float4 cj = *reinterpret_cast<const float4*>(ga[hh].cum + 32 * cg + j);
-              const float4 dj = *reinterpret_cast<const float4*>(ga[hh].d + 32 * cg + j);
-              const float v0 = j <= lane ? g[j] * (ex2(ci - cj.x) * dj.x) : 0.f;
-              const float v1 = j + 1 <= lane ? g[j + 1] * (ex2(ci - cj.y) * dj.y) : 0.f;
-              const float v2 = j + 2 <= lane ? g[j + 2] * (ex2(ci - cj.z) * dj.z) : 0.f;
-              const float v3 = j + 3 <= lane ? g[j + 3] * (ex2(ci - cj.w) * dj.w) : 0.f;
-              m[j / 2] = pack2_rn(v0, v1);
-              m[j / 2 + 1] = pack2_rn(v2, v3);
-            }
+        // 16 columns at a time: M of head h for them goes to 8 columns of their own place, so a
+        // warp overwrites nothing that another has yet to read.
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          const int j0 = 32 * cg + 16 * half;
+          const uint32_t at = lanes + kTG + j0;
+          float g[16];
+          if (cg <= q) {
+            tmem_ld16(at, g);
+            tmem_ld_wait();
           }
-          tmem_st16(lanes + kTG + 64 * hh + 16 * cg, m);
+#pragma unroll
+          for (int hh = 0; hh < kHeads; ++hh) {
+            uint32_t m[8];
+            if (cg > q) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) m[j] = 0u;
+            } else if (cg < q) {
+              // e^{G_i - G_j} d_j = e^{G_i - G_r} (e^{G_r - G_j} d_j), r between j and i: both
+              // exponents are at most 0, and one exponential per row is left
+              float ex = ga[hh].cum[row];
+              for (int b = cg + 1; b < q; ++b) ex += ga[hh].tot[b];
+              const float a = ex2(ex);
+#pragma unroll
+              for (int j = 0; j < 16; j += 4) {
+                const float4 u = *reinterpret_cast<const float4*>(ga[hh].u + j0 + j);
+                const float2 v0 = mul2(mul2(make_float2(u.x, u.y), make_float2(a, a)),
+                                       make_float2(g[j], g[j + 1]));
+                const float2 v1 = mul2(mul2(make_float2(u.z, u.w), make_float2(a, a)),
+                                       make_float2(g[j + 2], g[j + 3]));
+                m[j / 2] = pack2_rn(v0.x, v0.y);
+                m[j / 2 + 1] = pack2_rn(v1.x, v1.y);
+              }
+            } else {
+              const float ci = ga[hh].cum[row];
+              const int i = lane - 16 * half;  // columns j <= i are below the diagonal
+#pragma unroll
+              for (int j = 0; j < 16; j += 4) {
+                const float4 cj = *reinterpret_cast<const float4*>(ga[hh].cum + j0 + j);
+                const float4 dj = *reinterpret_cast<const float4*>(ga[hh].d + j0 + j);
+                const float v0 = j <= i ? g[j] * (ex2(ci - cj.x) * dj.x) : 0.f;
+                const float v1 = j + 1 <= i ? g[j + 1] * (ex2(ci - cj.y) * dj.y) : 0.f;
+                const float v2 = j + 2 <= i ? g[j + 2] * (ex2(ci - cj.z) * dj.z) : 0.f;
+                const float v3 = j + 3 <= i ? g[j + 3] * (ex2(ci - cj.w) * dj.w) : 0.f;
+                m[j / 2] = pack2_rn(v0, v1);
+                m[j / 2 + 1] = pack2_rn(v2, v3);
+              }
+            }
+            tmem_st8(at + 8 * hh, m);
+          }
         }
         // ---- Y = e^{G_i} (C S^T), in place
         wait(bars + kYS, c & 1);
@@ -653,7 +658,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         const uint64_t dx = desc_mnmajor(xb + hh * kBlock, kBlock);
 #pragma unroll
         for (int s = 0; s < 8; ++s)
-          mma_bf16_ts_w(tm + kTY + hh * 64, tm + kTG + hh * 64 + 8 * s,
+          mma_bf16_ts_w(tm + kTY + hh * 64, tm + kTG + 16 * s + 8 * hh,
                         dx + static_cast<uint64_t>((s * 2048) >> 4), kIdYM, 1);
       }
       mma_commit_w(bars + kYM);
@@ -667,102 +672,121 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         mbar_wait(bars + kYM, c & 1);
       }
     }
-  } else if (warp == 17) {
-    // ---------------------------------------------------------------- bulk copies
-    if (lane == 0) {
-      const int xc = (h0 * P) / 64, bc = grp * K::kNB;
-      auto load_x = [&](int c) {
-        const int st = c % K::kStages;
-        mbar_arrive_expect_tx(bars + kFullX + st, K::kXBytes);
-        tma_load_3d(sm + K::kX + st * K::kXBytes, &maps.x, bars + kFullX + st, 0, tok0 + c * kL, xc);
-      };
-      auto load_b = [&](int c) {
-        const int st = c % K::kStages;
-        mbar_arrive_expect_tx(bars + kFullB + st, K::kBBytes);
-        tma_load_3d(sm + K::kB + st * K::kBBytes, &maps.b, bars + kFullB + st, 0, tok0 + c * kL, bc);
-      };
-      auto load_c = [&](int c) {
-        mbar_arrive_expect_tx(bars + kFullC, K::kBBytes);
-        tma_load_3d(sm + K::kC, &maps.c, bars + kFullC, 0, tok0 + c * kL, bc);
-      };
-      if (chunks > 0) {
+  } else {
+    // ---------------------------------------------------------------- bulk copies and gates
+    const int xc = (h0 * P) / 64, bc = grp * K::kNB;
+    auto load_x = [&](int c) {
+      const int st = c % K::kStages;
+      mbar_arrive_expect_tx(bars + kFullX + st, K::kXBytes);
+      tma_load_3d(sm + K::kX + st * K::kXBytes, &maps.x, bars + kFullX + st, 0, tok0 + c * kL, xc);
+    };
+    auto load_b = [&](int c) {
+      const int st = c % K::kStages;
+      mbar_arrive_expect_tx(bars + kFullB + st, K::kBBytes);
+      tma_load_3d(sm + K::kB + st * K::kBBytes, &maps.b, bars + kFullB + st, 0, tok0 + c * kL, bc);
+    };
+    auto load_c = [&](int c) {
+      mbar_arrive_expect_tx(bars + kFullC, K::kBBytes);
+      tma_load_3d(sm + K::kC, &maps.c, bars + kFullC, 0, tok0 + c * kL, bc);
+    };
+    float neg_a[kHeads], dtb[kHeads], raw[kHeads][4];
+#pragma unroll
+    for (int hh = 0; hh < kHeads; ++hh) {
+      const int h = h0 + (hh < heads ? hh : 0);
+      neg_a[hh] = -expf(load_scalar(p.A_log, p.A_log_dtype, h));
+      dtb[hh] = load_scalar(p.dt_bias, p.dt_bias_dtype, h);
+    }
+    auto load_dt = [&](int c) {
+#pragma unroll
+      for (int hh = 0; hh < kHeads; ++hh) {
+        const int h = h0 + (hh < heads ? hh : 0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int t = c * kL + lane * 4 + k;
+          raw[hh][k] = t < tokens ? load_scalar(p.dt, p.dt_dtype,
+                                                (static_cast<int64_t>(tok0) + t) * p.H + h)
+                                  : 0.f;
+        }
+      }
+    };
+    auto gates_of = [&](int c) {  // of chunk c, whose dt is in raw; then the next one's dt
+      const int gs = c & 1;
+#pragma unroll
+      for (int hh = 0; hh < kHeads; ++hh)
+        write_gates(gates + gs * kHeads + hh, raw[hh], neg_a[hh], dtb[hh],
+                    hh < heads ? tokens - c * kL : 0, lane);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bars + kGatesFull + gs);
+      if (c + 1 < chunks) load_dt(c + 1);
+    };
+    if (chunks > 0) {
+      if (lane == 0) {
         load_b(0);
         if (!kStates) load_c(0);
         load_x(0);
+        for (int c = 1; c < K::kStages && c < chunks; ++c) {
+          load_b(c);
+          load_x(c);
+        }
       }
-      for (int c = 1; c < K::kStages && c < chunks; ++c) {
-        load_b(c);
-        load_x(c);
-      }
-      for (int c = 0; c < chunks; ++c) {
-        if (kStates) {
-          if (c + K::kStages < chunks) {
-            wait(bars + kDS + c % K::kStages, (c / K::kStages) & 1);  // x was read before it
+      __syncwarp();
+      load_dt(0);
+      gates_of(0);
+      if (chunks > 1) gates_of(1);
+    }
+    for (int c = 0; c < chunks; ++c) {
+      const int st = c % K::kStages, par = (c / K::kStages) & 1;
+      const bool more = c + K::kStages < chunks;
+      if (kStates) {
+        if (more) {
+          wait(bars + kDS + st, par);  // x was read before it
+          if (lane == 0) {
             load_b(c + K::kStages);
             load_x(c + K::kStages);
           }
-          continue;
+          __syncwarp();
         }
+      } else {
         if (c + 1 < chunks) {
           wait(bars + kYS, c & 1);
-          load_c(c + 1);
+          if (lane == 0) load_c(c + 1);
+          __syncwarp();
         }
-        if (c + K::kStages < chunks) {
-          wait(bars + kDS + c % K::kStages, (c / K::kStages) & 1);
-          load_b(c + K::kStages);
+        if (more) {
+          wait(bars + kDS + st, par);
+          if (lane == 0) load_b(c + K::kStages);
+          __syncwarp();
         }
-        if (c < chunks - 1 || tail == kL) {
-          wait(bars + kStaged + c % K::kStages, (c / K::kStages) & 1);
-          const uint8_t* xt = sm + K::kX + (c % K::kStages) * K::kXBytes;
+      }
+      if (c + 2 < chunks) {
+        wait(bars + kGatesFree + (c & 1), (c >> 1) & 1);
+        gates_of(c + 2);
+      }
+      if (!kStates && (c < chunks - 1 || tail == kL)) {
+        wait(bars + kStaged + st, par);
+        if (lane == 0) {
+          const uint8_t* xt = sm + K::kX + st * K::kXBytes;
           for (int b = 0; b < 2; ++b)
             if (kHeads == 1 || b < heads)
               tma_store_3d(&maps.out, xt + b * kBlock, 0, tok0 + c * kL, xc + b);
           bulk_commit();
-          if (c + K::kStages < chunks) {
+          if (more) {
             bulk_wait_read();
             load_x(c + K::kStages);
           }
         }
+        __syncwarp();
       }
-      if (!kStates) bulk_wait_all();
-      if (!wait.ok && chunks > 0) {
-        // copies still in flight land in this block's shared memory: let them
-        const int c = chunks - 1;
-        mbar_wait(bars + kFullX + c % K::kStages, (c / K::kStages) & 1);
-        mbar_wait(bars + kFullB + c % K::kStages, (c / K::kStages) & 1);
-        if (!kStates) mbar_wait(bars + kFullC, c & 1);
-      }
+    }
+    if (!kStates && lane == 0) bulk_wait_all();
+    if (!wait.ok && chunks > 0) {
+      // copies still in flight land in this block's shared memory: let them
+      const int c = chunks - 1;
+      mbar_wait(bars + kFullX + c % K::kStages, (c / K::kStages) & 1);
+      mbar_wait(bars + kFullB + c % K::kStages, (c / K::kStages) & 1);
+      if (!kStates) mbar_wait(bars + kFullC, c & 1);
     }
     __syncwarp();
-  } else if (warp - 18 < kHeads) {
-    // ---------------------------------------------------------------- gates of one head
-    const int hh = warp - 18;
-    const bool present = hh < heads;
-    const int h = h0 + (present ? hh : 0);
-    const float neg_a = -expf(load_scalar(p.A_log, p.A_log_dtype, h));
-    const float dtb = load_scalar(p.dt_bias, p.dt_bias_dtype, h);
-    auto load = [&](int c, float (&raw)[4]) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int t = c * kL + lane * 4 + k;
-        raw[k] = t < tokens
-                     ? load_scalar(p.dt, p.dt_dtype, (static_cast<int64_t>(tok0) + t) * p.H + h)
-                     : 0.f;
-      }
-    };
-    float raw[4];
-    if (chunks > 0) load(0, raw);
-    for (int c = 0; c < chunks; ++c) {
-      const int gs = c & 1;
-      float next[4] = {0.f, 0.f, 0.f, 0.f};
-      if (c + 1 < chunks) load(c + 1, next);
-      if (c >= 2) wait(bars + kGatesFree + gs, ((c >> 1) - 1) & 1);
-      write_gates(gates + gs * kHeads + hh, raw, neg_a, dtb, present ? tokens - c * kL : 0, lane);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bars + kGatesFull + gs);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) raw[k] = next[k];
-    }
   }
   if (!wait.ok) report_wait(p.status);
   tc_fence_before();
