@@ -250,14 +250,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&u)[16
       "r"(u[15])
       : "memory");
 }
-// 16 lanes x 16 columns from 8x8 fragments of 16-bit elements as ldmatrix hands them out
-// (a fragment is 8 lanes x 4 columns, thread t at lane t / 4, column t % 4): u[2 j] goes to
-// lanes 0-7, u[2 j + 1] to lanes 8-15 of columns 4 j to 4 j + 3.
-__device__ __forceinline__ void tmem_st_frag(uint32_t taddr, const uint32_t (&u)[8]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
-      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
-      : "memory");
+// 16 lanes x 8 columns from 8x8 fragments of 16-bit elements as ldmatrix hands them out (a
+// fragment is 8 lanes x 4 columns, thread t at lane t / 4, column t % 4): u[2 j] goes to lanes
+// 0-7, u[2 j + 1] to lanes 8-15 of columns 4 j to 4 j + 3.
+__device__ __forceinline__ void tmem_st_frag(uint32_t taddr, const uint32_t (&u)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr),
+               "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3])
+               : "memory");
 }
 // Four 8x8 matrices of 16-bit elements, transposed: lane l gives the address of row l % 8 of
 // matrix l / 8; thread t receives, of each, rows 2 (t % 4) and 2 (t % 4) + 1 of column t / 4.
@@ -347,6 +346,13 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
       "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
+}
+// The box into L2 only.
+__device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* map, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
 }
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int c0,
                                              int c1, int c2) {

@@ -27,9 +27,10 @@
 // each segment adds to the state and what it leaves of it; each block of the second kernel
 // then folds those of the segments before its own into its first state.
 //
-// Warps: 0-15 compute, 16 issues the products, 17 the bulk copies and the gates (up to two
-// chunks ahead). Every wait is bounded; a block that gives up reports it and
-// runs on without waiting, so no barrier is left short of its threads.
+// Warps: 0-7 the output (M, the scaling of Y, y), 8-15 the state (f x, S), which run at their own
+// pace and so cover each other's waits; 16 issues the products, 17 the bulk copies, 18 and 19
+// the gates (one head each, up to two chunks ahead). Every wait is bounded; a block that gives
+// up reports it and runs on without waiting, so no barrier is left short of its threads.
 #include "gdn_b200.h"
 #include "gdn_chunk_common.cuh"
 #include "ssm_launch.h"
@@ -44,7 +45,56 @@ using chunk::named_bar_sync;
 constexpr int kL = 128;             // tokens per chunk
 constexpr int kBlock = 16384;       // a [128 rows x 64 columns] bf16 tile
 constexpr int kComputeWarps = 16;
-constexpr int kThreads = 18 * 32;
+constexpr int kThreads = 20 * 32;
+
+// Registers per thread of the output kernel: 96 at launch (640 threads), then shared out anew
+// between the output's, the state's and the other warps: 256 x 104 + 256 x 96 + 128 x 80 is
+// what 640 x 96 were. Spills are what this avoids: the shared memory leaves L1 next to nothing,
+// and a few local accesses per chunk cost more than a product.
+constexpr int kLaunchRegs = 96, kOutRegs = 104, kStateRegs = 96, kMiscRegs = 80;
+static_assert(256 * kOutRegs + 256 * kStateRegs + 128 * kMiscRegs <= kThreads * kLaunchRegs, "");
+
+template <int kRegs>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+
+// Shared memory by 32-bit address.
+__device__ __forceinline__ float lds(uint32_t a) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float2 lds2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float4 lds4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint4 lds4u(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts4u(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w)
+               : "memory");
+}
+// Offset of row `row`'s 16-byte chunk 0 in a swizzled tile; chunk k is at this XOR 16 k.
+__device__ __forceinline__ uint32_t row_base(uint32_t row) { return row * 128u + ((row & 7u) << 4); }
 
 // TMEM columns
 constexpr uint32_t kTG = 0;         // C B^T; then M, 8 of every 16 columns per head
@@ -52,7 +102,8 @@ constexpr uint32_t kTY = 128;
 constexpr uint32_t kTD = 256;       // dS
 constexpr uint32_t kTF = 384;       // f x: hi 64 columns, lo 64 columns
 
-struct Gates {                      // of one head and chunk
+// Of one head and chunk; read by offset (the order is kCum to kTot).
+struct Gates {
   float cum[kL];                    // G from the start of the token's block of 32
   float dec[kL];                    // e^G
   float u[kL];                      // d_j e^{G_r - G_j}, r the end of j's block of 32
@@ -60,6 +111,8 @@ struct Gates {                      // of one head and chunk
   float d[kL];
   float tot[4];                     // G over each block of 32
 };
+constexpr uint32_t kCum = 0, kDec = 512, kU = 1024, kF = 1536, kD = 2048, kTot = 2560;
+static_assert(sizeof(Gates) == kTot + 16, "");
 
 struct Maps {
   CUtensorMap x, b, c, out;         // {64, T, columns / 64}, box {64, 128, blocks}
@@ -76,11 +129,15 @@ template <int P, int NS, bool kStates>
 struct Cfg {
   static constexpr int kHeads = 128 / P;
   static constexpr int kNB = NS / 64;
-  static constexpr int kStages = kStates ? 3 : 2;
+  // Stages: x stays until its y has left through the same memory; B and C are read early.
+  static constexpr int kXStages = 3, kBStages = kStates ? 3 : 1;
+  // Warps per TMEM lane quarter on the state: two beside the two on the output, or all four.
+  static constexpr int kParts = kStates ? 4 : 2;
+  static constexpr int kStateWarps = 4 * kParts;
   static constexpr uint32_t kXBytes = 2 * kBlock, kBBytes = kNB * kBlock;
   static constexpr uint32_t kX = 0;
-  static constexpr uint32_t kB = kX + kStages * kXBytes;
-  static constexpr uint32_t kC = kB + kStages * kBBytes;
+  static constexpr uint32_t kB = kX + kXStages * kXBytes;
+  static constexpr uint32_t kC = kB + kBStages * kBBytes;
   static constexpr uint32_t kS = kC + (kStates ? 0 : kBBytes);
   static constexpr uint32_t kGates = kS + (kStates ? 0 : kBBytes);
   static constexpr uint32_t kBars = kGates + 2 * kHeads * sizeof(Gates);
@@ -88,21 +145,21 @@ struct Cfg {
 };
 
 enum Bar {
-  kFullX = 0,       // [3], [2] and so on: one per stage
+  kFullX = 0,       // [3] one per stage
   kFullB = 3,       // [3]
   kFullC = 6,
   kGatesFull = 7,   // [2]
   kGatesFree = 9,   // [2]
   kCB = 11,         // products done: C B^T
   kYS = 12,         //   C S^T
-  kDS = 13,         //   dS [3]
+  kDS = 13,         //   dS [3, by stage of B]
   kYM = 16,         //   M x
   kFx = 17,         // operands written: f x [2] (the output kernel: one)
   kMy = 19,         //   M and the scaled Y
   kState = 20,      //   S
   kYFree = 21,      // Y read out
-  kStaged = 22,     // y in shared memory [2]
-  kZeroed = 24,
+  kStaged = 22,     // y in shared memory [3]
+  kZeroed = 25,
 };
 
 // Waits that stop waiting after the first that gave up.
@@ -226,7 +283,6 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
                  const __grid_constant__ Segments sg, int col_blocks) {
   using K = Cfg<P, NS, kStates>;
   constexpr int kHeads = K::kHeads;
-  constexpr int kNC = NS / 4;      // state columns per thread
   extern __shared__ uint8_t raw_smem[];
   uint8_t* const sm = align_smem<1024>(raw_smem);
   __shared__ int64_t s_where[2];
@@ -270,102 +326,264 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
 
   uint64_t* const bars = reinterpret_cast<uint64_t*>(sm + K::kBars);
   Gates* const gates = reinterpret_cast<Gates*>(sm + K::kGates);
+  constexpr int kOutWarps = kStates ? 0 : 8;  // warps 0-7; the state's warps follow
   if (threadIdx.x == 0) {
     for (int i = 0; i < 3; ++i) {
       mbar_init(bars + kFullX + i, 1);
       mbar_init(bars + kFullB + i, 1);
       mbar_init(bars + kDS + i, 1);
+      mbar_init(bars + kStaged + i, 8);
     }
     mbar_init(bars + kFullC, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bars + kGatesFull + i, 1);
+      mbar_init(bars + kGatesFull + i, kHeads);
       mbar_init(bars + kGatesFree + i, kComputeWarps);
-      mbar_init(bars + kFx + i, kComputeWarps);
-      mbar_init(bars + kStaged + i, kComputeWarps);
+      mbar_init(bars + kFx + i, K::kStateWarps);
     }
-    mbar_init(bars + kCB, 1);
-    mbar_init(bars + kYS, 1);
-    mbar_init(bars + kYM, 1);
-    for (int i : {kMy, kState, kYFree, kZeroed}) mbar_init(bars + i, kComputeWarps);
+    for (int i : {kCB, kYS, kYM}) mbar_init(bars + i, 1);
+    for (int i : {kMy, kYFree}) mbar_init(bars + i, 8);
+    for (int i : {kState, kZeroed}) mbar_init(bars + i, K::kStateWarps);
     fence_mbar_init();
   }
   if (warp == 16) tmem_alloc(&s_tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tm = s_tmem;
+  const uint32_t tm = s_tmem, sm_u = smem_u32(sm), gates_u = sm_u + K::kGates;
   Waiter wait;
+  const int q = warp & 3;                      // TMEM lane quarter
+  const uint32_t lanes = tm + (static_cast<uint32_t>(32 * q) << 16);
+  const int row = 32 * q + lane;               // token of a chunk / column of the block
+  auto arrive = [&](int bar) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bars + bar);
+  };
 
-  if (warp < kComputeWarps) {
-    const int q = warp & 3, cg = warp >> 2;
-    const uint32_t lanes = tm + (static_cast<uint32_t>(32 * q) << 16);
-    const int row = 32 * q + lane;               // token of a chunk / column of the block
+  if (warp < kOutWarps) {
+    if (!kStates) regs_inc<kOutRegs>();
+    // ---------------------------------------------------------------- output: token per thread
+    const int half = warp >> 2;
+    const int col_head = kHeads == 2 ? half : 0;  // head of columns 64 half to 64 half + 63
+    const float skip = p.D && col_head < heads ? load_scalar(p.D, p.D_dtype, h0 + col_head) : 0.f;
+    for (int c = 0; c < chunks; ++c) {
+      const int gs = c & 1;
+      const uint32_t ga = gates_u + gs * kHeads * static_cast<uint32_t>(sizeof(Gates));
+      wait(bars + kGatesFull + gs, (c >> 1) & 1);
+      wait(bars + kCB, c & 1);
+      tc_fence_after();
+      // ---- M over C B^T, 16 columns at a time: those of head h go to 8 columns of the same
+      // 16, so a warp overwrites nothing that another has yet to read. The two warps of a
+      // quarter take every other 16 (each has one piece on the diagonal).
+#pragma unroll 1
+      for (int k0 = 0; k0 < 4; k0 += 2) {
+        float g0[16], g1[16];
+        const uint32_t at = lanes + kTG + 32 * k0 + 16 * half;
+        if (k0 <= q) {
+          tmem_ld16(at, g0);
+          tmem_ld16(at + 32, g1);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int hh = 0; hh < kHeads; ++hh) {
+          const uint32_t gh = ga + hh * static_cast<uint32_t>(sizeof(Gates));
+          const float own = lds(gh + kCum + 4 * row);
+          auto piece = [&](int k, const float(&g)[16], uint32_t dst) {
+            const int j0 = 32 * k + 16 * half;
+            uint32_t m[8];
+            if (k < q) {
+              // e^{G_i - G_j} d_j = e^{G_i - G_r} (e^{G_r - G_j} d_j), r the end of j's block,
+              // between j and i: both exponents are at most 0, and one exponential per row
+              // is left
+              float ex = own;
+              for (int b = k + 1; b < q; ++b) ex += lds(gh + kTot + 4 * b);
+              const float e = ex2(ex);
+              const float2 a = make_float2(e, e);
+#pragma unroll
+              for (int j = 0; j < 16; j += 4) {
+                const float4 u = lds4(gh + kU + 4 * (j0 + j));
+                const float2 v0 =
+                    mul2(mul2(make_float2(u.x, u.y), a), make_float2(g[j], g[j + 1]));
+                const float2 v1 =
+                    mul2(mul2(make_float2(u.z, u.w), a), make_float2(g[j + 2], g[j + 3]));
+                m[j / 2] = pack2_rn(v0.x, v0.y);
+                m[j / 2 + 1] = pack2_rn(v1.x, v1.y);
+              }
+            } else if (k == q) {
+              const int i = row - j0;  // columns j <= i are on or below the diagonal
+#pragma unroll
+              for (int j = 0; j < 16; j += 4) {
+                const float4 cj = lds4(gh + kCum + 4 * (j0 + j));
+                const float4 dj = lds4(gh + kD + 4 * (j0 + j));
+                const float v0 = j <= i ? g[j] * (ex2(own - cj.x) * dj.x) : 0.f;
+                const float v1 = j + 1 <= i ? g[j + 1] * (ex2(own - cj.y) * dj.y) : 0.f;
+                const float v2 = j + 2 <= i ? g[j + 2] * (ex2(own - cj.z) * dj.z) : 0.f;
+                const float v3 = j + 3 <= i ? g[j + 3] * (ex2(own - cj.w) * dj.w) : 0.f;
+                m[j / 2] = pack2_rn(v0, v1);
+                m[j / 2 + 1] = pack2_rn(v2, v3);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) m[j] = 0u;
+            }
+            tmem_st8(dst + 8 * hh, m);
+          };
+          piece(k0, g0, at);
+          piece(k0 + 1, g1, at + 32);
+        }
+      }
+      // ---- Y = e^{G_i} (C S^T), in place
+      wait(bars + kYS, c & 1);
+      tc_fence_after();
+      {
+        const float e = lds(ga + col_head * static_cast<uint32_t>(sizeof(Gates)) + kDec + 4 * row);
+        const float2 e2 = make_float2(e, e);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t ty = lanes + kTY + 64 * half + 32 * k;
+          float y[32];
+          tmem_ld32(ty, y);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float2 v = mul2(make_float2(y[i], y[i + 1]), e2);
+            y[i] = v.x;
+            y[i + 1] = v.y;
+          }
+          tmem_st32(ty, y);
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      arrive(kMy);
+      arrive(kGatesFree + gs);
+      // ---- y: out of TMEM, D x added, over the chunk's x in shared memory
+      const int st = c % K::kXStages;
+      const uint32_t xrow = sm_u + K::kX + st * K::kXBytes + half * kBlock + row_base(row);
+      wait(bars + kYM, c & 1);
+      tc_fence_after();
+      {
+#pragma unroll
+        for (int k0 = 0; k0 < 8; k0 += 4) {
+          float y[32];
+          tmem_ld32(lanes + kTY + 64 * half + 8 * k0, y);
+          tmem_ld_wait();
+          if (k0 == 4) {
+            tc_fence_before();
+            arrive(kYFree);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t at = xrow ^ (16 * (k0 + k));
+            uint32_t w[4];
+            if (p.D) {
+              const uint4 xv = lds4u(at);
+              const uint32_t u[4] = {xv.x, xv.y, xv.z, xv.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 v = fma2(make_float2(skip, skip),
+                                      make_float2(__uint_as_float(u[e] << 16),
+                                                  __uint_as_float(u[e] & 0xffff0000u)),
+                                      make_float2(y[8 * k + 2 * e], y[8 * k + 2 * e + 1]));
+                w[e] = pack2_rn(v.x, v.y);
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w[e] = pack2_rn(y[8 * k + 2 * e], y[8 * k + 2 * e + 1]);
+            }
+            sts4u(at, w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      if (c < chunks - 1 || tail == kL) {
+        fence_async_smem();
+        arrive(kStaged + st);  // a bulk store takes the whole tile
+      } else {
+        // only the sequence's rows: 16 lanes write the 256 bytes of one
+        named_bar_sync(1, 256);
+        uint8_t* const xt = sm + K::kX + st * K::kXBytes;
+        const int l = lane & 15, blk = l >> 3;
+        const int64_t base = (static_cast<int64_t>(tok0) + c * kL) * p.H + h0;
+        if (kHeads == 1 || blk < heads) {
+          for (int r = warp * 2 + (lane >> 4); r < tail; r += 16) {
+            const uint4 v =
+                *reinterpret_cast<const uint4*>(xt + blk * kBlock + sw128_chunk(r, l & 7));
+            *reinterpret_cast<uint4*>(p.out + (base + static_cast<int64_t>(r) * p.H) * P + l * 8) =
+                v;
+          }
+        }
+      }
+    }
+  } else if (warp < kComputeWarps) {
+    if (!kStates) regs_inc<kStateRegs>();
+    // ---------------------------------------------------------------- state: column per thread
+    constexpr int kTok = kL / K::kParts;         // tokens of f x per warp
+    constexpr int kNC = NS / K::kParts;          // state columns per thread
+    const int part = (warp - kOutWarps) >> 2;
     const int row_head = kHeads == 2 ? q >> 1 : 0;   // head of column `row`
-    const int col_head = kHeads == 2 ? cg >> 1 : 0;  // head of columns 32 cg to 32 cg + 31
     const int64_t st_off =
-        ((n * p.H + h0) * static_cast<int64_t>(P) + row) * NS + kNC * cg;
+        ((n * p.H + h0) * static_cast<int64_t>(P) + row) * NS + kNC * part;
     const bool mine = row_head < heads;
     float S[kNC];
 #pragma unroll
     for (int i = 0; i < kNC; ++i) S[i] = 0.f;
     float left = 1.f;
 
-    if (!kStates) {
-      if (p.state && mine) {
+    if (!kStates && mine) {
+      if (p.state) {
         const float* src = static_cast<const float*>(p.state) + st_off;
 #pragma unroll
-        for (int i = 0; i < kNC; i += 4)
-          *reinterpret_cast<float4*>(S + i) = *reinterpret_cast<const float4*>(src + i);
+        for (int i = 0; i < kNC; i += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(src + i);
+          S[i] = v.x;
+          S[i + 1] = v.y;
+          S[i + 2] = v.z;
+          S[i + 3] = v.w;
+        }
       }
-      if (mine) {  // the segments of this sequence before this one
-        for (int64_t r = slot - seg; r < slot; ++r) {
-          const float g = sg.left[r * p.H + h0 + row_head];
-          const float* src =
-              sg.add + ((r * p.H + h0) * static_cast<int64_t>(P) + row) * NS + kNC * cg;
+      for (int64_t r = slot - seg; r < slot; ++r) {  // this sequence's segments before this one
+        const float g = sg.left[r * p.H + h0 + row_head];
+        const float* src =
+            sg.add + ((r * p.H + h0) * static_cast<int64_t>(P) + row) * NS + kNC * part;
 #pragma unroll
-          for (int i = 0; i < kNC; i += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(src + i);
-            S[i] = fmaf(g, S[i], v.x);
-            S[i + 1] = fmaf(g, S[i + 1], v.y);
-            S[i + 2] = fmaf(g, S[i + 2], v.z);
-            S[i + 3] = fmaf(g, S[i + 3], v.w);
-          }
+        for (int i = 0; i < kNC; i += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(src + i);
+          S[i] = fmaf(g, S[i], v.x);
+          S[i + 1] = fmaf(g, S[i + 1], v.y);
+          S[i + 2] = fmaf(g, S[i + 2], v.z);
+          S[i + 3] = fmaf(g, S[i + 3], v.w);
         }
       }
     }
 
     // The state as the operand of the next chunk's C S^T: row = column of the block, n
     // contiguous (K-major).
+    const uint32_t s_row = sm_u + K::kS + (kNC * part >> 6) * kBlock + row_base(row);
     auto write_state = [&]() {
 #pragma unroll
-      for (int k = 0; k < kNC / 8; ++k) {
-        const int nn = kNC * cg + 8 * k;
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = pack2_rn(S[8 * k + 2 * e], S[8 * k + 2 * e + 1]);
-        *reinterpret_cast<uint4*>(sm + K::kS + (nn >> 6) * kBlock +
-                                  sw128_chunk(row, (nn >> 3) & 7)) =
-            make_uint4(w[0], w[1], w[2], w[3]);
-      }
+      for (int k = 0; k < kNC / 8; ++k)
+        sts4u(s_row ^ (16 * (((kNC * part >> 3) + k) & 7)), pack2_rn(S[8 * k], S[8 * k + 1]),
+              pack2_rn(S[8 * k + 2], S[8 * k + 3]), pack2_rn(S[8 * k + 4], S[8 * k + 5]),
+              pack2_rn(S[8 * k + 6], S[8 * k + 7]));
       fence_async_smem();
-    };
-    auto arrive = [&](int bar) {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bars + bar);
+      arrive(kState);
     };
 
-    // (f x)^T of chunk c into TMEM, tokens 32 cg to 32 cg + 31 of columns 32 q to 32 q + 31:
-    // transposed by ldmatrix, scaled, split and stored as the fragments come.
+    // (f x)^T of chunk c into TMEM: this warp's tokens of columns 32 q to 32 q + 31, transposed
+    // by ldmatrix, scaled, split and stored as the fragments come, 16 tokens at a time.
+    // lane l gives ldmatrix token t0 + 8 (l / 16) + l % 8, columns 8 ((l / 8) % 2) to + 7 (and
+    // 16 on) of the quarter's 32
+    const uint32_t x_lane =
+        row_base(8 * (lane >> 4) + (lane & 7)) ^ (16 * ((q & 1) * 4 + ((lane >> 3) & 1)));
     auto write_fx = [&](int c) {
-      const int st = c % K::kStages, par = (c / K::kStages) & 1, gs = c & 1;
+      const int st = c % K::kXStages, gs = c & 1;
       uint8_t* const xt = sm + K::kX + st * K::kXBytes;
-      wait(bars + kFullX + st, par);
+      wait(bars + kFullX + st, (c / K::kXStages) & 1);
       if (c == chunks - 1 && tail < kL) {
         // Rows behind the sequence hold other tokens or nothing: zeros, so that neither they
         // nor a NaN among them enters a product.
-        uint8_t* const bt = sm + K::kB + st * K::kBBytes;
-        wait(bars + kFullB + st, par);
-        for (int i = threadIdx.x; i < (kL - tail) * 8; i += kComputeWarps * 32) {
+        uint8_t* const bt = sm + K::kB + (c % K::kBStages) * K::kBBytes;
+        wait(bars + kFullB + c % K::kBStages, (c / K::kBStages) & 1);
+        for (int i = threadIdx.x - kOutWarps * 32; i < (kL - tail) * 8; i += K::kStateWarps * 32) {
           const uint32_t off = (tail + (i >> 3)) * 128 + (i & 7) * 16;
           const uint4 z = make_uint4(0u, 0u, 0u, 0u);
           *reinterpret_cast<uint4*>(xt + off) = z;
@@ -374,36 +592,32 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
           for (int b = 0; b < K::kNB; ++b) *reinterpret_cast<uint4*>(bt + b * kBlock + off) = z;
         }
         fence_async_smem();
-        named_bar_sync(5, kComputeWarps * 32);
+        named_bar_sync(2, K::kStateWarps * 32);
         arrive(kZeroed);
       }
       wait(bars + kGatesFull + gs, (c >> 1) & 1);
-      const float* f = gates[gs * kHeads + row_head].f + 32 * cg + 2 * (lane & 3);
-      float2 fv[4];
+      const uint32_t f = gates_u + (gs * kHeads + row_head) * static_cast<uint32_t>(sizeof(Gates)) +
+                         kF + 8 * (lane & 3);
+      const uint32_t xb = sm_u + K::kX + st * K::kXBytes + (q >> 1) * kBlock + x_lane;
+      const uint32_t t_hi = lanes + (kStates && (c & 1) ? kTG : kTF);
+#pragma unroll 1
+      for (int t0 = part * kTok; t0 < (part + 1) * kTok; t0 += 16) {
+        const float2 f0 = lds2(f + 4 * t0), f1 = lds2(f + 4 * t0 + 32);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) fv[j] = *reinterpret_cast<const float2*>(f + 8 * j);
-      const uint32_t xb = smem_u32(xt + (q >> 1) * kBlock);
-      const uint32_t t_hi = lanes + (kStates && (c & 1) ? kTG : kTF) + 16 * cg;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t hi[8], lo[8];
-#pragma unroll
-        for (int jj = 0; jj < 2; ++jj) {
-          uint32_t u[4];  // tokens 8 (2 jj): columns 0-7, 8-15; tokens 8 (2 jj + 1): the same
-          const int tok = 32 * cg + 8 * (2 * jj + (lane >> 4)) + (lane & 7);
-          const int ch = (q & 1) * 4 + half * 2 + ((lane >> 3) & 1);
-          ldmatrix_x4_trans(xb + sw128_chunk(tok, ch), u);
+        for (int h = 0; h < 2; ++h) {
+          uint32_t u[4], hi[4], lo[4];  // tokens t0 to + 7: columns 0-7, 8-15; t0 + 8: the same
+          ldmatrix_x4_trans((xb + 128 * t0) ^ (32 * h), u);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float2 s = fv[2 * jj + (k >> 1)];
             const float2 v = mul2(make_float2(__uint_as_float(u[k] << 16),
                                               __uint_as_float(u[k] & 0xffff0000u)),
-                                  s);
-            split2(v.x, v.y, hi[4 * jj + k], lo[4 * jj + k]);
+                                  k < 2 ? f0 : f1);
+            split2(v.x, v.y, hi[k], lo[k]);
           }
+          const uint32_t at = t_hi + t0 / 2 + (static_cast<uint32_t>(16 * h) << 16);
+          tmem_st_frag(at, hi);
+          tmem_st_frag(at + 64, lo);
         }
-        tmem_st_frag(t_hi + (static_cast<uint32_t>(16 * half) << 16), hi);
-        tmem_st_frag(t_hi + 64 + (static_cast<uint32_t>(16 * half) << 16), lo);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -412,191 +626,63 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
 
     // The state behind chunk c, from what the chunk adds.
     auto update_state = [&](int c) {
-      const int gs = c & 1;
-      wait(bars + kDS + c % K::kStages, (c / K::kStages) & 1);
+      wait(bars + kDS + c % K::kBStages, (c / K::kBStages) & 1);
       tc_fence_after();
-      const float g = gates[gs * kHeads + row_head].dec[kL - 1];
-      const uint32_t td = lanes + (kStates && (c & 1) ? kTY : kTD) + kNC * cg;
-      if constexpr (kNC == 32) {
-        float v[32];
-        tmem_ld32(td, v);
-        tmem_ld_wait();
+      const float g =
+          lds(gates_u + ((c & 1) * kHeads + row_head) * static_cast<uint32_t>(sizeof(Gates)) + kDec +
+              4 * (kL - 1));
+      const float2 g2 = make_float2(g, g);
+      const uint32_t td = lanes + (kStates && (c & 1) ? kTY : kTD) + kNC * part;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) S[i] = fmaf(g, S[i], v[i]);
-      } else {
+      for (int i0 = 0; i0 < kNC; i0 += 16) {
         float v[16];
-        tmem_ld16(td, v);
+        tmem_ld16(td + i0, v);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) S[i] = fmaf(g, S[i], v[i]);
+        for (int i = 0; i < 16; i += 2) {
+          const float2 s = fma2(g2, make_float2(S[i0 + i], S[i0 + i + 1]),
+                                make_float2(v[i], v[i + 1]));
+          S[i0 + i] = s.x;
+          S[i0 + i + 1] = s.y;
+        }
       }
       if (kStates) left *= g;
       tc_fence_before();
+      arrive(kGatesFree + (c & 1));
     };
 
-    if (kStates) {
-      if (chunks > 0) write_fx(0);
-      for (int c = 0; c < chunks; ++c) {
-        // fx and dS alternate between two places, so the next operand is written while the
-        // product of this one runs
-        if (c + 1 < chunks) write_fx(c + 1);
-        update_state(c);
-        arrive(kGatesFree + (c & 1));
-      }
-    } else if (chunks > 0) {
-      write_state();
-      arrive(kState);
+    if (chunks > 0) {
+      if (!kStates) write_state();
       write_fx(0);
-      for (int c = 0; c < chunks; ++c) {
-        const int gs = c & 1;
-        const Gates* const ga = gates + gs * kHeads;
-        // ---- M, over C B^T (this warp: tokens 32 q + lane, 32 cg to 32 cg + 31)
-        wait(bars + kCB, c & 1);
-        tc_fence_after();
-        // 16 columns at a time: M of head h for them goes to 8 columns of their own place, so a
-        // warp overwrites nothing that another has yet to read.
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-          const int j0 = 32 * cg + 16 * half;
-          const uint32_t at = lanes + kTG + j0;
-          float g[16];
-          if (cg <= q) {
-            tmem_ld16(at, g);
-            tmem_ld_wait();
-          }
-#pragma unroll
-          for (int hh = 0; hh < kHeads; ++hh) {
-            uint32_t m[8];
-            if (cg > q) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) m[j] = 0u;
-            } else if (cg < q) {
-              // e^{G_i - G_j} d_j = e^{G_i - G_r} (e^{G_r - G_j} d_j), r between j and i: both
-              // exponents are at most 0, and one exponential per row is left
-              float ex = ga[hh].cum[row];
-              for (int b = cg + 1; b < q; ++b) ex += ga[hh].tot[b];
-              const float a = ex2(ex);
-#pragma unroll
-              for (int j = 0; j < 16; j += 4) {
-                const float4 u = *reinterpret_cast<const float4*>(ga[hh].u + j0 + j);
-                const float2 v0 = mul2(mul2(make_float2(u.x, u.y), make_float2(a, a)),
-                                       make_float2(g[j], g[j + 1]));
-                const float2 v1 = mul2(mul2(make_float2(u.z, u.w), make_float2(a, a)),
-                                       make_float2(g[j + 2], g[j + 3]));
-                m[j / 2] = pack2_rn(v0.x, v0.y);
-                m[j / 2 + 1] = pack2_rn(v1.x, v1.y);
-              }
-            } else {
-              const float ci = ga[hh].cum[row];
-              const int i = lane - 16 * half;  // columns j <= i are below the diagonal
-#pragma unroll
-              for (int j = 0; j < 16; j += 4) {
-                const float4 cj = *reinterpret_cast<const float4*>(ga[hh].cum + j0 + j);
-                const float4 dj = *reinterpret_cast<const float4*>(ga[hh].d + j0 + j);
-                const float v0 = j <= i ? g[j] * (ex2(ci - cj.x) * dj.x) : 0.f;
-                const float v1 = j + 1 <= i ? g[j + 1] * (ex2(ci - cj.y) * dj.y) : 0.f;
-                const float v2 = j + 2 <= i ? g[j + 2] * (ex2(ci - cj.z) * dj.z) : 0.f;
-                const float v3 = j + 3 <= i ? g[j + 3] * (ex2(ci - cj.w) * dj.w) : 0.f;
-                m[j / 2] = pack2_rn(v0, v1);
-                m[j / 2 + 1] = pack2_rn(v2, v3);
-              }
-            }
-            tmem_st8(at + 8 * hh, m);
-          }
-        }
-        // ---- Y = e^{G_i} (C S^T), in place
-        wait(bars + kYS, c & 1);
-        tc_fence_after();
-        {
-          float y[32];
-          const uint32_t ty = lanes + kTY + 32 * cg;
-          tmem_ld32(ty, y);
-          const float e = ga[col_head].dec[row];
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) y[i] *= e;
-          tmem_st32(ty, y);
-        }
-        tmem_st_wait();
-        tc_fence_before();
-        arrive(kMy);
-        // ---- state
-        update_state(c);
-        arrive(kGatesFree + gs);
-        if (c + 1 < chunks) {
-          write_state();
-          arrive(kState);
-          write_fx(c + 1);
-        }
-        // ---- y: out of TMEM, D x added, over the chunk's x in shared memory
-        const int st = c % K::kStages;
-        uint8_t* const xrow = sm + K::kX + st * K::kXBytes + (cg >> 1) * kBlock;
-        wait(bars + kYM, c & 1);
-        tc_fence_after();
-        {
-          float y[32];
-          tmem_ld32(lanes + kTY + 32 * cg, y);
-          tmem_ld_wait();
-          tc_fence_before();
-          arrive(kYFree);
-          const float skip =
-              p.D && col_head < heads ? load_scalar(p.D, p.D_dtype, h0 + col_head) : 0.f;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint4* const at =
-                reinterpret_cast<uint4*>(xrow + sw128_chunk(row, (cg & 1) * 4 + k));
-            if (p.D) {
-              const uint4 xv = *at;
-              const uint32_t u[4] = {xv.x, xv.y, xv.z, xv.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                y[8 * k + 2 * e] = fmaf(skip, __uint_as_float(u[e] << 16), y[8 * k + 2 * e]);
-                y[8 * k + 2 * e + 1] =
-                    fmaf(skip, __uint_as_float(u[e] & 0xffff0000u), y[8 * k + 2 * e + 1]);
-              }
-            }
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = pack2_rn(y[8 * k + 2 * e], y[8 * k + 2 * e + 1]);
-            *at = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-        if (c < chunks - 1 || tail == kL) {
-          fence_async_smem();
-          arrive(kStaged + st);  // a bulk store takes the whole tile
-        } else {
-          // only the sequence's rows: 16 lanes write the 256 bytes of one
-          named_bar_sync(5, kComputeWarps * 32);
-          uint8_t* const xt = sm + K::kX + st * K::kXBytes;
-          const int l = lane & 15, blk = l >> 3;
-          const int64_t base = (static_cast<int64_t>(tok0) + c * kL) * p.H + h0;
-          if (kHeads == 1 || blk < heads) {
-            for (int r = warp * 2 + (lane >> 4); r < tail; r += kComputeWarps * 2) {
-              const uint4 v =
-                  *reinterpret_cast<const uint4*>(xt + blk * kBlock + sw128_chunk(r, l & 7));
-              *reinterpret_cast<uint4*>(p.out + (base + static_cast<int64_t>(r) * p.H) * P +
-                                        l * 8) = v;
-            }
-          }
-        }
+    }
+    for (int c = 0; c < chunks; ++c) {
+      // states kernel: f x and dS alternate between two places, so the next operand is
+      // written while the product of this one runs
+      if (kStates && c + 1 < chunks) write_fx(c + 1);
+      update_state(c);
+      if (!kStates && c + 1 < chunks) {
+        write_fx(c + 1);
+        wait(bars + kYS, c & 1);  // the product has read the state it replaces
+        write_state();
       }
     }
     if (mine) {
+      float* dst = nullptr;
       if (kStates) {
-        float* dst =
-            sg.add + ((slot * p.H + h0) * static_cast<int64_t>(P) + row) * NS + kNC * cg;
-#pragma unroll
-        for (int i = 0; i < kNC; i += 4)
-          *reinterpret_cast<float4*>(dst + i) = make_float4(S[i], S[i + 1], S[i + 2], S[i + 3]);
-        if (cg == 0 && row % P == 0) sg.left[slot * p.H + h0 + row_head] = left;
+        dst = sg.add + ((slot * p.H + h0) * static_cast<int64_t>(P) + row) * NS + kNC * part;
+        if (part == 0 && row % P == 0) sg.left[slot * p.H + h0 + row_head] = left;
       } else if (last) {
-        float* dst = static_cast<float*>(p.new_state) + st_off;
+        dst = static_cast<float*>(p.new_state) + st_off;
+      }
+      if (dst) {
 #pragma unroll
         for (int i = 0; i < kNC; i += 4)
           *reinterpret_cast<float4*>(dst + i) = make_float4(S[i], S[i + 1], S[i + 2], S[i + 3]);
       }
     }
-  } else if (warp == 16) {
+  } else {
+    if (!kStates) regs_dec<kMiscRegs>();
+    if (warp == 16) {
     // ---------------------------------------------------------------- products
     constexpr uint32_t kIdCB = idesc_bf16(128, 128, false, false);
     constexpr uint32_t kIdDS = idesc_bf16(128, NS, false, true);
@@ -605,8 +691,8 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     const uint64_t d_s = desc_kmajor(smem_u32(sm + K::kS));
     auto kstep = [](int s) { return static_cast<uint64_t>(((s >> 2) * kBlock + (s & 3) * 32) >> 4); };
     for (int c = 0; c < chunks; ++c) {
-      const int st = c % K::kStages, par = (c / K::kStages) & 1;
-      const uint32_t xb = smem_u32(sm + K::kX + st * K::kXBytes);
+      const int st = c % K::kBStages, par = (c / K::kBStages) & 1;
+      const uint32_t xb = smem_u32(sm + K::kX + (c % K::kXStages) * K::kXBytes);
       const uint32_t bb = smem_u32(sm + K::kB + st * K::kBBytes);
       const bool zeroed = c == chunks - 1 && tail < kL;
       auto issue_ds = [&](uint32_t td, uint32_t tf) {
@@ -667,126 +753,104 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     if (chunks > 0) {
       const int c = chunks - 1;
       if (kStates) {
-        mbar_wait(bars + kDS + c % K::kStages, (c / K::kStages) & 1);
+        mbar_wait(bars + kDS + c % K::kBStages, (c / K::kBStages) & 1);
       } else {
         mbar_wait(bars + kYM, c & 1);
       }
     }
-  } else {
-    // ---------------------------------------------------------------- bulk copies and gates
-    const int xc = (h0 * P) / 64, bc = grp * K::kNB;
-    auto load_x = [&](int c) {
-      const int st = c % K::kStages;
-      mbar_arrive_expect_tx(bars + kFullX + st, K::kXBytes);
-      tma_load_3d(sm + K::kX + st * K::kXBytes, &maps.x, bars + kFullX + st, 0, tok0 + c * kL, xc);
-    };
-    auto load_b = [&](int c) {
-      const int st = c % K::kStages;
-      mbar_arrive_expect_tx(bars + kFullB + st, K::kBBytes);
-      tma_load_3d(sm + K::kB + st * K::kBBytes, &maps.b, bars + kFullB + st, 0, tok0 + c * kL, bc);
-    };
-    auto load_c = [&](int c) {
-      mbar_arrive_expect_tx(bars + kFullC, K::kBBytes);
-      tma_load_3d(sm + K::kC, &maps.c, bars + kFullC, 0, tok0 + c * kL, bc);
-    };
-    float neg_a[kHeads], dtb[kHeads], raw[kHeads][4];
-#pragma unroll
-    for (int hh = 0; hh < kHeads; ++hh) {
-      const int h = h0 + (hh < heads ? hh : 0);
-      neg_a[hh] = -expf(load_scalar(p.A_log, p.A_log_dtype, h));
-      dtb[hh] = load_scalar(p.dt_bias, p.dt_bias_dtype, h);
-    }
-    auto load_dt = [&](int c) {
-#pragma unroll
-      for (int hh = 0; hh < kHeads; ++hh) {
-        const int h = h0 + (hh < heads ? hh : 0);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int t = c * kL + lane * 4 + k;
-          raw[hh][k] = t < tokens ? load_scalar(p.dt, p.dt_dtype,
-                                                (static_cast<int64_t>(tok0) + t) * p.H + h)
-                                  : 0.f;
-        }
+  } else if (warp == 17) {
+    // ---------------------------------------------------------------- bulk copies
+    if (lane == 0) {
+      const int xc = (h0 * P) / 64, bc = grp * K::kNB;
+      auto load_x = [&](int c) {
+        const int st = c % K::kXStages;
+        mbar_arrive_expect_tx(bars + kFullX + st, K::kXBytes);
+        tma_load_3d(sm + K::kX + st * K::kXBytes, &maps.x, bars + kFullX + st, 0, tok0 + c * kL, xc);
+      };
+      auto load_b = [&](int c) {
+        const int st = c % K::kBStages;
+        mbar_arrive_expect_tx(bars + kFullB + st, K::kBBytes);
+        tma_load_3d(sm + K::kB + st * K::kBBytes, &maps.b, bars + kFullB + st, 0, tok0 + c * kL, bc);
+      };
+      auto load_c = [&](int c) {
+        mbar_arrive_expect_tx(bars + kFullC, K::kBBytes);
+        tma_load_3d(sm + K::kC, &maps.c, bars + kFullC, 0, tok0 + c * kL, bc);
+      };
+      for (int c = 0; c < K::kXStages && c < chunks; ++c) {
+        if (c < K::kBStages) load_b(c);
+        if (!kStates && c == 0) load_c(c);
+        load_x(c);
       }
-    };
-    auto gates_of = [&](int c) {  // of chunk c, whose dt is in raw; then the next one's dt
-      const int gs = c & 1;
-#pragma unroll
-      for (int hh = 0; hh < kHeads; ++hh)
-        write_gates(gates + gs * kHeads + hh, raw[hh], neg_a[hh], dtb[hh],
-                    hh < heads ? tokens - c * kL : 0, lane);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bars + kGatesFull + gs);
-      if (c + 1 < chunks) load_dt(c + 1);
-    };
-    if (chunks > 0) {
-      if (lane == 0) {
-        load_b(0);
-        if (!kStates) load_c(0);
-        load_x(0);
-        for (int c = 1; c < K::kStages && c < chunks; ++c) {
-          load_b(c);
-          load_x(c);
+      for (int c = 0; c < chunks; ++c) {
+        if (!kStates && c + 2 < chunks) {
+          // B and C have one stage: bring the next but one chunk's into L2, so that the copy
+          // that has to wait for the stage takes only L2's latency
+          tma_prefetch_3d(&maps.b, 0, tok0 + (c + 2) * kL, bc);
+          tma_prefetch_3d(&maps.c, 0, tok0 + (c + 2) * kL, bc);
         }
-      }
-      __syncwarp();
-      load_dt(0);
-      gates_of(0);
-      if (chunks > 1) gates_of(1);
-    }
-    for (int c = 0; c < chunks; ++c) {
-      const int st = c % K::kStages, par = (c / K::kStages) & 1;
-      const bool more = c + K::kStages < chunks;
-      if (kStates) {
-        if (more) {
-          wait(bars + kDS + st, par);  // x was read before it
-          if (lane == 0) {
-            load_b(c + K::kStages);
-            load_x(c + K::kStages);
-          }
-          __syncwarp();
-        }
-      } else {
-        if (c + 1 < chunks) {
+        if (!kStates && c + 1 < chunks) {
           wait(bars + kYS, c & 1);
-          if (lane == 0) load_c(c + 1);
-          __syncwarp();
+          load_c(c + 1);
         }
-        if (more) {
-          wait(bars + kDS + st, par);
-          if (lane == 0) load_b(c + K::kStages);
-          __syncwarp();
+        if (c + K::kBStages < chunks) {
+          wait(bars + kDS + c % K::kBStages, (c / K::kBStages) & 1);
+          load_b(c + K::kBStages);
+          if (kStates) load_x(c + K::kXStages);  // x was read before the product
         }
-      }
-      if (c + 2 < chunks) {
-        wait(bars + kGatesFree + (c & 1), (c >> 1) & 1);
-        gates_of(c + 2);
-      }
-      if (!kStates && (c < chunks - 1 || tail == kL)) {
-        wait(bars + kStaged + st, par);
-        if (lane == 0) {
+        if (!kStates && (c < chunks - 1 || tail == kL)) {
+          const int st = c % K::kXStages;
+          wait(bars + kStaged + st, (c / K::kXStages) & 1);
           const uint8_t* xt = sm + K::kX + st * K::kXBytes;
           for (int b = 0; b < 2; ++b)
             if (kHeads == 1 || b < heads)
               tma_store_3d(&maps.out, xt + b * kBlock, 0, tok0 + c * kL, xc + b);
           bulk_commit();
-          if (more) {
+          if (c + K::kXStages < chunks) {
             bulk_wait_read();
-            load_x(c + K::kStages);
+            load_x(c + K::kXStages);
           }
         }
-        __syncwarp();
+      }
+      if (!kStates) bulk_wait_all();
+      if (!wait.ok && chunks > 0) {
+        // copies still in flight land in this block's shared memory: let them
+        const int c = chunks - 1;
+        mbar_wait(bars + kFullX + c % K::kXStages, (c / K::kXStages) & 1);
+        mbar_wait(bars + kFullB + c % K::kBStages, (c / K::kBStages) & 1);
+        if (!kStates) mbar_wait(bars + kFullC, c & 1);
       }
     }
-    if (!kStates && lane == 0) bulk_wait_all();
-    if (!wait.ok && chunks > 0) {
-      // copies still in flight land in this block's shared memory: let them
-      const int c = chunks - 1;
-      mbar_wait(bars + kFullX + c % K::kStages, (c / K::kStages) & 1);
-      mbar_wait(bars + kFullB + c % K::kStages, (c / K::kStages) & 1);
-      if (!kStates) mbar_wait(bars + kFullC, c & 1);
-    }
     __syncwarp();
+  } else if (warp - 18 < kHeads) {
+    // ---------------------------------------------------------------- gates of one head
+    const int hh = warp - 18;
+    const bool present = hh < heads;
+    const int h = h0 + (present ? hh : 0);
+    const float neg_a = -expf(load_scalar(p.A_log, p.A_log_dtype, h));
+    const float dtb = load_scalar(p.dt_bias, p.dt_bias_dtype, h);
+    auto load = [&](int c, float (&raw)[4]) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int t = c * kL + lane * 4 + k;
+        raw[k] = t < tokens
+                     ? load_scalar(p.dt, p.dt_dtype, (static_cast<int64_t>(tok0) + t) * p.H + h)
+                     : 0.f;
+      }
+    };
+    float raw[4];
+    if (chunks > 0) load(0, raw);
+    for (int c = 0; c < chunks; ++c) {
+      const int gs = c & 1;
+      float next[4] = {0.f, 0.f, 0.f, 0.f};
+      if (c + 1 < chunks) load(c + 1, next);
+      if (c >= 2) wait(bars + kGatesFree + gs, ((c >> 1) - 1) & 1);
+      write_gates(gates + gs * kHeads + hh, raw, neg_a, dtb, present ? tokens - c * kL : 0, lane);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bars + kGatesFull + gs);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) raw[k] = next[k];
+    }
+  }
   }
   if (!wait.ok) report_wait(p.status);
   tc_fence_before();
@@ -856,6 +920,12 @@ int launch_as(const SsmParams& p, cudaStream_t stream) {
   }
   using K = Cfg<P, NS, false>;
   auto fn = ssm_chunk_kernel<P, NS, false>;
+  // the new shares wait for registers that the launch has to have brought
+  static const bool regs_ok = [&] {
+    cudaFuncAttributes at;
+    return cudaFuncGetAttributes(&at, fn) == cudaSuccess && at.numRegs == kLaunchRegs;
+  }();
+  if (!regs_ok) return GDN_ERR_CUDA;
   if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, K::kBytes) !=
       cudaSuccess)
     return GDN_ERR_CUDA;
