@@ -44,15 +44,13 @@ using chunk::named_bar_sync;
 
 constexpr int kL = 128;             // tokens per chunk
 constexpr int kBlock = 16384;       // a [128 rows x 64 columns] bf16 tile
-constexpr int kComputeWarps = 16;
-constexpr int kThreads = 20 * 32;
 
 // Registers per thread of the output kernel: 96 at launch (640 threads), then shared out anew
-// between the output's, the state's and the other warps: 256 x 104 + 256 x 96 + 128 x 80 is
+// between the output's, the state's and the other warps: 256 x 96 + 256 x 112 + 128 x 64 is
 // what 640 x 96 were. Spills are what this avoids: the shared memory leaves L1 next to nothing,
 // and a few local accesses per chunk cost more than a product.
-constexpr int kLaunchRegs = 96, kOutRegs = 104, kStateRegs = 96, kMiscRegs = 80;
-static_assert(256 * kOutRegs + 256 * kStateRegs + 128 * kMiscRegs <= kThreads * kLaunchRegs, "");
+constexpr int kLaunchRegs = 96, kOutRegs = 96, kStateRegs = 112, kMiscRegs = 64;
+static_assert(256 * kOutRegs + 256 * kStateRegs + 128 * kMiscRegs <= 640 * kLaunchRegs, "");
 
 template <int kRegs>
 __device__ __forceinline__ void regs_inc() {
@@ -69,6 +67,9 @@ __device__ __forceinline__ float lds(uint32_t a) {
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
   return v;
 }
+__device__ __forceinline__ void sts(uint32_t a, float v) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
+}
 __device__ __forceinline__ float2 lds2(uint32_t a) {
   float2 v;
   asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
@@ -81,6 +82,7 @@ __device__ __forceinline__ float4 lds4(uint32_t a) {
                : "r"(a));
   return v;
 }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
 __device__ __forceinline__ uint4 lds4u(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
@@ -100,7 +102,8 @@ __device__ __forceinline__ uint32_t row_base(uint32_t row) { return row * 128u +
 constexpr uint32_t kTG = 0;         // C B^T; then M, 8 of every 16 columns per head
 constexpr uint32_t kTY = 128;
 constexpr uint32_t kTD = 256;       // dS
-constexpr uint32_t kTF = 384;       // f x: hi 64 columns, lo 64 columns
+constexpr uint32_t kTF = 384;       // f x: 48 columns per place (the states kernel: from 0 on)
+constexpr int kTerms = 3;           // bf16 terms of f x
 
 // Of one head and chunk; read by offset (the order is kCum to kTot).
 struct Gates {
@@ -131,9 +134,10 @@ struct Cfg {
   static constexpr int kNB = NS / 64;
   // Stages: x stays until its y has left through the same memory; B and C are read early.
   static constexpr int kXStages = 3, kBStages = kStates ? 3 : 1;
-  // Warps per TMEM lane quarter on the state: two beside the two on the output, or all four.
-  static constexpr int kParts = kStates ? 4 : 2;
-  static constexpr int kStateWarps = 4 * kParts;
+  // f x is written by 32 tokens, into places in turn.
+  static constexpr int kPlaces = kStates ? 4 : 2;
+  static constexpr int kOutWarps = kStates ? 0 : 8, kStateWarps = 8;
+  static constexpr int kThreads = 32 * (kOutWarps + kStateWarps + 4);
   static constexpr uint32_t kXBytes = 2 * kBlock, kBBytes = kNB * kBlock;
   static constexpr uint32_t kX = 0;
   static constexpr uint32_t kB = kX + kXStages * kXBytes;
@@ -141,7 +145,7 @@ struct Cfg {
   static constexpr uint32_t kS = kC + (kStates ? 0 : kBBytes);
   static constexpr uint32_t kGates = kS + (kStates ? 0 : kBBytes);
   static constexpr uint32_t kBars = kGates + 2 * kHeads * sizeof(Gates);
-  static constexpr uint32_t kBytes = kBars + 256 + 1024;  // and the alignment
+  static constexpr uint32_t kBytes = kBars + 272 + 1024;  // and the alignment
 };
 
 enum Bar {
@@ -154,23 +158,37 @@ enum Bar {
   kYS = 12,         //   C S^T
   kDS = 13,         //   dS [3, by stage of B]
   kYM = 16,         //   M x
-  kFx = 17,         // operands written: f x [2] (the output kernel: one)
-  kMy = 19,         //   M and the scaled Y
-  kState = 20,      //   S
-  kYFree = 21,      // Y read out
-  kStaged = 22,     // y in shared memory [3]
-  kZeroed = 25,
+  kFx = 17,         // f x written [4, by place]
+  kFxFree = 21,     // f x read by its products [4]
+  kMy = 25,         // M and the scaled Y written
+  kState = 26,      // S written, dS read [2]
+  kYFree = 28,      // Y read out
+  kStaged = 29,     // y in shared memory [3]
+  kZeroed = 32,
 };
 
-// Waits that stop waiting after the first that gave up.
+// Bounded waits in few instructions (the roles' code has to stay in the instruction cache: see
+// the note on code size below). A wait gives up after kTries polls of at most kPollNs each,
+// a second or two; later waits of the thread then do not wait at all.
 struct Waiter {
-  bool ok = true;
-  __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t parity) {
-    if (ok) ok = mbar_wait(bar, parity);
+  static constexpr uint32_t kTries = 1u << 20, kPollNs = 2000;
+  uint32_t left = kTries;
+  __device__ __forceinline__ void operator()(uint32_t bar, uint32_t parity) {
+    uint32_t i = left;
+    for (; i; --i) {
+      uint32_t done;
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(done)
+          : "r"(bar), "r"(parity), "r"(kPollNs)
+          : "memory");
+      if (done) return;
+    }
+    left = 0;
   }
-  __device__ __forceinline__ void spin(uint64_t* bar, uint32_t parity) {
-    if (ok) ok = mbar_wait_spin(bar, parity);
-  }
+  __device__ __forceinline__ bool ok() const { return left != 0; }
 };
 
 __device__ __forceinline__ int64_t clamp_bound(const SsmParams& p, int64_t i) {
@@ -223,62 +241,57 @@ __device__ __forceinline__ void find_segment(const SsmParams& p, const Segments&
   n = p.N;
 }
 
-// Gates of a chunk's first `valid` tokens (the others: d = 0, no decay) of one head, four per
-// lane. All sums run over terms of one sign, so none of them cancels.
-__device__ __forceinline__ void write_gates(Gates* g, const float (&raw)[4], float neg_a,
-                                            float dtb, int valid, int lane) {
-  float d[4], lg[4];
-#pragma unroll
+// Gates of a chunk's first `valid` tokens (the others: d = 0, no decay) of one head, a block of
+// 32 tokens at a time, token per lane; raw: dt of the four blocks. All sums run over terms of
+// one sign, so none of them cancels.
+__device__ __forceinline__ void write_gates(uint32_t g, const float (&raw)[4], float neg_a, float dtb,
+                                            int valid, int lane) {
+  float tot[4];
+#pragma unroll 1
   for (int k = 0; k < 4; ++k) {
-    const bool in = lane * 4 + k < valid;
-    d[k] = in ? softplus_ref(raw[k] + dtb) : 0.f;
-    const float l = in ? neg_a * d[k] * kLog2e : 0.f;
+    const bool in = 32 * k + lane < valid;
+    const float r = k == 0 ? raw[0] : (k == 1 ? raw[1] : (k == 2 ? raw[2] : raw[3]));
+    const float d = in ? softplus_ref(r + dtb) : 0.f;
+    float lg = in ? neg_a * d * kLog2e : 0.f;
     // 2^-127 is zero to ex2: a stronger decay changes nothing, and the sums stay small. A NaN
     // stays one.
-    lg[k] = l < -127.f ? -127.f : l;
-  }
-  // sums over the block of 32 tokens (8 lanes) up to and from this lane
-  float pre = (lg[0] + lg[1]) + (lg[2] + lg[3]), suf = pre;
+    lg = lg < -127.f ? -127.f : lg;
+    float pre = lg, suf = lg;  // over the block, up to and from this token
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    const float a = __shfl_up_sync(0xffffffffu, pre, o, 8);
-    const float b = __shfl_down_sync(0xffffffffu, suf, o, 8);
-    if ((lane & 7) >= o) pre += a;
-    if ((lane & 7) + o < 8) suf += b;
+    for (int o = 1; o < 32; o <<= 1) {
+      const float a = __shfl_up_sync(0xffffffffu, pre, o);
+      const float b = __shfl_down_sync(0xffffffffu, suf, o);
+      if (lane >= o) pre += a;
+      if (lane + o < 32) suf += b;
+    }
+    float behind = __shfl_down_sync(0xffffffffu, suf, 1);
+    if (lane == 31) behind = 0.f;
+    const float t = __shfl_sync(0xffffffffu, pre, 31);
+    const uint32_t at = g + 4 * (32 * k + lane);
+    sts(at + kCum, pre);
+    sts(at + kD, d);
+    sts(at + kU, d * ex2(behind));
+    sts(at + kF, behind);  // until the blocks behind are known
+    if (lane == 0) sts(g + kTot + 4 * k, t);
+    tot[0] = k == 0 ? t : tot[0];
+    tot[1] = k == 1 ? t : tot[1];
+    tot[2] = k == 2 ? t : tot[2];
+    tot[3] = t;
   }
-  float before = __shfl_up_sync(0xffffffffu, pre, 1, 8);
-  float behind = __shfl_down_sync(0xffffffffu, suf, 1, 8);
-  if ((lane & 7) == 0) before = 0.f;
-  if ((lane & 7) == 7) behind = 0.f;
-  const float b0 = __shfl_sync(0xffffffffu, pre, 7), b1 = __shfl_sync(0xffffffffu, pre, 15);
-  const float b2 = __shfl_sync(0xffffffffu, pre, 23), b3 = __shfl_sync(0xffffffffu, pre, 31);
-  const int blk = lane >> 3;
-  const float head = blk == 0 ? 0.f : (blk == 1 ? b0 : (blk == 2 ? b0 + b1 : b0 + b1 + b2));
-  const float tail = blk == 3 ? 0.f : (blk == 2 ? b3 : (blk == 1 ? b2 + b3 : b1 + b2 + b3));
-  float c[4], w[4];  // from the block's start, inclusive; to its end, exclusive
-  c[0] = before + lg[0];
-  c[1] = c[0] + lg[1];
-  c[2] = c[1] + lg[2];
-  c[3] = c[2] + lg[3];
-  w[3] = behind;
-  w[2] = w[3] + lg[3];
-  w[1] = w[2] + lg[2];
-  w[0] = w[1] + lg[1];
-  const int at = lane * 4;
-  *reinterpret_cast<float4*>(g->cum + at) = make_float4(c[0], c[1], c[2], c[3]);
-  *reinterpret_cast<float4*>(g->dec + at) =
-      make_float4(ex2(head + c[0]), ex2(head + c[1]), ex2(head + c[2]), ex2(head + c[3]));
-  *reinterpret_cast<float4*>(g->u + at) =
-      make_float4(d[0] * ex2(w[0]), d[1] * ex2(w[1]), d[2] * ex2(w[2]), d[3] * ex2(w[3]));
-  *reinterpret_cast<float4*>(g->f + at) =
-      make_float4(d[0] * ex2(w[0] + tail), d[1] * ex2(w[1] + tail), d[2] * ex2(w[2] + tail),
-                  d[3] * ex2(w[3] + tail));
-  *reinterpret_cast<float4*>(g->d + at) = make_float4(d[0], d[1], d[2], d[3]);
-  if ((lane & 7) == 7) g->tot[blk] = pre;
+#pragma unroll 1
+  for (int k = 0; k < 4; ++k) {
+    const float head = k == 0 ? 0.f : (k == 1 ? tot[0] : (k == 2 ? tot[0] + tot[1]
+                                                                 : tot[0] + tot[1] + tot[2]));
+    const float tail = k == 3 ? 0.f : (k == 2 ? tot[3] : (k == 1 ? tot[2] + tot[3]
+                                                                 : tot[1] + tot[2] + tot[3]));
+    const uint32_t at = g + 4 * (32 * k + lane);  // this lane's own values
+    sts(at + kDec, ex2(head + lds(at + kCum)));
+    sts(at + kF, lds(at + kD) * ex2(lds(at + kF) + tail));
+  }
 }
 
 template <int P, int NS, bool kStates>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Cfg<P, NS, kStates>::kThreads, 1)
 ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Maps maps,
                  const __grid_constant__ Segments sg, int col_blocks) {
   using K = Cfg<P, NS, kStates>;
@@ -325,8 +338,8 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
   const int tok0 = static_cast<int>(t_begin);
 
   uint64_t* const bars = reinterpret_cast<uint64_t*>(sm + K::kBars);
-  Gates* const gates = reinterpret_cast<Gates*>(sm + K::kGates);
-  constexpr int kOutWarps = kStates ? 0 : 8;  // warps 0-7; the state's warps follow
+  constexpr int kOutWarps = K::kOutWarps;                   // first, then the state's
+  constexpr int kMisc = kOutWarps + K::kStateWarps;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 3; ++i) {
       mbar_init(bars + kFullX + i, 1);
@@ -337,20 +350,25 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     mbar_init(bars + kFullC, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(bars + kGatesFull + i, kHeads);
-      mbar_init(bars + kGatesFree + i, kComputeWarps);
+      mbar_init(bars + kGatesFree + i, kOutWarps + K::kStateWarps);
+      mbar_init(bars + kState + i, K::kStateWarps);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(bars + kFx + i, K::kStateWarps);
+      mbar_init(bars + kFxFree + i, 1);
     }
     for (int i : {kCB, kYS, kYM}) mbar_init(bars + i, 1);
     for (int i : {kMy, kYFree}) mbar_init(bars + i, 8);
-    for (int i : {kState, kZeroed}) mbar_init(bars + i, K::kStateWarps);
+    mbar_init(bars + kZeroed, K::kStateWarps);
     fence_mbar_init();
   }
-  if (warp == 16) tmem_alloc(&s_tmem, 512);
+  if (warp == kMisc) tmem_alloc(&s_tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tm = s_tmem, sm_u = smem_u32(sm), gates_u = sm_u + K::kGates;
-  Waiter wait;
+  const uint32_t tm = s_tmem, sm_u = smem_u32(sm), gates_u = sm_u + K::kGates,
+                 bars_u = sm_u + K::kBars;
+  Waiter wait, finally;  // the second for what a block that gave up still has to wait for
   const int q = warp & 3;                      // TMEM lane quarter
   const uint32_t lanes = tm + (static_cast<uint32_t>(32 * q) << 16);
   const int row = 32 * q + lane;               // token of a chunk / column of the block
@@ -368,76 +386,70 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     for (int c = 0; c < chunks; ++c) {
       const int gs = c & 1;
       const uint32_t ga = gates_u + gs * kHeads * static_cast<uint32_t>(sizeof(Gates));
-      wait(bars + kGatesFull + gs, (c >> 1) & 1);
-      wait(bars + kCB, c & 1);
+      wait(bars_u + 8 * (kGatesFull + gs), (c >> 1) & 1);
+      wait(bars_u + 8 * (kCB), c & 1);
       tc_fence_after();
       // ---- M over C B^T, 16 columns at a time: those of head h go to 8 columns of the same
       // 16, so a warp overwrites nothing that another has yet to read. The two warps of a
       // quarter take every other 16 (each has one piece on the diagonal).
 #pragma unroll 1
-      for (int k0 = 0; k0 < 4; k0 += 2) {
-        float g0[16], g1[16];
-        const uint32_t at = lanes + kTG + 32 * k0 + 16 * half;
-        if (k0 <= q) {
-          tmem_ld16(at, g0);
-          tmem_ld16(at + 32, g1);
+      for (int k = 0; k < 4; ++k) {  // piece k: columns 32 k + 16 half on, in block k of 32
+        const int j0 = 32 * k + 16 * half;
+        const uint32_t at = lanes + kTG + j0;
+        float g[16];
+        if (k <= q) {
+          tmem_ld16(at, g);
           tmem_ld_wait();
         }
-#pragma unroll
+#pragma unroll 1
         for (int hh = 0; hh < kHeads; ++hh) {
           const uint32_t gh = ga + hh * static_cast<uint32_t>(sizeof(Gates));
-          const float own = lds(gh + kCum + 4 * row);
-          auto piece = [&](int k, const float(&g)[16], uint32_t dst) {
-            const int j0 = 32 * k + 16 * half;
-            uint32_t m[8];
-            if (k < q) {
-              // e^{G_i - G_j} d_j = e^{G_i - G_r} (e^{G_r - G_j} d_j), r the end of j's block,
-              // between j and i: both exponents are at most 0, and one exponential per row
-              // is left
-              float ex = own;
-              for (int b = k + 1; b < q; ++b) ex += lds(gh + kTot + 4 * b);
-              const float e = ex2(ex);
-              const float2 a = make_float2(e, e);
+          uint32_t m[8];
+          if (k < q) {
+            // e^{G_i - G_j} d_j = e^{G_i - G_r} (e^{G_r - G_j} d_j), r the end of j's block,
+            // between j and i: both exponents are at most 0, and one exponential per row is left
+            float ex = lds(gh + kCum + 4 * row);
+            if (k + 1 < q) ex += lds(gh + kTot + 4 * (k + 1));
+            if (k + 2 < q) ex += lds(gh + kTot + 4 * (k + 2));
+            const float e = ex2(ex);
+            const float2 a = make_float2(e, e);
 #pragma unroll
-              for (int j = 0; j < 16; j += 4) {
-                const float4 u = lds4(gh + kU + 4 * (j0 + j));
-                const float2 v0 =
-                    mul2(mul2(make_float2(u.x, u.y), a), make_float2(g[j], g[j + 1]));
-                const float2 v1 =
-                    mul2(mul2(make_float2(u.z, u.w), a), make_float2(g[j + 2], g[j + 3]));
-                m[j / 2] = pack2_rn(v0.x, v0.y);
-                m[j / 2 + 1] = pack2_rn(v1.x, v1.y);
-              }
-            } else if (k == q) {
-              const int i = row - j0;  // columns j <= i are on or below the diagonal
-#pragma unroll
-              for (int j = 0; j < 16; j += 4) {
-                const float4 cj = lds4(gh + kCum + 4 * (j0 + j));
-                const float4 dj = lds4(gh + kD + 4 * (j0 + j));
-                const float v0 = j <= i ? g[j] * (ex2(own - cj.x) * dj.x) : 0.f;
-                const float v1 = j + 1 <= i ? g[j + 1] * (ex2(own - cj.y) * dj.y) : 0.f;
-                const float v2 = j + 2 <= i ? g[j + 2] * (ex2(own - cj.z) * dj.z) : 0.f;
-                const float v3 = j + 3 <= i ? g[j + 3] * (ex2(own - cj.w) * dj.w) : 0.f;
-                m[j / 2] = pack2_rn(v0, v1);
-                m[j / 2 + 1] = pack2_rn(v2, v3);
-              }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) m[j] = 0u;
+            for (int j = 0; j < 16; j += 4) {
+              const float4 u = lds4(gh + kU + 4 * (j0 + j));
+              const float2 v0 = mul2(mul2(make_float2(u.x, u.y), a), make_float2(g[j], g[j + 1]));
+              const float2 v1 =
+                  mul2(mul2(make_float2(u.z, u.w), a), make_float2(g[j + 2], g[j + 3]));
+              m[j / 2] = pack2_rn(v0.x, v0.y);
+              m[j / 2 + 1] = pack2_rn(v1.x, v1.y);
             }
-            tmem_st8(dst + 8 * hh, m);
-          };
-          piece(k0, g0, at);
-          piece(k0 + 1, g1, at + 32);
+          } else if (k == q) {
+            const float own = lds(gh + kCum + 4 * row);
+            const int i = row - j0;  // columns j <= i are on or below the diagonal
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+              const float4 cj = lds4(gh + kCum + 4 * (j0 + j));
+              const float4 dj = lds4(gh + kD + 4 * (j0 + j));
+              const float v0 = j <= i ? g[j] * (ex2(own - cj.x) * dj.x) : 0.f;
+              const float v1 = j + 1 <= i ? g[j + 1] * (ex2(own - cj.y) * dj.y) : 0.f;
+              const float v2 = j + 2 <= i ? g[j + 2] * (ex2(own - cj.z) * dj.z) : 0.f;
+              const float v3 = j + 3 <= i ? g[j + 3] * (ex2(own - cj.w) * dj.w) : 0.f;
+              m[j / 2] = pack2_rn(v0, v1);
+              m[j / 2 + 1] = pack2_rn(v2, v3);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m[j] = 0u;
+          }
+          tmem_st8(at + 8 * hh, m);
         }
       }
       // ---- Y = e^{G_i} (C S^T), in place
-      wait(bars + kYS, c & 1);
+      wait(bars_u + 8 * (kYS), c & 1);
       tc_fence_after();
       {
         const float e = lds(ga + col_head * static_cast<uint32_t>(sizeof(Gates)) + kDec + 4 * row);
         const float2 e2 = make_float2(e, e);
-#pragma unroll
+#pragma unroll 1
         for (int k = 0; k < 2; ++k) {
           const uint32_t ty = lanes + kTY + 64 * half + 32 * k;
           float y[32];
@@ -459,10 +471,10 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       // ---- y: out of TMEM, D x added, over the chunk's x in shared memory
       const int st = c % K::kXStages;
       const uint32_t xrow = sm_u + K::kX + st * K::kXBytes + half * kBlock + row_base(row);
-      wait(bars + kYM, c & 1);
+      wait(bars_u + 8 * (kYM), c & 1);
       tc_fence_after();
       {
-#pragma unroll
+#pragma unroll 1
         for (int k0 = 0; k0 < 8; k0 += 4) {
           float y[32];
           tmem_ld32(lanes + kTY + 64 * half + 8 * k0, y);
@@ -474,21 +486,16 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t at = xrow ^ (16 * (k0 + k));
+            const uint4 xv = p.D ? lds4u(at) : make_uint4(0u, 0u, 0u, 0u);
+            const uint32_t u[4] = {xv.x, xv.y, xv.z, xv.w};
             uint32_t w[4];
-            if (p.D) {
-              const uint4 xv = lds4u(at);
-              const uint32_t u[4] = {xv.x, xv.y, xv.z, xv.w};
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 v = fma2(make_float2(skip, skip),
-                                      make_float2(__uint_as_float(u[e] << 16),
-                                                  __uint_as_float(u[e] & 0xffff0000u)),
-                                      make_float2(y[8 * k + 2 * e], y[8 * k + 2 * e + 1]));
-                w[e] = pack2_rn(v.x, v.y);
-              }
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) w[e] = pack2_rn(y[8 * k + 2 * e], y[8 * k + 2 * e + 1]);
+            for (int e = 0; e < 4; ++e) {
+              const float2 v = fma2(make_float2(skip, skip),
+                                    make_float2(__uint_as_float(u[e] << 16),
+                                                __uint_as_float(u[e] & 0xffff0000u)),
+                                    make_float2(y[8 * k + 2 * e], y[8 * k + 2 * e + 1]));
+              w[e] = pack2_rn(v.x, v.y);
             }
             sts4u(at, w[0], w[1], w[2], w[3]);
           }
@@ -513,11 +520,10 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         }
       }
     }
-  } else if (warp < kComputeWarps) {
+  } else if (warp < kMisc) {
     if (!kStates) regs_inc<kStateRegs>();
     // ---------------------------------------------------------------- state: column per thread
-    constexpr int kTok = kL / K::kParts;         // tokens of f x per warp
-    constexpr int kNC = NS / K::kParts;          // state columns per thread
+    constexpr int kNC = NS / 2;                  // state columns per thread
     const int part = (warp - kOutWarps) >> 2;
     const int row_head = kHeads == 2 ? q >> 1 : 0;   // head of column `row`
     const int64_t st_off =
@@ -538,6 +544,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
           S[i + 1] = v.y;
           S[i + 2] = v.z;
           S[i + 3] = v.w;
+          if (i % 16 == 12) asm volatile("" ::: "memory");  // no more loads in flight than that
         }
       }
       for (int64_t r = slot - seg; r < slot; ++r) {  // this sequence's segments before this one
@@ -551,6 +558,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
           S[i + 1] = fmaf(g, S[i + 1], v.y);
           S[i + 2] = fmaf(g, S[i + 2], v.z);
           S[i + 3] = fmaf(g, S[i + 3], v.w);
+          if (i % 16 == 12) asm volatile("" ::: "memory");
         }
       }
     }
@@ -558,7 +566,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     // The state as the operand of the next chunk's C S^T: row = column of the block, n
     // contiguous (K-major).
     const uint32_t s_row = sm_u + K::kS + (kNC * part >> 6) * kBlock + row_base(row);
-    auto write_state = [&]() {
+    auto arrive_state = [&]() {
 #pragma unroll
       for (int k = 0; k < kNC / 8; ++k)
         sts4u(s_row ^ (16 * (((kNC * part >> 3) + k) & 7)), pack2_rn(S[8 * k], S[8 * k + 1]),
@@ -568,21 +576,20 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       arrive(kState);
     };
 
-    // (f x)^T of chunk c into TMEM: this warp's tokens of columns 32 q to 32 q + 31, transposed
-    // by ldmatrix, scaled, split and stored as the fragments come, 16 tokens at a time.
-    // lane l gives ldmatrix token t0 + 8 (l / 16) + l % 8, columns 8 ((l / 8) % 2) to + 7 (and
-    // 16 on) of the quarter's 32
-    const uint32_t x_lane =
-        row_base(8 * (lane >> 4) + (lane & 7)) ^ (16 * ((q & 1) * 4 + ((lane >> 3) & 1)));
-    auto write_fx = [&](int c) {
-      const int st = c % K::kXStages, gs = c & 1;
+    // (f x)^T into TMEM, 32 tokens at a time (this warp: 16 of them, of columns 32 q to
+    // 32 q + 31): transposed by ldmatrix, scaled, split and stored as the fragments come. Lane
+    // l gives ldmatrix token l % 8 + 8 (l / 16) of the 16, columns 8 ((l / 8) % 2) on.
+    const uint32_t x_lane = row_base(16 * part + 8 * (lane >> 4) + (lane & 7)) ^
+                            (16 * ((q & 1) * 4 + ((lane >> 3) & 1)));
+    auto begin_fx = [&](int c) {
+      const int st = c % K::kXStages;
       uint8_t* const xt = sm + K::kX + st * K::kXBytes;
-      wait(bars + kFullX + st, (c / K::kXStages) & 1);
+      wait(bars_u + 8 * (kFullX + st), (c / K::kXStages) & 1);
       if (c == chunks - 1 && tail < kL) {
         // Rows behind the sequence hold other tokens or nothing: zeros, so that neither they
         // nor a NaN among them enters a product.
         uint8_t* const bt = sm + K::kB + (c % K::kBStages) * K::kBBytes;
-        wait(bars + kFullB + c % K::kBStages, (c / K::kBStages) & 1);
+        wait(bars_u + 8 * (kFullB + c % K::kBStages), (c / K::kBStages) & 1);
         for (int i = threadIdx.x - kOutWarps * 32; i < (kL - tail) * 8; i += K::kStateWarps * 32) {
           const uint32_t off = (tail + (i >> 3)) * 128 + (i & 7) * 16;
           const uint4 z = make_uint4(0u, 0u, 0u, 0u);
@@ -595,44 +602,53 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         named_bar_sync(2, K::kStateWarps * 32);
         arrive(kZeroed);
       }
-      wait(bars + kGatesFull + gs, (c >> 1) & 1);
-      const uint32_t f = gates_u + (gs * kHeads + row_head) * static_cast<uint32_t>(sizeof(Gates)) +
-                         kF + 8 * (lane & 3);
-      const uint32_t xb = sm_u + K::kX + st * K::kXBytes + (q >> 1) * kBlock + x_lane;
-      const uint32_t t_hi = lanes + (kStates && (c & 1) ? kTG : kTF);
-#pragma unroll 1
-      for (int t0 = part * kTok; t0 < (part + 1) * kTok; t0 += 16) {
-        const float2 f0 = lds2(f + 4 * t0), f1 = lds2(f + 4 * t0 + 32);
+      wait(bars_u + 8 * (kGatesFull + (c & 1)), (c >> 1) & 1);
+    };
+    auto write_fx = [&](int c, int t) {  // tokens 32 t to 32 t + 31 of chunk c
+      const int k = 4 * c + t, place = k % K::kPlaces;
+      const uint32_t f = gates_u +
+                         ((c & 1) * kHeads + row_head) * static_cast<uint32_t>(sizeof(Gates)) + kF +
+                         4 * (32 * t + 16 * part) + 8 * (lane & 3);
+      const float2 f0 = lds2(f), f1 = lds2(f + 32);
+      const uint32_t xa = sm_u + K::kX + (c % K::kXStages) * K::kXBytes + (q >> 1) * kBlock +
+                          128 * 32 * t + x_lane;
+      if (k >= K::kPlaces) wait(bars_u + 8 * (kFxFree + place), (k / K::kPlaces - 1) & 1);
+      const uint32_t at = lanes + (kStates ? 0 : kTF) + 16 * kTerms * place + 8 * part;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t u[4], hi[4], lo[4];  // tokens t0 to + 7: columns 0-7, 8-15; t0 + 8: the same
-          ldmatrix_x4_trans((xb + 128 * t0) ^ (32 * h), u);
+      for (int h = 0; h < 2; ++h) {
+        uint32_t u[4], w[kTerms][4];  // tokens 0-7 of columns 0-7 and 8-15, then tokens 8-15
+        ldmatrix_x4_trans(xa ^ (32 * h), u);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 v = mul2(make_float2(__uint_as_float(u[k] << 16),
-                                              __uint_as_float(u[k] & 0xffff0000u)),
-                                  k < 2 ? f0 : f1);
-            split2(v.x, v.y, hi[k], lo[k]);
+        for (int i = 0; i < 4; ++i) {
+          float2 v = mul2(make_float2(__uint_as_float(u[i] << 16),
+                                      __uint_as_float(u[i] & 0xffff0000u)),
+                          i < 2 ? f0 : f1);
+#pragma unroll
+          for (int r = 0; r < kTerms - 1; ++r) {
+            w[r][i] = pack2_rn(v.x, v.y);
+            v = add2(v, make_float2(__uint_as_float((w[r][i] << 16) ^ 0x80000000u),
+                                    __uint_as_float((w[r][i] & 0xffff0000u) ^ 0x80000000u)));
           }
-          const uint32_t at = t_hi + t0 / 2 + (static_cast<uint32_t>(16 * h) << 16);
-          tmem_st_frag(at, hi);
-          tmem_st_frag(at + 64, lo);
+          w[kTerms - 1][i] = pack2_rn(v.x, v.y);
         }
+#pragma unroll
+        for (int r = 0; r < kTerms; ++r)
+          tmem_st_frag(at + 16 * r + (static_cast<uint32_t>(16 * h) << 16), w[r]);
       }
       tmem_st_wait();
       tc_fence_before();
-      arrive(kFx + (kStates ? (c & 1) : 0));
+      arrive(kFx + place);
     };
 
     // The state behind chunk c, from what the chunk adds.
     auto update_state = [&](int c) {
-      wait(bars + kDS + c % K::kBStages, (c / K::kBStages) & 1);
+      wait(bars_u + 8 * (kDS + c % K::kBStages), (c / K::kBStages) & 1);
       tc_fence_after();
       const float g =
           lds(gates_u + ((c & 1) * kHeads + row_head) * static_cast<uint32_t>(sizeof(Gates)) + kDec +
               4 * (kL - 1));
       const float2 g2 = make_float2(g, g);
-      const uint32_t td = lanes + (kStates && (c & 1) ? kTY : kTD) + kNC * part;
+      const uint32_t td = lanes + kTD + (kStates ? 128 * (c & 1) : 0) + kNC * part;
 #pragma unroll
       for (int i0 = 0; i0 < kNC; i0 += 16) {
         float v[16];
@@ -651,19 +667,24 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       arrive(kGatesFree + (c & 1));
     };
 
+    // Turn i of the loop writes quarter i % 4 of chunk i / 4, and updates the state with the chunk
+    // before after the first quarter, while the products of that chunk's end still run; one
+    // more turn updates it with the last chunk. (One loop: each part of the code exists once.)
     if (chunks > 0) {
-      if (!kStates) write_state();
-      write_fx(0);
-    }
-    for (int c = 0; c < chunks; ++c) {
-      // states kernel: f x and dS alternate between two places, so the next operand is
-      // written while the product of this one runs
-      if (kStates && c + 1 < chunks) write_fx(c + 1);
-      update_state(c);
-      if (!kStates && c + 1 < chunks) {
-        write_fx(c + 1);
-        wait(bars + kYS, c & 1);  // the product has read the state it replaces
-        write_state();
+      if (!kStates) arrive_state();
+#pragma unroll 1
+      for (int i = 0; i <= 4 * chunks; ++i) {
+        const int c = i >> 2, t = i & 3;
+        if (c < chunks) {
+          if (t == 0) begin_fx(c);
+          write_fx(c, t);
+        }
+        if (t == 0 && c > 0) {
+          update_state(c - 1);
+          // C S^T has read the state it replaces: it came before dS
+          if (!kStates && c < chunks) arrive_state();
+          if (kStates) arrive(kState + ((c - 1) & 1));
+        }
       }
     }
     if (mine) {
@@ -682,70 +703,89 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     }
   } else {
     if (!kStates) regs_dec<kMiscRegs>();
-    if (warp == 16) {
+    if (warp == kMisc) {
     // ---------------------------------------------------------------- products
     constexpr uint32_t kIdCB = idesc_bf16(128, 128, false, false);
     constexpr uint32_t kIdDS = idesc_bf16(128, NS, false, true);
     constexpr uint32_t kIdYM = idesc_bf16(128, P, false, true);
-    const uint64_t d_c = desc_kmajor(smem_u32(sm + K::kC));
-    const uint64_t d_s = desc_kmajor(smem_u32(sm + K::kS));
-    auto kstep = [](int s) { return static_cast<uint64_t>(((s >> 2) * kBlock + (s & 3) * 32) >> 4); };
+    // Descriptors differ in their start address alone: built where they are used, from bases
+    // that look new in every chunk, or all of them would be kept in registers.
+    const uint64_t d_k = desc_kmajor(0), d_mn = desc_mnmajor(0, kBlock);
+    auto fresh = [](uint32_t v) {
+      uint32_t r;
+      asm volatile("mov.u32 %0, %1;" : "=r"(r) : "r"(v));
+      return r;
+    };
+    auto desc = [](uint64_t kind, uint32_t base, uint32_t off) {
+      return kind | static_cast<uint64_t>((base + off) >> 4);
+    };
+    auto kstep = [](int s) { return static_cast<uint32_t>((s >> 2) * kBlock + (s & 3) * 32); };
     for (int c = 0; c < chunks; ++c) {
       const int st = c % K::kBStages, par = (c / K::kBStages) & 1;
-      const uint32_t xb = smem_u32(sm + K::kX + (c % K::kXStages) * K::kXBytes);
-      const uint32_t bb = smem_u32(sm + K::kB + st * K::kBBytes);
+      const uint32_t xb = sm_u + K::kX + (c % K::kXStages) * K::kXBytes;
+      const uint32_t bb = sm_u + K::kB + st * K::kBBytes;
       const bool zeroed = c == chunks - 1 && tail < kL;
-      auto issue_ds = [&](uint32_t td, uint32_t tf) {
-        const uint64_t db = desc_mnmajor(bb, kBlock);
+      auto issue_ds = [&](uint32_t td) {
+#pragma unroll 1
+        for (int t = 0; t < 4; ++t) {
+          const int k = 4 * c + t, place = k % K::kPlaces;
+          wait(bars_u + 8 * (kFx + place), (k / K::kPlaces) & 1);
+          tc_fence_after();
+          const uint32_t tf = tm + (kStates ? 0 : kTF) + 16 * kTerms * place;
+          const uint32_t b0 = fresh(bb + t * 4096);
 #pragma unroll
-        for (int s = 0; s < 8; ++s)
-          mma_bf16_ts_w(td, tf + 8 * s, db + static_cast<uint64_t>((s * 2048) >> 4), kIdDS, s > 0);
+          for (int r = 0; r < kTerms; ++r) {
 #pragma unroll
-        for (int s = 0; s < 8; ++s)
-          mma_bf16_ts_w(td, tf + 64 + 8 * s, db + static_cast<uint64_t>((s * 2048) >> 4), kIdDS, 1);
+            for (int s = 0; s < 2; ++s)
+              mma_bf16_ts_w(td, tf + 16 * r + 8 * s, desc(d_mn, b0, s * 2048), kIdDS,
+                            t > 0 || r > 0 || s > 0);
+          }
+          mma_commit_w(bars + kFxFree + place);
+        }
+        mma_commit_w(bars + kDS + st);
       };
       if (kStates) {
-        wait.spin(bars + kFullB + st, par);
-        wait.spin(bars + kFx + (c & 1), (c >> 1) & 1);
-        tc_fence_after();
-        issue_ds(tm + (c & 1 ? kTY : kTD), tm + (c & 1 ? kTG : kTF));
-        mma_commit_w(bars + kDS + st);
+        wait(bars_u + 8 * (kFullB + st), par);
+        if (c >= 2) wait(bars_u + 8 * (kState + (c & 1)), ((c >> 1) - 1) & 1);
+        issue_ds(tm + kTD + 128 * (c & 1));
         continue;
       }
       // C B^T: over the place of the last chunk's M
-      wait.spin(bars + kFullB + st, par);
-      wait.spin(bars + kFullC, c & 1);
-      if (zeroed) wait.spin(bars + kZeroed, 0);
-      if (c > 0) wait.spin(bars + kYM, (c - 1) & 1);
+      wait(bars_u + 8 * (kFullB + st), par);
+      wait(bars_u + 8 * (kFullC), c & 1);
+      if (zeroed) wait(bars_u + 8 * (kZeroed), 0);
+      if (c > 0) wait(bars_u + 8 * (kYM), (c - 1) & 1);
       tc_fence_after();
-      const uint64_t d_b = desc_kmajor(bb);
-#pragma unroll
-      for (int s = 0; s < NS / 16; ++s)
-        mma_bf16_w(tm + kTG, d_c + kstep(s), d_b + kstep(s), kIdCB, s > 0);
+      {
+        const uint32_t b0 = fresh(bb), c0 = fresh(sm_u + K::kC);
+#pragma unroll 4
+        for (int s = 0; s < NS / 16; ++s)
+          mma_bf16_w(tm + kTG, desc(d_k, c0, kstep(s)), desc(d_k, b0, kstep(s)), kIdCB, s > 0);
+      }
       mma_commit_w(bars + kCB);
       // C S^T
-      wait.spin(bars + kState, c & 1);
-      if (c > 0) wait.spin(bars + kYFree, (c - 1) & 1);
+      wait(bars_u + 8 * (kState), c & 1);
+      if (c > 0) wait(bars_u + 8 * (kYFree), (c - 1) & 1);
       tc_fence_after();
-#pragma unroll
-      for (int s = 0; s < NS / 16; ++s)
-        mma_bf16_w(tm + kTY, d_c + kstep(s), d_s + kstep(s), kIdCB, s > 0);
+      {
+        const uint32_t s0 = fresh(sm_u + K::kS), c0 = fresh(sm_u + K::kC);
+#pragma unroll 4
+        for (int s = 0; s < NS / 16; ++s)
+          mma_bf16_w(tm + kTY, desc(d_k, c0, kstep(s)), desc(d_k, s0, kstep(s)), kIdCB, s > 0);
+      }
       mma_commit_w(bars + kYS);
       // (f x)^T B
-      wait.spin(bars + kFx, c & 1);
-      tc_fence_after();
-      issue_ds(tm + kTD, tm + kTF);
-      mma_commit_w(bars + kDS + st);
+      issue_ds(tm + kTD);
       // M x
-      wait.spin(bars + kMy, c & 1);
+      wait(bars_u + 8 * (kMy), c & 1);
       tc_fence_after();
-#pragma unroll
+#pragma unroll 1
       for (int hh = 0; hh < kHeads; ++hh) {
-        const uint64_t dx = desc_mnmajor(xb + hh * kBlock, kBlock);
-#pragma unroll
+        const uint32_t x0 = fresh(xb + hh * kBlock);
+#pragma unroll 4
         for (int s = 0; s < 8; ++s)
           mma_bf16_ts_w(tm + kTY + hh * 64, tm + kTG + 16 * s + 8 * hh,
-                        dx + static_cast<uint64_t>((s * 2048) >> 4), kIdYM, 1);
+                        desc(d_mn, x0, s * 2048), kIdYM, 1);
       }
       mma_commit_w(bars + kYM);
     }
@@ -753,12 +793,12 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     if (chunks > 0) {
       const int c = chunks - 1;
       if (kStates) {
-        mbar_wait(bars + kDS + c % K::kBStages, (c / K::kBStages) & 1);
+        finally(bars_u + 8 * (kDS + c % K::kBStages), (c / K::kBStages) & 1);
       } else {
-        mbar_wait(bars + kYM, c & 1);
+        finally(bars_u + 8 * (kYM), c & 1);
       }
     }
-  } else if (warp == 17) {
+  } else if (warp == kMisc + 1) {
     // ---------------------------------------------------------------- bulk copies
     if (lane == 0) {
       const int xc = (h0 * P) / 64, bc = grp * K::kNB;
@@ -789,17 +829,17 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
           tma_prefetch_3d(&maps.c, 0, tok0 + (c + 2) * kL, bc);
         }
         if (!kStates && c + 1 < chunks) {
-          wait(bars + kYS, c & 1);
+          wait(bars_u + 8 * (kYS), c & 1);
           load_c(c + 1);
         }
         if (c + K::kBStages < chunks) {
-          wait(bars + kDS + c % K::kBStages, (c / K::kBStages) & 1);
+          wait(bars_u + 8 * (kDS + c % K::kBStages), (c / K::kBStages) & 1);
           load_b(c + K::kBStages);
           if (kStates) load_x(c + K::kXStages);  // x was read before the product
         }
         if (!kStates && (c < chunks - 1 || tail == kL)) {
           const int st = c % K::kXStages;
-          wait(bars + kStaged + st, (c / K::kXStages) & 1);
+          wait(bars_u + 8 * (kStaged + st), (c / K::kXStages) & 1);
           const uint8_t* xt = sm + K::kX + st * K::kXBytes;
           for (int b = 0; b < 2; ++b)
             if (kHeads == 1 || b < heads)
@@ -812,18 +852,18 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         }
       }
       if (!kStates) bulk_wait_all();
-      if (!wait.ok && chunks > 0) {
+      if (!wait.ok() && chunks > 0) {
         // copies still in flight land in this block's shared memory: let them
         const int c = chunks - 1;
-        mbar_wait(bars + kFullX + c % K::kXStages, (c / K::kXStages) & 1);
-        mbar_wait(bars + kFullB + c % K::kBStages, (c / K::kBStages) & 1);
-        if (!kStates) mbar_wait(bars + kFullC, c & 1);
+        finally(bars_u + 8 * (kFullX + c % K::kXStages), (c / K::kXStages) & 1);
+        finally(bars_u + 8 * (kFullB + c % K::kBStages), (c / K::kBStages) & 1);
+        if (!kStates) finally(bars_u + 8 * (kFullC), c & 1);
       }
     }
     __syncwarp();
-  } else if (warp - 18 < kHeads) {
+  } else if (warp - kMisc - 2 < kHeads) {
     // ---------------------------------------------------------------- gates of one head
-    const int hh = warp - 18;
+    const int hh = warp - kMisc - 2;
     const bool present = hh < heads;
     const int h = h0 + (present ? hh : 0);
     const float neg_a = -expf(load_scalar(p.A_log, p.A_log_dtype, h));
@@ -831,7 +871,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     auto load = [&](int c, float (&raw)[4]) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int t = c * kL + lane * 4 + k;
+        const int t = c * kL + 32 * k + lane;
         raw[k] = t < tokens
                      ? load_scalar(p.dt, p.dt_dtype, (static_cast<int64_t>(tok0) + t) * p.H + h)
                      : 0.f;
@@ -843,8 +883,8 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       const int gs = c & 1;
       float next[4] = {0.f, 0.f, 0.f, 0.f};
       if (c + 1 < chunks) load(c + 1, next);
-      if (c >= 2) wait(bars + kGatesFree + gs, ((c >> 1) - 1) & 1);
-      write_gates(gates + gs * kHeads + hh, raw, neg_a, dtb, present ? tokens - c * kL : 0, lane);
+      if (c >= 2) wait(bars_u + 8 * (kGatesFree + gs), ((c >> 1) - 1) & 1);
+      write_gates(gates_u + (gs * kHeads + hh) * static_cast<uint32_t>(sizeof(Gates)), raw, neg_a, dtb, present ? tokens - c * kL : 0, lane);
       __syncwarp();
       if (lane == 0) mbar_arrive(bars + kGatesFull + gs);
 #pragma unroll
@@ -852,11 +892,11 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     }
   }
   }
-  if (!wait.ok) report_wait(p.status);
+  if (!wait.ok()) report_wait(p.status);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 16) tmem_dealloc(tm, 512);
+  if (warp == kMisc) tmem_dealloc(tm, 512);
 }
 
 bool encode(CUtensorMap* map, const void* base, int64_t T, int64_t cols, uint32_t blocks) {
@@ -915,7 +955,7 @@ int launch_as(const SsmParams& p, cudaStream_t stream) {
     if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, K::kBytes) !=
         cudaSuccess)
       return GDN_ERR_CUDA;
-    fn<<<grid, kThreads, K::kBytes, stream>>>(p, maps, sg, cols);
+    fn<<<grid, K::kThreads, K::kBytes, stream>>>(p, maps, sg, cols);
     if (cudaGetLastError() != cudaSuccess) return GDN_ERR_CUDA;
   }
   using K = Cfg<P, NS, false>;
@@ -929,7 +969,7 @@ int launch_as(const SsmParams& p, cudaStream_t stream) {
   if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, K::kBytes) !=
       cudaSuccess)
     return GDN_ERR_CUDA;
-  fn<<<grid, kThreads, K::kBytes, stream>>>(p, maps, sg, cols);
+  fn<<<grid, K::kThreads, K::kBytes, stream>>>(p, maps, sg, cols);
   return cudaGetLastError() == cudaSuccess ? 0 : GDN_ERR_CUDA;
 }
 
