@@ -31,6 +31,22 @@ def require_cuda(name: str, t: torch.Tensor, device: torch.device) -> None:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
+def require_all(device: torch.device, names: tuple, tensors: tuple) -> None:
+    """require_cuda for each tensor that is given (None: left out), quick where all is well."""
+    try:
+        if device.type == "cuda":
+            for t in tensors:
+                if t is not None and t.device != device:
+                    break
+            else:
+                return
+    except AttributeError:
+        pass
+    for name, t in zip(names, tensors):
+        if t is not None:
+            require_cuda(name, t, device)
+
+
 def as_bf16(name: str, t: torch.Tensor) -> torch.Tensor:
     if t.dtype != torch.bfloat16:
         raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
@@ -80,7 +96,14 @@ def on_device(device: torch.device):
     return _SAME if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
+# The handle of the current stream without a Stream object around it (2 us a call), where
+# this torch has it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_handle(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 

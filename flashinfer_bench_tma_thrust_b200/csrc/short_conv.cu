@@ -39,14 +39,6 @@ __device__ __forceinline__ void unpack(const Row& r, float (&v)[kVec]) {
   }
 }
 
-__device__ __forceinline__ Row pack(const float (&v)[kVec]) {
-  uint32_t u[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
-  return Row{make_uint4(u[0], u[1], u[2], u[3])};
-}
-
 // Channels [c, c + 8) of a row; with kWide one 16-byte access (the launcher has checked
 // alignment and that 8 divides every section), else one access per channel below C.
 template <bool kWide>
@@ -76,24 +68,63 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* row, int c, int C, cons
     if (c + i < C) p[c + i] = static_cast<unsigned short>(u[i >> 1] >> ((i & 1) * 16));
 }
 
-// What a thread knows of its channels.
+// What a thread knows of its channels, in pairs.
 template <int W>
 struct Taps {
-  float w[W][kVec];
-  float bias[kVec];
+  float2 w[W][kVec / 2];
+  float2 bias[kVec / 2];
 };
+
+// kN consecutive fp32 or bf16 parameters from element i on (16-byte aligned) as floats.
+template <int kN>
+__device__ __forceinline__ void load_params(const void* base, int dtype, int64_t i, float (&v)[kN]) {
+  if (dtype == kBF16) {
+    const uint4* p = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(base) + i);
+#pragma unroll
+    for (int k = 0; k < kN / 8; ++k) {
+      float f[kVec];
+      unpack(Row{p[k]}, f);
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) v[8 * k + e] = f[e];
+    }
+  } else {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + i);
+#pragma unroll
+    for (int k = 0; k < kN / 4; ++k) {
+      const float4 f = p[k];
+      v[4 * k] = f.x;
+      v[4 * k + 1] = f.y;
+      v[4 * k + 2] = f.z;
+      v[4 * k + 3] = f.w;
+    }
+  }
+}
 
 template <int W, bool kWide>
 __device__ __forceinline__ Taps<W> load_taps(const ConvParams& p, int c) {
+  float w[kVec * W], b[kVec];
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) b[i] = 0.f;
+  if (kWide) {
+    load_params(p.weight, p.weight_dtype, static_cast<int64_t>(c) * W, w);
+    if (p.bias) load_params(p.bias, p.bias_dtype, c, b);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const bool in = c + i < p.C;
+      if (in && p.bias) b[i] = load_scalar(p.bias, p.bias_dtype, c + i);
+#pragma unroll
+      for (int k = 0; k < W; ++k)
+        w[i * W + k] =
+            in ? load_scalar(p.weight, p.weight_dtype, static_cast<int64_t>(c + i) * W + k) : 0.f;
+    }
+  }
   Taps<W> t;
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) {
-    const int ch = c + i;
-    const bool in = kWide || ch < p.C;
-    t.bias[i] = p.bias && in ? load_scalar(p.bias, p.bias_dtype, ch) : 0.f;
+  for (int i = 0; i < kVec / 2; ++i) {
+    t.bias[i] = make_float2(b[2 * i], b[2 * i + 1]);
 #pragma unroll
-    for (int k = 0; k < W; ++k)
-      t.w[k][i] = in ? load_scalar(p.weight, p.weight_dtype, static_cast<int64_t>(ch) * W + k) : 0.f;
+    for (int k = 0; k < W; ++k) t.w[k][i] = make_float2(w[2 * i * W + k], w[(2 * i + 1) * W + k]);
   }
   return t;
 }
@@ -110,38 +141,61 @@ __device__ __forceinline__ Place place_of(const ConvParams& p, int c) {
   return Place{p.out[s], p.begin[s + 1] - p.begin[s], c - p.begin[s], p.normed[s]};
 }
 
-__device__ __forceinline__ float silu(float v) {
-  float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-kLog2e * v));
-  return __fdividef(v, 1.f + e);
+__device__ __forceinline__ float2 pair(uint32_t u) {
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
 
-// One output row: activation, norm of the head (16 lanes), store. All lanes of the warp call
-// it; `live` says whether this thread's channels exist.
-template <bool kWide>
-__device__ __forceinline__ void finish(const ConvParams& p, const Place& pl, int c, int64_t row,
-                                       float (&v)[kVec], bool live) {
+// v / (1 + e^-v) of two values with three MUFU operations instead of four: one reciprocal of
+// the product of the denominators. The exponent is capped at 2^63 so that the product stays
+// finite; below v = -43 the result is then -43 2^-63 and the like instead of even less.
+__device__ __forceinline__ float2 silu2(float2 v) {
+  float e0, e1, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(fminf(-kLog2e * v.x, 63.f)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(fminf(-kLog2e * v.y, 63.f)));
+  const float a = 1.f + e0, b = 1.f + e1;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
+  return make_float2(v.x * (r * b), v.y * (r * a));
+}
+
+// One output row: the taps over W rows, activation, norm of the head (16 lanes), store. All
+// lanes of the warp call it; `live` says whether this thread's channels exist.
+template <int W, bool kWide>
+__device__ __forceinline__ void output_row(const ConvParams& p, const Taps<W>& taps, const Place& pl,
+                                           int c, int64_t row, const Row* const (&in)[W],
+                                           bool live) {
+  float2 y[kVec / 2];
+#pragma unroll
+  for (int i = 0; i < kVec / 2; ++i) y[i] = taps.bias[i];
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+    const uint32_t u[4] = {in[k]->w.x, in[k]->w.y, in[k]->w.z, in[k]->w.w};
+#pragma unroll
+    for (int i = 0; i < kVec / 2; ++i) y[i] = __ffma2_rn(taps.w[k][i], pair(u[i]), y[i]);
+  }
   if (p.silu) {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) v[i] = silu(v[i]);
+    for (int i = 0; i < kVec / 2; ++i) y[i] = silu2(y[i]);
   }
   if (pl.normed) {  // the same for all 16 lanes of a head
-    float q = 0.f;
+    float2 q2 = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) q = fmaf(v[i], v[i], q);
+    for (int i = 0; i < kVec / 2; ++i) q2 = __ffma2_rn(y[i], y[i], q2);
+    float q = q2.x + q2.y;
     const uint32_t lanes = 0xffffu << (threadIdx.x & 16);
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) q += __shfl_xor_sync(lanes, q, o);
     const float r = rsqrtf(q + p.eps);
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) v[i] *= r;
+    for (int i = 0; i < kVec / 2; ++i) y[i] = __fmul2_rn(y[i], make_float2(r, r));
   }
   if (!live) return;
-  const Row r = pack(v);
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(y[i].y), "f"(y[i].x));
   if (kWide) {
-    *reinterpret_cast<uint4*>(pl.out + row * pl.width + pl.at) = r.w;
+    *reinterpret_cast<uint4*>(pl.out + row * pl.width + pl.at) = make_uint4(u[0], u[1], u[2], u[3]);
   } else {
-    const uint32_t u[4] = {r.w.x, r.w.y, r.w.z, r.w.w};
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
       if (c + i >= p.C) break;
@@ -174,7 +228,7 @@ __device__ __forceinline__ int64_t bound(const ConvParams& p, int64_t i) {
 
 // Prompts. Blocks [0, tiles) of grid.y take `run` tokens each; the N behind them write one
 // sequence's new state (its last W-1 inputs, from the state where it is shorter).
-constexpr int kAhead = 8;  // rows loaded before the first is used
+constexpr int kAhead = 4;  // rows per batch; the next batch's are loaded meanwhile
 
 template <int W, bool kWide>
 __global__ void __launch_bounds__(kThreads) conv_prefill_kernel(const __grid_constant__ ConvParams p,
@@ -218,29 +272,51 @@ __global__ void __launch_bounds__(kThreads) conv_prefill_kernel(const __grid_con
   const Taps<W> taps = load_taps<W, kWide>(p, cl);
   Place pl = place_of(p, cl);
   if (!live) pl.normed = 0;  // no lane waits in the head's shuffles for one without channels
-  float win[W - 1][kVec];  // the W-1 rows before the token
+  // rows[0 .. W-2]: the W-1 rows before the batch; behind them the batch's own
+  Row rows[W - 1 + kAhead];
+  const Row zero{make_uint4(0u, 0u, 0u, 0u)};
 #pragma unroll
-  for (int r = 0; r < W - 1; ++r) {
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) win[r][i] = 0.f;
-  }
+  for (int r = 0; r < W - 1; ++r) rows[r] = zero;
   if (n < p.N && start < t0) {  // the tile begins inside a sequence
 #pragma unroll
     for (int r = 0; r < W - 1; ++r) {
       const int64_t u = t0 - (W - 1) + r;
       if (u >= start) {
-        unpack(load_row<kWide>(p.x + u * p.x_stride, cl, p.C), win[r]);
+        rows[r] = load_row<kWide>(p.x + u * p.x_stride, cl, p.C);
       } else if (p.state) {
-        unpack(load_row<kWide>(p.state + (n * (W - 1) + (u - start) + (W - 1)) * p.C, cl, p.C), win[r]);
+        rows[r] = load_row<kWide>(p.state + (n * (W - 1) + (u - start) + (W - 1)) * p.C, cl, p.C);
       }
     }
   }
+  Row next[kAhead];  // the batch after, on its way
+#pragma unroll
+  for (int a = 0; a < kAhead; ++a)
+    next[a] = load_row<kWide>(p.x + min(t0 + a, p.T - 1) * p.x_stride, cl, p.C);
   for (int64_t tb = t0; tb < t1; tb += kAhead) {
-    Row rows[kAhead];
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a)
-      rows[a] = load_row<kWide>(p.x + min(tb + a, p.T - 1) * p.x_stride, cl, p.C);
+    for (int a = 0; a < kAhead; ++a) rows[W - 1 + a] = next[a];
+    if (tb + kAhead < t1) {
 #pragma unroll
+      for (int a = 0; a < kAhead; ++a)
+        next[a] = load_row<kWide>(p.x + min(tb + kAhead + a, p.T - 1) * p.x_stride, cl, p.C);
+    }
+    if (n < p.N && start < tb && tb + kAhead <= min(end, t1)) {
+      // all of the batch and the rows before it lie in one sequence
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        const Row* in[W];
+#pragma unroll
+        for (int k = 0; k < W; ++k) in[k] = &rows[a + k];
+        output_row<W, kWide>(p, taps, pl, cl, tb + a, in, live);
+      }
+#pragma unroll
+      for (int r = 0; r < W - 1; ++r) rows[r] = rows[kAhead + r];
+      continue;
+    }
+    Row win[W];  // token by token, over the sequences' bounds
+#pragma unroll
+    for (int r = 0; r < W - 1; ++r) win[r] = rows[r];
+#pragma unroll 1
     for (int a = 0; a < kAhead; ++a) {
       const int64_t t = tb + a;
       if (t >= t1) break;
@@ -255,72 +331,66 @@ __global__ void __launch_bounds__(kThreads) conv_prefill_kernel(const __grid_con
       if (n >= p.N || t < start) continue;  // a token of no sequence
       if (t == start) {
 #pragma unroll
-        for (int r = 0; r < W - 1; ++r) {
-          Row v{make_uint4(0u, 0u, 0u, 0u)};
-          if (p.state) v = load_row<kWide>(p.state + (n * (W - 1) + r) * p.C, cl, p.C);
-          unpack(v, win[r]);
-        }
+        for (int r = 0; r < W - 1; ++r)
+          win[r] = p.state ? load_row<kWide>(p.state + (n * (W - 1) + r) * p.C, cl, p.C) : zero;
       }
-      float cur[kVec], y[kVec];
-      unpack(rows[a], cur);
+      win[W - 1] = load_row<kWide>(p.x + t * p.x_stride, cl, p.C);  // (again: a is no constant)
+      const Row* in[W];
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        float s = taps.bias[i];
+      for (int k = 0; k < W; ++k) in[k] = &win[k];
+      output_row<W, kWide>(p, taps, pl, cl, t, in, live);
 #pragma unroll
-        for (int k = 0; k < W - 1; ++k) s = fmaf(taps.w[k][i], win[k][i], s);
-        y[i] = fmaf(taps.w[W - 1][i], cur[i], s);
-      }
-#pragma unroll
-      for (int r = 0; r + 1 < W - 1; ++r) {
-#pragma unroll
-        for (int i = 0; i < kVec; ++i) win[r][i] = win[r + 1][i];
-      }
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) win[W - 2][i] = cur[i];
-      finish<kWide>(p, pl, cl, t, y, live);
+      for (int r = 0; r < W - 1; ++r) win[r] = win[r + 1];
     }
+#pragma unroll
+    for (int r = 0; r < W - 1; ++r) rows[r] = win[r];
   }
 }
 
 // One token per sequence: each thread reads its 8 channels of the W-1 state rows and of x,
 // and writes the rows moved up by one, so the new state may be the old one's memory.
 template <int W, bool kWide>
-__global__ void __launch_bounds__(kThreads) conv_decode_kernel(const __grid_constant__ ConvParams p) {
+__global__ void __launch_bounds__(kThreads) conv_decode_kernel(const __grid_constant__ ConvParams p,
+                                                              int per_thread) {
   const int c = (blockIdx.x * kThreads + threadIdx.x) * kVec;
   const bool live = c < p.C;
-  const int64_t n = blockIdx.y + static_cast<int64_t>(blockIdx.z) * gridDim.y;
-  if (n >= p.N) return;
+  const int64_t by = blockIdx.y + static_cast<int64_t>(blockIdx.z) * gridDim.y;
+  const int64_t n0 = by * per_thread, n1 = min(n0 + per_thread, p.N);
+  if (n0 >= p.N) return;
   const int cl = live ? c : 0;
-  Row rows[W];
+  auto load = [&](int64_t n, Row(&rows)[W]) {
 #pragma unroll
-  for (int r = 0; r < W - 1; ++r)
-    rows[r] = p.state ? load_row<kWide>(p.state + (n * (W - 1) + r) * p.C, cl, p.C)
-                      : Row{make_uint4(0u, 0u, 0u, 0u)};
-  rows[W - 1] = load_row<kWide>(p.x + n * p.x_stride, cl, p.C);
+    for (int r = 0; r < W - 1; ++r)
+      rows[r] = p.state ? load_row<kWide>(p.state + (n * (W - 1) + r) * p.C, cl, p.C)
+                        : Row{make_uint4(0u, 0u, 0u, 0u)};
+    rows[W - 1] = load_row<kWide>(p.x + n * p.x_stride, cl, p.C);
+  };
+  Row next[W];
+  load(n0, next);
   const Taps<W> taps = load_taps<W, kWide>(p, cl);
   Place pl = place_of(p, cl);
   if (!live) pl.normed = 0;
-  float y[kVec];
+  for (int64_t n = n0; n < n1; ++n) {
+    Row rows[W];
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) y[i] = taps.bias[i];
+    for (int r = 0; r < W; ++r) rows[r] = next[r];
+    if (n + 1 < n1) load(n + 1, next);
+    if (live) {
 #pragma unroll
-  for (int k = 0; k < W; ++k) {
-    float v[kVec];
-    unpack(rows[k], v);
+      for (int r = 0; r < W - 1; ++r)
+        store_row<kWide>(p.new_state + (n * (W - 1) + r) * p.C, c, p.C, rows[r + 1]);
+    }
+    const Row* in[W];
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) y[i] = fmaf(taps.w[k][i], v[i], y[i]);
+    for (int k = 0; k < W; ++k) in[k] = &rows[k];
+    output_row<W, kWide>(p, taps, pl, cl, n, in, live);
   }
-  if (live) {
-#pragma unroll
-    for (int r = 0; r < W - 1; ++r)
-      store_row<kWide>(p.new_state + (n * (W - 1) + r) * p.C, c, p.C, rows[r + 1]);
-  }
-  finish<kWide>(p, pl, cl, n, y, live);
 }
 
 bool wide_ok(const ConvParams& p) {
   auto al = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; };
-  if (!al(p.x) || p.x_stride % kVec || p.C % kVec || !al(p.new_state) || (p.state && !al(p.state)))
+  if (!al(p.x) || p.x_stride % kVec || p.C % kVec || !al(p.new_state) || (p.state && !al(p.state)) ||
+      !al(p.weight) || (p.bias && !al(p.bias)))
     return false;
   for (int s = 0; s < p.sections; ++s)
     if (p.begin[s + 1] % kVec || !al(p.out[s])) return false;
@@ -338,7 +408,7 @@ int prefill_w(const ConvParams& p, cudaStream_t stream) {
   const unsigned bx = (p.C + kThreads * kVec - 1) / (kThreads * kVec);
   // A run of `run` tokens reads W-1 rows again; short runs fill the SMs for short prompts.
   int run = 64;
-  while (run > kAhead && bx * ((p.T + run - 1) / run) < 148 * 8) run /= 2;
+  while (run > 8 && bx * ((p.T + run - 1) / run) < 148 * 8) run /= 2;
   const int64_t tiles = (p.T + run - 1) / run;
   const int64_t rows = tiles + p.N;
   if (rows > (int64_t{1} << 30)) return GDN_ERR_UNSUPPORTED_SHAPE;
@@ -355,11 +425,14 @@ template <int W>
 int decode_w(const ConvParams& p, cudaStream_t stream) {
   const unsigned bx = (p.C + kThreads * kVec - 1) / (kThreads * kVec);
   if (p.N > (int64_t{1} << 30)) return GDN_ERR_UNSUPPORTED_SHAPE;
-  const dim3 grid = rows_grid(bx, p.N);
+  // Several sequences per thread share the load of its taps once the grid covers the SMs.
+  int per_thread = 1;
+  while (per_thread < 8 && bx * (p.N / (2 * per_thread)) >= 148 * 8) per_thread *= 2;
+  const dim3 grid = rows_grid(bx, (p.N + per_thread - 1) / per_thread);
   if (wide_ok(p)) {
-    conv_decode_kernel<W, true><<<grid, kThreads, 0, stream>>>(p);
+    conv_decode_kernel<W, true><<<grid, kThreads, 0, stream>>>(p, per_thread);
   } else {
-    conv_decode_kernel<W, false><<<grid, kThreads, 0, stream>>>(p);
+    conv_decode_kernel<W, false><<<grid, kThreads, 0, stream>>>(p, per_thread);
   }
   return cudaGetLastError() == cudaSuccess ? 0 : GDN_ERR_CUDA;
 }

@@ -80,14 +80,16 @@ __device__ __forceinline__ float bf16_at(const __nv_bfloat16* p) {
 }
 
 // ---------------------------------------------------------------- one token per sequence
-// HBM bounds it: the state goes through once (5 flop per 8 bytes). A warp has kRows loads
-// of kPer rows each in flight before it reduces any of them. Blocks of 4 warps share a
-// head's rows (p.P rows over `splits` blocks).
+// HBM bounds it: the state goes through once (5 flop per 8 bytes). A warp takes kRows * kPer
+// rows (at most 32: lane r holds x and y of row r) with all its loads in flight before it
+// reduces any of them. Blocks of 4 warps share a head's rows, `splits` blocks a head.
 template <typename S, int kLanes, int kPieces, int kRows>
 __global__ void __launch_bounds__(128) ssm_decode_kernel(const __grid_constant__ SsmParams p,
-                                                        int splits, int rows_per_warp) {
+                                                        int splits) {
   constexpr int kE = Piece<S>::kE;
   constexpr int kPer = 32 / kLanes;  // rows per load
+  constexpr int kWarpRows = kRows * kPer;
+  static_assert(kWarpRows <= 32, "");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int l = lane % kLanes, sub = lane / kLanes;
   const int64_t head = blockIdx.x / splits;  // flattened (sequence, head)
@@ -95,10 +97,25 @@ __global__ void __launch_bounds__(128) ssm_decode_kernel(const __grid_constant__
   const int64_t n = head / p.H;
   const int h = static_cast<int>(head - n * p.H);
   const int64_t grp = n * p.G + h / (p.H / p.G);
-  const int row0 = (split * 4 + warp) * rows_per_warp;
-  const int row1 = min(row0 + rows_per_warp, p.P);
-  if (row0 >= row1) return;
+  const int row0 = (split * 4 + warp) * kWarpRows;
+  if (row0 >= p.P) return;
 
+  float s[kRows][kPieces][kE];
+  const int64_t at0 = (head * p.P + row0 + sub) * p.Ns + l * kE;
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) {
+      if (p.state && row0 + i * kPer + sub < p.P) {
+        Piece<S>::load(p.state, at0 + i * kPer * p.Ns + j * kLanes * kE, s[i][j]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < kE; ++k) s[i][j][k] = 0.f;
+      }
+    }
+  }
+  const bool own = lane < kWarpRows && row0 + lane < p.P;
+  const float x_lane = own ? bf16_at(p.x + head * p.P + row0 + lane) : 0.f;
   const float v = load_scalar(p.dt, p.dt_dtype, head) + load_scalar(p.dt_bias, p.dt_bias_dtype, h);
   const float d = softplus_ref(v);
   const float g = expf(-expf(load_scalar(p.A_log, p.A_log_dtype, h)) * d);
@@ -114,47 +131,29 @@ __global__ void __launch_bounds__(128) ssm_decode_kernel(const __grid_constant__
   }
   bc = row_sum<kLanes>(bc);
 
-  for (int r0 = row0; r0 < row1; r0 += kRows * kPer) {
-    float s[kRows][kPieces][kE];
-    float x[kRows];
+  float y = 0.f;
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const int r = r0 + i * kPer + sub;
-      const bool in = r < row1;
-      const int64_t at = (head * p.P + r) * p.Ns + l * kE;
+  for (int i = 0; i < kRows; ++i) {
+    const float dx = d * __shfl_sync(0xffffffffu, x_lane, i * kPer + sub);
+    float dot = 0.f;
 #pragma unroll
-      for (int j = 0; j < kPieces; ++j) {
-        if (in && p.state) {
-          Piece<S>::load(p.state, at + j * kLanes * kE, s[i][j]);
-        } else {
+    for (int j = 0; j < kPieces; ++j) {
+      float w[kE];
 #pragma unroll
-          for (int k = 0; k < kE; ++k) s[i][j][k] = 0.f;
-        }
+      for (int k = 0; k < kE; ++k) {
+        dot = fmaf(s[i][j][k], c[j][k], dot);
+        w[k] = fmaf(g, s[i][j][k], dx * b[j][k]);
       }
-      x[i] = in ? bf16_at(p.x + head * p.P + r) : 0.f;
+      if (row0 + i * kPer + sub < p.P)
+        Piece<S>::store(p.new_state, at0 + i * kPer * p.Ns + j * kLanes * kE, w);
     }
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const int r = r0 + i * kPer + sub;
-      const bool in = r < row1;
-      const int64_t at = (head * p.P + r) * p.Ns + l * kE;
-      const float dx = d * x[i];
-      float dot = 0.f;
-#pragma unroll
-      for (int j = 0; j < kPieces; ++j) {
-        float w[kE];
-#pragma unroll
-        for (int k = 0; k < kE; ++k) {
-          dot = fmaf(s[i][j][k], c[j][k], dot);
-          w[k] = fmaf(g, s[i][j][k], dx * b[j][k]);
-        }
-        if (in) Piece<S>::store(p.new_state, at + j * kLanes * kE, w);
-      }
-      dot = row_sum<kLanes>(dot);
-      if (in && l == 0)
-        p.out[head * p.P + r] = __float2bfloat16_rn(fmaf(g, dot, fmaf(dx, bc, skip * x[i])));
-    }
+    dot = row_sum<kLanes>(dot);
+    const float yi = fmaf(g, dot, dx * bc);
+    // row i * kPer + (lane % kPer) is in the lanes of that sub
+    const float mine = kPer == 1 ? yi : __shfl_sync(0xffffffffu, yi, (lane % kPer) * kLanes);
+    if (lane / kPer == i) y = mine;
   }
+  if (own) p.out[head * p.P + row0 + lane] = __float2bfloat16_rn(fmaf(skip, x_lane, y));
 }
 
 // ---------------------------------------------------------------- prompts, token by token
@@ -262,14 +261,12 @@ __global__ void __launch_bounds__(128) ssm_recurrent_kernel(const __grid_constan
 
 template <typename S, int kLanes, int kPieces, int kRows>
 int decode_as(const SsmParams& p, cudaStream_t stream) {
-  constexpr int kPer = 32 / kLanes;
+  constexpr int kBlockRows = 4 * kRows * (32 / kLanes);
   const int64_t heads = p.N * p.H;
-  // Rows per warp: a whole load batch, more warps per head while the grid leaves SMs idle.
-  int splits = (p.P + 4 * kRows * kPer - 1) / (4 * kRows * kPer);
-  const int rows_per_warp = (p.P + splits * 4 - 1) / (splits * 4);
+  const int splits = (p.P + kBlockRows - 1) / kBlockRows;
   if (heads * splits > 0x7fffffffLL) return GDN_ERR_UNSUPPORTED_SHAPE;
   ssm_decode_kernel<S, kLanes, kPieces, kRows>
-      <<<static_cast<unsigned>(heads * splits), 128, 0, stream>>>(p, splits, rows_per_warp);
+      <<<static_cast<unsigned>(heads * splits), 128, 0, stream>>>(p, splits);
   return cudaGetLastError() == cudaSuccess ? 0 : GDN_ERR_CUDA;
 }
 
@@ -289,7 +286,7 @@ int recurrent_as(const SsmParams& p, cudaStream_t stream) {
 int launch_ssm_decode(const SsmParams& p, cudaStream_t stream) {
   if (p.state_bf16) {
     switch (p.Ns) {
-      case 16: return decode_as<__nv_bfloat16, 2, 1, 4>(p, stream);
+      case 16: return decode_as<__nv_bfloat16, 2, 1, 2>(p, stream);
       case 32: return decode_as<__nv_bfloat16, 4, 1, 4>(p, stream);
       case 64: return decode_as<__nv_bfloat16, 8, 1, 4>(p, stream);
       case 128: return decode_as<__nv_bfloat16, 16, 1, 4>(p, stream);
@@ -298,7 +295,7 @@ int launch_ssm_decode(const SsmParams& p, cudaStream_t stream) {
     return GDN_ERR_UNSUPPORTED_SHAPE;
   }
   switch (p.Ns) {
-    case 16: return decode_as<float, 4, 1, 8>(p, stream);
+    case 16: return decode_as<float, 4, 1, 4>(p, stream);
     case 32: return decode_as<float, 8, 1, 8>(p, stream);
     case 64: return decode_as<float, 16, 1, 8>(p, stream);
     case 128: return decode_as<float, 32, 1, 8>(p, stream);

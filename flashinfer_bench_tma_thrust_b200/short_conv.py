@@ -30,6 +30,7 @@ call on a device allocates its status words: make it before a stream capture.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -39,29 +40,29 @@ from . import _lib, _status
 MAX_SECTIONS = 8
 
 
+_NAMES = ("x", "weight", "bias", "state", "cu_seqlens")
+
+
 def _taps(x, weight, bias):
-    """(weight, code, bias, code, C, W), checked."""
-    dev, ch = x.device, x.shape[-1]
-    C.require_cuda("weight", weight, dev)
+    """(weight, code, bias, code, W), checked."""
+    ch = x.shape[-1]
     if weight.dim() == 3 and weight.shape[1] == 1:
         weight = weight[:, 0]
-    if weight.dim() != 2 or weight.shape[0] != ch or not 2 <= weight.shape[1] <= 4:
-        raise ValueError(f"weight must be [{ch}, W] with 2 to 4 taps, got {tuple(weight.shape)}")
+    shape = weight.shape
+    if len(shape) != 2 or shape[0] != ch or not 2 <= shape[1] <= 4:
+        raise ValueError(f"weight must be [{ch}, W] with 2 to 4 taps, got {tuple(shape)}")
     w, w_t = C.as_gate("weight", weight)
-    b, b_t = None, 0
-    if bias is not None:
-        C.require_cuda("bias", bias, dev)
-        if tuple(bias.shape) != (ch,):
-            raise ValueError(f"bias must be [{ch}], got {tuple(bias.shape)}")
-        b, b_t = C.as_gate("bias", bias)
-    return w, w_t, b, b_t, ch, weight.shape[1]
+    if bias is None:
+        return w, w_t, None, 0, shape[1]
+    if bias.shape != (ch,):
+        raise ValueError(f"bias must be [{ch}], got {tuple(bias.shape)}")
+    return w, w_t, *C.as_gate("bias", bias), shape[1]
 
 
-def _state(state, shape, dev):
+def _state(state, shape):
     if state is None:
         return None
-    C.require_cuda("state", state, dev)
-    if tuple(state.shape) != shape:
+    if state.shape != shape:
         raise ValueError(f"state must be {list(shape)}, got {tuple(state.shape)}")
     return C.as_bf16("state", state)
 
@@ -74,7 +75,10 @@ def _rows(x):
     return x if x.stride(-1) == 1 else x.contiguous()
 
 
+@functools.lru_cache(maxsize=256)
 def _sections(ch, split, l2norm):
+    """(widths, the library's arrays of widths and norms), checked; `split` and `l2norm` as the
+    caller gave them, sequences as tuples."""
     widths = (ch,) if split is None else tuple(int(w) for w in split)
     if not 1 <= len(widths) <= MAX_SECTIONS or min(widths) <= 0 or sum(widths) != ch:
         raise ValueError(f"split must be 1 to {MAX_SECTIONS} positive widths summing to {ch}, "
@@ -91,7 +95,12 @@ def _sections(ch, split, l2norm):
             raise ValueError("a section with l2norm must begin at and span whole heads of "
                              f"{C.HEAD_DIM} channels, got begin {at}, width {w}")
         at += w
-    return widths, normed
+    i32 = ctypes.c_int32 * len(widths)
+    return widths, i32(*widths), i32(*normed), ctypes.c_void_p * len(widths)
+
+
+def _hashable(v):
+    return v if v is None or isinstance(v, (bool, tuple)) else tuple(v)
 
 
 def _activation(activation) -> int:
@@ -102,13 +111,6 @@ def _activation(activation) -> int:
     raise ValueError(f"activation must be 'silu' or None, got {activation!r}")
 
 
-def _outputs(lead, widths, normed, dev):
-    k = len(widths)
-    outs = [torch.empty(*lead, w, dtype=torch.bfloat16, device=dev) for w in widths]
-    i32 = ctypes.c_int32 * k
-    return outs, i32(*widths), i32(*normed), (ctypes.c_void_p * k)(*[o.data_ptr() for o in outs])
-
-
 def prefill(x, weight, bias=None, state=None, cu_seqlens=None, *, activation="silu", split=None,
             l2norm=None, eps=1e-6, check=False):
     """The convolution over packed prompts: (output [T, C] or a tuple of sections, new_state
@@ -116,28 +118,29 @@ def prefill(x, weight, bias=None, state=None, cu_seqlens=None, *, activation="si
     next call on the device, or at this one with ``check=True`` (which synchronises)."""
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
         raise ValueError("x must be a [T, C] tensor")
-    dev = x.device
-    C.require_cuda("x", x, dev)
-    w, w_t, b, b_t, ch, taps = _taps(x, weight, bias)
     if cu_seqlens is None:
         raise ValueError("cu_seqlens is required")
-    C.require_cuda("cu_seqlens", cu_seqlens, dev)
+    dev = x.device
+    C.require_all(dev, _NAMES, (x, weight, bias, state, cu_seqlens))
+    w, w_t, b, b_t, taps = _taps(x, weight, bias)
+    ch = x.shape[-1]
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
         raise ValueError("cu_seqlens must be a 1-D tensor of length num_seqs + 1")
     cu, cu_t = C.as_index("cu_seqlens", cu_seqlens)
     n, t = cu.numel() - 1, x.shape[0]
-    s = _state(state, (n, taps - 1, ch), dev)
+    s = _state(state, (n, taps - 1, ch))
     x = _rows(x)
-    widths, normed = _sections(ch, split, l2norm)
+    widths, wa, na, pointers = _sections(ch, _hashable(split), _hashable(l2norm))
     act = _activation(activation)
     lib = _lib.load()
     with C.on_device(dev):
         status = _status.address(dev.index)
-        outs, wa, na, oa = _outputs((t,), widths, normed, dev)
+        outs = [torch.empty(t, v, dtype=torch.bfloat16, device=dev) for v in widths]
         new_state = torch.empty(n, taps - 1, ch, dtype=torch.bfloat16, device=dev)
         rc = lib.gdn_conv_prefill_fwd(
             x.data_ptr(), x.stride(0), w.data_ptr(), w_t, C.ptr(b), b_t, C.ptr(s), cu.data_ptr(),
-            cu_t, act, len(widths), wa, na, eps, oa, new_state.data_ptr(), t, n, ch, taps, status,
+            cu_t, act, len(widths), wa, na, eps, pointers(*[o.data_ptr() for o in outs]),
+            new_state.data_ptr(), t, n, ch, taps, status,
             C.stream_handle(dev))
         _lib.check(rc, "gdn_conv_prefill_fwd")
         _status.finish(dev.index, check)
@@ -148,21 +151,23 @@ def _decode(x, weight, bias, state, activation, split, l2norm, eps, inplace):
     if not isinstance(x, torch.Tensor) or x.dim() != 3 or x.shape[1] != 1:
         raise ValueError("x must be a [B, 1, C] tensor")
     dev = x.device
-    C.require_cuda("x", x, dev)
-    w, w_t, b, b_t, ch, taps = _taps(x, weight, bias)
+    C.require_all(dev, _NAMES, (x, weight, bias, state, None))
+    w, w_t, b, b_t, taps = _taps(x, weight, bias)
+    ch = x.shape[-1]
     n = x.shape[0]
-    s = _state(state, (n, taps - 1, ch), dev)
+    s = _state(state, (n, taps - 1, ch))
     x = _rows(x)
-    widths, normed = _sections(ch, split, l2norm)
+    widths, wa, na, pointers = _sections(ch, _hashable(split), _hashable(l2norm))
     act = _activation(activation)
     lib = _lib.load()
     with C.on_device(dev):
-        outs, wa, na, oa = _outputs((n, 1), widths, normed, dev)
+        outs = [torch.empty(n, 1, v, dtype=torch.bfloat16, device=dev) for v in widths]
         new_state = state if inplace else \
             torch.empty(n, taps - 1, ch, dtype=torch.bfloat16, device=dev)
         rc = lib.gdn_conv_decode_fwd(
             x.data_ptr(), x.stride(0), w.data_ptr(), w_t, C.ptr(b), b_t, C.ptr(s), act,
-            len(widths), wa, na, eps, oa, new_state.data_ptr(), n, ch, taps, C.stream_handle(dev))
+            len(widths), wa, na, eps, pointers(*[o.data_ptr() for o in outs]),
+            new_state.data_ptr(), n, ch, taps, C.stream_handle(dev))
     _lib.check(rc, "gdn_conv_decode_fwd")
     return (outs[0] if split is None else tuple(outs)), new_state
 

@@ -39,58 +39,64 @@ def _aligned(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _vector(name, t, h, dev):
-    K.require_cuda(name, t, dev)
-    if tuple(t.shape) != (h,):
-        raise ValueError(f"{name} must be [{h}], got {tuple(t.shape)}")
+_NAMES = ("x", "dt", "A_log", "B", "C", "D", "dt_bias", "state", "cu_seqlens")
+
+
+def _gate(name, t, shape):
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {tuple(t.shape)}")
     return K.as_gate(name, t)
 
 
-def _args(x, dt, A_log, B, C, D, dt_bias, lead: int) -> _Args:
+def _args(x, dt, A_log, B, C, D, dt_bias, state, cu, lead: int) -> _Args:
     """Checks shared by prompts (lead = 1) and tokens (lead = 2: [B, 1, ...])."""
     a = _Args()
-    if not isinstance(x, torch.Tensor) or x.dim() != lead + 2 or (lead == 2 and x.shape[1] != 1):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"x must be a torch.Tensor, got {type(x).__name__}")
+    dev, shape = x.device, tuple(x.shape)
+    if len(shape) != lead + 2 or (lead == 2 and shape[1] != 1):
         raise ValueError("x must be a %s tensor" % ("[T, H, P]" if lead == 1 else "[B, 1, H, P]"))
-    dev = x.device
-    for name, t in (("x", x), ("dt", dt), ("B", B), ("C", C)):
-        K.require_cuda(name, t, dev)
-    head = tuple(x.shape[:lead])
-    a.dev, a.T, a.H, a.P = dev, x.shape[0], x.shape[-2], x.shape[-1]
-    if B.dim() != lead + 2 or tuple(B.shape[:lead]) != head or B.shape != C.shape:
-        raise ValueError(f"B and C must be {list(head)} + [G, Ns], got {tuple(B.shape)} and "
+    K.require_all(dev, _NAMES, (x, dt, A_log, B, C, D, dt_bias, state, cu))
+    of_b, head = tuple(B.shape), shape[:lead]
+    T, H, P = shape[0], shape[-2], shape[-1]
+    if len(of_b) != lead + 2 or of_b[:lead] != head or C.shape != of_b:
+        raise ValueError(f"B and C must be {list(head)} + [G, Ns], got {of_b} and "
                          f"{tuple(C.shape)}")
-    a.G, a.Ns = B.shape[-2], B.shape[-1]
-    if a.Ns not in STATE_DIMS:
-        raise ValueError(f"the state size must be one of {STATE_DIMS}, got {a.Ns}")
-    if not 1 <= a.P <= MAX_HEAD_DIM:
-        raise ValueError(f"the head size must be 1 to {MAX_HEAD_DIM}, got {a.P}")
-    if a.G <= 0 or a.H <= 0 or a.H % a.G:
-        raise ValueError(f"num_heads ({a.H}) must be a positive multiple of num_groups ({a.G})")
-    if tuple(dt.shape) != head + (a.H,):
-        raise ValueError(f"dt must be {list(head) + [a.H]}, got {tuple(dt.shape)}")
-    a.x = K.as_bf16("x", x)
-    a.B, a.C = _aligned(K.as_bf16("B", B)), _aligned(K.as_bf16("C", C))
-    a.dt, a.dt_t = K.as_gate("dt", dt)
-    a.A, a.A_t = _vector("A_log", A_log, a.H, dev)
-    a.dtb, a.dtb_t = _vector("dt_bias", dt_bias, a.H, dev)
-    a.D, a.D_t = (None, 0) if D is None else _vector("D", D, a.H, dev)
+    G, Ns = of_b[-2], of_b[-1]
+    if Ns not in STATE_DIMS:
+        raise ValueError(f"the state size must be one of {STATE_DIMS}, got {Ns}")
+    if not 1 <= P <= MAX_HEAD_DIM:
+        raise ValueError(f"the head size must be 1 to {MAX_HEAD_DIM}, got {P}")
+    if G <= 0 or H <= 0 or H % G:
+        raise ValueError(f"num_heads ({H}) must be a positive multiple of num_groups ({G})")
+    a.dev, a.T, a.H, a.P, a.G, a.Ns = dev, T, H, P, G, Ns
+    a.x, a.B, a.C = K.as_bf16("x", x), K.as_bf16("B", B), K.as_bf16("C", C)
+    if (a.B.data_ptr() | a.C.data_ptr()) % 16:
+        a.B, a.C = _aligned(a.B), _aligned(a.C)
+    a.dt, a.dt_t = _gate("dt", dt, head + (H,))
+    vec = (H,)
+    a.A, a.A_t = _gate("A_log", A_log, vec)
+    a.dtb, a.dtb_t = _gate("dt_bias", dt_bias, vec)
+    a.D, a.D_t = (None, 0) if D is None else _gate("D", D, vec)
     return a
 
 
 def _prefill_args(x, dt, A_log, B, C, D, dt_bias, state, cu_seqlens) -> _Args:
-    a = _args(x, dt, A_log, B, C, D, dt_bias, 1)
-    K.require_cuda("cu_seqlens", cu_seqlens, a.dev)
+    if cu_seqlens is None:
+        raise ValueError("cu_seqlens is required")
+    a = _args(x, dt, A_log, B, C, D, dt_bias, state, cu_seqlens, 1)
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
         raise ValueError("cu_seqlens must be a 1-D tensor of length num_seqs + 1")
     a.cu, a.cu_t = K.as_index("cu_seqlens", cu_seqlens)
     a.N = a.cu.numel() - 1
     a.state = None
     if state is not None:
-        K.require_cuda("state", state, a.dev)
-        if tuple(state.shape) != (a.N, a.H, a.P, a.Ns):
+        if state.shape != (a.N, a.H, a.P, a.Ns):
             raise ValueError(f"state must be [{a.N}, {a.H}, {a.P}, {a.Ns}], "
                              f"got {tuple(state.shape)}")
-        a.state = _aligned(state.float().contiguous())
+        if state.dtype != torch.float32:
+            state = state.float()
+        a.state = _aligned(state.contiguous())
     return a
 
 
@@ -138,12 +144,11 @@ def prefill(x, dt, A_log, B, C, D, dt_bias, state, cu_seqlens, *, check=False):
 
 
 def _decode(x, dt, A_log, B, C, D, dt_bias, state, inplace):
-    a = _args(x, dt, A_log, B, C, D, dt_bias, 2)
+    a = _args(x, dt, A_log, B, C, D, dt_bias, state, None, 2)
     shape = (a.T, a.H, a.P, a.Ns)
     s = state
     if state is not None:
-        K.require_cuda("state", state, a.dev)
-        if tuple(state.shape) != shape:
+        if state.shape != shape:
             raise ValueError(f"state must be {list(shape)}, got {tuple(state.shape)}")
         if not inplace:
             if s.dtype not in (torch.float32, torch.bfloat16):
@@ -153,7 +158,7 @@ def _decode(x, dt, A_log, B, C, D, dt_bias, state, inplace):
     lib = _lib.load()
     with K.on_device(a.dev):
         out = torch.empty(a.T, 1, a.H, a.P, dtype=torch.bfloat16, device=a.dev)
-        new_state = state if inplace else torch.empty(shape, dtype=s_dtype, device=a.dev)
+        new_state = state if inplace else torch.empty(*shape, dtype=s_dtype, device=a.dev)
         rc = lib.gdn_ssm_decode_fwd(
             a.x.data_ptr(), a.dt.data_ptr(), a.dt_t, a.A.data_ptr(), a.A_t, a.B.data_ptr(),
             a.C.data_ptr(), K.ptr(a.D), a.D_t, a.dtb.data_ptr(), a.dtb_t, K.ptr(s),

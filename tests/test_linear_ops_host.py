@@ -121,7 +121,7 @@ def test_cpu_tensors_are_refused():
 def any_device(monkeypatch):
     """Let CPU tensors through the device check: everything refused below is refused before
     the launch."""
-    monkeypatch.setattr(_checks, "require_cuda", lambda name, t, device: None)
+    monkeypatch.setattr(_checks, "require_all", lambda device, names, tensors: None)
 
 
 def _bf(*shape):
