@@ -8,12 +8,15 @@
 // and in a normed section every head of 128 channels is divided by sqrt(sum y^2 + eps).
 // 2 W flop stand against 4 bytes of traffic per element, so HBM bounds it: each input is
 // read once, a run of tokens per thread keeps the last W-1 rows in registers, and the
-// outputs leave in 16-byte stores, each section to its own dense tensor (what the operators
+// outputs leave in vector stores, each section to its own dense tensor (what the operators
 // behind it take) with no pass of its own for split, silu or norm.
 //
-// A thread owns 8 adjacent channels (16 bytes of a row), so a head is 16 lanes of a warp and
-// its norm four shuffles. Sums are fp32; silu takes ex2.approx and an approximate division
-// (a few fp32 ulp, far below the bf16 rounding of the output, the only other one).
+// A thread owns 8 adjacent channels (16 bytes of a row), so a head is 16 lanes. For prompts its
+// rows arrive by asynchronous copies in a ring of its own in shared memory, 12 to 16 rows ahead:
+// with rows in flight in registers (4 per thread, 16 warps per SM) HBM's latency was not
+// covered. No thread waits for another. Sums are fp32; silu takes ex2.approx and a shared
+// approximate reciprocal (a few fp32 ulp, far below the bf16 rounding of the output, the only
+// other one).
 #include "gdn_b200.h"
 #include "gdn_common.cuh"
 #include "ssm_launch.h"
@@ -23,6 +26,7 @@ namespace {
 
 constexpr int kVec = 8;         // channels per thread
 constexpr int kThreads = 128;   // 1024 channels per block
+constexpr int kP = kVec / 2;    // pairs of channels
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Eight channels of one row as stored.
@@ -30,13 +34,14 @@ struct Row {
   uint4 w;
 };
 
-__device__ __forceinline__ void unpack(const Row& r, float (&v)[kVec]) {
-  const uint32_t u[4] = {r.w.x, r.w.y, r.w.z, r.w.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(u[i] << 16);
-    v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-  }
+__device__ __forceinline__ float2 pair(uint32_t u) {
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+__device__ __forceinline__ void pairs(const Row& r, float2 (&v)[kP]) {
+  v[0] = pair(r.w.x);
+  v[1] = pair(r.w.y);
+  v[2] = pair(r.w.z);
+  v[3] = pair(r.w.w);
 }
 
 // Channels [c, c + 8) of a row; with kWide one 16-byte access (the launcher has checked
@@ -45,9 +50,9 @@ template <bool kWide>
 __device__ __forceinline__ Row load_row(const __nv_bfloat16* row, int c, int C) {
   if (kWide) return Row{*reinterpret_cast<const uint4*>(row + c)};
   const unsigned short* p = reinterpret_cast<const unsigned short*>(row);
-  uint32_t u[4];
+  uint32_t u[kP];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kP; ++i) {
     const uint32_t lo = c + 2 * i < C ? p[c + 2 * i] : 0u;
     const uint32_t hi = c + 2 * i + 1 < C ? p[c + 2 * i + 1] : 0u;
     u[i] = lo | (hi << 16);
@@ -62,7 +67,7 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* row, int c, int C, cons
     return;
   }
   unsigned short* p = reinterpret_cast<unsigned short*>(row);
-  const uint32_t u[4] = {r.w.x, r.w.y, r.w.z, r.w.w};
+  const uint32_t u[kP] = {r.w.x, r.w.y, r.w.z, r.w.w};
 #pragma unroll
   for (int i = 0; i < kVec; ++i)
     if (c + i < C) p[c + i] = static_cast<unsigned short>(u[i >> 1] >> ((i & 1) * 16));
@@ -71,8 +76,8 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* row, int c, int C, cons
 // What a thread knows of its channels, in pairs.
 template <int W>
 struct Taps {
-  float2 w[W][kVec / 2];
-  float2 bias[kVec / 2];
+  float2 w[W][kP];
+  float2 bias[kP];
 };
 
 // kN consecutive fp32 or bf16 parameters from element i on (16-byte aligned) as floats.
@@ -82,10 +87,13 @@ __device__ __forceinline__ void load_params(const void* base, int dtype, int64_t
     const uint4* p = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(base) + i);
 #pragma unroll
     for (int k = 0; k < kN / 8; ++k) {
-      float f[kVec];
-      unpack(Row{p[k]}, f);
+      float2 f[kP];
+      pairs(Row{p[k]}, f);
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) v[8 * k + e] = f[e];
+      for (int e = 0; e < kP; ++e) {
+        v[8 * k + 2 * e] = f[e].x;
+        v[8 * k + 2 * e + 1] = f[e].y;
+      }
     }
   } else {
     const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + i);
@@ -121,7 +129,7 @@ __device__ __forceinline__ Taps<W> load_taps(const ConvParams& p, int c) {
   }
   Taps<W> t;
 #pragma unroll
-  for (int i = 0; i < kVec / 2; ++i) {
+  for (int i = 0; i < kP; ++i) {
     t.bias[i] = make_float2(b[2 * i], b[2 * i + 1]);
 #pragma unroll
     for (int k = 0; k < W; ++k) t.w[k][i] = make_float2(w[2 * i * W + k], w[(2 * i + 1) * W + k]);
@@ -132,7 +140,8 @@ __device__ __forceinline__ Taps<W> load_taps(const ConvParams& p, int c) {
 // Where a thread's channels go: its section (kWide: all 8 channels lie in one).
 struct Place {
   __nv_bfloat16* out;
-  int width, at, normed;
+  int64_t width;
+  int at, normed;
 };
 __device__ __forceinline__ Place place_of(const ConvParams& p, int c) {
   int s = 0;
@@ -141,67 +150,118 @@ __device__ __forceinline__ Place place_of(const ConvParams& p, int c) {
   return Place{p.out[s], p.begin[s + 1] - p.begin[s], c - p.begin[s], p.normed[s]};
 }
 
-__device__ __forceinline__ float2 pair(uint32_t u) {
-  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-}
-
 // v / (1 + e^-v) of two values with three MUFU operations instead of four: one reciprocal of
 // the product of the denominators. The exponent is capped at 2^63 so that the product stays
 // finite; below v = -43 the result is then -43 2^-63 and the like instead of even less.
 __device__ __forceinline__ float2 silu2(float2 v) {
-  float e0, e1, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(fminf(-kLog2e * v.x, 63.f)));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(fminf(-kLog2e * v.y, 63.f)));
-  const float a = 1.f + e0, b = 1.f + e1;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a * b));
-  return make_float2(v.x * (r * b), v.y * (r * a));
+  const float2 z = __fmul2_rn(v, make_float2(-kLog2e, -kLog2e));
+  float2 e;
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(fminf(z.x, 63.f)));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(fminf(z.y, 63.f)));
+  const float2 a = __fadd2_rn(e, make_float2(1.f, 1.f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a.x * a.y));
+  return __fmul2_rn(v, __fmul2_rn(make_float2(a.y, a.x), make_float2(r, r)));
 }
 
-// One output row: the taps over W rows, activation, norm of the head (16 lanes), store. All
-// lanes of the warp call it; `live` says whether this thread's channels exist.
-template <int W, bool kWide>
-__device__ __forceinline__ void output_row(const ConvParams& p, const Taps<W>& taps, const Place& pl,
-                                           int c, int64_t row, const Row* const (&in)[W],
-                                           bool live) {
-  float2 y[kVec / 2];
+// The W-1 rows before the current one, as floats.
+template <int W>
+struct Window {
+  float2 v[W - 1][kP];
+  __device__ __forceinline__ void set(int r, const Row& row) {
+    pairs(row, v[r]);
+  }
+};
+
+// Sums of kTok values per lane over 16 lanes, each in every lane. Four values: two exchanges
+// that leave one value per lane, two more steps on it, and four broadcasts, 9 shuffles for 16.
+template <int kTok>
+__device__ __forceinline__ void head_sums(float (&q)[kTok]) {
+  const uint32_t lanes = 0xffffu << (threadIdx.x & 16);
+  if constexpr (kTok == 4) {
+    const bool hi = threadIdx.x & 1, hi2 = threadIdx.x & 2;
+    const float a = (hi ? q[1] : q[0]) + __shfl_xor_sync(lanes, hi ? q[0] : q[1], 1);
+    const float b = (hi ? q[3] : q[2]) + __shfl_xor_sync(lanes, hi ? q[2] : q[3], 1);
+    float s = (hi2 ? b : a) + __shfl_xor_sync(lanes, hi2 ? a : b, 2);
+    s += __shfl_xor_sync(lanes, s, 4);
+    s += __shfl_xor_sync(lanes, s, 8);
 #pragma unroll
-  for (int i = 0; i < kVec / 2; ++i) y[i] = taps.bias[i];
+    for (int t = 0; t < 4; ++t) q[t] = __shfl_sync(lanes, s, t, 16);
+  } else {
 #pragma unroll
-  for (int k = 0; k < W; ++k) {
-    const uint32_t u[4] = {in[k]->w.x, in[k]->w.y, in[k]->w.z, in[k]->w.w};
+    for (int t = 0; t < kTok; ++t) {
 #pragma unroll
-    for (int i = 0; i < kVec / 2; ++i) y[i] = __ffma2_rn(taps.w[k][i], pair(u[i]), y[i]);
+      for (int o = 8; o > 0; o >>= 1) q[t] += __shfl_xor_sync(lanes, q[t], o);
+    }
+  }
+}
+
+// kTok output rows from row `at` on (kWide: at `out`): the taps over the window and `rows` (which enter the
+// window one by one), activation, norm of the head (16 lanes), store. All lanes of the warp
+// call it; `live` says whether this thread's channels exist.
+template <int W, bool kWide, int kTok>
+__device__ __forceinline__ void output_rows(const ConvParams& p, const Taps<W>& taps, const Place& pl,
+                                            int c, int64_t at, __nv_bfloat16* out, Window<W>& win,
+                                            const Row (&rows)[kTok], bool live) {
+  float2 y[kTok][kP];
+#pragma unroll
+  for (int t = 0; t < kTok; ++t) {
+    float2 in[kP];
+    pairs(rows[t], in);
+#pragma unroll
+    for (int i = 0; i < kP; ++i) {
+      const float2 cur = in[i];
+      float2 s = taps.bias[i];
+#pragma unroll
+      for (int k = 0; k < W - 1; ++k) s = __ffma2_rn(taps.w[k][i], win.v[k][i], s);
+      y[t][i] = __ffma2_rn(taps.w[W - 1][i], cur, s);
+#pragma unroll
+      for (int k = 0; k + 1 < W - 1; ++k) win.v[k][i] = win.v[k + 1][i];
+      win.v[W - 2][i] = cur;
+    }
   }
   if (p.silu) {
 #pragma unroll
-    for (int i = 0; i < kVec / 2; ++i) y[i] = silu2(y[i]);
+    for (int t = 0; t < kTok; ++t) {
+#pragma unroll
+      for (int i = 0; i < kP; ++i) y[t][i] = silu2(y[t][i]);
+    }
   }
-  if (pl.normed) {  // the same for all 16 lanes of a head
-    float2 q2 = make_float2(0.f, 0.f);
+  if (pl.normed) {  // the same for the 16 lanes of a head
+    float q[kTok];
 #pragma unroll
-    for (int i = 0; i < kVec / 2; ++i) q2 = __ffma2_rn(y[i], y[i], q2);
-    float q = q2.x + q2.y;
-    const uint32_t lanes = 0xffffu << (threadIdx.x & 16);
+    for (int t = 0; t < kTok; ++t) {
+      float2 q2 = __fmul2_rn(y[t][0], y[t][0]);
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) q += __shfl_xor_sync(lanes, q, o);
-    const float r = rsqrtf(q + p.eps);
+      for (int i = 1; i < kP; ++i) q2 = __ffma2_rn(y[t][i], y[t][i], q2);
+      q[t] = q2.x + q2.y;
+    }
+    head_sums(q);
 #pragma unroll
-    for (int i = 0; i < kVec / 2; ++i) y[i] = __fmul2_rn(y[i], make_float2(r, r));
+    for (int t = 0; t < kTok; ++t) {
+      const float r = rsqrtf(q[t] + p.eps);
+#pragma unroll
+      for (int i = 0; i < kP; ++i) y[t][i] = __fmul2_rn(y[t][i], make_float2(r, r));
+    }
   }
   if (!live) return;
-  uint32_t u[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(y[i].y), "f"(y[i].x));
-  if (kWide) {
-    *reinterpret_cast<uint4*>(pl.out + row * pl.width + pl.at) = make_uint4(u[0], u[1], u[2], u[3]);
-  } else {
+  for (int t = 0; t < kTok; ++t) {
+    uint32_t u[kP];
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      if (c + i >= p.C) break;
-      const Place q = place_of(p, c + i);
-      reinterpret_cast<unsigned short*>(q.out)[row * q.width + q.at] =
-          static_cast<unsigned short>(u[i >> 1] >> ((i & 1) * 16));
+    for (int i = 0; i < kP; ++i)
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[i]) : "f"(y[t][i].y), "f"(y[t][i].x));
+    if (kWide) {
+      *reinterpret_cast<uint4*>(out) = make_uint4(u[0], u[1], u[2], u[3]);
+      out += pl.width;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        if (c + i >= p.C) break;
+        const Place q = place_of(p, c + i);
+        reinterpret_cast<unsigned short*>(q.out)[(at + t) * q.width + q.at] =
+            static_cast<unsigned short>(u[i >> 1] >> ((i & 1) * 16));
+      }
     }
   }
 }
@@ -228,7 +288,14 @@ __device__ __forceinline__ int64_t bound(const ConvParams& p, int64_t i) {
 
 // Prompts. Blocks [0, tiles) of grid.y take `run` tokens each; the N behind them write one
 // sequence's new state (its last W-1 inputs, from the state where it is shorter).
-constexpr int kAhead = 4;  // rows per batch; the next batch's are loaded meanwhile
+constexpr int kAhead = 4, kSlots = 4;  // rows per batch, batches in the ring
+
+__device__ __forceinline__ void copy16_async(uint4* to, const __nv_bfloat16* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(to))),
+               "l"(from)
+               : "memory");
+}
 
 template <int W, bool kWide>
 __global__ void __launch_bounds__(kThreads) conv_prefill_kernel(const __grid_constant__ ConvParams p,
@@ -271,53 +338,59 @@ __global__ void __launch_bounds__(kThreads) conv_prefill_kernel(const __grid_con
   const int cl = live ? c : 0;
   const Taps<W> taps = load_taps<W, kWide>(p, cl);
   Place pl = place_of(p, cl);
-  if (!live) pl.normed = 0;  // no lane waits in the head's shuffles for one without channels
-  // rows[0 .. W-2]: the W-1 rows before the batch; behind them the batch's own
-  Row rows[W - 1 + kAhead];
+  if (!live) pl.normed = 0;  // (a normed section is whole warps)
+  Window<W> win;
   const Row zero{make_uint4(0u, 0u, 0u, 0u)};
 #pragma unroll
-  for (int r = 0; r < W - 1; ++r) rows[r] = zero;
+  for (int r = 0; r < W - 1; ++r) win.set(r, zero);
   if (n < p.N && start < t0) {  // the tile begins inside a sequence
 #pragma unroll
     for (int r = 0; r < W - 1; ++r) {
       const int64_t u = t0 - (W - 1) + r;
       if (u >= start) {
-        rows[r] = load_row<kWide>(p.x + u * p.x_stride, cl, p.C);
+        win.set(r, load_row<kWide>(p.x + u * p.x_stride, cl, p.C));
       } else if (p.state) {
-        rows[r] = load_row<kWide>(p.state + (n * (W - 1) + (u - start) + (W - 1)) * p.C, cl, p.C);
+        win.set(r, load_row<kWide>(p.state + (n * (W - 1) + (u - start) + (W - 1)) * p.C, cl, p.C));
       }
     }
   }
-  Row next[kAhead];  // the batch after, on its way
-#pragma unroll
-  for (int a = 0; a < kAhead; ++a)
-    next[a] = load_row<kWide>(p.x + min(t0 + a, p.T - 1) * p.x_stride, cl, p.C);
-  for (int64_t tb = t0; tb < t1; tb += kAhead) {
-#pragma unroll
-    for (int a = 0; a < kAhead; ++a) rows[W - 1 + a] = next[a];
-    if (tb + kAhead < t1) {
-#pragma unroll
-      for (int a = 0; a < kAhead; ++a)
-        next[a] = load_row<kWide>(p.x + min(tb + kAhead + a, p.T - 1) * p.x_stride, cl, p.C);
-    }
-    if (n < p.N && start < tb && tb + kAhead <= min(end, t1)) {
-      // all of the batch and the rows before it lie in one sequence
+  // The ring: batch b of kAhead rows in slot b % kSlots, at this thread's own place.
+  __shared__ uint4 ring[kSlots][kAhead][kThreads];
+  const int batches = static_cast<int>((t1 - t0 + kAhead - 1) / kAhead);
+  const __nv_bfloat16* from = p.x + t0 * p.x_stride + cl;
+  auto fetch = [&](int b) {
+    if (kWide && b < batches) {
+      uint4* const to = &ring[b % kSlots][0][threadIdx.x];
 #pragma unroll
       for (int a = 0; a < kAhead; ++a) {
-        const Row* in[W];
-#pragma unroll
-        for (int k = 0; k < W; ++k) in[k] = &rows[a + k];
-        output_row<W, kWide>(p, taps, pl, cl, tb + a, in, live);
+        if (t0 + b * kAhead + a < t1) copy16_async(to + a * kThreads, from);
+        from += p.x_stride;
       }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto fetched = [&](int b, int a) {
+    return kWide ? Row{ring[b % kSlots][a][threadIdx.x]}
+                 : load_row<kWide>(p.x + (t0 + b * kAhead + a) * p.x_stride, cl, p.C);
+  };
+#pragma unroll 1
+  for (int b = 0; b < kSlots - 1; ++b) fetch(b);
+  __nv_bfloat16* to = pl.out + t0 * pl.width + pl.at;  // kWide: the batch's first output row
+#pragma unroll 1
+  for (int b = 0; b < batches; ++b, to += kAhead * pl.width) {
+    const int64_t tb = t0 + b * kAhead;
+    fetch(b + kSlots - 1);  // its slot's rows are in registers or behind
+    asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 1) : "memory");
+    if (n < p.N && start < tb && tb + kAhead <= min(end, t1)) {
+      // all of the batch and the rows before it lie in one sequence
+      Row rows[kAhead];
 #pragma unroll
-      for (int r = 0; r < W - 1; ++r) rows[r] = rows[kAhead + r];
+      for (int a = 0; a < kAhead; ++a) rows[a] = fetched(b, a);
+      output_rows<W, kWide, kAhead>(p, taps, pl, cl, tb, to, win, rows, live);
       continue;
     }
-    Row win[W];  // token by token, over the sequences' bounds
-#pragma unroll
-    for (int r = 0; r < W - 1; ++r) win[r] = rows[r];
 #pragma unroll 1
-    for (int a = 0; a < kAhead; ++a) {
+    for (int a = 0; a < kAhead; ++a) {  // token by token, over the sequences' bounds
       const int64_t t = tb + a;
       if (t >= t1) break;
       while (t >= end && n < p.N) {  // into the next sequence that has tokens
@@ -332,19 +405,13 @@ __global__ void __launch_bounds__(kThreads) conv_prefill_kernel(const __grid_con
       if (t == start) {
 #pragma unroll
         for (int r = 0; r < W - 1; ++r)
-          win[r] = p.state ? load_row<kWide>(p.state + (n * (W - 1) + r) * p.C, cl, p.C) : zero;
+          win.set(r, p.state ? load_row<kWide>(p.state + (n * (W - 1) + r) * p.C, cl, p.C) : zero);
       }
-      win[W - 1] = load_row<kWide>(p.x + t * p.x_stride, cl, p.C);  // (again: a is no constant)
-      const Row* in[W];
-#pragma unroll
-      for (int k = 0; k < W; ++k) in[k] = &win[k];
-      output_row<W, kWide>(p, taps, pl, cl, t, in, live);
-#pragma unroll
-      for (int r = 0; r < W - 1; ++r) win[r] = win[r + 1];
+      const Row row[1] = {fetched(b, a)};
+      output_rows<W, kWide, 1>(p, taps, pl, cl, t, to + a * pl.width, win, row, live);
     }
-#pragma unroll
-    for (int r = 0; r < W - 1; ++r) rows[r] = win[r];
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // One token per sequence: each thread reads its 8 channels of the W-1 state rows and of x,
@@ -380,10 +447,11 @@ __global__ void __launch_bounds__(kThreads) conv_decode_kernel(const __grid_cons
       for (int r = 0; r < W - 1; ++r)
         store_row<kWide>(p.new_state + (n * (W - 1) + r) * p.C, c, p.C, rows[r + 1]);
     }
-    const Row* in[W];
+    Window<W> win;
 #pragma unroll
-    for (int k = 0; k < W; ++k) in[k] = &rows[k];
-    output_row<W, kWide>(p, taps, pl, cl, n, in, live);
+    for (int r = 0; r < W - 1; ++r) win.set(r, rows[r]);
+    const Row row[1] = {rows[W - 1]};
+    output_rows<W, kWide, 1>(p, taps, pl, cl, n, pl.out + n * pl.width + pl.at, win, row, live);
   }
 }
 

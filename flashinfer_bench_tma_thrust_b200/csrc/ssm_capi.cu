@@ -25,7 +25,7 @@ int fill_conv(gdn::ConvParams* p, const void* x, int64_t x_row_stride, const voi
   int64_t at = 0;
   for (int32_t s = 0; s < sections; ++s) {
     if (widths[s] <= 0) return GDN_ERR_UNSUPPORTED_SHAPE;
-    // the heads of a normed section are whole groups of 16 threads
+    // the heads of a normed section are whole warps
     if (normed[s] && (at % 128 || widths[s] % 128)) return GDN_ERR_UNSUPPORTED_SHAPE;
     p->begin[s] = static_cast<int>(at);
     p->normed[s] = normed[s] != 0;

@@ -24,47 +24,56 @@ struct Piece;
 template <>
 struct Piece<float> {
   static constexpr int kE = 4;
-  static __device__ __forceinline__ void load(const void* base, int64_t i, float (&v)[4]) {
-    const float4 f = ld_stream_f4(static_cast<const float*>(base) + i);
-    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+  static __device__ __forceinline__ void unpack(const uint4& u, float2 (&v)[2]) {
+    v[0] = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+    v[1] = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
   }
-  static __device__ __forceinline__ void store(void* base, int64_t i, const float (&v)[4]) {
-    st_stream_f4(static_cast<float*>(base) + i, make_float4(v[0], v[1], v[2], v[3]));
+  static __device__ __forceinline__ uint4 pack(const float2 (&v)[2]) {
+    return make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x),
+                      __float_as_uint(v[1].y));
   }
 };
 template <>
 struct Piece<__nv_bfloat16> {
   static constexpr int kE = 8;
-  static __device__ __forceinline__ void load(const void* base, int64_t i, float (&v)[8]) {
-    uint32_t u[4];
-    asm volatile("ld.global.cs.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3])
-                 : "l"(static_cast<const __nv_bfloat16*>(base) + i));
+  static __device__ __forceinline__ void unpack(const uint4& w, float2 (&v)[4]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      v[2 * k] = __uint_as_float(u[k] << 16);
-      v[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
-    }
+    for (int k = 0; k < 4; ++k)
+      v[k] = make_float2(__uint_as_float(u[k] << 16), __uint_as_float(u[k] & 0xffff0000u));
   }
-  static __device__ __forceinline__ void store(void* base, int64_t i, const float (&v)[8]) {
+  static __device__ __forceinline__ uint4 pack(const float2 (&v)[4]) {
     uint32_t u[4];  // the state's own type: one rounding per step, the user's choice of it
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[k]) : "f"(v[2 * k + 1]), "f"(v[2 * k]));
-    asm volatile("st.global.cs.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(
-                     static_cast<__nv_bfloat16*>(base) + i),
-                 "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3])
-                 : "memory");
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u[k]) : "f"(v[k].y), "f"(v[k].x));
+    return make_uint4(u[0], u[1], u[2], u[3]);
   }
 };
+// Streaming access to the state: each element is touched once per launch.
+template <typename S>
+__device__ __forceinline__ uint4 load_piece(const void* base, int64_t i) {
+  uint4 u;
+  asm volatile("ld.global.cs.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+               : "l"(static_cast<const S*>(base) + i));
+  return u;
+}
+template <typename S>
+__device__ __forceinline__ void store_piece(void* base, int64_t i, const uint4& u) {
+  asm volatile("st.global.cs.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(static_cast<S*>(base) + i),
+               "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w)
+               : "memory");
+}
 
-// kE consecutive bf16 values (kE = 4 or 8, aligned to their size) as floats.
+// kE consecutive bf16 values (kE = 4 or 8, aligned to their size) as pairs of floats.
 template <int kE>
-__device__ __forceinline__ void load_bf16(const __nv_bfloat16* p, float (&v)[kE]) {
+__device__ __forceinline__ void load_bf16(const __nv_bfloat16* p, float2 (&v)[kE / 2]) {
 #pragma unroll
   for (int k = 0; k < kE; k += 4) {
     const float4 f = load_bf16x4(p + k);
-    v[k] = f.x; v[k + 1] = f.y; v[k + 2] = f.z; v[k + 3] = f.w;
+    v[k / 2] = make_float2(f.x, f.y);
+    v[k / 2 + 1] = make_float2(f.z, f.w);
   }
 }
 
@@ -80,16 +89,16 @@ __device__ __forceinline__ float bf16_at(const __nv_bfloat16* p) {
 }
 
 // ---------------------------------------------------------------- one token per sequence
-// HBM bounds it: the state goes through once (5 flop per 8 bytes). A warp takes kRows * kPer
-// rows (at most 32: lane r holds x and y of row r) with all its loads in flight before it
-// reduces any of them. Blocks of 4 warps share a head's rows, `splits` blocks a head.
-template <typename S, int kLanes, int kPieces, int kRows>
+// HBM bounds it: the state goes through once (5 flop per 8 bytes). A warp takes batches of
+// kRows * kPer rows (at most 32: lane r holds x and y of row r); a batch's loads are all in
+// flight, and the next batch's too, before it is used. Blocks of 4 warps share a head's rows.
+template <typename S, int kLanes, int kPieces, int kRows, bool kLoop>
 __global__ void __launch_bounds__(128) ssm_decode_kernel(const __grid_constant__ SsmParams p,
-                                                        int splits) {
-  constexpr int kE = Piece<S>::kE;
+                                                        int splits, int batches) {
+  constexpr int kE = Piece<S>::kE, kH = kE / 2;
   constexpr int kPer = 32 / kLanes;  // rows per load
-  constexpr int kWarpRows = kRows * kPer;
-  static_assert(kWarpRows <= 32, "");
+  constexpr int kBatch = kRows * kPer;
+  static_assert(kBatch <= 32, "");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int l = lane % kLanes, sub = lane / kLanes;
   const int64_t head = blockIdx.x / splits;  // flattened (sequence, head)
@@ -97,63 +106,84 @@ __global__ void __launch_bounds__(128) ssm_decode_kernel(const __grid_constant__
   const int64_t n = head / p.H;
   const int h = static_cast<int>(head - n * p.H);
   const int64_t grp = n * p.G + h / (p.H / p.G);
-  const int row0 = (split * 4 + warp) * kWarpRows;
-  if (row0 >= p.P) return;
+  const int first = (split * 4 + warp) * batches * kBatch;
+  const int end = min(first + batches * kBatch, p.P);
+  if (first >= end) return;
 
-  float s[kRows][kPieces][kE];
-  const int64_t at0 = (head * p.P + row0 + sub) * p.Ns + l * kE;
+  // without kLoop (one batch) `next` is the batch itself
+  uint4 next[kRows][kPieces];
+  auto load = [&](int row0) {
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
+    for (int i = 0; i < kRows; ++i) {
+      const int r = row0 + i * kPer + sub;
 #pragma unroll
-    for (int j = 0; j < kPieces; ++j) {
-      if (p.state && row0 + i * kPer + sub < p.P) {
-        Piece<S>::load(p.state, at0 + i * kPer * p.Ns + j * kLanes * kE, s[i][j]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < kE; ++k) s[i][j][k] = 0.f;
-      }
+      for (int j = 0; j < kPieces; ++j)
+        next[i][j] = p.state && r < end
+                         ? load_piece<S>(p.state, (head * p.P + r) * p.Ns + (j * kLanes + l) * kE)
+                         : make_uint4(0u, 0u, 0u, 0u);
     }
-  }
-  const bool own = lane < kWarpRows && row0 + lane < p.P;
-  const float x_lane = own ? bf16_at(p.x + head * p.P + row0 + lane) : 0.f;
+  };
+  load(first);
   const float v = load_scalar(p.dt, p.dt_dtype, head) + load_scalar(p.dt_bias, p.dt_bias_dtype, h);
-  const float d = softplus_ref(v);
-  const float g = expf(-expf(load_scalar(p.A_log, p.A_log_dtype, h)) * d);
+  const float a_log = load_scalar(p.A_log, p.A_log_dtype, h);
   const float skip = p.D ? load_scalar(p.D, p.D_dtype, h) : 0.f;
-  float b[kPieces][kE], c[kPieces][kE], bc = 0.f;
+  float2 b[kPieces][kH], c[kPieces][kH];
 #pragma unroll
   for (int j = 0; j < kPieces; ++j) {
     const int64_t at = grp * p.Ns + (j * kLanes + l) * kE;
     load_bf16<kE>(p.B + at, b[j]);
     load_bf16<kE>(p.C + at, c[j]);
+  }
+  const float d = softplus_ref(v);
+  const float g = expf(-expf(a_log) * d);
+  float bc = 0.f;
 #pragma unroll
-    for (int k = 0; k < kE; ++k) bc = fmaf(b[j][k], c[j][k], bc);
+  for (int j = 0; j < kPieces; ++j) {
+#pragma unroll
+    for (int k = 0; k < kH; ++k) bc = fmaf(b[j][k].x, c[j][k].x, fmaf(b[j][k].y, c[j][k].y, bc));
   }
   bc = row_sum<kLanes>(bc);
+  const float2 g2 = make_float2(g, g);
 
-  float y = 0.f;
+#pragma unroll 1
+  for (int row0 = first; row0 < end; row0 += kBatch) {
+    uint4 s[kRows][kPieces];
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    const float dx = d * __shfl_sync(0xffffffffu, x_lane, i * kPer + sub);
-    float dot = 0.f;
+    for (int i = 0; i < kRows; ++i) {
 #pragma unroll
-    for (int j = 0; j < kPieces; ++j) {
-      float w[kE];
-#pragma unroll
-      for (int k = 0; k < kE; ++k) {
-        dot = fmaf(s[i][j][k], c[j][k], dot);
-        w[k] = fmaf(g, s[i][j][k], dx * b[j][k]);
-      }
-      if (row0 + i * kPer + sub < p.P)
-        Piece<S>::store(p.new_state, at0 + i * kPer * p.Ns + j * kLanes * kE, w);
+      for (int j = 0; j < kPieces; ++j) s[i][j] = next[i][j];
     }
-    dot = row_sum<kLanes>(dot);
-    const float yi = fmaf(g, dot, dx * bc);
-    // row i * kPer + (lane % kPer) is in the lanes of that sub
-    const float mine = kPer == 1 ? yi : __shfl_sync(0xffffffffu, yi, (lane % kPer) * kLanes);
-    if (lane / kPer == i) y = mine;
+    if (kLoop && row0 + kBatch < end) load(row0 + kBatch);
+    const bool own = lane < kBatch && row0 + lane < end;
+    const float x_lane = own ? bf16_at(p.x + head * p.P + row0 + lane) : 0.f;
+    float y = 0.f;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int r = row0 + i * kPer + sub;
+      const float dx = d * __shfl_sync(0xffffffffu, x_lane, i * kPer + sub);
+      const float2 dx2 = make_float2(dx, dx);
+      float2 dot = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j) {
+        float2 w[kH];
+        Piece<S>::unpack(s[i][j], w);
+#pragma unroll
+        for (int k = 0; k < kH; ++k) {
+          dot = __ffma2_rn(w[k], c[j][k], dot);
+          w[k] = __ffma2_rn(g2, w[k], __fmul2_rn(dx2, b[j][k]));
+        }
+        if (r < end)
+          store_piece<S>(p.new_state, (head * p.P + r) * p.Ns + (j * kLanes + l) * kE,
+                         Piece<S>::pack(w));
+      }
+      const float yi = fmaf(g, row_sum<kLanes>(dot.x + dot.y), dx * bc);
+      // row i * kPer + (lane % kPer) is in the lanes of that sub
+      const float mine = kPer == 1 ? yi : __shfl_sync(0xffffffffu, yi, (lane % kPer) * kLanes);
+      if (lane / kPer == i) y = mine;
+    }
+    if (own) p.out[head * p.P + row0 + lane] = __float2bfloat16_rn(fmaf(skip, x_lane, y));
+    if (!kLoop) break;
   }
-  if (own) p.out[head * p.P + row0 + lane] = __float2bfloat16_rn(fmaf(skip, x_lane, y));
 }
 
 // ---------------------------------------------------------------- prompts, token by token
@@ -165,7 +195,7 @@ constexpr int kStep = 4;
 template <int kLanes, int kPieces, int kRows>
 __global__ void __launch_bounds__(128) ssm_recurrent_kernel(const __grid_constant__ SsmParams p,
                                                            int tiles) {
-  constexpr int kE = 4;
+  constexpr int kE = 4, kH = 2;
   constexpr int kPer = 32 / kLanes;
   constexpr int kWarpRows = kRows * kPer;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -186,26 +216,24 @@ __global__ void __launch_bounds__(128) ssm_recurrent_kernel(const __grid_constan
   start = start < 0 ? 0 : (start > p.T ? p.T : start);
   end = end < 0 ? 0 : (end > p.T ? p.T : end);
 
-  float s[kRows][kPieces][kE];
+  float2 s[kRows][kPieces][kH];
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
     const int r = row0 + i * kPer + sub;
 #pragma unroll
-    for (int j = 0; j < kPieces; ++j) {
-      if (p.state && r < p.P) {
-        Piece<float>::load(p.state, (head * p.P + r) * p.Ns + (j * kLanes + l) * kE, s[i][j]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < kE; ++k) s[i][j][k] = 0.f;
-      }
-    }
+    for (int j = 0; j < kPieces; ++j)
+      Piece<float>::unpack(p.state && r < p.P ? load_piece<float>(p.state, (head * p.P + r) * p.Ns +
+                                                                               (j * kLanes + l) * kE)
+                                              : make_uint4(0u, 0u, 0u, 0u),
+                           s[i][j]);
   }
   const float neg_a = -expf(load_scalar(p.A_log, p.A_log_dtype, h));
   const float dtb = load_scalar(p.dt_bias, p.dt_bias_dtype, h);
   const float skip = p.D ? load_scalar(p.D, p.D_dtype, h) : 0.f;
 
   for (int64_t t0 = start; t0 < end; t0 += kStep) {
-    float b[kStep][kPieces][kE], c[kStep][kPieces][kE], x[kStep][kRows], d[kStep], g[kStep];
+    float2 b[kStep][kPieces][kH], c[kStep][kPieces][kH];
+    float x[kStep][kRows], d[kStep], g[kStep];
 #pragma unroll
     for (int a = 0; a < kStep; ++a) {
       const int64_t t = min(t0 + a, end - 1);
@@ -233,16 +261,17 @@ __global__ void __launch_bounds__(128) ssm_recurrent_kernel(const __grid_constan
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
         const float dx = d[a] * x[a][i];
-        float dot = 0.f;
+        const float2 dx2 = make_float2(dx, dx), g2 = make_float2(g[a], g[a]);
+        float2 dot2 = make_float2(0.f, 0.f);
 #pragma unroll
         for (int j = 0; j < kPieces; ++j) {
 #pragma unroll
-          for (int k = 0; k < kE; ++k) {
-            s[i][j][k] = fmaf(g[a], s[i][j][k], dx * b[a][j][k]);
-            dot = fmaf(s[i][j][k], c[a][j][k], dot);
+          for (int k = 0; k < kH; ++k) {
+            s[i][j][k] = __ffma2_rn(g2, s[i][j][k], __fmul2_rn(dx2, b[a][j][k]));
+            dot2 = __ffma2_rn(s[i][j][k], c[a][j][k], dot2);
           }
         }
-        dot = row_sum<kLanes>(dot);
+        const float dot = row_sum<kLanes>(dot2.x + dot2.y);
         const int r = row0 + i * kPer + sub;
         if (l == 0 && r < p.P)
           p.out[((t0 + a) * p.H + h) * p.P + r] = __float2bfloat16_rn(fmaf(skip, x[a][i], dot));
@@ -255,18 +284,27 @@ __global__ void __launch_bounds__(128) ssm_recurrent_kernel(const __grid_constan
     if (r >= p.P) continue;
 #pragma unroll
     for (int j = 0; j < kPieces; ++j)
-      Piece<float>::store(p.new_state, (head * p.P + r) * p.Ns + (j * kLanes + l) * kE, s[i][j]);
+      store_piece<float>(p.new_state, (head * p.P + r) * p.Ns + (j * kLanes + l) * kE,
+                         Piece<float>::pack(s[i][j]));
   }
 }
 
 template <typename S, int kLanes, int kPieces, int kRows>
-int decode_as(const SsmParams& p, cudaStream_t stream) {
+int decode_as(const SsmParams& p, cudaStream_t stream, int most_batches) {
   constexpr int kBlockRows = 4 * kRows * (32 / kLanes);
   const int64_t heads = p.N * p.H;
-  const int splits = (p.P + kBlockRows - 1) / kBlockRows;
+  const int whole = (p.P + kBlockRows - 1) / kBlockRows;  // batches of a whole head
+  int batches = 1;
+  while (batches < most_batches && batches < whole && heads * (whole / (2 * batches)) >= 148 * 16)
+    batches *= 2;
+  const int splits = (whole + batches - 1) / batches;
   if (heads * splits > 0x7fffffffLL) return GDN_ERR_UNSUPPORTED_SHAPE;
-  ssm_decode_kernel<S, kLanes, kPieces, kRows>
-      <<<static_cast<unsigned>(heads * splits), 128, 0, stream>>>(p, splits);
+  const unsigned grid = static_cast<unsigned>(heads * splits);
+  if (batches > 1) {
+    ssm_decode_kernel<S, kLanes, kPieces, kRows, true><<<grid, 128, 0, stream>>>(p, splits, batches);
+  } else {
+    ssm_decode_kernel<S, kLanes, kPieces, kRows, false><<<grid, 128, 0, stream>>>(p, splits, 1);
+  }
   return cudaGetLastError() == cudaSuccess ? 0 : GDN_ERR_CUDA;
 }
 
@@ -283,23 +321,27 @@ int recurrent_as(const SsmParams& p, cudaStream_t stream) {
 
 }  // namespace
 
+// Batches per warp at most, where the grid stays full: a warp's gates and its B and C cost as much
+// as a batch of bf16 rows.
+constexpr int kF32Batches = 1, kBf16Batches = 4;
+
 int launch_ssm_decode(const SsmParams& p, cudaStream_t stream) {
   if (p.state_bf16) {
     switch (p.Ns) {
-      case 16: return decode_as<__nv_bfloat16, 2, 1, 2>(p, stream);
-      case 32: return decode_as<__nv_bfloat16, 4, 1, 4>(p, stream);
-      case 64: return decode_as<__nv_bfloat16, 8, 1, 4>(p, stream);
-      case 128: return decode_as<__nv_bfloat16, 16, 1, 4>(p, stream);
-      case 256: return decode_as<__nv_bfloat16, 32, 1, 4>(p, stream);
+      case 16: return decode_as<__nv_bfloat16, 2, 1, 2>(p, stream, kBf16Batches);
+      case 32: return decode_as<__nv_bfloat16, 4, 1, 4>(p, stream, kBf16Batches);
+      case 64: return decode_as<__nv_bfloat16, 8, 1, 4>(p, stream, kBf16Batches);
+      case 128: return decode_as<__nv_bfloat16, 16, 1, 4>(p, stream, kBf16Batches);
+      case 256: return decode_as<__nv_bfloat16, 32, 1, 4>(p, stream, kBf16Batches);
     }
     return GDN_ERR_UNSUPPORTED_SHAPE;
   }
   switch (p.Ns) {
-    case 16: return decode_as<float, 4, 1, 4>(p, stream);
-    case 32: return decode_as<float, 8, 1, 8>(p, stream);
-    case 64: return decode_as<float, 16, 1, 8>(p, stream);
-    case 128: return decode_as<float, 32, 1, 8>(p, stream);
-    case 256: return decode_as<float, 32, 2, 4>(p, stream);
+    case 16: return decode_as<float, 4, 1, 4>(p, stream, kF32Batches);
+    case 32: return decode_as<float, 8, 1, 8>(p, stream, kF32Batches);
+    case 64: return decode_as<float, 16, 1, 8>(p, stream, kF32Batches);
+    case 128: return decode_as<float, 32, 1, 8>(p, stream, kF32Batches);
+    case 256: return decode_as<float, 32, 2, 4>(p, stream, kF32Batches);
   }
   return GDN_ERR_UNSUPPORTED_SHAPE;
 }
