@@ -173,20 +173,18 @@ struct Window {
   }
 };
 
-// Sums of kTok values per lane over 16 lanes, each in every lane. Four values: two exchanges
-// that leave one value per lane, two more steps on it, and four broadcasts, 9 shuffles for 16.
+// Sums of kTok values per lane over 16 lanes, each in every lane. Two values: an exchange that
+// leaves one value per lane, three more steps on it, and two broadcasts, 6 shuffles for 8.
 template <int kTok>
 __device__ __forceinline__ void head_sums(float (&q)[kTok]) {
   const uint32_t lanes = 0xffffu << (threadIdx.x & 16);
-  if constexpr (kTok == 4) {
-    const bool hi = threadIdx.x & 1, hi2 = threadIdx.x & 2;
-    const float a = (hi ? q[1] : q[0]) + __shfl_xor_sync(lanes, hi ? q[0] : q[1], 1);
-    const float b = (hi ? q[3] : q[2]) + __shfl_xor_sync(lanes, hi ? q[2] : q[3], 1);
-    float s = (hi2 ? b : a) + __shfl_xor_sync(lanes, hi2 ? a : b, 2);
-    s += __shfl_xor_sync(lanes, s, 4);
-    s += __shfl_xor_sync(lanes, s, 8);
+  if constexpr (kTok == 2) {
+    const bool hi = threadIdx.x & 1;
+    float s = (hi ? q[1] : q[0]) + __shfl_xor_sync(lanes, hi ? q[0] : q[1], 1);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) q[t] = __shfl_sync(lanes, s, t, 16);
+    for (int o = 2; o < 16; o <<= 1) s += __shfl_xor_sync(lanes, s, o);
+    q[0] = __shfl_sync(lanes, s, 0, 16);
+    q[1] = __shfl_sync(lanes, s, 1, 16);
   } else {
 #pragma unroll
     for (int t = 0; t < kTok; ++t) {
@@ -383,10 +381,11 @@ __global__ void __launch_bounds__(kThreads) conv_prefill_kernel(const __grid_con
     asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 1) : "memory");
     if (n < p.N && start < tb && tb + kAhead <= min(end, t1)) {
       // all of the batch and the rows before it lie in one sequence
-      Row rows[kAhead];
 #pragma unroll
-      for (int a = 0; a < kAhead; ++a) rows[a] = fetched(b, a);
-      output_rows<W, kWide, kAhead>(p, taps, pl, cl, tb, to, win, rows, live);
+      for (int a = 0; a < kAhead; a += 2) {  // two rows at a time: more take too many registers
+        const Row rows[2] = {fetched(b, a), fetched(b, a + 1)};
+        output_rows<W, kWide, 2>(p, taps, pl, cl, tb + a, to + a * pl.width, win, rows, live);
+      }
       continue;
     }
 #pragma unroll 1
@@ -474,9 +473,11 @@ dim3 rows_grid(unsigned bx, int64_t rows) {
 template <int W>
 int prefill_w(const ConvParams& p, cudaStream_t stream) {
   const unsigned bx = (p.C + kThreads * kVec - 1) / (kThreads * kVec);
-  // A run of `run` tokens reads W-1 rows again; short runs fill the SMs for short prompts.
-  int run = 64;
-  while (run > 8 && bx * ((p.T + run - 1) / run) < 148 * 8) run /= 2;
+  // A run reads W-1 rows and the taps again (128 against 64 tokens: 4 % less on 65536 x 6144),
+  // but the grid wants some five rounds of blocks (three per SM) for an even end: runs of 128 on
+  // 19679 x 8192, under three rounds, lose 7 %. Short prompts take short runs to fill the SMs.
+  int run = 128;
+  while (run > 8 && bx * ((p.T + run - 1) / run) < 148 * 16) run /= 2;
   const int64_t tiles = (p.T + run - 1) / run;
   const int64_t rows = tiles + p.N;
   if (rows > (int64_t{1} << 30)) return GDN_ERR_UNSUPPORTED_SHAPE;
