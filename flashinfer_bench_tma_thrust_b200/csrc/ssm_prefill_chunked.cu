@@ -145,7 +145,7 @@ struct Cfg {
   static constexpr uint32_t kS = kC + (kStates ? 0 : kBBytes);
   static constexpr uint32_t kGates = kS + (kStates ? 0 : kBBytes);
   static constexpr uint32_t kBars = kGates + 2 * kHeads * sizeof(Gates);
-  static constexpr uint32_t kBytes = kBars + 272 + 1024;  // and the alignment
+  static constexpr uint32_t kBytes = kBars + 8 * 34 + 1024;  // and the alignment
 };
 
 enum Bar {
@@ -165,6 +165,7 @@ enum Bar {
   kYFree = 28,      // Y read out
   kStaged = 29,     // y in shared memory [3]
   kZeroed = 32,
+  kXRead = 33,      // x read by the state's warps, so that y may replace it
 };
 
 // Bounded waits in few instructions (the roles' code has to stay in the instruction cache: see
@@ -360,6 +361,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     for (int i : {kCB, kYS, kYM}) mbar_init(bars + i, 1);
     for (int i : {kMy, kYFree}) mbar_init(bars + i, 8);
     mbar_init(bars + kZeroed, K::kStateWarps);
+    mbar_init(bars + kXRead, K::kStateWarps);
     fence_mbar_init();
   }
   if (warp == kMisc) tmem_alloc(&s_tmem, 512);
@@ -472,12 +474,17 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       const int st = c % K::kXStages;
       const uint32_t xrow = sm_u + K::kX + st * K::kXBytes + half * kBlock + row_base(row);
       wait(bars_u + 8 * (kYM), c & 1);
+      wait(bars_u + 8 * (kXRead), c & 1);
       tc_fence_after();
       {
 #pragma unroll 1
         for (int k0 = 0; k0 < 8; k0 += 4) {
           float y[32];
+          uint4 xv[4];
           tmem_ld32(lanes + kTY + 64 * half + 8 * k0, y);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            xv[k] = p.D ? lds4u(xrow ^ (16 * (k0 + k))) : make_uint4(0u, 0u, 0u, 0u);
           tmem_ld_wait();
           if (k0 == 4) {
             tc_fence_before();
@@ -485,9 +492,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t at = xrow ^ (16 * (k0 + k));
-            const uint4 xv = p.D ? lds4u(at) : make_uint4(0u, 0u, 0u, 0u);
-            const uint32_t u[4] = {xv.x, xv.y, xv.z, xv.w};
+            const uint32_t u[4] = {xv[k].x, xv[k].y, xv[k].z, xv[k].w};
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -497,7 +502,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
                                     make_float2(y[8 * k + 2 * e], y[8 * k + 2 * e + 1]));
               w[e] = pack2_rn(v.x, v.y);
             }
-            sts4u(at, w[0], w[1], w[2], w[3]);
+            sts4u(xrow ^ (16 * (k0 + k)), w[0], w[1], w[2], w[3]);
           }
         }
       }
@@ -638,6 +643,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       tmem_st_wait();
       tc_fence_before();
       arrive(kFx + place);
+      if (!kStates && t == 3) arrive(kXRead);
     };
 
     // The state behind chunk c, from what the chunk adds.
@@ -725,29 +731,32 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       const uint32_t xb = sm_u + K::kX + (c % K::kXStages) * K::kXBytes;
       const uint32_t bb = sm_u + K::kB + st * K::kBBytes;
       const bool zeroed = c == chunks - 1 && tail < kL;
-      auto issue_ds = [&](uint32_t td) {
-#pragma unroll 1
-        for (int t = 0; t < 4; ++t) {
-          const int k = 4 * c + t, place = k % K::kPlaces;
-          wait(bars_u + 8 * (kFx + place), (k / K::kPlaces) & 1);
-          tc_fence_after();
-          const uint32_t tf = tm + (kStates ? 0 : kTF) + 16 * kTerms * place;
-          const uint32_t b0 = fresh(bb + t * 4096);
+      // dS by quarter t of the chunk's tokens, whose f x is in its place
+      auto issue_ds = [&](uint32_t td, int t) {
+        const int place = (4 * c + t) % K::kPlaces;
+        const uint32_t tf = tm + (kStates ? 0 : kTF) + 16 * kTerms * place;
+        const uint32_t b0 = fresh(bb + t * 4096);
+        tc_fence_after();
 #pragma unroll
-          for (int r = 0; r < kTerms; ++r) {
+        for (int r = 0; r < kTerms; ++r) {
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
-              mma_bf16_ts_w(td, tf + 16 * r + 8 * s, desc(d_mn, b0, s * 2048), kIdDS,
-                            t > 0 || r > 0 || s > 0);
-          }
-          mma_commit_w(bars + kFxFree + place);
+          for (int s = 0; s < 2; ++s)
+            mma_bf16_ts_w(td, tf + 16 * r + 8 * s, desc(d_mn, b0, s * 2048), kIdDS,
+                          t > 0 || r > 0 || s > 0);
         }
-        mma_commit_w(bars + kDS + st);
+        mma_commit_w(bars + kFxFree + place);
+        if (t == 3) mma_commit_w(bars + kDS + st);
       };
+      auto fx_bar = [&](int t) { return bars_u + 8 * (kFx + (4 * c + t) % K::kPlaces); };
+      auto fx_par = [&](int t) { return static_cast<uint32_t>(((4 * c + t) / K::kPlaces) & 1); };
       if (kStates) {
         wait(bars_u + 8 * (kFullB + st), par);
         if (c >= 2) wait(bars_u + 8 * (kState + (c & 1)), ((c >> 1) - 1) & 1);
-        issue_ds(tm + kTD + 128 * (c & 1));
+#pragma unroll 1
+        for (int t = 0; t < 4; ++t) {
+          wait(fx_bar(t), fx_par(t));
+          issue_ds(tm + kTD + 128 * (c & 1), t);
+        }
         continue;
       }
       // C B^T: over the place of the last chunk's M
@@ -774,20 +783,34 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
           mma_bf16_w(tm + kTY, desc(d_k, c0, kstep(s)), desc(d_k, s0, kstep(s)), kIdCB, s > 0);
       }
       mma_commit_w(bars + kYS);
-      // (f x)^T B
-      issue_ds(tm + kTD);
-      // M x
-      wait(bars_u + 8 * (kMy), c & 1);
-      tc_fence_after();
+      // (f x)^T B by quarters, and M x, each as soon as its operands are there
+      bool todo = true, force = !wait.ok();  // M x is; a block that gave up does not wait
+      int t = 0;
+      uint32_t polls = 1u << 24;  // of some 50 cycles
 #pragma unroll 1
-      for (int hh = 0; hh < kHeads; ++hh) {
-        const uint32_t x0 = fresh(xb + hh * kBlock);
+      while (t < 4 || todo) {
+        if (todo && (force || mbar_test_wait(bars_u + 8 * kMy, c & 1))) {
+          todo = false;
+          tc_fence_after();
+#pragma unroll 1
+          for (int hh = 0; hh < kHeads; ++hh) {
+            const uint32_t x0 = fresh(xb + hh * kBlock);
 #pragma unroll 4
-        for (int s = 0; s < 8; ++s)
-          mma_bf16_ts_w(tm + kTY + hh * 64, tm + kTG + 16 * s + 8 * hh,
-                        desc(d_mn, x0, s * 2048), kIdYM, 1);
+            for (int s = 0; s < 8; ++s)
+              mma_bf16_ts_w(tm + kTY + hh * 64, tm + kTG + 16 * s + 8 * hh, desc(d_mn, x0, s * 2048),
+                            kIdYM, 1);
+          }
+          mma_commit_w(bars + kYM);
+        }
+        if (t < 4 && (force || mbar_test_wait(fx_bar(t), fx_par(t)))) {
+          issue_ds(tm + kTD, t);
+          ++t;
+        }
+        if (!force && --polls == 0) {
+          force = true;
+          wait.left = 0;
+        }
       }
-      mma_commit_w(bars + kYM);
     }
     // the block's TMEM may go once the last product is done
     if (chunks > 0) {
