@@ -82,7 +82,9 @@ __device__ __forceinline__ float4 lds4(uint32_t a) {
                : "r"(a));
   return v;
 }
-__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) {
+  return __fadd2_rn(a, make_float2(-b.x, -b.y));
+}
 __device__ __forceinline__ uint4 lds4u(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
@@ -248,7 +250,7 @@ __device__ __forceinline__ void find_segment(const SsmParams& p, const Segments&
 __device__ __forceinline__ void write_gates(uint32_t g, const float (&raw)[4], float neg_a, float dtb,
                                             int valid, int lane) {
   float tot[4];
-#pragma unroll 1
+#pragma unroll 2
   for (int k = 0; k < 4; ++k) {
     const bool in = 32 * k + lane < valid;
     const float r = k == 0 ? raw[0] : (k == 1 ? raw[1] : (k == 2 ? raw[2] : raw[3]));
@@ -279,7 +281,7 @@ __device__ __forceinline__ void write_gates(uint32_t g, const float (&raw)[4], f
     tot[2] = k == 2 ? t : tot[2];
     tot[3] = t;
   }
-#pragma unroll 1
+#pragma unroll 2
   for (int k = 0; k < 4; ++k) {
     const float head = k == 0 ? 0.f : (k == 1 ? tot[0] : (k == 2 ? tot[0] + tot[1]
                                                                  : tot[0] + tot[1] + tot[2]));
@@ -617,28 +619,35 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       const float2 f0 = lds2(f), f1 = lds2(f + 32);
       const uint32_t xa = sm_u + K::kX + (c % K::kXStages) * K::kXBytes + (q >> 1) * kBlock +
                           128 * 32 * t + x_lane;
+      uint32_t u[2][4];  // [columns 0-15, 16-31]: tokens 0-7 of columns 0-7, 8-15; tokens 8-15
+      ldmatrix_x4_trans(xa, u[0]);
+      ldmatrix_x4_trans(xa ^ 32, u[1]);
       if (k >= K::kPlaces) wait(bars_u + 8 * (kFxFree + place), (k / K::kPlaces - 1) & 1);
       const uint32_t at = lanes + (kStates ? 0 : kTF) + 16 * kTerms * place + 8 * part;
+      uint32_t w[2][kTerms][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t u[4], w[kTerms][4];  // tokens 0-7 of columns 0-7 and 8-15, then tokens 8-15
-        ldmatrix_x4_trans(xa ^ (32 * h), u);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float2 v = mul2(make_float2(__uint_as_float(u[i] << 16),
-                                      __uint_as_float(u[i] & 0xffff0000u)),
+          // 24 bits in three bf16 terms of 8 by truncation: their sum is x f to the last bit
+          float2 v = mul2(make_float2(__uint_as_float(u[h][i] << 16),
+                                      __uint_as_float(u[h][i] & 0xffff0000u)),
                           i < 2 ? f0 : f1);
 #pragma unroll
-          for (int r = 0; r < kTerms - 1; ++r) {
-            w[r][i] = pack2_rn(v.x, v.y);
-            v = add2(v, make_float2(__uint_as_float((w[r][i] << 16) ^ 0x80000000u),
-                                    __uint_as_float((w[r][i] & 0xffff0000u) ^ 0x80000000u)));
+          for (int r = 0; r < kTerms; ++r) {
+            const uint32_t a = __float_as_uint(v.x), b = __float_as_uint(v.y);
+            w[h][r][i] = __byte_perm(a, b, 0x7632);
+            if (r + 1 < kTerms)
+              v = sub2(v, make_float2(__uint_as_float(a & 0xffff0000u),
+                                      __uint_as_float(b & 0xffff0000u)));
           }
-          w[kTerms - 1][i] = pack2_rn(v.x, v.y);
         }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
         for (int r = 0; r < kTerms; ++r)
-          tmem_st_frag(at + 16 * r + (static_cast<uint32_t>(16 * h) << 16), w[r]);
+          tmem_st_frag(at + 16 * r + (static_cast<uint32_t>(16 * h) << 16), w[h][r]);
       }
       tmem_st_wait();
       tc_fence_before();
