@@ -46,10 +46,10 @@ constexpr int kL = 128;             // tokens per chunk
 constexpr int kBlock = 16384;       // a [128 rows x 64 columns] bf16 tile
 
 // Registers per thread of the output kernel: 96 at launch (640 threads), then shared out anew
-// between the output's, the state's and the other warps: 256 x 96 + 256 x 112 + 128 x 64 is
+// between the output's, the state's and the other warps: 256 x 88 + 256 x 120 + 128 x 64 is
 // what 640 x 96 were. Spills are what this avoids: the shared memory leaves L1 next to nothing,
 // and a few local accesses per chunk cost more than a product.
-constexpr int kLaunchRegs = 96, kOutRegs = 96, kStateRegs = 112, kMiscRegs = 64;
+constexpr int kLaunchRegs = 96, kOutRegs = 88, kStateRegs = 120, kMiscRegs = 64;
 static_assert(256 * kOutRegs + 256 * kStateRegs + 128 * kMiscRegs <= 640 * kLaunchRegs, "");
 
 template <int kRegs>
@@ -382,7 +382,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
   };
 
   if (warp < kOutWarps) {
-    if (!kStates) regs_inc<kOutRegs>();
+    if (!kStates) regs_dec<kOutRegs>();
     // ---------------------------------------------------------------- output: token per thread
     const int half = warp >> 2;
     const int col_head = kHeads == 2 ? half : 0;  // head of columns 64 half to 64 half + 63
@@ -768,38 +768,49 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         }
         continue;
       }
-      // C B^T: over the place of the last chunk's M
-      wait(bars_u + 8 * (kFullB + st), par);
-      wait(bars_u + 8 * (kFullC), c & 1);
-      if (zeroed) wait(bars_u + 8 * (kZeroed), 0);
-      if (c > 0) wait(bars_u + 8 * (kYM), (c - 1) & 1);
-      tc_fence_after();
-      {
-        const uint32_t b0 = fresh(bb), c0 = fresh(sm_u + K::kC);
-#pragma unroll 4
-        for (int s = 0; s < NS / 16; ++s)
-          mma_bf16_w(tm + kTG, desc(d_k, c0, kstep(s)), desc(d_k, b0, kstep(s)), kIdCB, s > 0);
-      }
-      mma_commit_w(bars + kCB);
-      // C S^T
-      wait(bars_u + 8 * (kState), c & 1);
-      if (c > 0) wait(bars_u + 8 * (kYFree), (c - 1) & 1);
-      tc_fence_after();
-      {
-        const uint32_t s0 = fresh(sm_u + K::kS), c0 = fresh(sm_u + K::kC);
-#pragma unroll 4
-        for (int s = 0; s < NS / 16; ++s)
-          mma_bf16_w(tm + kTY, desc(d_k, c0, kstep(s)), desc(d_k, s0, kstep(s)), kIdCB, s > 0);
-      }
-      mma_commit_w(bars + kYS);
-      // (f x)^T B by quarters, and M x, each as soon as its operands are there
-      bool todo = true, force = !wait.ok();  // M x is; a block that gave up does not wait
+      // The chunk's products, each as soon as its operands are there and its place is free. What
+      // the order has to keep: B's stage is free with the last quarter of dS, so C B^T comes
+      // before that; C's stage and the state's operand are free with C S^T, which so follows
+      // C B^T and precedes the last quarter.
+      bool cb = false, ys = false, ym = false, b_in = false, state_in = false;
+      bool force = !wait.ok();  // a block that gave up does not wait
       int t = 0;
-      uint32_t polls = 1u << 24;  // of some 50 cycles
+      uint32_t polls = 1u << 23;  // of some 100 cycles
+      auto ready = [&](int bar, uint32_t parity) {
+        return force || mbar_test_wait(bars_u + 8 * bar, parity);
+      };
 #pragma unroll 1
-      while (t < 4 || todo) {
-        if (todo && (force || mbar_test_wait(bars_u + 8 * kMy, c & 1))) {
-          todo = false;
+      while (!ym || t < 4) {
+        b_in = b_in || ready(kFullB + st, par);
+        state_in = state_in || ready(kState, c & 1);
+        if (b_in && state_in && t < (ys ? 4 : 3) &&
+            ready(kFx + (4 * c + t) % K::kPlaces, ((4 * c + t) / K::kPlaces) & 1)) {
+          issue_ds(tm + kTD, t);
+          ++t;
+        }
+        if (!cb) {  // over the place of the last chunk's M
+          if (b_in && ready(kFullC, c & 1) && (!zeroed || ready(kZeroed, 0)) &&
+              (c == 0 || ready(kYM, (c - 1) & 1))) {
+            cb = true;
+            tc_fence_after();
+            const uint32_t b0 = fresh(bb), c0 = fresh(sm_u + K::kC);
+#pragma unroll 4
+            for (int s = 0; s < NS / 16; ++s)
+              mma_bf16_w(tm + kTG, desc(d_k, c0, kstep(s)), desc(d_k, b0, kstep(s)), kIdCB, s > 0);
+            mma_commit_w(bars + kCB);
+          }
+        } else if (!ys) {
+          if (state_in && (c == 0 || ready(kYFree, (c - 1) & 1))) {
+            ys = true;
+            tc_fence_after();
+            const uint32_t s0 = fresh(sm_u + K::kS), c0 = fresh(sm_u + K::kC);
+#pragma unroll 4
+            for (int s = 0; s < NS / 16; ++s)
+              mma_bf16_w(tm + kTY, desc(d_k, c0, kstep(s)), desc(d_k, s0, kstep(s)), kIdCB, s > 0);
+            mma_commit_w(bars + kYS);
+          }
+        } else if (!ym && ready(kMy, c & 1)) {
+          ym = true;
           tc_fence_after();
 #pragma unroll 1
           for (int hh = 0; hh < kHeads; ++hh) {
@@ -810,10 +821,6 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
                             kIdYM, 1);
           }
           mma_commit_w(bars + kYM);
-        }
-        if (t < 4 && (force || mbar_test_wait(fx_bar(t), fx_par(t)))) {
-          issue_ds(tm + kTD, t);
-          ++t;
         }
         if (!force && --polls == 0) {
           force = true;
