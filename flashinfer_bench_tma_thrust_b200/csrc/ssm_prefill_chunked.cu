@@ -46,10 +46,10 @@ constexpr int kL = 128;             // tokens per chunk
 constexpr int kBlock = 16384;       // a [128 rows x 64 columns] bf16 tile
 
 // Registers per thread of the output kernel: 96 at launch (640 threads), then shared out anew
-// between the output's, the state's and the other warps: 256 x 88 + 256 x 120 + 128 x 64 is
+// between the output's, the state's and the other warps: 256 x 96 + 256 x 112 + 128 x 64 is
 // what 640 x 96 were. Spills are what this avoids: the shared memory leaves L1 next to nothing,
 // and a few local accesses per chunk cost more than a product.
-constexpr int kLaunchRegs = 96, kOutRegs = 88, kStateRegs = 120, kMiscRegs = 64;
+constexpr int kLaunchRegs = 96, kOutRegs = kLaunchRegs, kStateRegs = 112, kMiscRegs = 64;
 static_assert(256 * kOutRegs + 256 * kStateRegs + 128 * kMiscRegs <= 640 * kLaunchRegs, "");
 
 template <int kRegs>
@@ -143,9 +143,12 @@ struct Cfg {
   static constexpr uint32_t kXBytes = 2 * kBlock, kBBytes = kNB * kBlock;
   static constexpr uint32_t kX = 0;
   static constexpr uint32_t kB = kX + kXStages * kXBytes;
-  static constexpr uint32_t kC = kB + kBStages * kBBytes;
-  static constexpr uint32_t kS = kC + (kStates ? 0 : kBBytes);
-  static constexpr uint32_t kGates = kS + (kStates ? 0 : kBBytes);
+  // Output kernel: behind each 64-wide block of B the same block of the state, 128 rows of each,
+  // so that both are one operand of 256 rows.
+  static constexpr uint32_t kBStep = kStates ? kBlock : 2 * kBlock;
+  static constexpr uint32_t kS = kB + kBlock;
+  static constexpr uint32_t kC = kB + kBStages * kNB * kBStep;
+  static constexpr uint32_t kGates = kC + (kStates ? 0 : kBBytes);
   static constexpr uint32_t kBars = kGates + 2 * kHeads * sizeof(Gates);
   static constexpr uint32_t kBytes = kBars + 8 * 34 + 1024;  // and the alignment
 };
@@ -156,8 +159,7 @@ enum Bar {
   kFullC = 6,
   kGatesFull = 7,   // [2]
   kGatesFree = 9,   // [2]
-  kCB = 11,         // products done: C B^T
-  kYS = 12,         //   C S^T
+  kCB = 11,         // products done: C [B; S]^T
   kDS = 13,         //   dS [3, by stage of B]
   kYM = 16,         //   M x
   kFx = 17,         // f x written [4, by place]
@@ -360,7 +362,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       mbar_init(bars + kFx + i, K::kStateWarps);
       mbar_init(bars + kFxFree + i, 1);
     }
-    for (int i : {kCB, kYS, kYM}) mbar_init(bars + i, 1);
+    for (int i : {kCB, kYM}) mbar_init(bars + i, 1);
     for (int i : {kMy, kYFree}) mbar_init(bars + i, 8);
     mbar_init(bars + kZeroed, K::kStateWarps);
     mbar_init(bars + kXRead, K::kStateWarps);
@@ -382,7 +384,6 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
   };
 
   if (warp < kOutWarps) {
-    if (!kStates) regs_dec<kOutRegs>();
     // ---------------------------------------------------------------- output: token per thread
     const int half = warp >> 2;
     const int col_head = kHeads == 2 ? half : 0;  // head of columns 64 half to 64 half + 63
@@ -405,7 +406,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
           tmem_ld16(at, g);
           tmem_ld_wait();
         }
-#pragma unroll 1
+#pragma unroll
         for (int hh = 0; hh < kHeads; ++hh) {
           const uint32_t gh = ga + hh * static_cast<uint32_t>(sizeof(Gates));
           uint32_t m[8];
@@ -448,8 +449,6 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         }
       }
       // ---- Y = e^{G_i} (C S^T), in place
-      wait(bars_u + 8 * (kYS), c & 1);
-      tc_fence_after();
       {
         const float e = lds(ga + col_head * static_cast<uint32_t>(sizeof(Gates)) + kDec + 4 * row);
         const float2 e2 = make_float2(e, e);
@@ -476,36 +475,31 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       const int st = c % K::kXStages;
       const uint32_t xrow = sm_u + K::kX + st * K::kXBytes + half * kBlock + row_base(row);
       wait(bars_u + 8 * (kYM), c & 1);
-      wait(bars_u + 8 * (kXRead), c & 1);
       tc_fence_after();
       {
-#pragma unroll 1
-        for (int k0 = 0; k0 < 8; k0 += 4) {
-          float y[32];
-          uint4 xv[4];
-          tmem_ld32(lanes + kTY + 64 * half + 8 * k0, y);
+        float y[2][32];
+        tmem_ld32(lanes + kTY + 64 * half, y[0]);
+        tmem_ld32(lanes + kTY + 64 * half + 32, y[1]);
+        tmem_ld_wait();
+        tc_fence_before();
+        arrive(kYFree);  // the next chunk's first product may start
+        wait(bars_u + 8 * (kXRead), c & 1);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            xv[k] = p.D ? lds4u(xrow ^ (16 * (k0 + k))) : make_uint4(0u, 0u, 0u, 0u);
-          tmem_ld_wait();
-          if (k0 == 4) {
-            tc_fence_before();
-            arrive(kYFree);
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t at = xrow ^ (16 * k);
+          const uint4 xv = p.D ? lds4u(at) : make_uint4(0u, 0u, 0u, 0u);
+          const uint32_t u[4] = {xv.x, xv.y, xv.z, xv.w};
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 v = fma2(make_float2(skip, skip),
+                                  make_float2(__uint_as_float(u[e] << 16),
+                                              __uint_as_float(u[e] & 0xffff0000u)),
+                                  make_float2(y[k >> 2][8 * (k & 3) + 2 * e],
+                                              y[k >> 2][8 * (k & 3) + 2 * e + 1]));
+            w[e] = pack2_rn(v.x, v.y);
           }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t u[4] = {xv[k].x, xv[k].y, xv[k].z, xv[k].w};
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 v = fma2(make_float2(skip, skip),
-                                    make_float2(__uint_as_float(u[e] << 16),
-                                                __uint_as_float(u[e] & 0xffff0000u)),
-                                    make_float2(y[8 * k + 2 * e], y[8 * k + 2 * e + 1]));
-              w[e] = pack2_rn(v.x, v.y);
-            }
-            sts4u(xrow ^ (16 * (k0 + k)), w[0], w[1], w[2], w[3]);
-          }
+          sts4u(at, w[0], w[1], w[2], w[3]);
         }
       }
       if (c < chunks - 1 || tail == kL) {
@@ -572,7 +566,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
 
     // The state as the operand of the next chunk's C S^T: row = column of the block, n
     // contiguous (K-major).
-    const uint32_t s_row = sm_u + K::kS + (kNC * part >> 6) * kBlock + row_base(row);
+    const uint32_t s_row = sm_u + K::kS + (kNC * part >> 6) * K::kBStep + row_base(row);
     auto arrive_state = [&]() {
 #pragma unroll
       for (int k = 0; k < kNC / 8; ++k)
@@ -603,7 +597,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
           *reinterpret_cast<uint4*>(xt + off) = z;
           *reinterpret_cast<uint4*>(xt + kBlock + off) = z;
 #pragma unroll
-          for (int b = 0; b < K::kNB; ++b) *reinterpret_cast<uint4*>(bt + b * kBlock + off) = z;
+          for (int b = 0; b < K::kNB; ++b) *reinterpret_cast<uint4*>(bt + b * K::kBStep + off) = z;
         }
         fence_async_smem();
         named_bar_sync(2, K::kStateWarps * 32);
@@ -624,9 +618,9 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       ldmatrix_x4_trans(xa ^ 32, u[1]);
       if (k >= K::kPlaces) wait(bars_u + 8 * (kFxFree + place), (k / K::kPlaces - 1) & 1);
       const uint32_t at = lanes + (kStates ? 0 : kTF) + 16 * kTerms * place + 8 * part;
-      uint32_t w[2][kTerms][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        uint32_t w[kTerms][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           // 24 bits in three bf16 terms of 8 by truncation: their sum is x f to the last bit
@@ -636,18 +630,15 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
 #pragma unroll
           for (int r = 0; r < kTerms; ++r) {
             const uint32_t a = __float_as_uint(v.x), b = __float_as_uint(v.y);
-            w[h][r][i] = __byte_perm(a, b, 0x7632);
+            w[r][i] = __byte_perm(a, b, 0x7632);
             if (r + 1 < kTerms)
               v = sub2(v, make_float2(__uint_as_float(a & 0xffff0000u),
                                       __uint_as_float(b & 0xffff0000u)));
           }
         }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
 #pragma unroll
         for (int r = 0; r < kTerms; ++r)
-          tmem_st_frag(at + 16 * r + (static_cast<uint32_t>(16 * h) << 16), w[h][r]);
+          tmem_st_frag(at + 16 * r + (static_cast<uint32_t>(16 * h) << 16), w[r]);
       }
       tmem_st_wait();
       tc_fence_before();
@@ -696,7 +687,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         }
         if (t == 0 && c > 0) {
           update_state(c - 1);
-          // C S^T has read the state it replaces: it came before dS
+          // C S^T has read the state it replaces: it came before dS's end
           if (!kStates && c < chunks) arrive_state();
           if (kStates) arrive(kState + ((c - 1) & 1));
         }
@@ -720,12 +711,13 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     if (!kStates) regs_dec<kMiscRegs>();
     if (warp == kMisc) {
     // ---------------------------------------------------------------- products
-    constexpr uint32_t kIdCB = idesc_bf16(128, 128, false, false);
+    constexpr uint32_t kIdCB = idesc_bf16(128, 256, false, false);
     constexpr uint32_t kIdDS = idesc_bf16(128, NS, false, true);
     constexpr uint32_t kIdYM = idesc_bf16(128, P, false, true);
     // Descriptors differ in their start address alone: built where they are used, from bases
     // that look new in every chunk, or all of them would be kept in registers.
-    const uint64_t d_k = desc_kmajor(0), d_mn = desc_mnmajor(0, kBlock);
+    const uint64_t d_k = desc_kmajor(0), d_x = desc_mnmajor(0, kBlock),
+                   d_b = desc_mnmajor(0, K::kBStep);
     auto fresh = [](uint32_t v) {
       uint32_t r;
       asm volatile("mov.u32 %0, %1;" : "=r"(r) : "r"(v));
@@ -734,7 +726,9 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     auto desc = [](uint64_t kind, uint32_t base, uint32_t off) {
       return kind | static_cast<uint64_t>((base + off) >> 4);
     };
-    auto kstep = [](int s) { return static_cast<uint32_t>((s >> 2) * kBlock + (s & 3) * 32); };
+    auto kstep = [](int s, uint32_t block) {
+      return static_cast<uint32_t>((s >> 2) * block + (s & 3) * 32);
+    };
     for (int c = 0; c < chunks; ++c) {
       const int st = c % K::kBStages, par = (c / K::kBStages) & 1;
       const uint32_t xb = sm_u + K::kX + (c % K::kXStages) * K::kXBytes;
@@ -750,7 +744,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         for (int r = 0; r < kTerms; ++r) {
 #pragma unroll
           for (int s = 0; s < 2; ++s)
-            mma_bf16_ts_w(td, tf + 16 * r + 8 * s, desc(d_mn, b0, s * 2048), kIdDS,
+            mma_bf16_ts_w(td, tf + 16 * r + 8 * s, desc(d_b, b0, s * 2048), kIdDS,
                           t > 0 || r > 0 || s > 0);
         }
         mma_commit_w(bars + kFxFree + place);
@@ -769,10 +763,9 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         continue;
       }
       // The chunk's products, each as soon as its operands are there and its place is free. What
-      // the order has to keep: B's stage is free with the last quarter of dS, so C B^T comes
-      // before that; C's stage and the state's operand are free with C S^T, which so follows
-      // C B^T and precedes the last quarter.
-      bool cb = false, ys = false, ym = false, b_in = false, state_in = false;
+      // the order has to keep: B's stage and the state's operand are free with the last quarter
+      // of dS, so C [B; S]^T comes before that.
+      bool cb = false, ym = false, b_in = false, state_in = false;
       bool force = !wait.ok();  // a block that gave up does not wait
       int t = 0;
       uint32_t polls = 1u << 23;  // of some 100 cycles
@@ -783,31 +776,22 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       while (!ym || t < 4) {
         b_in = b_in || ready(kFullB + st, par);
         state_in = state_in || ready(kState, c & 1);
-        if (b_in && state_in && t < (ys ? 4 : 3) &&
+        if (b_in && state_in && t < (cb ? 4 : 3) &&
             ready(kFx + (4 * c + t) % K::kPlaces, ((4 * c + t) / K::kPlaces) & 1)) {
           issue_ds(tm + kTD, t);
           ++t;
         }
-        if (!cb) {  // over the place of the last chunk's M
-          if (b_in && ready(kFullC, c & 1) && (!zeroed || ready(kZeroed, 0)) &&
-              (c == 0 || ready(kYM, (c - 1) & 1))) {
+        if (!cb) {  // over the places of the last chunk's M and Y
+          if (b_in && state_in && ready(kFullC, c & 1) && (!zeroed || ready(kZeroed, 0)) &&
+              (c == 0 || ready(kYFree, (c - 1) & 1))) {
             cb = true;
             tc_fence_after();
             const uint32_t b0 = fresh(bb), c0 = fresh(sm_u + K::kC);
 #pragma unroll 4
             for (int s = 0; s < NS / 16; ++s)
-              mma_bf16_w(tm + kTG, desc(d_k, c0, kstep(s)), desc(d_k, b0, kstep(s)), kIdCB, s > 0);
+              mma_bf16_w(tm + kTG, desc(d_k, c0, kstep(s, kBlock)),
+                         desc(d_k, b0, kstep(s, K::kBStep)), kIdCB, s > 0);
             mma_commit_w(bars + kCB);
-          }
-        } else if (!ys) {
-          if (state_in && (c == 0 || ready(kYFree, (c - 1) & 1))) {
-            ys = true;
-            tc_fence_after();
-            const uint32_t s0 = fresh(sm_u + K::kS), c0 = fresh(sm_u + K::kC);
-#pragma unroll 4
-            for (int s = 0; s < NS / 16; ++s)
-              mma_bf16_w(tm + kTY, desc(d_k, c0, kstep(s)), desc(d_k, s0, kstep(s)), kIdCB, s > 0);
-            mma_commit_w(bars + kYS);
           }
         } else if (!ym && ready(kMy, c & 1)) {
           ym = true;
@@ -817,7 +801,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
             const uint32_t x0 = fresh(xb + hh * kBlock);
 #pragma unroll 4
             for (int s = 0; s < 8; ++s)
-              mma_bf16_ts_w(tm + kTY + hh * 64, tm + kTG + 16 * s + 8 * hh, desc(d_mn, x0, s * 2048),
+              mma_bf16_ts_w(tm + kTY + hh * 64, tm + kTG + 16 * s + 8 * hh, desc(d_x, x0, s * 2048),
                             kIdYM, 1);
           }
           mma_commit_w(bars + kYM);
@@ -849,7 +833,9 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       auto load_b = [&](int c) {
         const int st = c % K::kBStages;
         mbar_arrive_expect_tx(bars + kFullB + st, K::kBBytes);
-        tma_load_3d(sm + K::kB + st * K::kBBytes, &maps.b, bars + kFullB + st, 0, tok0 + c * kL, bc);
+        for (int b = 0; b < K::kNB; ++b)
+          tma_load_3d(sm + K::kB + st * K::kBBytes + b * K::kBStep, &maps.b, bars + kFullB + st, 0,
+                      tok0 + c * kL, bc + b);
       };
       auto load_c = [&](int c) {
         mbar_arrive_expect_tx(bars + kFullC, K::kBBytes);
@@ -864,11 +850,12 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         if (!kStates && c + 2 < chunks) {
           // B and C have one stage: bring the next but one chunk's into L2, so that the copy
           // that has to wait for the stage takes only L2's latency
-          tma_prefetch_3d(&maps.b, 0, tok0 + (c + 2) * kL, bc);
+          for (int b = 0; b < K::kNB; ++b)
+            tma_prefetch_3d(&maps.b, 0, tok0 + (c + 2) * kL, bc + b);
           tma_prefetch_3d(&maps.c, 0, tok0 + (c + 2) * kL, bc);
         }
         if (!kStates && c + 1 < chunks) {
-          wait(bars_u + 8 * (kYS), c & 1);
+          wait(bars_u + 8 * (kCB), c & 1);
           load_c(c + 1);
         }
         if (c + K::kBStages < chunks) {
@@ -980,7 +967,7 @@ int launch_as(const SsmParams& p, cudaStream_t stream) {
   const int64_t T = p.T > 0 ? p.T : 1;
   const bool any = p.T > 0;
   if (!encode(&maps.x, any ? static_cast<const void*>(p.x) : p.new_state, T, hp, 2) ||
-      !encode(&maps.b, any ? static_cast<const void*>(p.B) : p.new_state, T, gn, NS / 64) ||
+      !encode(&maps.b, any ? static_cast<const void*>(p.B) : p.new_state, T, gn, 1) ||
       !encode(&maps.c, any ? static_cast<const void*>(p.C) : p.new_state, T, gn, NS / 64) ||
       !encode(&maps.out, any ? static_cast<const void*>(p.out) : p.new_state, T, hp, 1))
     return GDN_ERR_CUDA;
