@@ -46,10 +46,10 @@ constexpr int kL = 128;             // tokens per chunk
 constexpr int kBlock = 16384;       // a [128 rows x 64 columns] bf16 tile
 
 // Registers per thread of the output kernel: 96 at launch (640 threads), then shared out anew
-// between the output's, the state's and the other warps: 256 x 96 + 256 x 112 + 128 x 64 is
+// between the output's, the state's and the other warps: 256 x 96 + 256 x 104 + 128 x 80 is
 // what 640 x 96 were. Spills are what this avoids: the shared memory leaves L1 next to nothing,
 // and a few local accesses per chunk cost more than a product.
-constexpr int kLaunchRegs = 96, kOutRegs = kLaunchRegs, kStateRegs = 112, kMiscRegs = 64;
+constexpr int kLaunchRegs = 96, kOutRegs = kLaunchRegs, kStateRegs = 104, kMiscRegs = 80;
 static_assert(256 * kOutRegs + 256 * kStateRegs + 128 * kMiscRegs <= 640 * kLaunchRegs, "");
 
 template <int kRegs>
@@ -383,12 +383,71 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     if (lane == 0) mbar_arrive(bars + bar);
   };
 
+  const int part = (warp >> 2) & 1;            // of the two warps of a quarter in each role
+  const int row_head = kHeads == 2 ? q >> 1 : 0;  // head of column `row`
+  // (f x)^T of tokens 32 t to 32 t + 31 of chunk c into TMEM (this warp: 16 of them, of columns
+  // 32 q to 32 q + 31): transposed by ldmatrix, scaled, split and stored as the fragments come.
+  // Lane l gives ldmatrix token l % 8 + 8 (l / 16) of the 16, columns 8 ((l / 8) % 2) on.
+  const uint32_t x_lane = 2048 * part + (row_base(8 * (lane >> 4) + (lane & 7)) ^
+                                         (16 * ((q & 1) * 4 + ((lane >> 3) & 1))));
+  auto write_fx = [&](int c, int t) {
+    const int k = 4 * c + t, place = k % K::kPlaces;
+    const uint32_t f = gates_u +
+                       ((c & 1) * kHeads + row_head) * static_cast<uint32_t>(sizeof(Gates)) + kF +
+                       4 * (32 * t + 16 * part) + 8 * (lane & 3);
+    const float2 f0 = lds2(f), f1 = lds2(f + 32);
+    const uint32_t xa = sm_u + K::kX + (c % K::kXStages) * K::kXBytes + (q >> 1) * kBlock +
+                        128 * 32 * t + x_lane;
+    uint32_t u[2][4];  // [columns 0-15, 16-31]: tokens 0-7 of columns 0-7, 8-15; tokens 8-15
+    ldmatrix_x4_trans(xa, u[0]);
+    ldmatrix_x4_trans(xa ^ 32, u[1]);
+    if (k >= K::kPlaces) wait(bars_u + 8 * (kFxFree + place), (k / K::kPlaces - 1) & 1);
+    const uint32_t at = lanes + (kStates ? 0 : kTF) + 16 * kTerms * place + 8 * part;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t w[kTerms][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // 24 bits in three bf16 terms of 8 by truncation: their sum is x f to the last bit
+        float2 v = mul2(make_float2(__uint_as_float(u[h][i] << 16),
+                                    __uint_as_float(u[h][i] & 0xffff0000u)),
+                        i < 2 ? f0 : f1);
+#pragma unroll
+        for (int r = 0; r < kTerms; ++r) {
+          const uint32_t a = __float_as_uint(v.x), b = __float_as_uint(v.y);
+          w[r][i] = __byte_perm(a, b, 0x7632);
+          if (r + 1 < kTerms)
+            v = sub2(v, make_float2(__uint_as_float(a & 0xffff0000u),
+                                    __uint_as_float(b & 0xffff0000u)));
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < kTerms; ++r)
+        tmem_st_frag(at + 16 * r + (static_cast<uint32_t>(16 * h) << 16), w[r]);
+    }
+    tmem_st_wait();
+    tc_fence_before();
+    arrive(kFx + place);
+    if (!kStates && t == 3) arrive(kXRead);
+  };
+
   if (warp < kOutWarps) {
     // ---------------------------------------------------------------- output: token per thread
-    const int half = warp >> 2;
+    const int half = part;
     const int col_head = kHeads == 2 ? half : 0;  // head of columns 64 half to 64 half + 63
     const float skip = p.D && col_head < heads ? load_scalar(p.D, p.D_dtype, h0 + col_head) : 0.f;
-    for (int c = 0; c < chunks; ++c) {
+    // f x of a chunk's first quarter is this role's: it is written while M x runs, and keeps the
+    // state's warps, which have the longer way, from waiting on their own products.
+    auto first_fx = [&](int c) {
+      wait(bars_u + 8 * (kFullX + c % K::kXStages), (c / K::kXStages) & 1);
+      if (c == chunks - 1 && tail < kL) wait(bars_u + 8 * (kZeroed), 0);
+      wait(bars_u + 8 * (kGatesFull + (c & 1)), (c >> 1) & 1);
+      write_fx(c, 0);
+    };
+    // (turn -1 only writes the first chunk's)
+#pragma unroll 1
+    for (int c = -1; c < chunks; ++c) {
+     if (c >= 0) {
       const int gs = c & 1;
       const uint32_t ga = gates_u + gs * kHeads * static_cast<uint32_t>(sizeof(Gates));
       wait(bars_u + 8 * (kGatesFull + gs), (c >> 1) & 1);
@@ -471,6 +530,9 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       tc_fence_before();
       arrive(kMy);
       arrive(kGatesFree + gs);
+     }
+     if (c + 1 < chunks) first_fx(c + 1);
+     if (c >= 0) {
       // ---- y: out of TMEM, D x added, over the chunk's x in shared memory
       const int st = c % K::kXStages;
       const uint32_t xrow = sm_u + K::kX + st * K::kXBytes + half * kBlock + row_base(row);
@@ -520,13 +582,12 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
           }
         }
       }
+     }
     }
   } else if (warp < kMisc) {
     if (!kStates) regs_inc<kStateRegs>();
     // ---------------------------------------------------------------- state: column per thread
     constexpr int kNC = NS / 2;                  // state columns per thread
-    const int part = (warp - kOutWarps) >> 2;
-    const int row_head = kHeads == 2 ? q >> 1 : 0;   // head of column `row`
     const int64_t st_off =
         ((n * p.H + h0) * static_cast<int64_t>(P) + row) * NS + kNC * part;
     const bool mine = row_head < heads;
@@ -577,11 +638,6 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       arrive(kState);
     };
 
-    // (f x)^T into TMEM, 32 tokens at a time (this warp: 16 of them, of columns 32 q to
-    // 32 q + 31): transposed by ldmatrix, scaled, split and stored as the fragments come. Lane
-    // l gives ldmatrix token l % 8 + 8 (l / 16) of the 16, columns 8 ((l / 8) % 2) on.
-    const uint32_t x_lane = row_base(16 * part + 8 * (lane >> 4) + (lane & 7)) ^
-                            (16 * ((q & 1) * 4 + ((lane >> 3) & 1)));
     auto begin_fx = [&](int c) {
       const int st = c % K::kXStages;
       uint8_t* const xt = sm + K::kX + st * K::kXBytes;
@@ -605,47 +661,6 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       }
       wait(bars_u + 8 * (kGatesFull + (c & 1)), (c >> 1) & 1);
     };
-    auto write_fx = [&](int c, int t) {  // tokens 32 t to 32 t + 31 of chunk c
-      const int k = 4 * c + t, place = k % K::kPlaces;
-      const uint32_t f = gates_u +
-                         ((c & 1) * kHeads + row_head) * static_cast<uint32_t>(sizeof(Gates)) + kF +
-                         4 * (32 * t + 16 * part) + 8 * (lane & 3);
-      const float2 f0 = lds2(f), f1 = lds2(f + 32);
-      const uint32_t xa = sm_u + K::kX + (c % K::kXStages) * K::kXBytes + (q >> 1) * kBlock +
-                          128 * 32 * t + x_lane;
-      uint32_t u[2][4];  // [columns 0-15, 16-31]: tokens 0-7 of columns 0-7, 8-15; tokens 8-15
-      ldmatrix_x4_trans(xa, u[0]);
-      ldmatrix_x4_trans(xa ^ 32, u[1]);
-      if (k >= K::kPlaces) wait(bars_u + 8 * (kFxFree + place), (k / K::kPlaces - 1) & 1);
-      const uint32_t at = lanes + (kStates ? 0 : kTF) + 16 * kTerms * place + 8 * part;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t w[kTerms][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // 24 bits in three bf16 terms of 8 by truncation: their sum is x f to the last bit
-          float2 v = mul2(make_float2(__uint_as_float(u[h][i] << 16),
-                                      __uint_as_float(u[h][i] & 0xffff0000u)),
-                          i < 2 ? f0 : f1);
-#pragma unroll
-          for (int r = 0; r < kTerms; ++r) {
-            const uint32_t a = __float_as_uint(v.x), b = __float_as_uint(v.y);
-            w[r][i] = __byte_perm(a, b, 0x7632);
-            if (r + 1 < kTerms)
-              v = sub2(v, make_float2(__uint_as_float(a & 0xffff0000u),
-                                      __uint_as_float(b & 0xffff0000u)));
-          }
-        }
-#pragma unroll
-        for (int r = 0; r < kTerms; ++r)
-          tmem_st_frag(at + 16 * r + (static_cast<uint32_t>(16 * h) << 16), w[r]);
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      arrive(kFx + place);
-      if (!kStates && t == 3) arrive(kXRead);
-    };
-
     // The state behind chunk c, from what the chunk adds.
     auto update_state = [&](int c) {
       wait(bars_u + 8 * (kDS + c % K::kBStages), (c / K::kBStages) & 1);
@@ -673,23 +688,28 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       arrive(kGatesFree + (c & 1));
     };
 
-    // Turn i of the loop writes quarter i % 4 of chunk i / 4, and updates the state with the chunk
-    // before after the first quarter, while the products of that chunk's end still run; one
-    // more turn updates it with the last chunk. (One loop: each part of the code exists once.)
+    // Turn i of the loop writes one quarter of f x (the output kernel: its other warps write each
+    // chunk's first) and, with a chunk's first turn, updates the state with the chunk before;
+    // one more turn updates it with the last chunk. (One loop: each part of the code exists once.)
     if (chunks > 0) {
+      constexpr int kTurns = kStates ? 4 : 3;
       if (!kStates) arrive_state();
+      int c = 0, t = 4 - kTurns;
 #pragma unroll 1
-      for (int i = 0; i <= 4 * chunks; ++i) {
-        const int c = i >> 2, t = i & 3;
-        if (c < chunks) {
-          if (t == 0) begin_fx(c);
-          write_fx(c, t);
-        }
-        if (t == 0 && c > 0) {
+      for (int i = 0; i <= kTurns * chunks; ++i) {
+        const bool first = t == 4 - kTurns;
+        if (first && c < chunks) begin_fx(c);
+        if (kStates && c < chunks) write_fx(c, t);  // while the last chunk's products still run
+        if (first && c > 0) {
           update_state(c - 1);
           // C S^T has read the state it replaces: it came before dS's end
           if (!kStates && c < chunks) arrive_state();
           if (kStates) arrive(kState + ((c - 1) & 1));
+        }
+        if (!kStates && c < chunks) write_fx(c, t);
+        if (++t == 4) {
+          t = 4 - kTurns;
+          ++c;
         }
       }
     }
