@@ -138,7 +138,8 @@ struct Cfg {
   static constexpr int kXStages = 3, kBStages = kStates ? 3 : 1;
   // f x is written by 32 tokens, into places in turn.
   static constexpr int kPlaces = kStates ? 4 : 2;
-  static constexpr int kOutWarps = kStates ? 0 : 8, kStateWarps = 8;
+  static constexpr int kOutWarps = kStates ? 0 : 8, kStateWarps = kStates ? 16 : 8;
+  static constexpr int kFxWarps = 8;  // that write one quarter of a chunk's f x
   static constexpr int kThreads = 32 * (kOutWarps + kStateWarps + 4);
   static constexpr uint32_t kXBytes = 2 * kBlock, kBBytes = kNB * kBlock;
   static constexpr uint32_t kX = 0;
@@ -359,7 +360,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       mbar_init(bars + kState + i, K::kStateWarps);
     }
     for (int i = 0; i < 4; ++i) {
-      mbar_init(bars + kFx + i, K::kStateWarps);
+      mbar_init(bars + kFx + i, K::kFxWarps);
       mbar_init(bars + kFxFree + i, 1);
     }
     for (int i : {kCB, kYM}) mbar_init(bars + i, 1);
@@ -587,9 +588,10 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
   } else if (warp < kMisc) {
     if (!kStates) regs_inc<kStateRegs>();
     // ---------------------------------------------------------------- state: column per thread
-    constexpr int kNC = NS / 2;                  // state columns per thread
+    constexpr int kNC = NS * 4 / K::kStateWarps;  // state columns per thread, from kNC * sp on
+    const int sp = (warp - kOutWarps) >> 2;
     const int64_t st_off =
-        ((n * p.H + h0) * static_cast<int64_t>(P) + row) * NS + kNC * part;
+        ((n * p.H + h0) * static_cast<int64_t>(P) + row) * NS + kNC * sp;
     const bool mine = row_head < heads;
     float S[kNC];
 #pragma unroll
@@ -612,7 +614,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       for (int64_t r = slot - seg; r < slot; ++r) {  // this sequence's segments before this one
         const float g = sg.left[r * p.H + h0 + row_head];
         const float* src =
-            sg.add + ((r * p.H + h0) * static_cast<int64_t>(P) + row) * NS + kNC * part;
+            sg.add + ((r * p.H + h0) * static_cast<int64_t>(P) + row) * NS + kNC * sp;
 #pragma unroll
         for (int i = 0; i < kNC; i += 4) {
           const float4 v = *reinterpret_cast<const float4*>(src + i);
@@ -627,11 +629,11 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
 
     // The state as the operand of the next chunk's C S^T: row = column of the block, n
     // contiguous (K-major).
-    const uint32_t s_row = sm_u + K::kS + (kNC * part >> 6) * K::kBStep + row_base(row);
+    const uint32_t s_row = sm_u + K::kS + (kNC * sp >> 6) * K::kBStep + row_base(row);
     auto arrive_state = [&]() {
 #pragma unroll
       for (int k = 0; k < kNC / 8; ++k)
-        sts4u(s_row ^ (16 * (((kNC * part >> 3) + k) & 7)), pack2_rn(S[8 * k], S[8 * k + 1]),
+        sts4u(s_row ^ (16 * (((kNC * sp >> 3) + k) & 7)), pack2_rn(S[8 * k], S[8 * k + 1]),
               pack2_rn(S[8 * k + 2], S[8 * k + 3]), pack2_rn(S[8 * k + 4], S[8 * k + 5]),
               pack2_rn(S[8 * k + 6], S[8 * k + 7]));
       fence_async_smem();
@@ -669,7 +671,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
           lds(gates_u + ((c & 1) * kHeads + row_head) * static_cast<uint32_t>(sizeof(Gates)) + kDec +
               4 * (kL - 1));
       const float2 g2 = make_float2(g, g);
-      const uint32_t td = lanes + kTD + (kStates ? 128 * (c & 1) : 0) + kNC * part;
+      const uint32_t td = lanes + kTD + (kStates ? 128 * (c & 1) : 0) + kNC * sp;
 #pragma unroll
       for (int i0 = 0; i0 < kNC; i0 += 16) {
         float v[16];
@@ -692,12 +694,14 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     // chunk's first) and, with a chunk's first turn, updates the state with the chunk before;
     // one more turn updates it with the last chunk. (One loop: each part of the code exists once.)
     if (chunks > 0) {
-      constexpr int kTurns = kStates ? 4 : 3;
+      // the states kernel's two times 8 warps take every other quarter
+      const int t0 = kStates ? warp >> 3 : 1;
+      constexpr int kStep = kStates ? 2 : 1, kTurns = kStates ? 2 : 3;
       if (!kStates) arrive_state();
-      int c = 0, t = 4 - kTurns;
+      int c = 0, t = t0;
 #pragma unroll 1
       for (int i = 0; i <= kTurns * chunks; ++i) {
-        const bool first = t == 4 - kTurns;
+        const bool first = t == t0;
         if (first && c < chunks) begin_fx(c);
         if (kStates && c < chunks) write_fx(c, t);  // while the last chunk's products still run
         if (first && c > 0) {
@@ -707,8 +711,8 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
           if (kStates) arrive(kState + ((c - 1) & 1));
         }
         if (!kStates && c < chunks) write_fx(c, t);
-        if (++t == 4) {
-          t = 4 - kTurns;
+        if ((t += kStep) >= 4) {
+          t = t0;
           ++c;
         }
       }
@@ -716,8 +720,8 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     if (mine) {
       float* dst = nullptr;
       if (kStates) {
-        dst = sg.add + ((slot * p.H + h0) * static_cast<int64_t>(P) + row) * NS + kNC * part;
-        if (part == 0 && row % P == 0) sg.left[slot * p.H + h0 + row_head] = left;
+        dst = sg.add + ((slot * p.H + h0) * static_cast<int64_t>(P) + row) * NS + kNC * sp;
+        if (sp == 0 && row % P == 0) sg.left[slot * p.H + h0 + row_head] = left;
       } else if (last) {
         dst = static_cast<float*>(p.new_state) + st_off;
       }
@@ -914,27 +918,32 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     const int h = h0 + (present ? hh : 0);
     const float neg_a = -expf(load_scalar(p.A_log, p.A_log_dtype, h));
     const float dtb = load_scalar(p.dt_bias, p.dt_bias_dtype, h);
-    auto load = [&](int c, float (&raw)[4]) {
+    // dt of a chunk as stored, asked for a chunk ahead: nothing may use a value before its chunk
+    // (a conversion here would wait for each of the four in turn, 800 cycles each)
+    const bool half = p.dt_dtype == kBF16;
+    auto load = [&](int c, uint32_t (&raw)[4]) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int t = c * kL + 32 * k + lane;
-        raw[k] = t < tokens
-                     ? load_scalar(p.dt, p.dt_dtype, (static_cast<int64_t>(tok0) + t) * p.H + h)
-                     : 0.f;
+        const int t = min(c * kL + 32 * k + lane, tokens - 1);
+        const int64_t at = (static_cast<int64_t>(tok0) + t) * p.H + h;
+        raw[k] = half ? static_cast<const unsigned short*>(p.dt)[at]
+                      : static_cast<const uint32_t*>(p.dt)[at];
       }
     };
-    float raw[4];
+    uint32_t raw[4];
     if (chunks > 0) load(0, raw);
+#pragma unroll 1
     for (int c = 0; c < chunks; ++c) {
       const int gs = c & 1;
-      float next[4] = {0.f, 0.f, 0.f, 0.f};
-      if (c + 1 < chunks) load(c + 1, next);
+      float dt[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) dt[k] = __uint_as_float(half ? raw[k] << 16 : raw[k]);
+      if (c + 1 < chunks) load(c + 1, raw);
       if (c >= 2) wait(bars_u + 8 * (kGatesFree + gs), ((c >> 1) - 1) & 1);
-      write_gates(gates_u + (gs * kHeads + hh) * static_cast<uint32_t>(sizeof(Gates)), raw, neg_a, dtb, present ? tokens - c * kL : 0, lane);
+      write_gates(gates_u + (gs * kHeads + hh) * static_cast<uint32_t>(sizeof(Gates)), dt, neg_a,
+                  dtb, present ? tokens - c * kL : 0, lane);
       __syncwarp();
       if (lane == 0) mbar_arrive(bars + kGatesFull + gs);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) raw[k] = next[k];
     }
   }
   }
