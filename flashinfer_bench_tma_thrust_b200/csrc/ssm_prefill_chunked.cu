@@ -70,6 +70,10 @@ __device__ __forceinline__ float lds(uint32_t a) {
 __device__ __forceinline__ void sts(uint32_t a, float v) {
   asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
 }
+__device__ __forceinline__ void sts4(uint32_t a, float x, float y, float z, float w) {
+  asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(a), "f"(x), "f"(y), "f"(z), "f"(w)
+               : "memory");
+}
 __device__ __forceinline__ float2 lds2(uint32_t a) {
   float2 v;
   asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
@@ -119,6 +123,10 @@ struct Gates {
 constexpr uint32_t kCum = 0, kDec = 512, kU = 1024, kF = 1536, kD = 2048, kTot = 2560;
 static_assert(sizeof(Gates) == kTot + 16, "");
 
+// Chunks whose gates there is room for. The gates' warp takes some 3000 cycles a chunk, in a chain
+// of short dependent steps: with two stages it was in the loop of the others' waits.
+constexpr int kGateStages = 4;
+
 struct Maps {
   CUtensorMap x, b, c, out;         // {64, T, columns / 64}, box {64, 128, blocks}
 };
@@ -150,27 +158,29 @@ struct Cfg {
   static constexpr uint32_t kS = kB + kBlock;
   static constexpr uint32_t kC = kB + kBStages * kNB * kBStep;
   static constexpr uint32_t kGates = kC + (kStates ? 0 : kBBytes);
-  static constexpr uint32_t kBars = kGates + 2 * kHeads * sizeof(Gates);
-  static constexpr uint32_t kBytes = kBars + 8 * 34 + 1024;  // and the alignment
+  static constexpr uint32_t kBars = kGates + kGateStages * kHeads * sizeof(Gates);
+  static constexpr uint32_t kBytes = kBars + 8 * 40 + 1024;  // and the alignment
 };
 
+static_assert(sizeof(Gates) % 16 == 0, "");
 enum Bar {
-  kFullX = 0,       // [3] one per stage
-  kFullB = 3,       // [3]
-  kFullC = 6,
-  kGatesFull = 7,   // [2]
-  kGatesFree = 9,   // [2]
-  kCB = 11,         // products done: C [B; S]^T
-  kDS = 13,         //   dS [3, by stage of B]
-  kYM = 16,         //   M x
-  kFx = 17,         // f x written [4, by place]
-  kFxFree = 21,     // f x read by its products [4]
-  kMy = 25,         // M and the scaled Y written
-  kState = 26,      // S written, dS read [2]
-  kYFree = 28,      // Y read out
-  kStaged = 29,     // y in shared memory [3]
-  kZeroed = 32,
-  kXRead = 33,      // x read by the state's warps, so that y may replace it
+  kFullX = 0,                          // [3] one per stage
+  kFullB = kFullX + 3,                 // [3]
+  kFullC = kFullB + 3,
+  kGatesFull = kFullC + 1,             // [kGateStages]
+  kGatesFree = kGatesFull + kGateStages,
+  kCB = kGatesFree + kGateStages,      // products done: C [B; S]^T
+  kDS = kCB + 1,                       //   dS [3, by stage of B]
+  kYM = kDS + 3,                       //   M x
+  kFx = kYM + 1,                       // f x written [4, by place]
+  kFxFree = kFx + 4,                   // f x read by its products [4]
+  kMy = kFxFree + 4,                   // M and the scaled Y written
+  kState = kMy + 1,                    // S written, dS read [2]
+  kYFree = kState + 2,                 // Y read out
+  kStaged = kYFree + 1,                // y in shared memory [3]
+  kZeroed = kStaged + 3,
+  kXRead = kZeroed + 1,                // x read by the state's warps, so that y may replace it
+  kBarCount = kXRead + 1,
 };
 
 // Bounded waits in few instructions (the roles' code has to stay in the instruction cache: see
@@ -247,53 +257,76 @@ __device__ __forceinline__ void find_segment(const SsmParams& p, const Segments&
   n = p.N;
 }
 
-// Gates of a chunk's first `valid` tokens (the others: d = 0, no decay) of one head, a block of
-// 32 tokens at a time, token per lane; raw: dt of the four blocks. All sums run over terms of
-// one sign, so none of them cancels.
+// softplus(v) = max(v, 0) + log(1 + u), u = e^-|v|, with log(1 + u) = 2 atanh(s) by its series in
+// s = u / (2 + u) <= 1/3: a tenth of the instructions of log1pf(expf(v)), which with one or two
+// warps on all of a chunk's gates set the pace of the kernel. The first term left out is below
+// 2^-28 of the sum; u has ex2.approx's 2 ulp and, through the exponent's rest, no more.
+__device__ __forceinline__ float softplus(float v) {
+  const float x = -fabsf(v);
+  const float z = x * kLog2e;
+  const float rest = fmaf(x, kLog2e, -z);  // what rounding z left
+  const float e = ex2(z);
+  const float u = fmaf(e * 0.6931472f, rest, e);
+  const float s = __fdividef(u, 2.f + u), q = s * s;
+  float p = 1.f / 15.f;
+  p = fmaf(p, q, 1.f / 13.f);
+  p = fmaf(p, q, 1.f / 11.f);
+  p = fmaf(p, q, 1.f / 9.f);
+  p = fmaf(p, q, 1.f / 7.f);
+  p = fmaf(p, q, 1.f / 5.f);
+  p = fmaf(p, q, 1.f / 3.f);
+  const float t = s + s;
+  return fmaxf(v, 0.f) + fmaf(t, p * q, t) + (v != v ? v : 0.f);  // (fmaxf drops a NaN)
+}
+
+// Gates of a chunk's first `valid` tokens (the others: d = 0, no decay) of one head, four tokens
+// per lane (a block of 32: eight lanes). All sums run over terms of one sign, so none cancels.
 __device__ __forceinline__ void write_gates(uint32_t g, const float (&raw)[4], float neg_a, float dtb,
                                             int valid, int lane) {
-  float tot[4];
-#pragma unroll 2
+  float d[4], lg[4];
+#pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const bool in = 32 * k + lane < valid;
-    const float r = k == 0 ? raw[0] : (k == 1 ? raw[1] : (k == 2 ? raw[2] : raw[3]));
-    const float d = in ? softplus_ref(r + dtb) : 0.f;
-    float lg = in ? neg_a * d * kLog2e : 0.f;
+    const bool in = lane * 4 + k < valid;
+    d[k] = in ? softplus(raw[k] + dtb) : 0.f;
+    const float l = in ? neg_a * d[k] * kLog2e : 0.f;
     // 2^-127 is zero to ex2: a stronger decay changes nothing, and the sums stay small. A NaN
     // stays one.
-    lg = lg < -127.f ? -127.f : lg;
-    float pre = lg, suf = lg;  // over the block, up to and from this token
+    lg[k] = l < -127.f ? -127.f : l;
+  }
+  float pre = (lg[0] + lg[1]) + (lg[2] + lg[3]), suf = pre;  // over the block, to and from here
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const float a = __shfl_up_sync(0xffffffffu, pre, o);
-      const float b = __shfl_down_sync(0xffffffffu, suf, o);
-      if (lane >= o) pre += a;
-      if (lane + o < 32) suf += b;
-    }
-    float behind = __shfl_down_sync(0xffffffffu, suf, 1);
-    if (lane == 31) behind = 0.f;
-    const float t = __shfl_sync(0xffffffffu, pre, 31);
-    const uint32_t at = g + 4 * (32 * k + lane);
-    sts(at + kCum, pre);
-    sts(at + kD, d);
-    sts(at + kU, d * ex2(behind));
-    sts(at + kF, behind);  // until the blocks behind are known
-    if (lane == 0) sts(g + kTot + 4 * k, t);
-    tot[0] = k == 0 ? t : tot[0];
-    tot[1] = k == 1 ? t : tot[1];
-    tot[2] = k == 2 ? t : tot[2];
-    tot[3] = t;
+  for (int o = 1; o < 8; o <<= 1) {
+    const float a = __shfl_up_sync(0xffffffffu, pre, o, 8);
+    const float b = __shfl_down_sync(0xffffffffu, suf, o, 8);
+    if ((lane & 7) >= o) pre += a;
+    if ((lane & 7) + o < 8) suf += b;
   }
-#pragma unroll 2
-  for (int k = 0; k < 4; ++k) {
-    const float head = k == 0 ? 0.f : (k == 1 ? tot[0] : (k == 2 ? tot[0] + tot[1]
-                                                                 : tot[0] + tot[1] + tot[2]));
-    const float tail = k == 3 ? 0.f : (k == 2 ? tot[3] : (k == 1 ? tot[2] + tot[3]
-                                                                 : tot[1] + tot[2] + tot[3]));
-    const uint32_t at = g + 4 * (32 * k + lane);  // this lane's own values
-    sts(at + kDec, ex2(head + lds(at + kCum)));
-    sts(at + kF, lds(at + kD) * ex2(lds(at + kF) + tail));
-  }
+  float before = __shfl_up_sync(0xffffffffu, pre, 1, 8);
+  float behind = __shfl_down_sync(0xffffffffu, suf, 1, 8);
+  if ((lane & 7) == 0) before = 0.f;
+  if ((lane & 7) == 7) behind = 0.f;
+  const float b0 = __shfl_sync(0xffffffffu, pre, 7), b1 = __shfl_sync(0xffffffffu, pre, 15);
+  const float b2 = __shfl_sync(0xffffffffu, pre, 23), b3 = __shfl_sync(0xffffffffu, pre, 31);
+  const int blk = lane >> 3;
+  const float head = blk == 0 ? 0.f : (blk == 1 ? b0 : (blk == 2 ? b0 + b1 : b0 + b1 + b2));
+  const float tail = blk == 3 ? 0.f : (blk == 2 ? b3 : (blk == 1 ? b2 + b3 : b1 + b2 + b3));
+  float c[4], w[4];  // from the block's start, inclusive; to its end, exclusive
+  c[0] = before + lg[0];
+  c[1] = c[0] + lg[1];
+  c[2] = c[1] + lg[2];
+  c[3] = c[2] + lg[3];
+  w[3] = behind;
+  w[2] = w[3] + lg[3];
+  w[1] = w[2] + lg[2];
+  w[0] = w[1] + lg[1];
+  const uint32_t at = g + 16 * lane;
+  sts4(at + kCum, c[0], c[1], c[2], c[3]);
+  sts4(at + kD, d[0], d[1], d[2], d[3]);
+  sts4(at + kDec, ex2(head + c[0]), ex2(head + c[1]), ex2(head + c[2]), ex2(head + c[3]));
+  sts4(at + kU, d[0] * ex2(w[0]), d[1] * ex2(w[1]), d[2] * ex2(w[2]), d[3] * ex2(w[3]));
+  sts4(at + kF, d[0] * ex2(w[0] + tail), d[1] * ex2(w[1] + tail), d[2] * ex2(w[2] + tail),
+       d[3] * ex2(w[3] + tail));
+  if ((lane & 7) == 7) sts(g + kTot + 4 * blk, pre);
 }
 
 template <int P, int NS, bool kStates>
@@ -354,11 +387,11 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       mbar_init(bars + kStaged + i, 8);
     }
     mbar_init(bars + kFullC, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kGateStages; ++i) {
       mbar_init(bars + kGatesFull + i, kHeads);
       mbar_init(bars + kGatesFree + i, kOutWarps + K::kStateWarps);
-      mbar_init(bars + kState + i, K::kStateWarps);
     }
+    for (int i = 0; i < 2; ++i) mbar_init(bars + kState + i, K::kStateWarps);
     for (int i = 0; i < 4; ++i) {
       mbar_init(bars + kFx + i, K::kFxWarps);
       mbar_init(bars + kFxFree + i, 1);
@@ -394,7 +427,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
   auto write_fx = [&](int c, int t) {
     const int k = 4 * c + t, place = k % K::kPlaces;
     const uint32_t f = gates_u +
-                       ((c & 1) * kHeads + row_head) * static_cast<uint32_t>(sizeof(Gates)) + kF +
+                       (c % kGateStages * kHeads + row_head) * static_cast<uint32_t>(sizeof(Gates)) + kF +
                        4 * (32 * t + 16 * part) + 8 * (lane & 3);
     const float2 f0 = lds2(f), f1 = lds2(f + 32);
     const uint32_t xa = sm_u + K::kX + (c % K::kXStages) * K::kXBytes + (q >> 1) * kBlock +
@@ -442,16 +475,16 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     auto first_fx = [&](int c) {
       wait(bars_u + 8 * (kFullX + c % K::kXStages), (c / K::kXStages) & 1);
       if (c == chunks - 1 && tail < kL) wait(bars_u + 8 * (kZeroed), 0);
-      wait(bars_u + 8 * (kGatesFull + (c & 1)), (c >> 1) & 1);
+      wait(bars_u + 8 * (kGatesFull + c % kGateStages), (c / kGateStages) & 1);
       write_fx(c, 0);
     };
     // (turn -1 only writes the first chunk's)
 #pragma unroll 1
     for (int c = -1; c < chunks; ++c) {
      if (c >= 0) {
-      const int gs = c & 1;
+      const int gs = c % kGateStages;
       const uint32_t ga = gates_u + gs * kHeads * static_cast<uint32_t>(sizeof(Gates));
-      wait(bars_u + 8 * (kGatesFull + gs), (c >> 1) & 1);
+      wait(bars_u + 8 * (kGatesFull + gs), (c / kGateStages) & 1);
       wait(bars_u + 8 * (kCB), c & 1);
       tc_fence_after();
       // ---- M over C B^T, 16 columns at a time: those of head h go to 8 columns of the same
@@ -661,14 +694,14 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         named_bar_sync(2, K::kStateWarps * 32);
         arrive(kZeroed);
       }
-      wait(bars_u + 8 * (kGatesFull + (c & 1)), (c >> 1) & 1);
+      wait(bars_u + 8 * (kGatesFull + c % kGateStages), (c / kGateStages) & 1);
     };
     // The state behind chunk c, from what the chunk adds.
     auto update_state = [&](int c) {
       wait(bars_u + 8 * (kDS + c % K::kBStages), (c / K::kBStages) & 1);
       tc_fence_after();
       const float g =
-          lds(gates_u + ((c & 1) * kHeads + row_head) * static_cast<uint32_t>(sizeof(Gates)) + kDec +
+          lds(gates_u + (c % kGateStages * kHeads + row_head) * static_cast<uint32_t>(sizeof(Gates)) + kDec +
               4 * (kL - 1));
       const float2 g2 = make_float2(g, g);
       const uint32_t td = lanes + kTD + (kStates ? 128 * (c & 1) : 0) + kNC * sp;
@@ -687,7 +720,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       }
       if (kStates) left *= g;
       tc_fence_before();
-      arrive(kGatesFree + (c & 1));
+      arrive(kGatesFree + c % kGateStages);
     };
 
     // Turn i of the loop writes one quarter of f x (the output kernel: its other warps write each
@@ -924,7 +957,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     auto load = [&](int c, uint32_t (&raw)[4]) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int t = min(c * kL + 32 * k + lane, tokens - 1);
+        const int t = min(c * kL + 4 * lane + k, tokens - 1);
         const int64_t at = (static_cast<int64_t>(tok0) + t) * p.H + h;
         raw[k] = half ? static_cast<const unsigned short*>(p.dt)[at]
                       : static_cast<const uint32_t*>(p.dt)[at];
@@ -934,12 +967,13 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     if (chunks > 0) load(0, raw);
 #pragma unroll 1
     for (int c = 0; c < chunks; ++c) {
-      const int gs = c & 1;
+      const int gs = c % kGateStages;
       float dt[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) dt[k] = __uint_as_float(half ? raw[k] << 16 : raw[k]);
       if (c + 1 < chunks) load(c + 1, raw);
-      if (c >= 2) wait(bars_u + 8 * (kGatesFree + gs), ((c >> 1) - 1) & 1);
+      if (c >= kGateStages)
+        wait(bars_u + 8 * (kGatesFree + gs), (c / kGateStages - 1) & 1);
       write_gates(gates_u + (gs * kHeads + hh) * static_cast<uint32_t>(sizeof(Gates)), dt, neg_a,
                   dtb, present ? tokens - c * kL : 0, lane);
       __syncwarp();
