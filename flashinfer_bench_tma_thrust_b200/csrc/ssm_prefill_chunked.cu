@@ -117,10 +117,10 @@ struct Gates {
   float dec[kL];                    // e^G
   float u[kL];                      // d_j e^{G_r - G_j}, r the end of j's block of 32
   float f[kL];                      // d_j e^{G_L - G_j}
-  float d[kL];
+  float h[kL];                      // log2 d_j - G_j, for pairs within a block
   float tot[4];                     // G over each block of 32
 };
-constexpr uint32_t kCum = 0, kDec = 512, kU = 1024, kF = 1536, kD = 2048, kTot = 2560;
+constexpr uint32_t kCum = 0, kDec = 512, kU = 1024, kF = 1536, kH = 2048, kTot = 2560;
 static_assert(sizeof(Gates) == kTot + 16, "");
 
 // Chunks whose gates there is room for. The gates' warp takes some 3000 cycles a chunk, in a chain
@@ -257,6 +257,12 @@ __device__ __forceinline__ void find_segment(const SsmParams& p, const Segments&
   n = p.N;
 }
 
+__device__ __forceinline__ float lg2(float x) {  // log2 0 = -inf
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // softplus(v) = max(v, 0) + log(1 + u), u = e^-|v|, with log(1 + u) = 2 atanh(s) by its series in
 // s = u / (2 + u) <= 1/3: a tenth of the instructions of log1pf(expf(v)), which with one or two
 // warps on all of a chunk's gates set the pace of the kernel. The first term left out is below
@@ -321,7 +327,7 @@ __device__ __forceinline__ void write_gates(uint32_t g, const float (&raw)[4], f
   w[0] = w[1] + lg[1];
   const uint32_t at = g + 16 * lane;
   sts4(at + kCum, c[0], c[1], c[2], c[3]);
-  sts4(at + kD, d[0], d[1], d[2], d[3]);
+  sts4(at + kH, lg2(d[0]) - c[0], lg2(d[1]) - c[1], lg2(d[2]) - c[2], lg2(d[3]) - c[3]);
   sts4(at + kDec, ex2(head + c[0]), ex2(head + c[1]), ex2(head + c[2]), ex2(head + c[3]));
   sts4(at + kU, d[0] * ex2(w[0]), d[1] * ex2(w[1]), d[2] * ex2(w[2]), d[3] * ex2(w[3]));
   sts4(at + kF, d[0] * ex2(w[0] + tail), d[1] * ex2(w[1] + tail), d[2] * ex2(w[2] + tail),
@@ -492,53 +498,78 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       // quarter take every other 16 (each has one piece on the diagonal).
 #pragma unroll 1
       for (int k = 0; k < 4; ++k) {  // piece k: columns 32 k + 16 half on, in block k of 32
+        float g[16];
         const int j0 = 32 * k + 16 * half;
         const uint32_t at = lanes + kTG + j0;
-        float g[16];
         if (k <= q) {
           tmem_ld16(at, g);
           tmem_ld_wait();
         }
-#pragma unroll
-        for (int hh = 0; hh < kHeads; ++hh) {
-          const uint32_t gh = ga + hh * static_cast<uint32_t>(sizeof(Gates));
-          uint32_t m[8];
+        {
+          uint32_t m[kHeads][8];
           if (k < q) {
             // e^{G_i - G_j} d_j = e^{G_i - G_r} (e^{G_r - G_j} d_j), r the end of j's block,
             // between j and i: both exponents are at most 0, and one exponential per row is left
-            float ex = lds(gh + kCum + 4 * row);
-            if (k + 1 < q) ex += lds(gh + kTot + 4 * (k + 1));
-            if (k + 2 < q) ex += lds(gh + kTot + 4 * (k + 2));
-            const float e = ex2(ex);
-            const float2 a = make_float2(e, e);
+            float ex[kHeads];
+            float4 u[kHeads][4];
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-              const float4 u = lds4(gh + kU + 4 * (j0 + j));
-              const float2 v0 = mul2(mul2(make_float2(u.x, u.y), a), make_float2(g[j], g[j + 1]));
-              const float2 v1 =
-                  mul2(mul2(make_float2(u.z, u.w), a), make_float2(g[j + 2], g[j + 3]));
-              m[j / 2] = pack2_rn(v0.x, v0.y);
-              m[j / 2 + 1] = pack2_rn(v1.x, v1.y);
+            for (int hh = 0; hh < kHeads; ++hh) {  // all loads before the first use
+              const uint32_t gh = ga + hh * static_cast<uint32_t>(sizeof(Gates));
+              ex[hh] = lds(gh + kCum + 4 * row);
+              if (k + 1 < q) ex[hh] += lds(gh + kTot + 4 * (k + 1));
+              if (k + 2 < q) ex[hh] += lds(gh + kTot + 4 * (k + 2));
+#pragma unroll
+              for (int j = 0; j < 4; ++j) u[hh][j] = lds4(gh + kU + 4 * (j0 + 4 * j));
+            }
+#pragma unroll
+            for (int hh = 0; hh < kHeads; ++hh) {
+              const float e = ex2(ex[hh]);
+              const float2 a = make_float2(e, e);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float4 v = u[hh][j];
+                const float2 v0 = mul2(mul2(make_float2(v.x, v.y), a),
+                                       make_float2(g[4 * j], g[4 * j + 1]));
+                const float2 v1 = mul2(mul2(make_float2(v.z, v.w), a),
+                                       make_float2(g[4 * j + 2], g[4 * j + 3]));
+                m[hh][2 * j] = pack2_rn(v0.x, v0.y);
+                m[hh][2 * j + 1] = pack2_rn(v1.x, v1.y);
+              }
             }
           } else if (k == q) {
-            const float own = lds(gh + kCum + 4 * row);
             const int i = row - j0;  // columns j <= i are on or below the diagonal
+            float own[kHeads];
+            float4 x[kHeads][4];
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-              const float4 cj = lds4(gh + kCum + 4 * (j0 + j));
-              const float4 dj = lds4(gh + kD + 4 * (j0 + j));
-              const float v0 = j <= i ? g[j] * (ex2(own - cj.x) * dj.x) : 0.f;
-              const float v1 = j + 1 <= i ? g[j + 1] * (ex2(own - cj.y) * dj.y) : 0.f;
-              const float v2 = j + 2 <= i ? g[j + 2] * (ex2(own - cj.z) * dj.z) : 0.f;
-              const float v3 = j + 3 <= i ? g[j + 3] * (ex2(own - cj.w) * dj.w) : 0.f;
-              m[j / 2] = pack2_rn(v0, v1);
-              m[j / 2 + 1] = pack2_rn(v2, v3);
+            for (int hh = 0; hh < kHeads; ++hh) {
+              const uint32_t gh = ga + hh * static_cast<uint32_t>(sizeof(Gates));
+              own[hh] = lds(gh + kCum + 4 * row);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) x[hh][j] = lds4(gh + kH + 4 * (j0 + 4 * j));
+            }
+#pragma unroll
+            for (int hh = 0; hh < kHeads; ++hh) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float4 v = x[hh][j];
+                const float* const gj = g + 4 * j;
+                const float v0 = 4 * j <= i ? gj[0] * ex2(own[hh] + v.x) : 0.f;
+                const float v1 = 4 * j + 1 <= i ? gj[1] * ex2(own[hh] + v.y) : 0.f;
+                const float v2 = 4 * j + 2 <= i ? gj[2] * ex2(own[hh] + v.z) : 0.f;
+                const float v3 = 4 * j + 3 <= i ? gj[3] * ex2(own[hh] + v.w) : 0.f;
+                m[hh][2 * j] = pack2_rn(v0, v1);
+                m[hh][2 * j + 1] = pack2_rn(v2, v3);
+              }
             }
           } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) m[j] = 0u;
+            for (int hh = 0; hh < kHeads; ++hh) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) m[hh][j] = 0u;
+            }
           }
-          tmem_st8(at + 8 * hh, m);
+#pragma unroll
+          for (int hh = 0; hh < kHeads; ++hh) tmem_st8(at + 8 * hh, m[hh]);
         }
       }
       // ---- Y = e^{G_i} (C S^T), in place
