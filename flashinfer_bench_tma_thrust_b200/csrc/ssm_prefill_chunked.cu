@@ -207,31 +207,45 @@ struct Waiter {
   __device__ __forceinline__ bool ok() const { return left != 0; }
 };
 
+__device__ __forceinline__ int64_t clamp_to(int64_t v, int64_t T) {
+  return v < 0 ? 0 : (v > T ? T : v);
+}
 __device__ __forceinline__ int64_t clamp_bound(const SsmParams& p, int64_t i) {
-  const int64_t v = load_index(p.cu_seqlens, p.cu_dtype, i);
-  return v < 0 ? 0 : (v > p.T ? p.T : v);
+  return clamp_to(load_index(p.cu_seqlens, p.cu_dtype, i), p.T);
 }
 
-// Segment `slot` in the order of the sequences: (sequence, segment of it). Whole warp.
+// Segment `slot` in the order of the sequences: (sequence, segment of it) and the sequence's
+// bounds as they stand in cu_seqlens. Whole warp.
 __device__ __forceinline__ void find_segment(const SsmParams& p, const Segments& sg, int64_t slot,
-                                             int64_t& n, int64_t& seg) {
+                                             int64_t& n, int64_t& seg, int64_t& lo, int64_t& hi) {
   const int lane = threadIdx.x & 31;
   seg = 0;
   if (sg.len == 0) {
     // One segment per sequence; up to 32 sequences go longest first, so that the longest do
     // not start last.
     n = slot;
-    if (p.N > 32) return;
-    int64_t len = -1;
-    if (lane < p.N) len = max(clamp_bound(p, lane + 1) - clamp_bound(p, lane), int64_t{0});
+    if (p.N > 32) {
+      lo = load_index(p.cu_seqlens, p.cu_dtype, n);
+      hi = load_index(p.cu_seqlens, p.cu_dtype, n + 1);
+      return;
+    }
+    int64_t a = 0, b = 0, len = -1;
+    if (lane < p.N) {
+      a = load_index(p.cu_seqlens, p.cu_dtype, lane);
+      b = load_index(p.cu_seqlens, p.cu_dtype, lane + 1);
+      len = max(clamp_to(b, p.T) - clamp_to(a, p.T), int64_t{0});
+    }
     int rank = 0;
     for (int k = 0; k < static_cast<int>(p.N); ++k) {
       const int64_t other = __shfl_sync(0xffffffffu, len, k);
       rank += other > len || (other == len && k < lane);
     }
     n = __ffs(__ballot_sync(0xffffffffu, lane < p.N && rank == slot)) - 1;
+    lo = __shfl_sync(0xffffffffu, a, static_cast<int>(n));
+    hi = __shfl_sync(0xffffffffu, b, static_cast<int>(n));
     return;
   }
+  lo = hi = 0;
   int64_t before = 0;
   for (int64_t n0 = 0; n0 < p.N; n0 += 32) {
     int64_t cnt = 0;
@@ -250,6 +264,8 @@ __device__ __forceinline__ void find_segment(const SsmParams& p, const Segments&
       const int src = __ffs(past) - 1;
       n = n0 + src;
       seg = slot - before - __shfl_sync(0xffffffffu, incl - cnt, src);
+      lo = load_index(p.cu_seqlens, p.cu_dtype, n);
+      hi = load_index(p.cu_seqlens, p.cu_dtype, n + 1);
       return;
     }
     before += __shfl_sync(0xffffffffu, incl, 31);
@@ -343,49 +359,27 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
   constexpr int kHeads = K::kHeads;
   extern __shared__ uint8_t raw_smem[];
   uint8_t* const sm = align_smem<1024>(raw_smem);
-  __shared__ int64_t s_where[2];
+  __shared__ int64_t s_where[4];
   __shared__ uint32_t s_tmem;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kOutWarps = K::kOutWarps;                   // first, then the state's
+  constexpr int kMisc = kOutWarps + K::kStateWarps;
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(sm + K::kBars);
 
   const int64_t slot = blockIdx.x / col_blocks;
   const int cb = static_cast<int>(blockIdx.x - slot * col_blocks);
   if (warp == 0) {
-    int64_t n, seg;
-    find_segment(p, sg, slot, n, seg);
+    int64_t n, seg, lo, hi;
+    find_segment(p, sg, slot, n, seg, lo, hi);
     if (lane == 0) {
       s_where[0] = n;
       s_where[1] = seg;
+      s_where[2] = clamp_to(lo, p.T);
+      s_where[3] = max(clamp_to(hi, p.T), clamp_to(lo, p.T));
+      if (cb == 0 && seg == 0 && n < p.N && (lo < 0 || hi > p.T || hi < lo))
+        report_bad_bounds(p.status);
     }
-  }
-  __syncthreads();
-  const int64_t n = s_where[0], seg = s_where[1];
-  if (n >= p.N) return;
-
-  const int rep = p.H / p.G;                                  // heads of a group
-  const int per_group = (rep + kHeads - 1) / kHeads;
-  const int grp = cb / per_group;
-  const int h0 = grp * rep + (cb - grp * per_group) * kHeads;  // first head of the block
-  const int heads = min(kHeads, (grp + 1) * rep - h0);
-  const int64_t s_begin = clamp_bound(p, n);
-  const int64_t s_end = max(clamp_bound(p, n + 1), s_begin);
-  if (cb == 0 && seg == 0 && threadIdx.x == 0) {
-    const int64_t lo = load_index(p.cu_seqlens, p.cu_dtype, n);
-    const int64_t hi = load_index(p.cu_seqlens, p.cu_dtype, n + 1);
-    if (lo < 0 || hi > p.T || hi < lo) report_bad_bounds(p.status);
-  }
-  const int64_t t_begin = sg.len ? s_begin + seg * sg.len : s_begin;
-  const int64_t t_end = sg.len ? min(t_begin + sg.len, s_end) : s_end;
-  const bool last = t_end >= s_end;
-  if (kStates && last) return;  // the second kernel computes the sequence's last state
-  const int tokens = static_cast<int>(t_end - t_begin);
-  const int chunks = (tokens + kL - 1) / kL;
-  const int tail = tokens - (chunks - 1) * kL;                // of the last chunk
-  const int tok0 = static_cast<int>(t_begin);
-
-  uint64_t* const bars = reinterpret_cast<uint64_t*>(sm + K::kBars);
-  constexpr int kOutWarps = K::kOutWarps;                   // first, then the state's
-  constexpr int kMisc = kOutWarps + K::kStateWarps;
-  if (threadIdx.x == 0) {
+  } else if (threadIdx.x == 32) {
     for (int i = 0; i < 3; ++i) {
       mbar_init(bars + kFullX + i, 1);
       mbar_init(bars + kFullB + i, 1);
@@ -407,11 +401,31 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     mbar_init(bars + kZeroed, K::kStateWarps);
     mbar_init(bars + kXRead, K::kStateWarps);
     fence_mbar_init();
+  } else if (warp == kMisc) {
+    tmem_alloc(&s_tmem, 512);
   }
-  if (warp == kMisc) tmem_alloc(&s_tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  const int64_t n = s_where[0], seg = s_where[1], s_begin = s_where[2], s_end = s_where[3];
+  const int64_t t_begin = sg.len ? s_begin + seg * sg.len : s_begin;
+  const int64_t t_end = sg.len ? min(t_begin + sg.len, s_end) : s_end;
+  const bool last = t_end >= s_end;
+  if (n >= p.N || (kStates && last)) {  // (the second kernel computes a sequence's last state)
+    if (warp == kMisc) tmem_dealloc(s_tmem, 512);
+    return;
+  }
+
+  const int rep = p.H / p.G;                                  // heads of a group
+  const int per_group = (rep + kHeads - 1) / kHeads;
+  const int grp = cb / per_group;
+  const int h0 = grp * rep + (cb - grp * per_group) * kHeads;  // first head of the block
+  const int heads = min(kHeads, (grp + 1) * rep - h0);
+  const int tokens = static_cast<int>(t_end - t_begin);
+  const int chunks = (tokens + kL - 1) / kL;
+  const int tail = tokens - (chunks - 1) * kL;                // of the last chunk
+  const int tok0 = static_cast<int>(t_begin);
+
   const uint32_t tm = s_tmem, sm_u = smem_u32(sm), gates_u = sm_u + K::kGates,
                  bars_u = sm_u + K::kBars;
   Waiter wait, finally;  // the second for what a block that gave up still has to wait for
