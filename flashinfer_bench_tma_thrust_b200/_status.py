@@ -8,13 +8,14 @@ of its device before it launches and raises for what an earlier call left there.
 """
 from __future__ import annotations
 
+import ctypes
 import threading
 
 import torch
 
 from . import _lib
 
-_words: dict = {}  # device index -> (pinned tensor, numpy view, address)
+_words: dict = {}  # device index -> (pinned tensor, its words as one 64-bit number, address)
 _lock = threading.Lock()
 
 
@@ -25,20 +26,20 @@ def _entry(index: int):
             e = _words.get(index)
             if e is None:
                 t = torch.zeros(2, dtype=torch.int32, pin_memory=True)
-                e = _words[index] = (t, t.numpy(), t.data_ptr())
+                e = _words[index] = (t, ctypes.c_int64.from_address(t.data_ptr()), t.data_ptr())
     return e
 
 
 def address(index: int) -> int:
     """Address of the device's words, after raising for what they already hold."""
-    e = _entry(index)
-    if e[1][0] or e[1][1]:
+    e = _words.get(index) or _entry(index)
+    if e[1].value:
         raise_for(index)
     return e[2]
 
 
 def raise_for(index: int) -> None:
-    wait, bounds = (int(v) for v in _entry(index)[1])
+    wait, bounds = _entry(index)[0].tolist()
     if wait or bounds:
         what = [w for w, on in (("a bounded wait gave up", wait),
                                 ("cu_seqlens is not a non-decreasing sequence within [0, T]",
@@ -47,11 +48,10 @@ def raise_for(index: int) -> None:
                             "are invalid. Clear with reset_device_status().")
 
 
-def finish(index: int, check: bool) -> None:
-    """With ``check``: wait for the current stream and raise for this call's own report."""
-    if check:
-        torch.cuda.current_stream(index).synchronize()
-        raise_for(index)
+def finish(index: int) -> None:
+    """Wait for the current stream and raise for what its calls reported."""
+    torch.cuda.current_stream(index).synchronize()
+    raise_for(index)
 
 
 def reset(device=None) -> None:
@@ -60,4 +60,4 @@ def reset(device=None) -> None:
     if index is None:
         index = torch.cuda.current_device()
     torch.cuda.synchronize(index)
-    _entry(index)[1][:] = 0
+    _entry(index)[1].value = 0

@@ -129,21 +129,25 @@ def prefill(x, weight, bias=None, state=None, cu_seqlens=None, *, activation="si
     cu, cu_t = C.as_index("cu_seqlens", cu_seqlens)
     n, t = cu.numel() - 1, x.shape[0]
     s = _state(state, (n, taps - 1, ch))
-    x = _rows(x)
+    if x.dtype is not torch.bfloat16 or x.stride(-1) != 1 or not ch:
+        x = _rows(x)
     widths, wa, na, pointers = _sections(ch, _hashable(split), _hashable(l2norm))
     act = _activation(activation)
     lib = _lib.load()
     with C.on_device(dev):
         status = _status.address(dev.index)
         outs = [torch.empty(t, v, dtype=torch.bfloat16, device=dev) for v in widths]
-        new_state = torch.empty(n, taps - 1, ch, dtype=torch.bfloat16, device=dev)
+        new_state = torch.empty(n, taps - 1, ch, dtype=torch.bfloat16, device=dev) \
+            if s is None else torch.empty_like(s)
         rc = lib.gdn_conv_prefill_fwd(
             x.data_ptr(), x.stride(0), w.data_ptr(), w_t, C.ptr(b), b_t, C.ptr(s), cu.data_ptr(),
             cu_t, act, len(widths), wa, na, eps, pointers(*[o.data_ptr() for o in outs]),
             new_state.data_ptr(), t, n, ch, taps, status,
             C.stream_handle(dev))
-        _lib.check(rc, "gdn_conv_prefill_fwd")
-        _status.finish(dev.index, check)
+        if rc:
+            _lib.check(rc, "gdn_conv_prefill_fwd")
+        if check:
+            _status.finish(dev.index)
     return (outs[0] if split is None else tuple(outs)), new_state
 
 
@@ -156,19 +160,22 @@ def _decode(x, weight, bias, state, activation, split, l2norm, eps, inplace):
     ch = x.shape[-1]
     n = x.shape[0]
     s = _state(state, (n, taps - 1, ch))
-    x = _rows(x)
+    if x.dtype is not torch.bfloat16 or x.stride(-1) != 1 or not ch:
+        x = _rows(x)
     widths, wa, na, pointers = _sections(ch, _hashable(split), _hashable(l2norm))
     act = _activation(activation)
     lib = _lib.load()
     with C.on_device(dev):
         outs = [torch.empty(n, 1, v, dtype=torch.bfloat16, device=dev) for v in widths]
-        new_state = state if inplace else \
-            torch.empty(n, taps - 1, ch, dtype=torch.bfloat16, device=dev)
+        new_state = state if inplace else (
+            torch.empty(n, taps - 1, ch, dtype=torch.bfloat16, device=dev) if s is None
+            else torch.empty_like(s))
         rc = lib.gdn_conv_decode_fwd(
             x.data_ptr(), x.stride(0), w.data_ptr(), w_t, C.ptr(b), b_t, C.ptr(s), act,
             len(widths), wa, na, eps, pointers(*[o.data_ptr() for o in outs]),
             new_state.data_ptr(), n, ch, taps, C.stream_handle(dev))
-    _lib.check(rc, "gdn_conv_decode_fwd")
+    if rc:
+        _lib.check(rc, "gdn_conv_decode_fwd")
     return (outs[0] if split is None else tuple(outs)), new_state
 
 

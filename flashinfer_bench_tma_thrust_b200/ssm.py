@@ -30,37 +30,42 @@ STATE_DIMS = (16, 32, 64, 128, 256)
 MAX_HEAD_DIM = 256
 
 
-class _Args:
-    __slots__ = ("dev", "T", "H", "G", "P", "Ns", "x", "dt", "dt_t", "A", "A_t", "B", "C", "D",
-                 "D_t", "dtb", "dtb_t", "state", "cu", "cu_t", "N")
+_NAMES = ("x", "dt", "A_log", "B", "C", "D", "dt_bias", "state", "cu_seqlens")
+_BF16, _F32 = torch.bfloat16, torch.float32
+_CODES = K._GATE_CODES
 
 
 def _aligned(t):
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-_NAMES = ("x", "dt", "A_log", "B", "C", "D", "dt_bias", "state", "cu_seqlens")
-
-
 def _gate(name, t, shape):
+    """A gate or parameter of the given shape: (contiguous tensor, dtype code)."""
     if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {tuple(t.shape)}")
+    code = _CODES.get(t.dtype)
+    if code is not None and t.is_contiguous():
+        return t, code
     return K.as_gate(name, t)
 
 
-def _args(x, dt, A_log, B, C, D, dt_bias, state, cu, lead: int) -> _Args:
-    """Checks shared by prompts (lead = 1) and tokens (lead = 2: [B, 1, ...])."""
-    a = _Args()
+def _bf16(name, t):
+    return t if t.dtype is _BF16 and t.is_contiguous() else K.as_bf16(name, t)
+
+
+def _args(x, dt, A_log, B, C, D, dt_bias, state, cu, lead: int):
+    """Checks shared by prompts (lead = 1) and tokens (lead = 2: [B, 1, ...]). Returns (sizes,
+    the tensors to keep, the library's arguments up to dt_bias)."""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"x must be a torch.Tensor, got {type(x).__name__}")
-    dev, shape = x.device, tuple(x.shape)
+    shape = x.shape
     if len(shape) != lead + 2 or (lead == 2 and shape[1] != 1):
         raise ValueError("x must be a %s tensor" % ("[T, H, P]" if lead == 1 else "[B, 1, H, P]"))
-    K.require_all(dev, _NAMES, (x, dt, A_log, B, C, D, dt_bias, state, cu))
-    of_b, head = tuple(B.shape), shape[:lead]
+    K.require_all(x.device, _NAMES, (x, dt, A_log, B, C, D, dt_bias, state, cu))
+    of_b, head = B.shape, shape[:lead]
     T, H, P = shape[0], shape[-2], shape[-1]
     if len(of_b) != lead + 2 or of_b[:lead] != head or C.shape != of_b:
-        raise ValueError(f"B and C must be {list(head)} + [G, Ns], got {of_b} and "
+        raise ValueError(f"B and C must be {list(head)} + [G, Ns], got {tuple(of_b)} and "
                          f"{tuple(C.shape)}")
     G, Ns = of_b[-2], of_b[-1]
     if Ns not in STATE_DIMS:
@@ -69,53 +74,58 @@ def _args(x, dt, A_log, B, C, D, dt_bias, state, cu, lead: int) -> _Args:
         raise ValueError(f"the head size must be 1 to {MAX_HEAD_DIM}, got {P}")
     if G <= 0 or H <= 0 or H % G:
         raise ValueError(f"num_heads ({H}) must be a positive multiple of num_groups ({G})")
-    a.dev, a.T, a.H, a.P, a.G, a.Ns = dev, T, H, P, G, Ns
-    a.x, a.B, a.C = K.as_bf16("x", x), K.as_bf16("B", B), K.as_bf16("C", C)
-    if (a.B.data_ptr() | a.C.data_ptr()) % 16:
-        a.B, a.C = _aligned(a.B), _aligned(a.C)
-    a.dt, a.dt_t = _gate("dt", dt, head + (H,))
+    x, B, C = _bf16("x", x), _bf16("B", B), _bf16("C", C)
+    if (B.data_ptr() | C.data_ptr()) % 16:
+        B, C = _aligned(B), _aligned(C)
+    if lead == 1 and x.data_ptr() % 16:  # (bulk copies read it)
+        x = x.clone()
+    dt, dt_t = _gate("dt", dt, shape[:-1])
     vec = (H,)
-    a.A, a.A_t = _gate("A_log", A_log, vec)
-    a.dtb, a.dtb_t = _gate("dt_bias", dt_bias, vec)
-    a.D, a.D_t = (None, 0) if D is None else _gate("D", D, vec)
-    return a
+    A_log, a_t = _gate("A_log", A_log, vec)
+    dt_bias, b_t = _gate("dt_bias", dt_bias, vec)
+    d_ptr, d_t = None, 0
+    if D is not None:
+        D, d_t = _gate("D", D, vec)
+        d_ptr = D.data_ptr()
+    return (T, H, G, P, Ns), (x, dt, A_log, B, C, D, dt_bias), (
+        x.data_ptr(), dt.data_ptr(), dt_t, A_log.data_ptr(), a_t, B.data_ptr(), C.data_ptr(),
+        d_ptr, d_t, dt_bias.data_ptr(), b_t)
 
 
-def _prefill_args(x, dt, A_log, B, C, D, dt_bias, state, cu_seqlens) -> _Args:
-    if cu_seqlens is None:
+def _prompt_args(x, dt, A_log, B, C, D, dt_bias, state, cu):
+    if cu is None:
         raise ValueError("cu_seqlens is required")
-    a = _args(x, dt, A_log, B, C, D, dt_bias, state, cu_seqlens, 1)
-    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+    sizes, keep, head = _args(x, dt, A_log, B, C, D, dt_bias, state, cu, 1)
+    if cu.dim() != 1 or cu.numel() < 1:
         raise ValueError("cu_seqlens must be a 1-D tensor of length num_seqs + 1")
-    a.cu, a.cu_t = K.as_index("cu_seqlens", cu_seqlens)
-    a.N = a.cu.numel() - 1
-    a.state = None
+    cu, cu_t = K.as_index("cu_seqlens", cu)
+    n = cu.numel() - 1
+    _, H, _, P, Ns = sizes
     if state is not None:
-        if state.shape != (a.N, a.H, a.P, a.Ns):
-            raise ValueError(f"state must be [{a.N}, {a.H}, {a.P}, {a.Ns}], "
-                             f"got {tuple(state.shape)}")
-        if state.dtype != torch.float32:
+        if state.shape != (n, H, P, Ns):
+            raise ValueError(f"state must be [{n}, {H}, {P}, {Ns}], got {tuple(state.shape)}")
+        if state.dtype is not _F32:
             state = state.float()
-        a.state = _aligned(state.contiguous())
-    return a
+        state = _aligned(state.contiguous())
+    return sizes, n, (keep, state, cu), head + (K.ptr(state), cu.data_ptr(), cu_t)
 
 
 def prefill_recurrent(x, dt, A_log, B, C, D, dt_bias, state, cu_seqlens, *, check=False):
     """The scan token by token (one launch): any head size, the independent check of the
     chunked kernel."""
-    a = _prefill_args(x, dt, A_log, B, C, D, dt_bias, state, cu_seqlens)
-    lib = _lib.load()
-    with K.on_device(a.dev):
-        status = _status.address(a.dev.index)
-        out = torch.empty(a.T, a.H, a.P, dtype=torch.bfloat16, device=a.dev)
-        new_state = torch.empty(a.N, a.H, a.P, a.Ns, dtype=torch.float32, device=a.dev)
+    (T, H, G, P, Ns), n, keep, head = _prompt_args(x, dt, A_log, B, C, D, dt_bias, state, cu_seqlens)
+    lib, dev = _lib.load(), x.device
+    with K.on_device(dev):
+        status = _status.address(dev.index)
+        out = torch.empty_like(keep[0][0])
+        new_state = torch.empty(n, H, P, Ns, dtype=_F32, device=dev)
         rc = lib.gdn_ssm_prefill_recurrent_fwd(
-            a.x.data_ptr(), a.dt.data_ptr(), a.dt_t, a.A.data_ptr(), a.A_t, a.B.data_ptr(),
-            a.C.data_ptr(), K.ptr(a.D), a.D_t, a.dtb.data_ptr(), a.dtb_t, K.ptr(a.state),
-            a.cu.data_ptr(), a.cu_t, out.data_ptr(), new_state.data_ptr(), a.T, a.N, a.H, a.G,
-            a.P, a.Ns, status, K.stream_handle(a.dev))
-        _lib.check(rc, "gdn_ssm_prefill_recurrent_fwd")
-        _status.finish(a.dev.index, check)
+            *head, out.data_ptr(), new_state.data_ptr(), T, n, H, G, P, Ns, status,
+            K.stream_handle(dev))
+        if rc:
+            _lib.check(rc, "gdn_ssm_prefill_recurrent_fwd")
+        if check:
+            _status.finish(dev.index)
     return out, new_state
 
 
@@ -124,47 +134,47 @@ def prefill(x, dt, A_log, B, C, D, dt_bias, state, cu_seqlens, *, check=False):
     A ``cu_seqlens`` that leaves [0, T] or decreases, or a bounded wait that gave up, raises
     GDNError at the next call on the device, or at this one with ``check=True`` (which
     synchronises)."""
-    a = _prefill_args(x, dt, A_log, B, C, D, dt_bias, state, cu_seqlens)
-    lib = _lib.load()
-    with K.on_device(a.dev):
-        status = _status.address(a.dev.index)
-        out = torch.empty(a.T, a.H, a.P, dtype=torch.bfloat16, device=a.dev)
-        new_state = torch.empty(a.N, a.H, a.P, a.Ns, dtype=torch.float32, device=a.dev)
-        nbytes = lib.gdn_ssm_prefill_workspace_size(a.T, a.N, a.H, a.G, a.P, a.Ns)
+    (T, H, G, P, Ns), n, keep, head = _prompt_args(x, dt, A_log, B, C, D, dt_bias, state, cu_seqlens)
+    lib, dev = _lib.load(), x.device
+    with K.on_device(dev):
+        status = _status.address(dev.index)
+        out = torch.empty_like(keep[0][0])
+        new_state = torch.empty(n, H, P, Ns, dtype=_F32, device=dev)
+        nbytes = lib.gdn_ssm_prefill_workspace_size(T, n, H, G, P, Ns)
         # of this call alone: calls on several streams and captured graphs share nothing
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=a.dev) if nbytes else None
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         rc = lib.gdn_ssm_prefill_fwd(
-            _aligned(a.x).data_ptr(), a.dt.data_ptr(), a.dt_t, a.A.data_ptr(), a.A_t,
-            a.B.data_ptr(), a.C.data_ptr(), K.ptr(a.D), a.D_t, a.dtb.data_ptr(), a.dtb_t,
-            K.ptr(a.state), a.cu.data_ptr(), a.cu_t, out.data_ptr(), new_state.data_ptr(), a.T,
-            a.N, a.H, a.G, a.P, a.Ns, K.ptr(ws), nbytes, status, K.stream_handle(a.dev))
-        _lib.check(rc, "gdn_ssm_prefill_fwd")
-        _status.finish(a.dev.index, check)
+            *head, out.data_ptr(), new_state.data_ptr(), T, n, H, G, P, Ns, K.ptr(ws), nbytes,
+            status, K.stream_handle(dev))
+        if rc:
+            _lib.check(rc, "gdn_ssm_prefill_fwd")
+        if check:
+            _status.finish(dev.index)
     return out, new_state
 
 
 def _decode(x, dt, A_log, B, C, D, dt_bias, state, inplace):
-    a = _args(x, dt, A_log, B, C, D, dt_bias, state, None, 2)
-    shape = (a.T, a.H, a.P, a.Ns)
-    s = state
+    (T, H, G, P, Ns), keep, head = _args(x, dt, A_log, B, C, D, dt_bias, state, None, 2)
+    dtype = _F32
     if state is not None:
-        if state.shape != shape:
-            raise ValueError(f"state must be {list(shape)}, got {tuple(state.shape)}")
+        if state.shape != (T, H, P, Ns):
+            raise ValueError(f"state must be {[T, H, P, Ns]}, got {tuple(state.shape)}")
         if not inplace:
-            if s.dtype not in (torch.float32, torch.bfloat16):
-                s = s.float()
-            s = _aligned(s.contiguous())
-    s_dtype = torch.float32 if s is None else s.dtype
-    lib = _lib.load()
-    with K.on_device(a.dev):
-        out = torch.empty(a.T, 1, a.H, a.P, dtype=torch.bfloat16, device=a.dev)
-        new_state = state if inplace else torch.empty(*shape, dtype=s_dtype, device=a.dev)
+            if state.dtype is not _F32 and state.dtype is not _BF16:
+                state = state.float()
+            state = _aligned(state.contiguous())
+        dtype = state.dtype
+    lib, dev = _lib.load(), x.device
+    with K.on_device(dev):
+        out = torch.empty_like(keep[0])
+        new_state = state if inplace else (
+            torch.empty(T, H, P, Ns, dtype=dtype, device=dev) if state is None
+            else torch.empty_like(state))
         rc = lib.gdn_ssm_decode_fwd(
-            a.x.data_ptr(), a.dt.data_ptr(), a.dt_t, a.A.data_ptr(), a.A_t, a.B.data_ptr(),
-            a.C.data_ptr(), K.ptr(a.D), a.D_t, a.dtb.data_ptr(), a.dtb_t, K.ptr(s),
-            _lib.DTYPE_F32 if s_dtype == torch.float32 else _lib.DTYPE_BF16, out.data_ptr(),
-            new_state.data_ptr(), a.T, a.H, a.G, a.P, a.Ns, K.stream_handle(a.dev))
-    _lib.check(rc, "gdn_ssm_decode_fwd")
+            *head, K.ptr(state), _CODES[dtype], out.data_ptr(), new_state.data_ptr(), T, H, G, P, Ns,
+            K.stream_handle(dev))
+    if rc:
+        _lib.check(rc, "gdn_ssm_decode_fwd")
     return out, new_state
 
 

@@ -216,7 +216,8 @@ def test_ssm_decode_refusals(any_device):
 
 def test_status_words_raise_and_name_the_cause(monkeypatch):
     words = torch.zeros(2, dtype=torch.int32)
-    monkeypatch.setitem(_status._words, 99, (words, words.numpy(), words.data_ptr()))
+    monkeypatch.setitem(_status._words, 99, (words, ctypes.c_int64.from_address(words.data_ptr()),
+                                             words.data_ptr()))
     assert _status.address(99) == words.data_ptr()
     words[1] = 1
     with pytest.raises(_lib.GDNError, match="cu_seqlens"):
