@@ -169,7 +169,8 @@ int gdn_ssm_prefill_recurrent_fwd(const void* x, const void* dt, int dt_dtype, c
 
 size_t gdn_ssm_prefill_workspace_size(int64_t T, int64_t N, int32_t H, int32_t G, int32_t P,
                                       int32_t Ns) {
-  if (T < 0 || N < 0 || H <= 0 || G <= 0 || H % G || !gdn::ssm_chunked_takes(P, Ns)) return 0;
+  if (T < 0 || N < 0 || H <= 0 || G <= 0 || H % G || !gdn::ssm_chunked_takes(P, Ns, T, N))
+    return 0;
   return gdn::ssm_chunked_workspace(T, N, H, G, P, Ns);
 }
 
@@ -189,7 +190,7 @@ int gdn_ssm_prefill_fwd(const void* x, const void* dt, int dt_dtype, const void*
   p.cu_seqlens = cu_seqlens;
   p.cu_dtype = cu_dtype;
   p.status = status;
-  if (!gdn::ssm_chunked_takes(P, Ns))
+  if (!gdn::ssm_chunked_takes(P, Ns, T, N))
     return gdn::launch_ssm_recurrent(p, static_cast<cudaStream_t>(stream));
   // bulk copies read x and write out; token coordinates are 32-bit
   if (!aligned16(x) || !aligned16(out) || !aligned16(workspace)) return GDN_ERR_INVALID_ARG;

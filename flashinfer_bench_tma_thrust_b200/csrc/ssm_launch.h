@@ -71,8 +71,8 @@ int launch_conv_prefill(const ConvParams& p, cudaStream_t stream);
 int launch_conv_decode(const ConvParams& p, cudaStream_t stream);
 int launch_ssm_decode(const SsmParams& p, cudaStream_t stream);
 int launch_ssm_recurrent(const SsmParams& p, cudaStream_t stream);
-// The chunked kernel: the sizes it takes, the workspace bytes of a call (0: none), the call.
-bool ssm_chunked_takes(int P, int Ns);
+// The chunked kernel: the calls it takes, the workspace bytes of a call (0: none), the call.
+bool ssm_chunked_takes(int P, int Ns, int64_t T, int64_t N);
 size_t ssm_chunked_workspace(int64_t T, int64_t N, int H, int G, int P, int Ns);
 int launch_ssm_chunked(const SsmParams& p, cudaStream_t stream);
 

@@ -128,13 +128,16 @@ static_assert(sizeof(Gates) == kTot + 16, "");
 constexpr int kGateStages = 4;
 
 struct Maps {
-  CUtensorMap x, b, c, out;         // {64, T, columns / 64}, box {64, 128, blocks}
+  CUtensorMap x, b, c, out;         // bf16 {64, T, columns / 64}, box {64, 128, blocks}
+  // fp32 states {32, rows of all heads, Ns / 32}, box {32, P, Ns / 32}: the first states, what
+  // the segments add, and where the kernel's last states go
+  CUtensorMap first, add, last;
 };
 
 struct Segments {
   int64_t slots;                    // grid: slots x column blocks
   int len;                          // tokens per segment; 0: one per sequence
-  float* add;                       // [slots, H, P, Ns]
+  float* add;                       // [slots, H, P, Ns] (through the maps)
   float* left;                      // [slots, H]
 };
 
@@ -159,10 +162,11 @@ struct Cfg {
   static constexpr uint32_t kC = kB + kBStages * kNB * kBStep;
   static constexpr uint32_t kGates = kC + (kStates ? 0 : kBBytes);
   static constexpr uint32_t kBars = kGates + kGateStages * kHeads * sizeof(Gates);
-  static constexpr uint32_t kBytes = kBars + 8 * 40 + 1024;  // and the alignment
+  static constexpr uint32_t kBytes = kBars + 8 * 48 + 1024;  // and the alignment
 };
 
 static_assert(sizeof(Gates) % 16 == 0, "");
+static_assert(3 + 3 + 1 + 2 * kGateStages + 1 + 3 + 1 + 4 + 4 + 1 + 2 + 1 + 3 + 1 + 1 + 2 <= 48, "");
 enum Bar {
   kFullX = 0,                          // [3] one per stage
   kFullB = kFullX + 3,                 // [3]
@@ -180,7 +184,9 @@ enum Bar {
   kStaged = kYFree + 1,                // y in shared memory [3]
   kZeroed = kStaged + 3,
   kXRead = kZeroed + 1,                // x read by the state's warps, so that y may replace it
-  kBarCount = kXRead + 1,
+  kFullState = kXRead + 1,             // a state in the second and third stage of x
+  kStateRead = kFullState + 1,
+  kBarCount = kStateRead + 1,
 };
 
 // Bounded waits in few instructions (the roles' code has to stay in the instruction cache: see
@@ -284,7 +290,7 @@ __device__ __forceinline__ float lg2(float x) {  // log2 0 = -inf
 // warps on all of a chunk's gates set the pace of the kernel. The first term left out is below
 // 2^-28 of the sum; u has ex2.approx's 2 ulp and, through the exponent's rest, no more.
 __device__ __forceinline__ float softplus(float v) {
-  const float x = -fabsf(v);
+  const float x = -fminf(fabsf(v), 200.f);  // (e^-200 is zero; an infinite v leaves no NaN)
   const float z = x * kLog2e;
   const float rest = fmaf(x, kLog2e, -z);  // what rounding z left
   const float e = ex2(z);
@@ -400,6 +406,8 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     for (int i : {kMy, kYFree}) mbar_init(bars + i, 8);
     mbar_init(bars + kZeroed, K::kStateWarps);
     mbar_init(bars + kXRead, K::kStateWarps);
+    mbar_init(bars + kFullState, 1);
+    mbar_init(bars + kStateRead, K::kStateWarps);
     fence_mbar_init();
   } else if (warp == kMisc) {
     tmem_alloc(&s_tmem, 512);
@@ -668,40 +676,38 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     // ---------------------------------------------------------------- state: column per thread
     constexpr int kNC = NS * 4 / K::kStateWarps;  // state columns per thread, from kNC * sp on
     const int sp = (warp - kOutWarps) >> 2;
-    const int64_t st_off =
-        ((n * p.H + h0) * static_cast<int64_t>(P) + row) * NS + kNC * sp;
     const bool mine = row_head < heads;
     float S[kNC];
 #pragma unroll
     for (int i = 0; i < kNC; ++i) S[i] = 0.f;
     float left = 1.f;
 
-    if (!kStates && mine) {
-      if (p.state) {
-        const float* src = static_cast<const float*>(p.state) + st_off;
+    // fp32 states pass through shared memory, by bulk copies in swizzled rows of 32 values: read
+    // or written by threads that each own a row, memory would see 16 bytes of every 512 at a
+    // time (4 us for 64 KB and the other loads behind it, against 1).
+    const uint32_t s_tile = row_head * (P * NS * 4) + row_base(row % P);
+    auto s_at = [&](uint32_t base, int i) {  // of S[i], i a multiple of 4
+      const int at = kNC * sp + i;
+      return base + (at >> 5) * (P * 128) + (s_tile ^ (16 * ((at >> 2) & 7)));
+    };
+    if (!kStates) {
+      const int items = (p.state ? 1 : 0) + static_cast<int>(seg);
+      for (int k = 0; k < items; ++k) {
+        // the sequence's first state, then its segments before this one
+        const int64_t r = slot - items + k;
+        const float g = p.state && k == 0 ? 0.f : (mine ? sg.left[r * p.H + h0 + row_head] : 0.f);
+        wait(bars_u + 8 * (kFullState), k & 1);
+        if (mine) {
 #pragma unroll
-        for (int i = 0; i < kNC; i += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(src + i);
-          S[i] = v.x;
-          S[i + 1] = v.y;
-          S[i + 2] = v.z;
-          S[i + 3] = v.w;
-          if (i % 16 == 12) asm volatile("" ::: "memory");  // no more loads in flight than that
+          for (int i = 0; i < kNC; i += 4) {
+            const float4 v = lds4(s_at(sm_u + K::kX + K::kXBytes, i));
+            S[i] = fmaf(g, S[i], v.x);
+            S[i + 1] = fmaf(g, S[i + 1], v.y);
+            S[i + 2] = fmaf(g, S[i + 2], v.z);
+            S[i + 3] = fmaf(g, S[i + 3], v.w);
+          }
         }
-      }
-      for (int64_t r = slot - seg; r < slot; ++r) {  // this sequence's segments before this one
-        const float g = sg.left[r * p.H + h0 + row_head];
-        const float* src =
-            sg.add + ((r * p.H + h0) * static_cast<int64_t>(P) + row) * NS + kNC * sp;
-#pragma unroll
-        for (int i = 0; i < kNC; i += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(src + i);
-          S[i] = fmaf(g, S[i], v.x);
-          S[i + 1] = fmaf(g, S[i + 1], v.y);
-          S[i + 2] = fmaf(g, S[i + 2], v.z);
-          S[i + 3] = fmaf(g, S[i + 3], v.w);
-          if (i % 16 == 12) asm volatile("" ::: "memory");
-        }
+        arrive(kStateRead);
       }
     }
 
@@ -795,19 +801,22 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         }
       }
     }
-    if (mine) {
-      float* dst = nullptr;
-      if (kStates) {
-        dst = sg.add + ((slot * p.H + h0) * static_cast<int64_t>(P) + row) * NS + kNC * sp;
-        if (sp == 0 && row % P == 0) sg.left[slot * p.H + h0 + row_head] = left;
-      } else if (last) {
-        dst = static_cast<float*>(p.new_state) + st_off;
-      }
-      if (dst) {
+    if (kStates && mine && sp == 0 && row % P == 0) sg.left[slot * p.H + h0 + row_head] = left;
+    if (kStates || last) {
+      // over B and the state's operand: the last dS is done, and with it all that reads them
 #pragma unroll
-        for (int i = 0; i < kNC; i += 4)
-          *reinterpret_cast<float4*>(dst + i) = make_float4(S[i], S[i + 1], S[i + 2], S[i + 3]);
+      for (int i = 0; i < kNC; i += 4)
+        sts4(s_at(sm_u + K::kB, i), S[i], S[i + 1], S[i + 2], S[i + 3]);
+      fence_async_smem();
+      named_bar_sync(2, K::kStateWarps * 32);
+      if (warp == kOutWarps && lane == 0) {
+        const int64_t to = ((kStates ? slot : n) * p.H + h0) * static_cast<int64_t>(P);
+        for (int hh = 0; hh < heads; ++hh)
+          tma_store_3d(&maps.last, sm + K::kB + hh * (P * NS * 4), 0, static_cast<int>(to) + hh * P, 0);
+        bulk_commit();
+        bulk_wait_all();
       }
+      __syncwarp();
     }
   } else {
     if (!kStates) regs_dec<kMiscRegs>();
@@ -943,9 +952,26 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         mbar_arrive_expect_tx(bars + kFullC, K::kBBytes);
         tma_load_3d(sm + K::kC, &maps.c, bars + kFullC, 0, tok0 + c * kL, bc);
       };
-      for (int c = 0; c < K::kXStages && c < chunks; ++c) {
+      if (chunks > 0) {
+        load_b(0);
+        if (!kStates) load_c(0);
+        load_x(0);
+      }
+      if (!kStates) {  // states, one after the other in the other stages of x
+        const int items = (p.state ? 1 : 0) + static_cast<int>(seg);
+        for (int k = 0; k < items; ++k) {
+          if (k > 0) wait(bars_u + 8 * (kStateRead), (k - 1) & 1);
+          const bool first = p.state && k == 0;
+          const int64_t from = ((first ? n : slot - items + k) * p.H + h0) * static_cast<int64_t>(P);
+          mbar_arrive_expect_tx(bars + kFullState, heads * P * NS * 4);
+          for (int hh = 0; hh < heads; ++hh)
+            tma_load_3d(sm + K::kX + K::kXBytes + hh * (P * NS * 4), first ? &maps.first : &maps.add,
+                        bars + kFullState, 0, static_cast<int>(from) + hh * P, 0);
+        }
+        if (items > 0) wait(bars_u + 8 * (kStateRead), (items - 1) & 1);
+      }
+      for (int c = 1; c < K::kXStages && c < chunks; ++c) {
         if (c < K::kBStages) load_b(c);
-        if (!kStates && c == 0) load_c(c);
         load_x(c);
       }
       for (int c = 0; c < chunks; ++c) {
@@ -1045,6 +1071,18 @@ bool encode(CUtensorMap* map, const void* base, int64_t T, int64_t cols, uint32_
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool encode_state(CUtensorMap* map, const void* base, int64_t rows, int P, int Ns) {
+  chunk::EncodeTiledFn enc = chunk::get_encode_fn();
+  if (!enc) return false;
+  const cuuint64_t dims[3] = {32, static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(Ns / 32)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(Ns) * 4, 128};
+  const cuuint32_t box[3] = {32, static_cast<cuuint32_t>(P), static_cast<cuuint32_t>(Ns / 32)};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(base), dims, strides, box,
+             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int column_blocks(int H, int G, int P) {
   const int heads = 128 / P;
   return G * ((H / G + heads - 1) / heads);
@@ -1079,11 +1117,18 @@ int launch_as(const SsmParams& p, cudaStream_t stream) {
       !encode(&maps.c, any ? static_cast<const void*>(p.C) : p.new_state, T, gn, NS / 64) ||
       !encode(&maps.out, any ? static_cast<const void*>(p.out) : p.new_state, T, hp, 1))
     return GDN_ERR_CUDA;
+  // (row coordinates are 32-bit)
+  if (p.N * hp > 0x7fffffffLL || sg.slots * hp > 0x7fffffffLL) return GDN_ERR_UNSUPPORTED_SHAPE;
+  const void* const first = p.state ? p.state : p.new_state;
+  if (!encode_state(&maps.first, first, p.N * hp, P, NS)) return GDN_ERR_CUDA;
+  maps.add = maps.last = maps.first;
   const unsigned grid = static_cast<unsigned>(sg.slots * cols);
   if (sg.len) {
     if (!p.workspace) return GDN_ERR_WORKSPACE;
     sg.add = p.workspace;
     sg.left = p.workspace + sg.slots * hp * NS;
+    if (!encode_state(&maps.add, sg.add, sg.slots * hp, P, NS)) return GDN_ERR_CUDA;
+    maps.last = maps.add;
     using K = Cfg<P, NS, true>;
     auto fn = ssm_chunk_kernel<P, NS, true>;
     if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, K::kBytes) !=
@@ -1092,6 +1137,7 @@ int launch_as(const SsmParams& p, cudaStream_t stream) {
     fn<<<grid, K::kThreads, K::kBytes, stream>>>(p, maps, sg, cols);
     if (cudaGetLastError() != cudaSuccess) return GDN_ERR_CUDA;
   }
+  if (!encode_state(&maps.last, p.new_state, p.N * hp, P, NS)) return GDN_ERR_CUDA;
   using K = Cfg<P, NS, false>;
   auto fn = ssm_chunk_kernel<P, NS, false>;
   // the new shares wait for registers that the launch has to have brought
@@ -1109,8 +1155,11 @@ int launch_as(const SsmParams& p, cudaStream_t stream) {
 
 }  // namespace
 
-bool ssm_chunked_takes(int P, int Ns) {
-  return (P == 64 || P == 128) && (Ns == 64 || Ns == 128);
+// Few tokens per sequence go token by token: with 32 heads of 128 and states of 128, us token by
+// token against chunked: one sequence of 8 tokens 8.0 / 10.8, of 16 13.4 / 10.8; 8 sequences of
+// 4 18.6 / 20.5, of 8 30.6 / 20.7; 64 of 4 132 / 140, of 8 220 / 140.
+bool ssm_chunked_takes(int P, int Ns, int64_t T, int64_t N) {
+  return (P == 64 || P == 128) && (Ns == 64 || Ns == 128) && T > 4 * N + 8;
 }
 
 size_t ssm_chunked_workspace(int64_t T, int64_t N, int H, int G, int P, int Ns) {

@@ -63,7 +63,7 @@ def gates(dt, dt_bias, A_log):
     1); exp and log1p err by at most 2 u each, with two more for the sum and the branch. log g
     has the error of exp(A_log) (2 u) and of the product (u) besides; exp turns a relative
     error of its argument z into |z| times it, and adds 2 u."""
-    v = dt.double().cpu() + dt_bias.double().cpu()
+    v = (dt.double().cpu() + dt_bias.double().cpu()).clamp(min=-700.0)  # softplus(-700) = 0 here
     d = torch.nn.functional.softplus(v, threshold=1e9)
     lg = -torch.exp(A_log.double().cpu()) * d
     de = (6 + v.abs()) * U

@@ -100,7 +100,7 @@ def test_ssm_chunked_workspace_and_alignment(cuda_lib):
     assert _ssm(lib, "chunked", **call) == -5
     assert _ssm(lib, "chunked", ws=P16, wb=need - 1, **call) == -5
     assert _ssm(lib, "chunked", ws=P16 + 4, wb=need, **call) == -1
-    assert _ssm(lib, "chunked", out=P16 + 2) == -1
+    assert _ssm(lib, "chunked", T=100, out=P16 + 2) == -1
     assert _ssm(lib, "chunked", T=0x7fffff01) == -2
 
 

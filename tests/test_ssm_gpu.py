@@ -112,6 +112,29 @@ def test_chunked_uncovered_rows_and_neighbours():
         assert not torch.isnan(got[0][5:300]).any() and not torch.isnan(got[1]).any()
 
 
+@pytest.mark.parametrize("lengths", [[1], [2, 3], [12], [13], [4] * 9, [5] * 9, [1] * 40])
+def test_short_prompts(lengths):
+    """Both sides of the rule that gives short prompts to the token-by-token kernel."""
+    a = make(lengths, H=3, G=1, P=64, Ns=128, seed=35)
+    check_prompt(ssm.prefill(*dev(a), check=True), a, True)
+
+
+def test_masked_tokens():
+    """dt of -infinity: the token adds nothing and the state keeps its value; whole sequences,
+    chunks and single tokens of it."""
+    a = make([300, 140], seed=36)
+    a[1][128:270] = float("-inf")
+    a[1][300:] = float("-inf")
+    for fn, chunked in ((ssm.prefill, True), (ssm.prefill_recurrent, False)):
+        got = fn(*dev(a), check=True)
+        check_prompt(got, a, chunked)
+        assert torch.equal(got[1][1].cpu(), a[7][1])
+    t = slice(300, 302)
+    tok = [a[0][t, None], a[1][t, None], a[2], a[3][t, None], a[4][t, None], a[5], a[6], a[7]]
+    out, ns = ssm.decode(*dev(tok))
+    assert torch.equal(ns.cpu(), a[7]) and not torch.isnan(out).any()
+
+
 def test_chunked_many_sequences():
     lengths = [(i * 37) % 140 for i in range(200)]
     a = make(lengths, H=2, G=1, seed=33)
