@@ -82,7 +82,8 @@ struct Taps {
 
 // kN consecutive fp32 or bf16 parameters from element i on (16-byte aligned) as floats.
 template <int kN>
-__device__ __forceinline__ void load_params(const void* base, int dtype, int64_t i, float (&v)[kN]) {
+__device__ __forceinline__ void load_params(const void* base, int dtype, int64_t i,
+                                            float (&v)[kN]) {
   if (dtype == kBF16) {
     const uint4* p = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(base) + i);
 #pragma unroll
@@ -151,9 +152,12 @@ __device__ __forceinline__ Place place_of(const ConvParams& p, int c) {
 }
 
 // v / (1 + e^-v) of two values with three MUFU operations instead of four: one reciprocal of
-// the product of the denominators. The exponent is capped at 2^63 so that the product stays
-// finite; below v = -43 the result is then -43 2^-63 and the like instead of even less.
+// the product of the denominators. v is held at -43.5, where silu is -43.5 2^-62.8, nothing to
+// bf16's neighbours, so that the product stays finite (and a v of -1e38 or -infinity gives that
+// too). A NaN is kept by the factor v but not by the exponent, which both values share.
 __device__ __forceinline__ float2 silu2(float2 v) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(-43.5f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(-43.5f));
   const float2 z = __fmul2_rn(v, make_float2(-kLog2e, -kLog2e));
   float2 e;
   float r;
@@ -194,12 +198,12 @@ __device__ __forceinline__ void head_sums(float (&q)[kTok]) {
   }
 }
 
-// kTok output rows from row `at` on (kWide: at `out`): the taps over the window and `rows` (which enter the
-// window one by one), activation, norm of the head (16 lanes), store. All lanes of the warp
-// call it; `live` says whether this thread's channels exist.
+// kTok output rows from row `at` on (kWide: at `out`): the taps over the window and `rows`
+// (which enter the window one by one), activation, norm of the head (16 lanes), store. All lanes
+// of the warp call it; `live` says whether this thread's channels exist.
 template <int W, bool kWide, int kTok>
-__device__ __forceinline__ void output_rows(const ConvParams& p, const Taps<W>& taps, const Place& pl,
-                                            int c, int64_t at, __nv_bfloat16* out, Window<W>& win,
+__device__ __forceinline__ void output_rows(const ConvParams& p, const Taps<W>& taps,
+                                            const Place& pl, int c, int64_t at, __nv_bfloat16* out, Window<W>& win,
                                             const Row (&rows)[kTok], bool live) {
   float2 y[kTok][kP];
 #pragma unroll
@@ -296,8 +300,8 @@ __device__ __forceinline__ void copy16_async(uint4* to, const __nv_bfloat16* fro
 }
 
 template <int W, bool kWide>
-__global__ void __launch_bounds__(kThreads) conv_prefill_kernel(const __grid_constant__ ConvParams p,
-                                                               int64_t tiles, int run) {
+__global__ void __launch_bounds__(kThreads)
+conv_prefill_kernel(const __grid_constant__ ConvParams p, int64_t tiles, int run) {
   const int c = (blockIdx.x * kThreads + threadIdx.x) * kVec;
   const bool live = c < p.C;
   const int64_t by = blockIdx.y + static_cast<int64_t>(blockIdx.z) * gridDim.y;
@@ -416,8 +420,8 @@ __global__ void __launch_bounds__(kThreads) conv_prefill_kernel(const __grid_con
 // One token per sequence: each thread reads its 8 channels of the W-1 state rows and of x,
 // and writes the rows moved up by one, so the new state may be the old one's memory.
 template <int W, bool kWide>
-__global__ void __launch_bounds__(kThreads) conv_decode_kernel(const __grid_constant__ ConvParams p,
-                                                              int per_thread) {
+__global__ void __launch_bounds__(kThreads)
+conv_decode_kernel(const __grid_constant__ ConvParams p, int per_thread) {
   const int c = (blockIdx.x * kThreads + threadIdx.x) * kVec;
   const bool live = c < p.C;
   const int64_t by = blockIdx.y + static_cast<int64_t>(blockIdx.z) * gridDim.y;
@@ -456,8 +460,8 @@ __global__ void __launch_bounds__(kThreads) conv_decode_kernel(const __grid_cons
 
 bool wide_ok(const ConvParams& p) {
   auto al = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; };
-  if (!al(p.x) || p.x_stride % kVec || p.C % kVec || !al(p.new_state) || (p.state && !al(p.state)) ||
-      !al(p.weight) || (p.bias && !al(p.bias)))
+  if (!al(p.x) || p.x_stride % kVec || p.C % kVec || !al(p.new_state) ||
+      (p.state && !al(p.state)) || !al(p.weight) || (p.bias && !al(p.bias)))
     return false;
   for (int s = 0; s < p.sections; ++s)
     if (p.begin[s + 1] % kVec || !al(p.out[s])) return false;

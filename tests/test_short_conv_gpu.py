@@ -75,6 +75,31 @@ def test_sections_and_norms(C, split, norm, wdtype):
     check(got, ns, x[:9], w, b, st, list(range(10)), split=split, norm=norm)
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf"), -3e38, 3e38])
+def test_one_channel_leaves_its_neighbours_alone(bad):
+    """A channel's extreme value reaches that channel's outputs, of its own and the next W - 1
+    tokens, and nothing else; silu of a value far below zero is next to nothing."""
+    x, w, b, s, cu = make([40], 256, 4, bias=False)
+    w[:, :3], w[:, 3] = 0, 1
+    want, _ = short_conv.prefill(*dev(x, w, None, s, cu))
+    for ch in (6, 7):
+        y = x.clone()
+        y[20, ch] = bad
+        for cols in (256, 255):  # in vectors, and channel by channel
+            got, _ = short_conv.prefill(*dev(y[:, :cols].contiguous(), w[:cols], None,
+                                             s[..., :cols].contiguous(), cu), check=True)
+            other = torch.ones(40, cols, dtype=torch.bool)
+            other[20:24, ch] = False
+            assert torch.equal(got.cpu()[other], want[:, :cols].cpu()[other])
+            v = got[20, ch].item()
+            if bad != bad:
+                assert v != v
+            elif bad < 0:
+                assert abs(v) < 1e-16
+            else:
+                assert v == pytest.approx(bad, rel=2 ** -8)  # (bf16's own rounding of it)
+
+
 def test_zero_head_norm_and_eps():
     """A head of zeros stays zero; eps enters under the root."""
     x, w, _, _, cu = make([5], 256, 4, bias=False, seed=3)
