@@ -10,27 +10,37 @@
 //
 // One block per (column block, segment): 128 columns of x, that is one head of 128 or two
 // heads of 64 of one group (they share C B^T), over the chunks of one segment of a sequence.
-// Four products per chunk on tcgen05, accumulators in TMEM (512 columns):
-//     CB  [token i, token j]   = C B^T            operands as TMA brings them
-//     Y   [token, column]      = C S^T            S rounded to bf16, written to shared memory
-//     dS  [column, n]          = (f x)^T B        f x transposed into TMEM as bf16 hi + lo
-//     Y                       += M x              M = CB masked and decayed, bf16 in TMEM
-// Between the second and the fourth the block multiplies Y by e^{G_i} in TMEM. The state stays
-// in fp32 registers (thread = column, a quarter of n) for the whole segment.
+// Three products per chunk on tcgen05, accumulators in TMEM (512 columns):
+//     [CB, Y] [token, token | column]  = C [B; S]^T   S rounded to bf16, in shared memory
+//                                                     behind B: one operand of 256 rows
+//     dS      [column, n]              = (f x)^T B    f x transposed into TMEM as three bf16
+//                                                     terms, by quarters of 32 tokens
+//     Y                               += M x          M = CB masked and decayed, bf16 in TMEM
+// Between the first and the last the block multiplies Y by e^{G_i} in TMEM. The state stays
+// in fp32 registers (thread = column, half of n) for the whole segment.
 //
-// Roundings: x, B and C are exact bf16 operands. f x is a hi + lo pair (each term of the state
-// is off by 2^-16 at most, measured 6e-7 over all: the state is an fp32 result). S and M are
-// rounded once to bf16 as operands: they reach only y, which is rounded to bf16 itself.
+// Roundings: x, B and C are exact bf16 operands, and so are the three terms of f x, whose sum
+// is the fp32 product (the state, an fp32 result, is off by 3e-7; two terms left 2e-6). S and M
+// are rounded once to bf16 as operands: they reach only y, which is rounded to bf16 itself.
 //
 // Segments. With few (sequence, column block) chains the sequences are cut into segments of a
-// multiple of 128 tokens. A first kernel (the same code, third product only) computes what
+// multiple of 128 tokens. A first kernel (the same code, second product only) computes what
 // each segment adds to the state and what it leaves of it; each block of the second kernel
 // then folds those of the segments before its own into its first state.
 //
-// Warps: 0-7 the output (M, the scaling of Y, y), 8-15 the state (f x, S), which run at their own
-// pace and so cover each other's waits; 16 issues the products, 17 the bulk copies, 18 and 19
-// the gates (one head each, up to two chunks ahead). Every wait is bounded; a block that gives
+// Warps: 0-7 the output (M, the scaling of Y, y, and a chunk's first quarter of f x), 8-15 the
+// state (the other quarters, S), which run at their own pace and so cover each other's waits; 16
+// issues the products, each as soon as its operands are there, 17 the bulk copies, 18 and 19
+// the gates (one head each, up to four chunks ahead). Every wait is bounded; a block that gives
 // up reports it and runs on without waiting, so no barrier is left short of its threads.
+//
+// What bounds it: shared memory. Per chunk of 128 x 128 with Ns = 128 a block moves about 5400
+// of its 128-byte lines (products' operands 1800, bulk copies 1000, the roles' own loads and
+// stores 2400) in 6300 cycles. With heads of 128 and states of 128, at the 1.7 to 1.9 GHz that
+// the power limit leaves: 4 x 32768 tokens of 32 heads 990 to 1090 us (3.0 to 3.3 TB/s of the
+// bytes that have to move), one sequence of 32768 of 64 heads of 64 424 us, of which the
+// segments' states take 129, and one chunk, mostly latency, 10.8 us. Two chunks per SM at a
+// time would need twice the shared memory.
 #include "gdn_b200.h"
 #include "gdn_chunk_common.cuh"
 #include "ssm_launch.h"
@@ -44,6 +54,7 @@ using chunk::named_bar_sync;
 
 constexpr int kL = 128;             // tokens per chunk
 constexpr int kBlock = 16384;       // a [128 rows x 64 columns] bf16 tile
+constexpr int kMaxBars = 48;
 
 // Registers per thread of the output kernel: 96 at launch (640 threads), then shared out anew
 // between the output's, the state's and the other warps: 256 x 96 + 256 x 104 + 128 x 80 is
@@ -102,7 +113,9 @@ __device__ __forceinline__ void sts4u(uint32_t a, uint32_t x, uint32_t y, uint32
                : "memory");
 }
 // Offset of row `row`'s 16-byte chunk 0 in a swizzled tile; chunk k is at this XOR 16 k.
-__device__ __forceinline__ uint32_t row_base(uint32_t row) { return row * 128u + ((row & 7u) << 4); }
+__device__ __forceinline__ uint32_t row_base(uint32_t row) {
+  return row * 128u + ((row & 7u) << 4);
+}
 
 // TMEM columns
 constexpr uint32_t kTG = 0;         // C B^T; then M, 8 of every 16 columns per head
@@ -121,7 +134,8 @@ struct Gates {
   float tot[4];                     // G over each block of 32
 };
 constexpr uint32_t kCum = 0, kDec = 512, kU = 1024, kF = 1536, kH = 2048, kTot = 2560;
-static_assert(sizeof(Gates) == kTot + 16, "");
+constexpr uint32_t kGatesBytes = sizeof(Gates);
+static_assert(kGatesBytes == kTot + 16 && kGatesBytes % 16 == 0, "");
 
 // Chunks whose gates there is room for. The gates' warp takes some 3000 cycles a chunk, in a chain
 // of short dependent steps: with two stages it was in the loop of the others' waits.
@@ -162,11 +176,9 @@ struct Cfg {
   static constexpr uint32_t kC = kB + kBStages * kNB * kBStep;
   static constexpr uint32_t kGates = kC + (kStates ? 0 : kBBytes);
   static constexpr uint32_t kBars = kGates + kGateStages * kHeads * sizeof(Gates);
-  static constexpr uint32_t kBytes = kBars + 8 * 48 + 1024;  // and the alignment
+  static constexpr uint32_t kBytes = kBars + 8 * kMaxBars + 1024;  // and the alignment
 };
 
-static_assert(sizeof(Gates) % 16 == 0, "");
-static_assert(3 + 3 + 1 + 2 * kGateStages + 1 + 3 + 1 + 4 + 4 + 1 + 2 + 1 + 3 + 1 + 1 + 2 <= 48, "");
 enum Bar {
   kFullX = 0,                          // [3] one per stage
   kFullB = kFullX + 3,                 // [3]
@@ -188,10 +200,11 @@ enum Bar {
   kStateRead = kFullState + 1,
   kBarCount = kStateRead + 1,
 };
+static_assert(kBarCount <= kMaxBars, "");
 
-// Bounded waits in few instructions (the roles' code has to stay in the instruction cache: see
-// the note on code size below). A wait gives up after kTries polls of at most kPollNs each,
-// a second or two; later waits of the thread then do not wait at all.
+// Bounded waits in few instructions (all roles' code together has to stay in the instruction
+// cache, or they wait for instructions more than for each other). A wait gives up after kTries
+// polls of at most kPollNs each, a second or two; later waits of the thread do not wait at all.
 struct Waiter {
   static constexpr uint32_t kTries = 1u << 20, kPollNs = 2000;
   uint32_t left = kTries;
@@ -309,8 +322,8 @@ __device__ __forceinline__ float softplus(float v) {
 
 // Gates of a chunk's first `valid` tokens (the others: d = 0, no decay) of one head, four tokens
 // per lane (a block of 32: eight lanes). All sums run over terms of one sign, so none cancels.
-__device__ __forceinline__ void write_gates(uint32_t g, const float (&raw)[4], float neg_a, float dtb,
-                                            int valid, int lane) {
+__device__ __forceinline__ void write_gates(uint32_t g, const float (&raw)[4], float neg_a,
+                                            float dtb, int valid, int lane) {
   float d[4], lg[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -454,8 +467,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
                                          (16 * ((q & 1) * 4 + ((lane >> 3) & 1))));
   auto write_fx = [&](int c, int t) {
     const int k = 4 * c + t, place = k % K::kPlaces;
-    const uint32_t f = gates_u +
-                       (c % kGateStages * kHeads + row_head) * static_cast<uint32_t>(sizeof(Gates)) + kF +
+    const uint32_t f = gates_u + (c % kGateStages * kHeads + row_head) * kGatesBytes + kF +
                        4 * (32 * t + 16 * part) + 8 * (lane & 3);
     const float2 f0 = lds2(f), f1 = lds2(f + 32);
     const uint32_t xa = sm_u + K::kX + (c % K::kXStages) * K::kXBytes + (q >> 1) * kBlock +
@@ -509,167 +521,167 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     // (turn -1 only writes the first chunk's)
 #pragma unroll 1
     for (int c = -1; c < chunks; ++c) {
-     if (c >= 0) {
-      const int gs = c % kGateStages;
-      const uint32_t ga = gates_u + gs * kHeads * static_cast<uint32_t>(sizeof(Gates));
-      wait(bars_u + 8 * (kGatesFull + gs), (c / kGateStages) & 1);
-      wait(bars_u + 8 * (kCB), c & 1);
-      tc_fence_after();
-      // ---- M over C B^T, 16 columns at a time: those of head h go to 8 columns of the same
-      // 16, so a warp overwrites nothing that another has yet to read. The two warps of a
-      // quarter take every other 16 (each has one piece on the diagonal).
-#pragma unroll 1
-      for (int k = 0; k < 4; ++k) {  // piece k: columns 32 k + 16 half on, in block k of 32
-        float g[16];
-        const int j0 = 32 * k + 16 * half;
-        const uint32_t at = lanes + kTG + j0;
-        if (k <= q) {
-          tmem_ld16(at, g);
-          tmem_ld_wait();
+      if (c >= 0) {
+        const int gs = c % kGateStages;
+        const uint32_t ga = gates_u + gs * kHeads * kGatesBytes;
+        wait(bars_u + 8 * (kGatesFull + gs), (c / kGateStages) & 1);
+        wait(bars_u + 8 * (kCB), c & 1);
+        tc_fence_after();
+        // ---- M over C B^T, 16 columns at a time: those of head h go to 8 columns of the same
+        // 16, so a warp overwrites nothing that another has yet to read. The two warps of a
+        // quarter take every other 16 (each has one piece on the diagonal).
+  #pragma unroll 1
+        for (int k = 0; k < 4; ++k) {  // piece k: columns 32 k + 16 half on, in block k of 32
+          float g[16];
+          const int j0 = 32 * k + 16 * half;
+          const uint32_t at = lanes + kTG + j0;
+          if (k <= q) {
+            tmem_ld16(at, g);
+            tmem_ld_wait();
+          }
+          {
+            uint32_t m[kHeads][8];
+            if (k < q) {
+              // e^{G_i - G_j} d_j = e^{G_i - G_r} (e^{G_r - G_j} d_j), r the end of j's block,
+              // between j and i: both exponents are at most 0, and one exponential per row is left
+              float ex[kHeads];
+              float4 u[kHeads][4];
+  #pragma unroll
+              for (int hh = 0; hh < kHeads; ++hh) {  // all loads before the first use
+                const uint32_t gh = ga + hh * kGatesBytes;
+                ex[hh] = lds(gh + kCum + 4 * row);
+                if (k + 1 < q) ex[hh] += lds(gh + kTot + 4 * (k + 1));
+                if (k + 2 < q) ex[hh] += lds(gh + kTot + 4 * (k + 2));
+  #pragma unroll
+                for (int j = 0; j < 4; ++j) u[hh][j] = lds4(gh + kU + 4 * (j0 + 4 * j));
+              }
+  #pragma unroll
+              for (int hh = 0; hh < kHeads; ++hh) {
+                const float e = ex2(ex[hh]);
+                const float2 a = make_float2(e, e);
+  #pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const float4 v = u[hh][j];
+                  const float2 v0 = mul2(mul2(make_float2(v.x, v.y), a),
+                                         make_float2(g[4 * j], g[4 * j + 1]));
+                  const float2 v1 = mul2(mul2(make_float2(v.z, v.w), a),
+                                         make_float2(g[4 * j + 2], g[4 * j + 3]));
+                  m[hh][2 * j] = pack2_rn(v0.x, v0.y);
+                  m[hh][2 * j + 1] = pack2_rn(v1.x, v1.y);
+                }
+              }
+            } else if (k == q) {
+              const int i = row - j0;  // columns j <= i are on or below the diagonal
+              float own[kHeads];
+              float4 x[kHeads][4];
+  #pragma unroll
+              for (int hh = 0; hh < kHeads; ++hh) {
+                const uint32_t gh = ga + hh * kGatesBytes;
+                own[hh] = lds(gh + kCum + 4 * row);
+  #pragma unroll
+                for (int j = 0; j < 4; ++j) x[hh][j] = lds4(gh + kH + 4 * (j0 + 4 * j));
+              }
+  #pragma unroll
+              for (int hh = 0; hh < kHeads; ++hh) {
+  #pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const float4 v = x[hh][j];
+                  const float* const gj = g + 4 * j;
+                  const float v0 = 4 * j <= i ? gj[0] * ex2(own[hh] + v.x) : 0.f;
+                  const float v1 = 4 * j + 1 <= i ? gj[1] * ex2(own[hh] + v.y) : 0.f;
+                  const float v2 = 4 * j + 2 <= i ? gj[2] * ex2(own[hh] + v.z) : 0.f;
+                  const float v3 = 4 * j + 3 <= i ? gj[3] * ex2(own[hh] + v.w) : 0.f;
+                  m[hh][2 * j] = pack2_rn(v0, v1);
+                  m[hh][2 * j + 1] = pack2_rn(v2, v3);
+                }
+              }
+            } else {
+  #pragma unroll
+              for (int hh = 0; hh < kHeads; ++hh) {
+  #pragma unroll
+                for (int j = 0; j < 8; ++j) m[hh][j] = 0u;
+              }
+            }
+  #pragma unroll
+            for (int hh = 0; hh < kHeads; ++hh) tmem_st8(at + 8 * hh, m[hh]);
+          }
         }
+        // ---- Y = e^{G_i} (C S^T), in place
         {
-          uint32_t m[kHeads][8];
-          if (k < q) {
-            // e^{G_i - G_j} d_j = e^{G_i - G_r} (e^{G_r - G_j} d_j), r the end of j's block,
-            // between j and i: both exponents are at most 0, and one exponential per row is left
-            float ex[kHeads];
-            float4 u[kHeads][4];
-#pragma unroll
-            for (int hh = 0; hh < kHeads; ++hh) {  // all loads before the first use
-              const uint32_t gh = ga + hh * static_cast<uint32_t>(sizeof(Gates));
-              ex[hh] = lds(gh + kCum + 4 * row);
-              if (k + 1 < q) ex[hh] += lds(gh + kTot + 4 * (k + 1));
-              if (k + 2 < q) ex[hh] += lds(gh + kTot + 4 * (k + 2));
-#pragma unroll
-              for (int j = 0; j < 4; ++j) u[hh][j] = lds4(gh + kU + 4 * (j0 + 4 * j));
+          const float e = lds(ga + col_head * kGatesBytes + kDec + 4 * row);
+          const float2 e2 = make_float2(e, e);
+  #pragma unroll 1
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t ty = lanes + kTY + 64 * half + 32 * k;
+            float y[32];
+            tmem_ld32(ty, y);
+            tmem_ld_wait();
+  #pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float2 v = mul2(make_float2(y[i], y[i + 1]), e2);
+              y[i] = v.x;
+              y[i + 1] = v.y;
             }
-#pragma unroll
-            for (int hh = 0; hh < kHeads; ++hh) {
-              const float e = ex2(ex[hh]);
-              const float2 a = make_float2(e, e);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float4 v = u[hh][j];
-                const float2 v0 = mul2(mul2(make_float2(v.x, v.y), a),
-                                       make_float2(g[4 * j], g[4 * j + 1]));
-                const float2 v1 = mul2(mul2(make_float2(v.z, v.w), a),
-                                       make_float2(g[4 * j + 2], g[4 * j + 3]));
-                m[hh][2 * j] = pack2_rn(v0.x, v0.y);
-                m[hh][2 * j + 1] = pack2_rn(v1.x, v1.y);
-              }
-            }
-          } else if (k == q) {
-            const int i = row - j0;  // columns j <= i are on or below the diagonal
-            float own[kHeads];
-            float4 x[kHeads][4];
-#pragma unroll
-            for (int hh = 0; hh < kHeads; ++hh) {
-              const uint32_t gh = ga + hh * static_cast<uint32_t>(sizeof(Gates));
-              own[hh] = lds(gh + kCum + 4 * row);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) x[hh][j] = lds4(gh + kH + 4 * (j0 + 4 * j));
-            }
-#pragma unroll
-            for (int hh = 0; hh < kHeads; ++hh) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float4 v = x[hh][j];
-                const float* const gj = g + 4 * j;
-                const float v0 = 4 * j <= i ? gj[0] * ex2(own[hh] + v.x) : 0.f;
-                const float v1 = 4 * j + 1 <= i ? gj[1] * ex2(own[hh] + v.y) : 0.f;
-                const float v2 = 4 * j + 2 <= i ? gj[2] * ex2(own[hh] + v.z) : 0.f;
-                const float v3 = 4 * j + 3 <= i ? gj[3] * ex2(own[hh] + v.w) : 0.f;
-                m[hh][2 * j] = pack2_rn(v0, v1);
-                m[hh][2 * j + 1] = pack2_rn(v2, v3);
-              }
-            }
-          } else {
-#pragma unroll
-            for (int hh = 0; hh < kHeads; ++hh) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) m[hh][j] = 0u;
-            }
+            tmem_st32(ty, y);
           }
-#pragma unroll
-          for (int hh = 0; hh < kHeads; ++hh) tmem_st8(at + 8 * hh, m[hh]);
         }
-      }
-      // ---- Y = e^{G_i} (C S^T), in place
-      {
-        const float e = lds(ga + col_head * static_cast<uint32_t>(sizeof(Gates)) + kDec + 4 * row);
-        const float2 e2 = make_float2(e, e);
-#pragma unroll 1
-        for (int k = 0; k < 2; ++k) {
-          const uint32_t ty = lanes + kTY + 64 * half + 32 * k;
-          float y[32];
-          tmem_ld32(ty, y);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float2 v = mul2(make_float2(y[i], y[i + 1]), e2);
-            y[i] = v.x;
-            y[i + 1] = v.y;
-          }
-          tmem_st32(ty, y);
-        }
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      arrive(kMy);
-      arrive(kGatesFree + gs);
-     }
-     if (c + 1 < chunks) first_fx(c + 1);
-     if (c >= 0) {
-      // ---- y: out of TMEM, D x added, over the chunk's x in shared memory
-      const int st = c % K::kXStages;
-      const uint32_t xrow = sm_u + K::kX + st * K::kXBytes + half * kBlock + row_base(row);
-      wait(bars_u + 8 * (kYM), c & 1);
-      tc_fence_after();
-      {
-        float y[2][32];
-        tmem_ld32(lanes + kTY + 64 * half, y[0]);
-        tmem_ld32(lanes + kTY + 64 * half + 32, y[1]);
-        tmem_ld_wait();
+        tmem_st_wait();
         tc_fence_before();
-        arrive(kYFree);  // the next chunk's first product may start
-        wait(bars_u + 8 * (kXRead), c & 1);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t at = xrow ^ (16 * k);
-          const uint4 xv = p.D ? lds4u(at) : make_uint4(0u, 0u, 0u, 0u);
-          const uint32_t u[4] = {xv.x, xv.y, xv.z, xv.w};
-          uint32_t w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 v = fma2(make_float2(skip, skip),
-                                  make_float2(__uint_as_float(u[e] << 16),
-                                              __uint_as_float(u[e] & 0xffff0000u)),
-                                  make_float2(y[k >> 2][8 * (k & 3) + 2 * e],
-                                              y[k >> 2][8 * (k & 3) + 2 * e + 1]));
-            w[e] = pack2_rn(v.x, v.y);
+        arrive(kMy);
+        arrive(kGatesFree + gs);
+      }
+      if (c + 1 < chunks) first_fx(c + 1);
+      if (c >= 0) {
+        // ---- y: out of TMEM, D x added, over the chunk's x in shared memory
+        const int st = c % K::kXStages;
+        const uint32_t xrow = sm_u + K::kX + st * K::kXBytes + half * kBlock + row_base(row);
+        wait(bars_u + 8 * (kYM), c & 1);
+        tc_fence_after();
+        {
+          float y[2][32];
+          tmem_ld32(lanes + kTY + 64 * half, y[0]);
+          tmem_ld32(lanes + kTY + 64 * half + 32, y[1]);
+          tmem_ld_wait();
+          tc_fence_before();
+          arrive(kYFree);  // the next chunk's first product may start
+          wait(bars_u + 8 * (kXRead), c & 1);
+  #pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t at = xrow ^ (16 * k);
+            const uint4 xv = p.D ? lds4u(at) : make_uint4(0u, 0u, 0u, 0u);
+            const uint32_t u[4] = {xv.x, xv.y, xv.z, xv.w};
+            uint32_t w[4];
+  #pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 v = fma2(make_float2(skip, skip),
+                                    make_float2(__uint_as_float(u[e] << 16),
+                                                __uint_as_float(u[e] & 0xffff0000u)),
+                                    make_float2(y[k >> 2][8 * (k & 3) + 2 * e],
+                                                y[k >> 2][8 * (k & 3) + 2 * e + 1]));
+              w[e] = pack2_rn(v.x, v.y);
+            }
+            sts4u(at, w[0], w[1], w[2], w[3]);
           }
-          sts4u(at, w[0], w[1], w[2], w[3]);
+        }
+        if (c < chunks - 1 || tail == kL) {
+          fence_async_smem();
+          arrive(kStaged + st);  // a bulk store takes the whole tile
+        } else {
+          // only the sequence's rows: 16 lanes write the 256 bytes of one
+          named_bar_sync(1, 256);
+          uint8_t* const xt = sm + K::kX + st * K::kXBytes;
+          const int l = lane & 15, blk = l >> 3;
+          const int64_t base = (static_cast<int64_t>(tok0) + c * kL) * p.H + h0;
+          if (kHeads == 1 || blk < heads) {
+            for (int r = warp * 2 + (lane >> 4); r < tail; r += 16) {
+              const uint4 v =
+                  *reinterpret_cast<const uint4*>(xt + blk * kBlock + sw128_chunk(r, l & 7));
+              const int64_t at = (base + static_cast<int64_t>(r) * p.H) * P + l * 8;
+              *reinterpret_cast<uint4*>(p.out + at) = v;
+            }
+          }
         }
       }
-      if (c < chunks - 1 || tail == kL) {
-        fence_async_smem();
-        arrive(kStaged + st);  // a bulk store takes the whole tile
-      } else {
-        // only the sequence's rows: 16 lanes write the 256 bytes of one
-        named_bar_sync(1, 256);
-        uint8_t* const xt = sm + K::kX + st * K::kXBytes;
-        const int l = lane & 15, blk = l >> 3;
-        const int64_t base = (static_cast<int64_t>(tok0) + c * kL) * p.H + h0;
-        if (kHeads == 1 || blk < heads) {
-          for (int r = warp * 2 + (lane >> 4); r < tail; r += 16) {
-            const uint4 v =
-                *reinterpret_cast<const uint4*>(xt + blk * kBlock + sw128_chunk(r, l & 7));
-            *reinterpret_cast<uint4*>(p.out + (base + static_cast<int64_t>(r) * p.H) * P + l * 8) =
-                v;
-          }
-        }
-      }
-     }
     }
   } else if (warp < kMisc) {
     if (!kStates) regs_inc<kStateRegs>();
@@ -752,8 +764,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       wait(bars_u + 8 * (kDS + c % K::kBStages), (c / K::kBStages) & 1);
       tc_fence_after();
       const float g =
-          lds(gates_u + (c % kGateStages * kHeads + row_head) * static_cast<uint32_t>(sizeof(Gates)) + kDec +
-              4 * (kL - 1));
+          lds(gates_u + (c % kGateStages * kHeads + row_head) * kGatesBytes + kDec + 4 * (kL - 1));
       const float2 g2 = make_float2(g, g);
       const uint32_t td = lanes + kTD + (kStates ? 128 * (c & 1) : 0) + kNC * sp;
 #pragma unroll
@@ -812,7 +823,8 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       if (warp == kOutWarps && lane == 0) {
         const int64_t to = ((kStates ? slot : n) * p.H + h0) * static_cast<int64_t>(P);
         for (int hh = 0; hh < heads; ++hh)
-          tma_store_3d(&maps.last, sm + K::kB + hh * (P * NS * 4), 0, static_cast<int>(to) + hh * P, 0);
+          tma_store_3d(&maps.last, sm + K::kB + hh * (P * NS * 4), 0, static_cast<int>(to) + hh * P,
+                       0);
         bulk_commit();
         bulk_wait_all();
       }
@@ -821,236 +833,239 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
   } else {
     if (!kStates) regs_dec<kMiscRegs>();
     if (warp == kMisc) {
-    // ---------------------------------------------------------------- products
-    constexpr uint32_t kIdCB = idesc_bf16(128, 256, false, false);
-    constexpr uint32_t kIdDS = idesc_bf16(128, NS, false, true);
-    constexpr uint32_t kIdYM = idesc_bf16(128, P, false, true);
-    // Descriptors differ in their start address alone: built where they are used, from bases
-    // that look new in every chunk, or all of them would be kept in registers.
-    const uint64_t d_k = desc_kmajor(0), d_x = desc_mnmajor(0, kBlock),
-                   d_b = desc_mnmajor(0, K::kBStep);
-    auto fresh = [](uint32_t v) {
-      uint32_t r;
-      asm volatile("mov.u32 %0, %1;" : "=r"(r) : "r"(v));
-      return r;
-    };
-    auto desc = [](uint64_t kind, uint32_t base, uint32_t off) {
-      return kind | static_cast<uint64_t>((base + off) >> 4);
-    };
-    auto kstep = [](int s, uint32_t block) {
-      return static_cast<uint32_t>((s >> 2) * block + (s & 3) * 32);
-    };
-    for (int c = 0; c < chunks; ++c) {
-      const int st = c % K::kBStages, par = (c / K::kBStages) & 1;
-      const uint32_t xb = sm_u + K::kX + (c % K::kXStages) * K::kXBytes;
-      const uint32_t bb = sm_u + K::kB + st * K::kBBytes;
-      const bool zeroed = c == chunks - 1 && tail < kL;
-      // dS by quarter t of the chunk's tokens, whose f x is in its place
-      auto issue_ds = [&](uint32_t td, int t) {
-        const int place = (4 * c + t) % K::kPlaces;
-        const uint32_t tf = tm + (kStates ? 0 : kTF) + 16 * kTerms * place;
-        const uint32_t b0 = fresh(bb + t * 4096);
-        tc_fence_after();
-#pragma unroll
-        for (int r = 0; r < kTerms; ++r) {
-#pragma unroll
-          for (int s = 0; s < 2; ++s)
-            mma_bf16_ts_w(td, tf + 16 * r + 8 * s, desc(d_b, b0, s * 2048), kIdDS,
-                          t > 0 || r > 0 || s > 0);
-        }
-        mma_commit_w(bars + kFxFree + place);
-        if (t == 3) mma_commit_w(bars + kDS + st);
+      // ---------------------------------------------------------------- products
+      constexpr uint32_t kIdCB = idesc_bf16(128, 256, false, false);
+      constexpr uint32_t kIdDS = idesc_bf16(128, NS, false, true);
+      constexpr uint32_t kIdYM = idesc_bf16(128, P, false, true);
+      // Descriptors differ in their start address alone: built where they are used, from bases
+      // that look new in every chunk, or all of them would be kept in registers.
+      const uint64_t d_k = desc_kmajor(0), d_x = desc_mnmajor(0, kBlock),
+                     d_b = desc_mnmajor(0, K::kBStep);
+      auto fresh = [](uint32_t v) {
+        uint32_t r;
+        asm volatile("mov.u32 %0, %1;" : "=r"(r) : "r"(v));
+        return r;
       };
-      auto fx_bar = [&](int t) { return bars_u + 8 * (kFx + (4 * c + t) % K::kPlaces); };
-      auto fx_par = [&](int t) { return static_cast<uint32_t>(((4 * c + t) / K::kPlaces) & 1); };
-      if (kStates) {
-        wait(bars_u + 8 * (kFullB + st), par);
-        if (c >= 2) wait(bars_u + 8 * (kState + (c & 1)), ((c >> 1) - 1) & 1);
-#pragma unroll 1
-        for (int t = 0; t < 4; ++t) {
-          wait(fx_bar(t), fx_par(t));
-          issue_ds(tm + kTD + 128 * (c & 1), t);
-        }
-        continue;
-      }
-      // The chunk's products, each as soon as its operands are there and its place is free. What
-      // the order has to keep: B's stage and the state's operand are free with the last quarter
-      // of dS, so C [B; S]^T comes before that.
-      bool cb = false, ym = false, b_in = false, state_in = false;
-      bool force = !wait.ok();  // a block that gave up does not wait
-      int t = 0;
-      uint32_t polls = 1u << 23;  // of some 100 cycles
-      auto ready = [&](int bar, uint32_t parity) {
-        return force || mbar_test_wait(bars_u + 8 * bar, parity);
+      auto desc = [](uint64_t kind, uint32_t base, uint32_t off) {
+        return kind | static_cast<uint64_t>((base + off) >> 4);
       };
-#pragma unroll 1
-      while (!ym || t < 4) {
-        b_in = b_in || ready(kFullB + st, par);
-        state_in = state_in || ready(kState, c & 1);
-        if (b_in && state_in && t < (cb ? 4 : 3) &&
-            ready(kFx + (4 * c + t) % K::kPlaces, ((4 * c + t) / K::kPlaces) & 1)) {
-          issue_ds(tm + kTD, t);
-          ++t;
-        }
-        if (!cb) {  // over the places of the last chunk's M and Y
-          if (b_in && state_in && ready(kFullC, c & 1) && (!zeroed || ready(kZeroed, 0)) &&
-              (c == 0 || ready(kYFree, (c - 1) & 1))) {
-            cb = true;
-            tc_fence_after();
-            const uint32_t b0 = fresh(bb), c0 = fresh(sm_u + K::kC);
-#pragma unroll 4
-            for (int s = 0; s < NS / 16; ++s)
-              mma_bf16_w(tm + kTG, desc(d_k, c0, kstep(s, kBlock)),
-                         desc(d_k, b0, kstep(s, K::kBStep)), kIdCB, s > 0);
-            mma_commit_w(bars + kCB);
-          }
-        } else if (!ym && ready(kMy, c & 1)) {
-          ym = true;
-          tc_fence_after();
-#pragma unroll 1
-          for (int hh = 0; hh < kHeads; ++hh) {
-            const uint32_t x0 = fresh(xb + hh * kBlock);
-#pragma unroll 4
-            for (int s = 0; s < 8; ++s)
-              mma_bf16_ts_w(tm + kTY + hh * 64, tm + kTG + 16 * s + 8 * hh, desc(d_x, x0, s * 2048),
-                            kIdYM, 1);
-          }
-          mma_commit_w(bars + kYM);
-        }
-        if (!force && --polls == 0) {
-          force = true;
-          wait.left = 0;
-        }
-      }
-    }
-    // the block's TMEM may go once the last product is done
-    if (chunks > 0) {
-      const int c = chunks - 1;
-      if (kStates) {
-        finally(bars_u + 8 * (kDS + c % K::kBStages), (c / K::kBStages) & 1);
-      } else {
-        finally(bars_u + 8 * (kYM), c & 1);
-      }
-    }
-  } else if (warp == kMisc + 1) {
-    // ---------------------------------------------------------------- bulk copies
-    if (lane == 0) {
-      const int xc = (h0 * P) / 64, bc = grp * K::kNB;
-      auto load_x = [&](int c) {
-        const int st = c % K::kXStages;
-        mbar_arrive_expect_tx(bars + kFullX + st, K::kXBytes);
-        tma_load_3d(sm + K::kX + st * K::kXBytes, &maps.x, bars + kFullX + st, 0, tok0 + c * kL, xc);
+      auto kstep = [](int s, uint32_t block) {
+        return static_cast<uint32_t>((s >> 2) * block + (s & 3) * 32);
       };
-      auto load_b = [&](int c) {
-        const int st = c % K::kBStages;
-        mbar_arrive_expect_tx(bars + kFullB + st, K::kBBytes);
-        for (int b = 0; b < K::kNB; ++b)
-          tma_load_3d(sm + K::kB + st * K::kBBytes + b * K::kBStep, &maps.b, bars + kFullB + st, 0,
-                      tok0 + c * kL, bc + b);
-      };
-      auto load_c = [&](int c) {
-        mbar_arrive_expect_tx(bars + kFullC, K::kBBytes);
-        tma_load_3d(sm + K::kC, &maps.c, bars + kFullC, 0, tok0 + c * kL, bc);
-      };
-      if (chunks > 0) {
-        load_b(0);
-        if (!kStates) load_c(0);
-        load_x(0);
-      }
-      if (!kStates) {  // states, one after the other in the other stages of x
-        const int items = (p.state ? 1 : 0) + static_cast<int>(seg);
-        for (int k = 0; k < items; ++k) {
-          if (k > 0) wait(bars_u + 8 * (kStateRead), (k - 1) & 1);
-          const bool first = p.state && k == 0;
-          const int64_t from = ((first ? n : slot - items + k) * p.H + h0) * static_cast<int64_t>(P);
-          mbar_arrive_expect_tx(bars + kFullState, heads * P * NS * 4);
-          for (int hh = 0; hh < heads; ++hh)
-            tma_load_3d(sm + K::kX + K::kXBytes + hh * (P * NS * 4), first ? &maps.first : &maps.add,
-                        bars + kFullState, 0, static_cast<int>(from) + hh * P, 0);
-        }
-        if (items > 0) wait(bars_u + 8 * (kStateRead), (items - 1) & 1);
-      }
-      for (int c = 1; c < K::kXStages && c < chunks; ++c) {
-        if (c < K::kBStages) load_b(c);
-        load_x(c);
-      }
       for (int c = 0; c < chunks; ++c) {
-        if (!kStates && c + 2 < chunks) {
-          // B and C have one stage: bring the next but one chunk's into L2, so that the copy
-          // that has to wait for the stage takes only L2's latency
-          for (int b = 0; b < K::kNB; ++b)
-            tma_prefetch_3d(&maps.b, 0, tok0 + (c + 2) * kL, bc + b);
-          tma_prefetch_3d(&maps.c, 0, tok0 + (c + 2) * kL, bc);
+        const int st = c % K::kBStages, par = (c / K::kBStages) & 1;
+        const uint32_t xb = sm_u + K::kX + (c % K::kXStages) * K::kXBytes;
+        const uint32_t bb = sm_u + K::kB + st * K::kBBytes;
+        const bool zeroed = c == chunks - 1 && tail < kL;
+        // dS by quarter t of the chunk's tokens, whose f x is in its place
+        auto issue_ds = [&](uint32_t td, int t) {
+          const int place = (4 * c + t) % K::kPlaces;
+          const uint32_t tf = tm + (kStates ? 0 : kTF) + 16 * kTerms * place;
+          const uint32_t b0 = fresh(bb + t * 4096);
+          tc_fence_after();
+  #pragma unroll
+          for (int r = 0; r < kTerms; ++r) {
+  #pragma unroll
+            for (int s = 0; s < 2; ++s)
+              mma_bf16_ts_w(td, tf + 16 * r + 8 * s, desc(d_b, b0, s * 2048), kIdDS,
+                            t > 0 || r > 0 || s > 0);
+          }
+          mma_commit_w(bars + kFxFree + place);
+          if (t == 3) mma_commit_w(bars + kDS + st);
+        };
+        auto fx_bar = [&](int t) { return bars_u + 8 * (kFx + (4 * c + t) % K::kPlaces); };
+        auto fx_par = [&](int t) { return static_cast<uint32_t>(((4 * c + t) / K::kPlaces) & 1); };
+        if (kStates) {
+          wait(bars_u + 8 * (kFullB + st), par);
+          if (c >= 2) wait(bars_u + 8 * (kState + (c & 1)), ((c >> 1) - 1) & 1);
+  #pragma unroll 1
+          for (int t = 0; t < 4; ++t) {
+            wait(fx_bar(t), fx_par(t));
+            issue_ds(tm + kTD + 128 * (c & 1), t);
+          }
+          continue;
         }
-        if (!kStates && c + 1 < chunks) {
-          wait(bars_u + 8 * (kCB), c & 1);
-          load_c(c + 1);
-        }
-        if (c + K::kBStages < chunks) {
-          wait(bars_u + 8 * (kDS + c % K::kBStages), (c / K::kBStages) & 1);
-          load_b(c + K::kBStages);
-          if (kStates) load_x(c + K::kXStages);  // x was read before the product
-        }
-        if (!kStates && (c < chunks - 1 || tail == kL)) {
-          const int st = c % K::kXStages;
-          wait(bars_u + 8 * (kStaged + st), (c / K::kXStages) & 1);
-          const uint8_t* xt = sm + K::kX + st * K::kXBytes;
-          for (int b = 0; b < 2; ++b)
-            if (kHeads == 1 || b < heads)
-              tma_store_3d(&maps.out, xt + b * kBlock, 0, tok0 + c * kL, xc + b);
-          bulk_commit();
-          if (c + K::kXStages < chunks) {
-            bulk_wait_read();
-            load_x(c + K::kXStages);
+        // The chunk's products, each as soon as its operands are there and its place is free. What
+        // the order has to keep: B's stage and the state's operand are free with the last quarter
+        // of dS, so C [B; S]^T comes before that.
+        bool cb = false, ym = false, b_in = false, state_in = false;
+        bool force = !wait.ok();  // a block that gave up does not wait
+        int t = 0;
+        uint32_t polls = 1u << 23;  // of some 100 cycles
+        auto ready = [&](int bar, uint32_t parity) {
+          return force || mbar_test_wait(bars_u + 8 * bar, parity);
+        };
+  #pragma unroll 1
+        while (!ym || t < 4) {
+          b_in = b_in || ready(kFullB + st, par);
+          state_in = state_in || ready(kState, c & 1);
+          if (b_in && state_in && t < (cb ? 4 : 3) &&
+              ready(kFx + (4 * c + t) % K::kPlaces, ((4 * c + t) / K::kPlaces) & 1)) {
+            issue_ds(tm + kTD, t);
+            ++t;
+          }
+          if (!cb) {  // over the places of the last chunk's M and Y
+            if (b_in && state_in && ready(kFullC, c & 1) && (!zeroed || ready(kZeroed, 0)) &&
+                (c == 0 || ready(kYFree, (c - 1) & 1))) {
+              cb = true;
+              tc_fence_after();
+              const uint32_t b0 = fresh(bb), c0 = fresh(sm_u + K::kC);
+  #pragma unroll 4
+              for (int s = 0; s < NS / 16; ++s)
+                mma_bf16_w(tm + kTG, desc(d_k, c0, kstep(s, kBlock)),
+                           desc(d_k, b0, kstep(s, K::kBStep)), kIdCB, s > 0);
+              mma_commit_w(bars + kCB);
+            }
+          } else if (!ym && ready(kMy, c & 1)) {
+            ym = true;
+            tc_fence_after();
+  #pragma unroll 1
+            for (int hh = 0; hh < kHeads; ++hh) {
+              const uint32_t x0 = fresh(xb + hh * kBlock);
+  #pragma unroll 4
+              for (int s = 0; s < 8; ++s)
+                mma_bf16_ts_w(tm + kTY + hh * 64, tm + kTG + 16 * s + 8 * hh,
+                              desc(d_x, x0, s * 2048), kIdYM, 1);
+            }
+            mma_commit_w(bars + kYM);
+          }
+          if (!force && --polls == 0) {
+            force = true;
+            wait.left = 0;
           }
         }
       }
-      if (!kStates) bulk_wait_all();
-      if (!wait.ok() && chunks > 0) {
-        // copies still in flight land in this block's shared memory: let them
+      // the block's TMEM may go once the last product is done
+      if (chunks > 0) {
         const int c = chunks - 1;
-        finally(bars_u + 8 * (kFullX + c % K::kXStages), (c / K::kXStages) & 1);
-        finally(bars_u + 8 * (kFullB + c % K::kBStages), (c / K::kBStages) & 1);
-        if (!kStates) finally(bars_u + 8 * (kFullC), c & 1);
+        if (kStates) {
+          finally(bars_u + 8 * (kDS + c % K::kBStages), (c / K::kBStages) & 1);
+        } else {
+          finally(bars_u + 8 * (kYM), c & 1);
+        }
       }
-    }
-    __syncwarp();
-  } else if (warp - kMisc - 2 < kHeads) {
-    // ---------------------------------------------------------------- gates of one head
-    const int hh = warp - kMisc - 2;
-    const bool present = hh < heads;
-    const int h = h0 + (present ? hh : 0);
-    const float neg_a = -expf(load_scalar(p.A_log, p.A_log_dtype, h));
-    const float dtb = load_scalar(p.dt_bias, p.dt_bias_dtype, h);
-    // dt of a chunk as stored, asked for a chunk ahead: nothing may use a value before its chunk
-    // (a conversion here would wait for each of the four in turn, 800 cycles each)
-    const bool half = p.dt_dtype == kBF16;
-    auto load = [&](int c, uint32_t (&raw)[4]) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int t = min(c * kL + 4 * lane + k, tokens - 1);
-        const int64_t at = (static_cast<int64_t>(tok0) + t) * p.H + h;
-        raw[k] = half ? static_cast<const unsigned short*>(p.dt)[at]
-                      : static_cast<const uint32_t*>(p.dt)[at];
+    } else if (warp == kMisc + 1) {
+      // ---------------------------------------------------------------- bulk copies
+      if (lane == 0) {
+        const int xc = (h0 * P) / 64, bc = grp * K::kNB;
+        auto load_x = [&](int c) {
+          const int st = c % K::kXStages;
+          mbar_arrive_expect_tx(bars + kFullX + st, K::kXBytes);
+          tma_load_3d(sm + K::kX + st * K::kXBytes, &maps.x, bars + kFullX + st, 0, tok0 + c * kL,
+                      xc);
+        };
+        auto load_b = [&](int c) {
+          const int st = c % K::kBStages;
+          mbar_arrive_expect_tx(bars + kFullB + st, K::kBBytes);
+          for (int b = 0; b < K::kNB; ++b)
+            tma_load_3d(sm + K::kB + st * K::kBBytes + b * K::kBStep, &maps.b, bars + kFullB + st,
+                        0, tok0 + c * kL, bc + b);
+        };
+        auto load_c = [&](int c) {
+          mbar_arrive_expect_tx(bars + kFullC, K::kBBytes);
+          tma_load_3d(sm + K::kC, &maps.c, bars + kFullC, 0, tok0 + c * kL, bc);
+        };
+        if (chunks > 0) {
+          load_b(0);
+          if (!kStates) load_c(0);
+          load_x(0);
+        }
+        if (!kStates) {  // states, one after the other in the other stages of x
+          const int items = (p.state ? 1 : 0) + static_cast<int>(seg);
+          for (int k = 0; k < items; ++k) {
+            if (k > 0) wait(bars_u + 8 * (kStateRead), (k - 1) & 1);
+            const bool first = p.state && k == 0;
+            const int64_t from =
+                ((first ? n : slot - items + k) * p.H + h0) * static_cast<int64_t>(P);
+            mbar_arrive_expect_tx(bars + kFullState, heads * P * NS * 4);
+            for (int hh = 0; hh < heads; ++hh)
+              tma_load_3d(sm + K::kX + K::kXBytes + hh * (P * NS * 4),
+                          first ? &maps.first : &maps.add, bars + kFullState, 0,
+                          static_cast<int>(from) + hh * P, 0);
+          }
+          if (items > 0) wait(bars_u + 8 * (kStateRead), (items - 1) & 1);
+        }
+        for (int c = 1; c < K::kXStages && c < chunks; ++c) {
+          if (c < K::kBStages) load_b(c);
+          load_x(c);
+        }
+        for (int c = 0; c < chunks; ++c) {
+          if (!kStates && c + 2 < chunks) {
+            // B and C have one stage: bring the next but one chunk's into L2, so that the copy
+            // that has to wait for the stage takes only L2's latency
+            for (int b = 0; b < K::kNB; ++b)
+              tma_prefetch_3d(&maps.b, 0, tok0 + (c + 2) * kL, bc + b);
+            tma_prefetch_3d(&maps.c, 0, tok0 + (c + 2) * kL, bc);
+          }
+          if (!kStates && c + 1 < chunks) {
+            wait(bars_u + 8 * (kCB), c & 1);
+            load_c(c + 1);
+          }
+          if (c + K::kBStages < chunks) {
+            wait(bars_u + 8 * (kDS + c % K::kBStages), (c / K::kBStages) & 1);
+            load_b(c + K::kBStages);
+            if (kStates) load_x(c + K::kXStages);  // x was read before the product
+          }
+          if (!kStates && (c < chunks - 1 || tail == kL)) {
+            const int st = c % K::kXStages;
+            wait(bars_u + 8 * (kStaged + st), (c / K::kXStages) & 1);
+            const uint8_t* xt = sm + K::kX + st * K::kXBytes;
+            for (int b = 0; b < 2; ++b)
+              if (kHeads == 1 || b < heads)
+                tma_store_3d(&maps.out, xt + b * kBlock, 0, tok0 + c * kL, xc + b);
+            bulk_commit();
+            if (c + K::kXStages < chunks) {
+              bulk_wait_read();
+              load_x(c + K::kXStages);
+            }
+          }
+        }
+        if (!kStates) bulk_wait_all();
+        if (!wait.ok() && chunks > 0) {
+          // copies still in flight land in this block's shared memory: let them
+          const int c = chunks - 1;
+          finally(bars_u + 8 * (kFullX + c % K::kXStages), (c / K::kXStages) & 1);
+          finally(bars_u + 8 * (kFullB + c % K::kBStages), (c / K::kBStages) & 1);
+          if (!kStates) finally(bars_u + 8 * (kFullC), c & 1);
+        }
       }
-    };
-    uint32_t raw[4];
-    if (chunks > 0) load(0, raw);
-#pragma unroll 1
-    for (int c = 0; c < chunks; ++c) {
-      const int gs = c % kGateStages;
-      float dt[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) dt[k] = __uint_as_float(half ? raw[k] << 16 : raw[k]);
-      if (c + 1 < chunks) load(c + 1, raw);
-      if (c >= kGateStages)
-        wait(bars_u + 8 * (kGatesFree + gs), (c / kGateStages - 1) & 1);
-      write_gates(gates_u + (gs * kHeads + hh) * static_cast<uint32_t>(sizeof(Gates)), dt, neg_a,
-                  dtb, present ? tokens - c * kL : 0, lane);
       __syncwarp();
-      if (lane == 0) mbar_arrive(bars + kGatesFull + gs);
+    } else if (warp - kMisc - 2 < kHeads) {
+      // ---------------------------------------------------------------- gates of one head
+      const int hh = warp - kMisc - 2;
+      const bool present = hh < heads;
+      const int h = h0 + (present ? hh : 0);
+      const float neg_a = -expf(load_scalar(p.A_log, p.A_log_dtype, h));
+      const float dtb = load_scalar(p.dt_bias, p.dt_bias_dtype, h);
+      // dt of a chunk as stored, asked for a chunk ahead: nothing may use a value before its chunk
+      // (a conversion here would wait for each of the four in turn, 800 cycles each)
+      const bool half = p.dt_dtype == kBF16;
+      auto load = [&](int c, uint32_t (&raw)[4]) {
+  #pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int t = min(c * kL + 4 * lane + k, tokens - 1);
+          const int64_t at = (static_cast<int64_t>(tok0) + t) * p.H + h;
+          raw[k] = half ? static_cast<const unsigned short*>(p.dt)[at]
+                        : static_cast<const uint32_t*>(p.dt)[at];
+        }
+      };
+      uint32_t raw[4];
+      if (chunks > 0) load(0, raw);
+  #pragma unroll 1
+      for (int c = 0; c < chunks; ++c) {
+        const int gs = c % kGateStages;
+        float dt[4];
+  #pragma unroll
+        for (int k = 0; k < 4; ++k) dt[k] = __uint_as_float(half ? raw[k] << 16 : raw[k]);
+        if (c + 1 < chunks) load(c + 1, raw);
+        if (c >= kGateStages)
+          wait(bars_u + 8 * (kGatesFree + gs), (c / kGateStages - 1) & 1);
+        write_gates(gates_u + (gs * kHeads + hh) * kGatesBytes, dt, neg_a,
+                    dtb, present ? tokens - c * kL : 0, lane);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars + kGatesFull + gs);
+      }
     }
-  }
   }
   if (!wait.ok()) report_wait(p.status);
   tc_fence_before();
@@ -1109,13 +1124,8 @@ int launch_as(const SsmParams& p, cudaStream_t stream) {
   if (sg.slots * cols > 0x7fffffffLL) return GDN_ERR_UNSUPPORTED_SHAPE;
   Maps maps;
   const int64_t hp = static_cast<int64_t>(p.H) * P, gn = static_cast<int64_t>(p.G) * NS;
-  // without tokens the maps are not read; any mapped memory will do
-  const int64_t T = p.T > 0 ? p.T : 1;
-  const bool any = p.T > 0;
-  if (!encode(&maps.x, any ? static_cast<const void*>(p.x) : p.new_state, T, hp, 2) ||
-      !encode(&maps.b, any ? static_cast<const void*>(p.B) : p.new_state, T, gn, 1) ||
-      !encode(&maps.c, any ? static_cast<const void*>(p.C) : p.new_state, T, gn, NS / 64) ||
-      !encode(&maps.out, any ? static_cast<const void*>(p.out) : p.new_state, T, hp, 1))
+  if (!encode(&maps.x, p.x, p.T, hp, 2) || !encode(&maps.b, p.B, p.T, gn, 1) ||
+      !encode(&maps.c, p.C, p.T, gn, NS / 64) || !encode(&maps.out, p.out, p.T, hp, 1))
     return GDN_ERR_CUDA;
   // (row coordinates are 32-bit)
   if (p.N * hp > 0x7fffffffLL || sg.slots * hp > 0x7fffffffLL) return GDN_ERR_UNSUPPORTED_SHAPE;

@@ -222,10 +222,11 @@ __global__ void __launch_bounds__(128) ssm_recurrent_kernel(const __grid_constan
     const int r = row0 + i * kPer + sub;
 #pragma unroll
     for (int j = 0; j < kPieces; ++j)
-      Piece<float>::unpack(p.state && r < p.P ? load_piece<float>(p.state, (head * p.P + r) * p.Ns +
-                                                                               (j * kLanes + l) * kE)
-                                              : make_uint4(0u, 0u, 0u, 0u),
-                           s[i][j]);
+      Piece<float>::unpack(
+          p.state && r < p.P
+              ? load_piece<float>(p.state, (head * p.P + r) * p.Ns + (j * kLanes + l) * kE)
+              : make_uint4(0u, 0u, 0u, 0u),
+          s[i][j]);
   }
   const float neg_a = -expf(load_scalar(p.A_log, p.A_log_dtype, h));
   const float dtb = load_scalar(p.dt_bias, p.dt_bias_dtype, h);
@@ -301,7 +302,8 @@ int decode_as(const SsmParams& p, cudaStream_t stream, int most_batches) {
   if (heads * splits > 0x7fffffffLL) return GDN_ERR_UNSUPPORTED_SHAPE;
   const unsigned grid = static_cast<unsigned>(heads * splits);
   if (batches > 1) {
-    ssm_decode_kernel<S, kLanes, kPieces, kRows, true><<<grid, 128, 0, stream>>>(p, splits, batches);
+    ssm_decode_kernel<S, kLanes, kPieces, kRows, true>
+        <<<grid, 128, 0, stream>>>(p, splits, batches);
   } else {
     ssm_decode_kernel<S, kLanes, kPieces, kRows, false><<<grid, 128, 0, stream>>>(p, splits, 1);
   }
@@ -321,8 +323,8 @@ int recurrent_as(const SsmParams& p, cudaStream_t stream) {
 
 }  // namespace
 
-// Batches per warp at most, where the grid stays full: a warp's gates and its B and C cost as much
-// as a batch of bf16 rows.
+// Batches per warp at most, where the grid stays full: a warp's gates and its B and C cost as
+// much as a batch of bf16 rows.
 constexpr int kF32Batches = 1, kBf16Batches = 4;
 
 int launch_ssm_decode(const SsmParams& p, cudaStream_t stream) {
