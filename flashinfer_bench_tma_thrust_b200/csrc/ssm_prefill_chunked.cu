@@ -1166,8 +1166,8 @@ int launch_as(const SsmParams& p, cudaStream_t stream) {
 }  // namespace
 
 // Few tokens per sequence go token by token: with 32 heads of 128 and states of 128, us token by
-// token against chunked: one sequence of 8 tokens 8.0 / 10.8, of 16 13.4 / 10.8; 8 sequences of
-// 4 18.6 / 20.5, of 8 30.6 / 20.7; 64 of 4 132 / 140, of 8 220 / 140.
+// token against chunked: one sequence of 8 tokens 6.4 / 10.5, of 16 10.4 / 10.5; 8 sequences of
+// 4 15.7 / 20.4, of 6 23.1 / 20.4; 64 of 4 113 / 140, of 6 166 / 140.
 bool ssm_chunked_takes(int P, int Ns, int64_t T, int64_t N) {
   return (P == 64 || P == 128) && (Ns == 64 || Ns == 128) && T > 4 * N + 8;
 }

@@ -7,7 +7,7 @@
 // A row needs only its x_p once g, d and B.C are known:
 //     y_p = g (S[p, :] . C) + d x_p (B . C) + D x_p
 // so one dot product per row, on the row as it was loaded.
-#include <algorithm>
+#include <type_traits>
 
 #include "gdn_b200.h"
 #include "gdn_common.cuh"
@@ -83,14 +83,37 @@ __device__ __forceinline__ float row_sum(float v) {
   for (int o = kLanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+// Sums of kRows rows over their kLanes lanes; lane l of a row's lanes is left with that of row
+// l / (kLanes / kRows). Each exchange halves the rows that a lane still sums: for 4 rows of 16
+// lanes 5 shuffles, not 16.
+template <int kLanes, int kRows>
+__device__ __forceinline__ float row_sums(float (&v)[kRows]) {
+  static_assert(kRows <= kLanes, "");
+  int o = kLanes / 2;
+#pragma unroll
+  for (int rows = kRows / 2; rows > 0; rows /= 2, o /= 2) {
+    const bool hi = threadIdx.x & o;
+#pragma unroll
+    for (int i = 0; i < rows; ++i) {
+      const float send = hi ? v[i] : v[i + rows], keep = hi ? v[i + rows] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+  }
+  float sum = v[0];
+#pragma unroll
+  for (; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
+}
 
 __device__ __forceinline__ float bf16_at(const __nv_bfloat16* p) {
   return __uint_as_float(static_cast<uint32_t>(*reinterpret_cast<const unsigned short*>(p)) << 16);
 }
 
 // ---------------------------------------------------------------- one token per sequence
-// HBM bounds it: the state goes through once (5 flop per 8 bytes). A warp takes batches of
-// kRows * kPer rows (at most 32: lane r holds x and y of row r); a batch's loads are all in
+// HBM bounds it: the state goes through once (5 flop per 8 bytes): 256 sequences of 32 heads of
+// 128 x 128 in fp32 take 161 us, 6.7 TB/s; 300 of 80 heads of 64 x 128 in bf16, with twice the
+// rows per byte, 134 us, 5.9 TB/s, near the issue limit. A warp takes batches of
+// kRows * kPer rows, of which each lane holds x and y of one; a batch's loads are all in
 // flight, and the next batch's too, before it is used. Blocks of 4 warps share a head's rows.
 template <typename S, int kLanes, int kPieces, int kRows, bool kLoop>
 __global__ void __launch_bounds__(128) ssm_decode_kernel(const __grid_constant__ SsmParams p,
@@ -98,7 +121,7 @@ __global__ void __launch_bounds__(128) ssm_decode_kernel(const __grid_constant__
   constexpr int kE = Piece<S>::kE, kH = kE / 2;
   constexpr int kPer = 32 / kLanes;  // rows per load
   constexpr int kBatch = kRows * kPer;
-  static_assert(kBatch <= 32, "");
+  constexpr int kShare = kLanes / kRows;  // lanes that end up with the same row's y
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int l = lane % kLanes, sub = lane / kLanes;
   const int64_t head = blockIdx.x / splits;  // flattened (sequence, head)
@@ -154,13 +177,14 @@ __global__ void __launch_bounds__(128) ssm_decode_kernel(const __grid_constant__
       for (int j = 0; j < kPieces; ++j) s[i][j] = next[i][j];
     }
     if (kLoop && row0 + kBatch < end) load(row0 + kBatch);
-    const bool own = lane < kBatch && row0 + lane < end;
-    const float x_lane = own ? bf16_at(p.x + head * p.P + row0 + lane) : 0.f;
-    float y = 0.f;
+    const int mine = row0 + l / kShare * kPer + sub;
+    const float x_mine = mine < end ? bf16_at(p.x + head * p.P + mine) : 0.f;
+    const float dx_mine = d * x_mine;
+    float dots[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       const int r = row0 + i * kPer + sub;
-      const float dx = d * __shfl_sync(0xffffffffu, x_lane, i * kPer + sub);
+      const float dx = __shfl_sync(0xffffffffu, dx_mine, i * kShare, kLanes);
       const float2 dx2 = make_float2(dx, dx);
       float2 dot = make_float2(0.f, 0.f);
 #pragma unroll
@@ -176,12 +200,11 @@ __global__ void __launch_bounds__(128) ssm_decode_kernel(const __grid_constant__
           store_piece<S>(p.new_state, (head * p.P + r) * p.Ns + (j * kLanes + l) * kE,
                          Piece<S>::pack(w));
       }
-      const float yi = fmaf(g, row_sum<kLanes>(dot.x + dot.y), dx * bc);
-      // row i * kPer + (lane % kPer) is in the lanes of that sub
-      const float mine = kPer == 1 ? yi : __shfl_sync(0xffffffffu, yi, (lane % kPer) * kLanes);
-      if (lane / kPer == i) y = mine;
+      dots[i] = dot.x + dot.y;
     }
-    if (own) p.out[head * p.P + row0 + lane] = __float2bfloat16_rn(fmaf(skip, x_lane, y));
+    const float y = fmaf(g, row_sums<kLanes>(dots), dx_mine * bc);
+    if (l % kShare == 0 && mine < end)
+      p.out[head * p.P + mine] = __float2bfloat16_rn(fmaf(skip, x_mine, y));
     if (!kLoop) break;
   }
 }
@@ -189,7 +212,9 @@ __global__ void __launch_bounds__(128) ssm_decode_kernel(const __grid_constant__
 // ---------------------------------------------------------------- prompts, token by token
 // A warp keeps kRows * kPer rows of one head's state in registers over the whole sequence;
 // the inputs of kStep tokens are loaded together. Any P, and the state sizes that the
-// chunked kernel does not take; the independent check of that kernel elsewhere.
+// chunked kernel does not take; the independent check of that kernel elsewhere. Bound by the
+// chain of a token's loads, products and reductions, 2 us for four tokens: 64 sequences of 4
+// tokens of 32 heads of 128 x 128 113 us, of which the states' way in and out is 85.
 constexpr int kStep = 4;
 
 template <int kLanes, int kPieces, int kRows>
@@ -198,6 +223,7 @@ __global__ void __launch_bounds__(128) ssm_recurrent_kernel(const __grid_constan
   constexpr int kE = 4, kH = 2;
   constexpr int kPer = 32 / kLanes;
   constexpr int kWarpRows = kRows * kPer;
+  constexpr int kShare = kLanes / kRows;  // lanes that end up with the same row's y
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int l = lane % kLanes, sub = lane / kLanes;
   const int64_t head = blockIdx.x / tiles;
@@ -259,6 +285,7 @@ __global__ void __launch_bounds__(128) ssm_recurrent_kernel(const __grid_constan
 #pragma unroll
     for (int a = 0; a < kStep; ++a) {
       if (t0 + a >= end) break;
+      float dots[kRows];
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
         const float dx = d[a] * x[a][i];
@@ -272,11 +299,13 @@ __global__ void __launch_bounds__(128) ssm_recurrent_kernel(const __grid_constan
             dot2 = __ffma2_rn(s[i][j][k], c[a][j][k], dot2);
           }
         }
-        const float dot = row_sum<kLanes>(dot2.x + dot2.y);
-        const int r = row0 + i * kPer + sub;
-        if (l == 0 && r < p.P)
-          p.out[((t0 + a) * p.H + h) * p.P + r] = __float2bfloat16_rn(fmaf(skip, x[a][i], dot));
+        dots[i] = dot2.x + dot2.y;
+        if (l == 0) dots[i] = fmaf(skip, x[a][i], dots[i]);
       }
+      const float y = row_sums<kLanes>(dots);
+      const int r = row0 + l / kShare * kPer + sub;
+      if (l % kShare == 0 && r < p.P)
+        p.out[((t0 + a) * p.H + h) * p.P + r] = __float2bfloat16_rn(y);
     }
   }
 #pragma unroll
@@ -291,18 +320,24 @@ __global__ void __launch_bounds__(128) ssm_recurrent_kernel(const __grid_constan
 }
 
 template <typename S, int kLanes, int kPieces, int kRows>
-int decode_as(const SsmParams& p, cudaStream_t stream, int most_batches) {
+int decode_as(const SsmParams& p, cudaStream_t stream) {
+  // Batches per warp at most, where the grid stays full. A warp's gates and its B and C cost as
+  // much as a batch of bf16 rows (300 x 80 heads of 64 x 128: 1 batch 148 us, 4 batches 134); with
+  // fp32 rows HBM has the next block's loads to do meanwhile (256 x 32 heads of 128 x 128: 161 us
+  // with 1 batch, 168 with 2).
+  constexpr bool kLoops = std::is_same_v<S, __nv_bfloat16>;
+  constexpr int kMostBatches = kLoops ? 4 : 1;
   constexpr int kBlockRows = 4 * kRows * (32 / kLanes);
   const int64_t heads = p.N * p.H;
   const int whole = (p.P + kBlockRows - 1) / kBlockRows;  // batches of a whole head
   int batches = 1;
-  while (batches < most_batches && batches < whole && heads * (whole / (2 * batches)) >= 148 * 16)
+  while (batches < kMostBatches && batches < whole && heads * (whole / (2 * batches)) >= 148 * 16)
     batches *= 2;
   const int splits = (whole + batches - 1) / batches;
   if (heads * splits > 0x7fffffffLL) return GDN_ERR_UNSUPPORTED_SHAPE;
   const unsigned grid = static_cast<unsigned>(heads * splits);
-  if (batches > 1) {
-    ssm_decode_kernel<S, kLanes, kPieces, kRows, true>
+  if (kLoops && batches > 1) {
+    ssm_decode_kernel<S, kLanes, kPieces, kRows, kLoops>
         <<<grid, 128, 0, stream>>>(p, splits, batches);
   } else {
     ssm_decode_kernel<S, kLanes, kPieces, kRows, false><<<grid, 128, 0, stream>>>(p, splits, 1);
@@ -323,27 +358,23 @@ int recurrent_as(const SsmParams& p, cudaStream_t stream) {
 
 }  // namespace
 
-// Batches per warp at most, where the grid stays full: a warp's gates and its B and C cost as
-// much as a batch of bf16 rows.
-constexpr int kF32Batches = 1, kBf16Batches = 4;
-
 int launch_ssm_decode(const SsmParams& p, cudaStream_t stream) {
   if (p.state_bf16) {
     switch (p.Ns) {
-      case 16: return decode_as<__nv_bfloat16, 2, 1, 2>(p, stream, kBf16Batches);
-      case 32: return decode_as<__nv_bfloat16, 4, 1, 4>(p, stream, kBf16Batches);
-      case 64: return decode_as<__nv_bfloat16, 8, 1, 4>(p, stream, kBf16Batches);
-      case 128: return decode_as<__nv_bfloat16, 16, 1, 4>(p, stream, kBf16Batches);
-      case 256: return decode_as<__nv_bfloat16, 32, 1, 4>(p, stream, kBf16Batches);
+      case 16: return decode_as<__nv_bfloat16, 2, 1, 2>(p, stream);
+      case 32: return decode_as<__nv_bfloat16, 4, 1, 4>(p, stream);
+      case 64: return decode_as<__nv_bfloat16, 8, 1, 4>(p, stream);
+      case 128: return decode_as<__nv_bfloat16, 16, 1, 4>(p, stream);
+      case 256: return decode_as<__nv_bfloat16, 32, 1, 4>(p, stream);
     }
     return GDN_ERR_UNSUPPORTED_SHAPE;
   }
   switch (p.Ns) {
-    case 16: return decode_as<float, 4, 1, 4>(p, stream, kF32Batches);
-    case 32: return decode_as<float, 8, 1, 8>(p, stream, kF32Batches);
-    case 64: return decode_as<float, 16, 1, 8>(p, stream, kF32Batches);
-    case 128: return decode_as<float, 32, 1, 8>(p, stream, kF32Batches);
-    case 256: return decode_as<float, 32, 2, 4>(p, stream, kF32Batches);
+    case 16: return decode_as<float, 4, 1, 4>(p, stream);
+    case 32: return decode_as<float, 8, 1, 8>(p, stream);
+    case 64: return decode_as<float, 16, 1, 8>(p, stream);
+    case 128: return decode_as<float, 32, 1, 4>(p, stream);
+    case 256: return decode_as<float, 32, 2, 4>(p, stream);
   }
   return GDN_ERR_UNSUPPORTED_SHAPE;
 }
