@@ -16,7 +16,9 @@
 // with rows in flight in registers (4 per thread, 16 warps per SM) HBM's latency was not
 // covered. No thread waits for another. Sums are fp32; silu takes ex2.approx and a shared
 // approximate reciprocal (a few fp32 ulp, far below the bf16 rounding of the output, the only
-// other one).
+// other one). 65536 x 6144 take 262 us (6.2 TB/s); 19679 x 8192 115 us, and 130 with the norm of
+// half of the channels: besides HBM the instructions per row (130 for 8 channels) come near a
+// bound then.
 #include "gdn_b200.h"
 #include "gdn_common.cuh"
 #include "ssm_launch.h"
@@ -203,7 +205,8 @@ __device__ __forceinline__ void head_sums(float (&q)[kTok]) {
 // of the warp call it; `live` says whether this thread's channels exist.
 template <int W, bool kWide, int kTok>
 __device__ __forceinline__ void output_rows(const ConvParams& p, const Taps<W>& taps,
-                                            const Place& pl, int c, int64_t at, __nv_bfloat16* out, Window<W>& win,
+                                            const Place& pl, int c, int64_t at,
+                                            __nv_bfloat16* out, Window<W>& win,
                                             const Row (&rows)[kTok], bool live) {
   float2 y[kTok][kP];
 #pragma unroll
@@ -417,10 +420,14 @@ conv_prefill_kernel(const __grid_constant__ ConvParams p, int64_t tiles, int run
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// One token per sequence: each thread reads its 8 channels of the W-1 state rows and of x,
+// One token per sequence, bound by HBM (1024 sequences of 8192 channels with 4 taps 26.7 us,
+// 5.0 TB/s with the launch): each thread reads its 8 channels of the W-1 state rows and of x,
 // and writes the rows moved up by one, so the new state may be the old one's memory.
+template <int W>
+constexpr int kDecodeBlocks = W == 4 ? 4 : (W == 3 ? 5 : 7);  // per SM, by the registers
+
 template <int W, bool kWide>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kDecodeBlocks<W>)
 conv_decode_kernel(const __grid_constant__ ConvParams p, int per_thread) {
   const int c = (blockIdx.x * kThreads + threadIdx.x) * kVec;
   const bool live = c < p.C;
@@ -478,8 +485,8 @@ template <int W>
 int prefill_w(const ConvParams& p, cudaStream_t stream) {
   const unsigned bx = (p.C + kThreads * kVec - 1) / (kThreads * kVec);
   // A run reads W-1 rows and the taps again (128 against 64 tokens: 4 % less on 65536 x 6144),
-  // but the grid wants some five rounds of blocks (three per SM) for an even end: runs of 128 on
-  // 19679 x 8192, under three rounds, lose 7 %. Short prompts take short runs to fill the SMs.
+  // but the grid wants some four rounds of blocks (four per SM) for an even end: runs of 128 on
+  // 19679 x 8192, two rounds, lose 5 %. Short prompts take short runs to fill the SMs.
   int run = 128;
   while (run > 8 && bx * ((p.T + run - 1) / run) < 148 * 16) run /= 2;
   const int64_t tiles = (p.T + run - 1) / run;
@@ -498,9 +505,11 @@ template <int W>
 int decode_w(const ConvParams& p, cudaStream_t stream) {
   const unsigned bx = (p.C + kThreads * kVec - 1) / (kThreads * kVec);
   if (p.N > (int64_t{1} << 30)) return GDN_ERR_UNSUPPORTED_SHAPE;
-  // Several sequences per thread share the load of its taps once the grid covers the SMs.
-  int per_thread = 1;
-  while (per_thread < 8 && bx * (p.N / (2 * per_thread)) >= 148 * 8) per_thread *= 2;
+  // One round of blocks: a thread's sequences share the load of its taps, and each one's rows are
+  // under way while it has the one before in hand (1024 x 8192: 14 in one round 26.7 us, 4 in three
+  // and a half 28.8, 1 each 32.3).
+  const int64_t round = 148 * kDecodeBlocks<W>;
+  const int per_thread = static_cast<int>((bx * p.N + round - 1) / round);
   const dim3 grid = rows_grid(bx, (p.N + per_thread - 1) / per_thread);
   if (wide_ok(p)) {
     conv_decode_kernel<W, true><<<grid, kThreads, 0, stream>>>(p, per_thread);
