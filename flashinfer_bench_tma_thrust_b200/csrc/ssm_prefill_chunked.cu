@@ -36,11 +36,11 @@
 //
 // What bounds it: shared memory. Per chunk of 128 x 128 with Ns = 128 a block moves about 5400
 // of its 128-byte lines (products' operands 1800, bulk copies 1000, the roles' own loads and
-// stores 2400) in 6300 cycles. With heads of 128 and states of 128, at the 1.7 to 1.9 GHz that
-// the power limit leaves: 4 x 32768 tokens of 32 heads 990 to 1090 us (3.0 to 3.3 TB/s of the
-// bytes that have to move), one sequence of 32768 of 64 heads of 64 424 us, of which the
-// segments' states take 129, and one chunk, mostly latency, 10.8 us. Two chunks per SM at a
-// time would need twice the shared memory.
+// stores 2400) in 6300 cycles, half of them with work for the tensor cores. With heads of 128
+// and states of 128, at the 1.7 to 1.9 GHz that the power limit leaves: 4 x 32768 tokens of 32
+// heads 945 to 1090 us (3.0 to 3.4 TB/s of the bytes that have to move), one sequence of 32768
+// of 64 heads of 64 410 us, of which the segments' states take 129, and one chunk, mostly
+// latency, 10.4 us. Two chunks per SM at a time would need twice the shared memory.
 #include "gdn_b200.h"
 #include "gdn_chunk_common.cuh"
 #include "ssm_launch.h"
