@@ -35,8 +35,9 @@ def require_all(device: torch.device, names: tuple, tensors: tuple) -> None:
     """require_cuda for each tensor that is given (None: left out), quick where all is well."""
     try:
         if device.type == "cuda":
+            index = device.index
             for t in tensors:
-                if t is not None and t.device != device:
+                if t is not None and t.get_device() != index:  # (-1: the CPU)
                     break
             else:
                 return
@@ -55,12 +56,12 @@ def as_bf16(name: str, t: torch.Tensor) -> torch.Tensor:
 
 def as_gate(name: str, t: torch.Tensor) -> tuple[torch.Tensor, int]:
     """Gate/parameter tensors: bf16 or fp32 pass through, other floats go to fp32."""
-    if t.dtype not in _GATE_CODES:
+    code = _GATE_CODES.get(t.dtype)
+    if code is None:
         if not t.dtype.is_floating_point:
             raise TypeError(f"{name} must be a floating tensor, got {t.dtype}")
-        t = t.float()
-    t = t.contiguous()
-    return t, _GATE_CODES[t.dtype]
+        t, code = t.float(), _lib.DTYPE_F32
+    return t.contiguous(), code
 
 
 def as_index(name: str, t: torch.Tensor) -> tuple[torch.Tensor, int]:
@@ -89,11 +90,13 @@ def check_heads(HQ: int, HV: int, D: int) -> None:
 
 
 _SAME = contextlib.nullcontext()
+# (without the check for an initialised CUDA: the callers hold tensors on the device)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def on_device(device: torch.device):
     """Context in which `device` is current; free where it is already (the usual call)."""
-    return _SAME if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _SAME if _current_device() == device.index else torch.cuda.device(device)
 
 
 # The handle of the current stream without a Stream object around it (2 us a call), where
