@@ -19,6 +19,8 @@
 // other one). 65536 x 6144 take 262 us (6.2 TB/s); 19679 x 8192 115 us, and 130 with the norm of
 // half of the channels: besides HBM the instructions per row (130 for 8 channels) come near a
 // bound then.
+#include <cmath>
+
 #include "gdn_b200.h"
 #include "gdn_common.cuh"
 #include "ssm_launch.h"
@@ -334,32 +336,9 @@ conv_prefill_kernel(const __grid_constant__ ConvParams p, int64_t tiles, int run
   }
   const int64_t t0 = by * run;
   const int64_t t1 = min(t0 + run, p.T);
-  int64_t n = find_sequence(p.cu_seqlens, p.cu_dtype, p.N, t0);
-  int64_t start = p.T, end = p.T;  // of sequence n; none left: nothing is written
-  if (n < p.N) {
-    start = bound(p, n);
-    end = bound(p, n + 1);
-  }
   const int cl = live ? c : 0;
-  const Taps<W> taps = load_taps<W, kWide>(p, cl);
-  Place pl = place_of(p, cl);
-  if (!live) pl.normed = 0;  // (a normed section is whole warps)
-  Window<W> win;
-  const Row zero{make_uint4(0u, 0u, 0u, 0u)};
-#pragma unroll
-  for (int r = 0; r < W - 1; ++r) win.set(r, zero);
-  if (n < p.N && start < t0) {  // the tile begins inside a sequence
-#pragma unroll
-    for (int r = 0; r < W - 1; ++r) {
-      const int64_t u = t0 - (W - 1) + r;
-      if (u >= start) {
-        win.set(r, load_row<kWide>(p.x + u * p.x_stride, cl, p.C));
-      } else if (p.state) {
-        win.set(r, load_row<kWide>(p.state + (n * (W - 1) + (u - start) + (W - 1)) * p.C, cl, p.C));
-      }
-    }
-  }
-  // The ring: batch b of kAhead rows in slot b % kSlots, at this thread's own place.
+  // The ring: batch b of kAhead rows in slot b % kSlots, at this thread's own place. Asked for
+  // before anything else: x needs no bounds.
   __shared__ uint4 ring[kSlots][kAhead][kThreads];
   const int batches = static_cast<int>((t1 - t0 + kAhead - 1) / kAhead);
   const __nv_bfloat16* from = p.x + t0 * p.x_stride + cl;
@@ -380,6 +359,30 @@ conv_prefill_kernel(const __grid_constant__ ConvParams p, int64_t tiles, int run
   };
 #pragma unroll 1
   for (int b = 0; b < kSlots - 1; ++b) fetch(b);
+  const Taps<W> taps = load_taps<W, kWide>(p, cl);
+  Place pl = place_of(p, cl);
+  if (!live) pl.normed = 0;  // (a normed section is whole warps)
+  int64_t n = find_sequence(p.cu_seqlens, p.cu_dtype, p.N, t0);
+  int64_t start = p.T, end = p.T;  // of sequence n; none left: nothing is written
+  if (n < p.N) {
+    start = bound(p, n);
+    end = bound(p, n + 1);
+  }
+  Window<W> win;
+  const Row zero{make_uint4(0u, 0u, 0u, 0u)};
+#pragma unroll
+  for (int r = 0; r < W - 1; ++r) win.set(r, zero);
+  if (n < p.N && start < t0) {  // the tile begins inside a sequence
+#pragma unroll
+    for (int r = 0; r < W - 1; ++r) {
+      const int64_t u = t0 - (W - 1) + r;
+      if (u >= start) {
+        win.set(r, load_row<kWide>(p.x + u * p.x_stride, cl, p.C));
+      } else if (p.state) {
+        win.set(r, load_row<kWide>(p.state + (n * (W - 1) + (u - start) + (W - 1)) * p.C, cl, p.C));
+      }
+    }
+  }
   __nv_bfloat16* to = pl.out + t0 * pl.width + pl.at;  // kWide: the batch's first output row
 #pragma unroll 1
   for (int b = 0; b < batches; ++b, to += kAhead * pl.width) {
@@ -484,11 +487,17 @@ dim3 rows_grid(unsigned bx, int64_t rows) {
 template <int W>
 int prefill_w(const ConvParams& p, cudaStream_t stream) {
   const unsigned bx = (p.C + kThreads * kVec - 1) / (kThreads * kVec);
-  // A run reads W-1 rows and the taps again (128 against 64 tokens: 4 % less on 65536 x 6144),
-  // but the grid wants some four rounds of blocks (four per SM) for an even end: runs of 128 on
-  // 19679 x 8192, two rounds, lose 5 %. Short prompts take short runs to fill the SMs.
-  int run = 128;
-  while (run > 8 && bx * ((p.T + run - 1) / run) < 148 * 16) run /= 2;
+  // Four blocks per SM run at a time. While one round of them covers the tokens in runs of 48 or
+  // less, it does: 8192 channels, 7 tokens 3.4 us in runs of 1 and 5.5 of 8; 1000 11.1 in runs of
+  // 16, 12.1 of 8; 3000 28.3 of 48, 31.7 of 8. Beyond, a run costs its rows and as long as 10 more
+  // (bounds, taps, W-1 rows again), and the last round is half empty: with `round` tokens to a
+  // round of runs of one, (round / run + 1/2) (run + 10) is least at sqrt(20 round). 5000 tokens
+  // 42.1 us in runs of 32, 43.9 of 48, 45.6 of 64; 19679 129.5 of 64, 135 of 32, 136 of 128; 65536
+  // x 6144 261 of 128, 267 of 72 or 144.
+  const int64_t round = (bx * p.T + 148 * 4 - 1) / (148 * 4);
+  const int run = round <= 2    ? static_cast<int>(round < 1 ? 1 : round)
+                  : round <= 48 ? static_cast<int>(round + 3) / 4 * 4
+                                : static_cast<int>(std::sqrt(20.0 * round) / 8 + 0.5) * 8;
   const int64_t tiles = (p.T + run - 1) / run;
   const int64_t rows = tiles + p.N;
   if (rows > (int64_t{1} << 30)) return GDN_ERR_UNSUPPORTED_SHAPE;
