@@ -95,7 +95,8 @@ def test_ssm_chunked_workspace_and_alignment(cuda_lib):
     assert size(5000, 1, 4, 2, 80, 64) == 0                # token by token
     assert size(-1, 1, 4, 2, 64, 64) == 0 and size(5000, 1, 3, 2, 64, 64) == 0
     need = size(2500, 1, 2, 1, 64, 128)
-    assert need == (2500 // 1024 + 1) * 2 * (64 * 128 + 1) * 4
+    assert need == (2500 // 256 + 1) * 2 * (64 * 128 + 1) * 4  # (segments of two chunks)
+    assert size(2500, 0, 2, 1, 64, 128) == 0               # no sequences
     call = dict(T=2500, N=1, H=2, G=1, P=64, Ns=128)
     assert _ssm(lib, "chunked", **call) == -5
     assert _ssm(lib, "chunked", ws=P16, wb=need - 1, **call) == -5

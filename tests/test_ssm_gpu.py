@@ -77,7 +77,8 @@ def test_chunked_heads(H, G, P):
     check_prompt(ssm.prefill(*dev(a), check=True), a, True)
 
 
-@pytest.mark.parametrize("lengths", [[2500], [1500, 0, 1100, 7], [1024, 1024], [2049]])
+@pytest.mark.parametrize("lengths", [[2500], [1500, 0, 1100, 7], [1024, 1024], [2049], [1100],
+                                     [20000], [0, 9000, 1]])
 @pytest.mark.parametrize("P,Ns", [(64, 128), (128, 64)])
 def test_chunked_segments(lengths, P, Ns):
     """Few heads and long sequences: cut into segments (two launches)."""
@@ -247,6 +248,14 @@ def test_empty_calls():
                a[7][:0]])
     out, ns = ssm.decode(*tok)
     assert out.shape == (0, 1, 4, 64) and ns.shape == (0, 4, 64, 64)
+
+
+def test_tokens_without_sequences():
+    """Rows that no sequence covers, as all are where there is none: nothing runs."""
+    a = dev(make([700], seed=27))
+    for fn in (ssm.prefill, ssm.prefill_recurrent):
+        out, ns = fn(*a[:7], None, torch.zeros(1, dtype=torch.int32, device="cuda"), check=True)
+        assert out.shape == (700, 4, 64) and ns.shape == (0, 4, 64, 64)
 
 
 def test_large_offsets():
