@@ -41,14 +41,15 @@ MAX_SECTIONS = 8
 
 
 _NAMES = ("x", "weight", "bias", "state", "cu_seqlens")
+_BF16, _empty, _empty_like = torch.bfloat16, torch.empty, torch.empty_like
 
 
 def _taps(x, weight, bias):
     """(weight, code, bias, code, W), checked."""
-    ch = x.shape[-1]
-    if weight.dim() == 3 and weight.shape[1] == 1:
+    ch, shape = x.shape[-1], weight.shape
+    if len(shape) == 3 and shape[1] == 1:
         weight = weight[:, 0]
-    shape = weight.shape
+        shape = weight.shape
     if len(shape) != 2 or shape[0] != ch or not 2 <= shape[1] <= 4:
         raise ValueError(f"weight must be [{ch}, W] with 2 to 4 taps, got {tuple(shape)}")
     w, w_t = C.as_gate("weight", weight)
@@ -129,16 +130,16 @@ def prefill(x, weight, bias=None, state=None, cu_seqlens=None, *, activation="si
     cu, cu_t = C.as_index("cu_seqlens", cu_seqlens)
     n, t = cu.numel() - 1, x.shape[0]
     s = _state(state, (n, taps - 1, ch))
-    if x.dtype is not torch.bfloat16 or x.stride(-1) != 1 or not ch:
+    if x.dtype is not _BF16 or x.stride(-1) != 1 or not ch:
         x = _rows(x)
     widths, wa, na, pointers = _sections(ch, _hashable(split), _hashable(l2norm))
     act = _activation(activation)
     lib = _lib.load()
     with C.on_device(dev):
         status = _status.address(dev.index)
-        outs = [torch.empty(t, v, dtype=torch.bfloat16, device=dev) for v in widths]
-        new_state = torch.empty(n, taps - 1, ch, dtype=torch.bfloat16, device=dev) \
-            if s is None else torch.empty_like(s)
+        outs = [_empty(t, v, dtype=_BF16, device=dev) for v in widths]
+        new_state = _empty(n, taps - 1, ch, dtype=_BF16, device=dev) \
+            if s is None else _empty_like(s)
         rc = lib.gdn_conv_prefill_fwd(
             x.data_ptr(), x.stride(0), w.data_ptr(), w_t, C.ptr(b), b_t, C.ptr(s), cu.data_ptr(),
             cu_t, act, len(widths), wa, na, eps, pointers(*[o.data_ptr() for o in outs]),
@@ -160,16 +161,16 @@ def _decode(x, weight, bias, state, activation, split, l2norm, eps, inplace):
     ch = x.shape[-1]
     n = x.shape[0]
     s = _state(state, (n, taps - 1, ch))
-    if x.dtype is not torch.bfloat16 or x.stride(-1) != 1 or not ch:
+    if x.dtype is not _BF16 or x.stride(-1) != 1 or not ch:
         x = _rows(x)
     widths, wa, na, pointers = _sections(ch, _hashable(split), _hashable(l2norm))
     act = _activation(activation)
     lib = _lib.load()
     with C.on_device(dev):
-        outs = [torch.empty(n, 1, v, dtype=torch.bfloat16, device=dev) for v in widths]
+        outs = [_empty(n, 1, v, dtype=_BF16, device=dev) for v in widths]
         new_state = state if inplace else (
-            torch.empty(n, taps - 1, ch, dtype=torch.bfloat16, device=dev) if s is None
-            else torch.empty_like(s))
+            _empty(n, taps - 1, ch, dtype=_BF16, device=dev) if s is None
+            else _empty_like(s))
         rc = lib.gdn_conv_decode_fwd(
             x.data_ptr(), x.stride(0), w.data_ptr(), w_t, C.ptr(b), b_t, C.ptr(s), act,
             len(widths), wa, na, eps, pointers(*[o.data_ptr() for o in outs]),

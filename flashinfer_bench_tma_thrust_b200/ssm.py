@@ -28,6 +28,8 @@ state where the recurrence may leave an infinity.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _checks as K
@@ -99,6 +101,11 @@ def _args(x, dt, A_log, B, C, D, dt_bias, state, cu, lead: int):
         d_ptr, d_t, dt_bias.data_ptr(), b_t)
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(*sizes):
+    return _lib.load().gdn_ssm_prefill_workspace_size(*sizes)
+
+
 def _prompt_args(x, dt, A_log, B, C, D, dt_bias, state, cu):
     if cu is None:
         raise ValueError("cu_seqlens is required")
@@ -147,7 +154,7 @@ def prefill(x, dt, A_log, B, C, D, dt_bias, state, cu_seqlens, *, check=False):
         status = _status.address(dev.index)
         out = torch.empty_like(keep[0][0])
         new_state = torch.empty(n, H, P, Ns, dtype=_F32, device=dev)
-        nbytes = lib.gdn_ssm_prefill_workspace_size(T, n, H, G, P, Ns)
+        nbytes = _workspace_bytes(T, n, H, G, P, Ns)
         # of this call alone: calls on several streams and captured graphs share nothing
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         rc = lib.gdn_ssm_prefill_fwd(
