@@ -20,7 +20,7 @@ int fill_conv(gdn::ConvParams* p, const void* x, int64_t x_row_stride, const voi
   if (sections < 1 || sections > gdn::kMaxSections || !widths || !normed || !outs)
     return GDN_ERR_INVALID_ARG;
   if (!real_ok(weight_dtype) || (bias && !real_ok(bias_dtype))) return GDN_ERR_UNSUPPORTED_DTYPE;
-  if (activation != 0 && activation != 1) return GDN_ERR_INVALID_ARG;
+  if ((activation != 0 && activation != 1) || !(eps >= 0.f)) return GDN_ERR_INVALID_ARG;
   *p = gdn::ConvParams{};
   int64_t at = 0;
   for (int32_t s = 0; s < sections; ++s) {

@@ -134,6 +134,8 @@ def prefill(x, weight, bias=None, state=None, cu_seqlens=None, *, activation="si
         x = _rows(x)
     widths, wa, na, pointers = _sections(ch, _hashable(split), _hashable(l2norm))
     act = _activation(activation)
+    if not eps >= 0:
+        raise ValueError(f"eps must be at least 0, got {eps}")
     lib = _lib.load()
     with C.on_device(dev):
         status = _status.address(dev.index)
@@ -165,6 +167,8 @@ def _decode(x, weight, bias, state, activation, split, l2norm, eps, inplace):
         x = _rows(x)
     widths, wa, na, pointers = _sections(ch, _hashable(split), _hashable(l2norm))
     act = _activation(activation)
+    if not eps >= 0:
+        raise ValueError(f"eps must be at least 0, got {eps}")
     lib = _lib.load()
     with C.on_device(dev):
         outs = [_empty(n, 1, v, dtype=_BF16, device=dev) for v in widths]

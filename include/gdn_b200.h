@@ -249,7 +249,7 @@ GDN_API int gdn_prefill_chunked_fwd_noalloc(const void* q, const void* k, const 
  *               (outs: host array of device pointers)
  *   normed      host array: where non-zero, each head of 128 channels of the section is
  *               divided by sqrt(sum of squares + eps); the section's begin and width must
- *               then be multiples of 128
+ *               then be multiples of 128 (eps at least 0)
  *   status      two int32 words (device or mapped host memory) or NULL: [1] becomes 1 when
  *               cu_seqlens has a bound outside [0, T] (used clamped) or a decreasing pair
  *
@@ -321,8 +321,9 @@ GDN_API int gdn_ssm_prefill_recurrent_fwd(const void* x, const void* dt, int dt_
  *
  * With P and Ns of 64 or 128 and more than 4 N + 8 tokens the chunked tensor-core kernels run
  * (chunks of 128 tokens; one launch, two where few long sequences are cut into segments; x and
- * out 16-byte aligned, T < 2^31 - 256); other calls run the token-by-token kernel. In a chunk an infinity or NaN
- * in x also reaches the outputs of up to 127 tokens before it, of the same channel.
+ * out 16-byte aligned, T < 2^31 - 256); other calls run the token-by-token kernel. In a chunk
+ * an infinity or NaN in x also reaches the outputs of up to 127 tokens before it, of the same
+ * channel.
  */
 GDN_API size_t gdn_ssm_prefill_workspace_size(int64_t T, int64_t N, int32_t H, int32_t G,
                                               int32_t P, int32_t Ns);

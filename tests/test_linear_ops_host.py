@@ -11,14 +11,14 @@ P16 = 4096  # a 16-byte aligned address that nothing reads
 
 
 def _conv(lib, fn="prefill", C=256, W=4, widths=(128, 128), normed=(1, 0), T=4, N=1, wdt=1,
-          cu_dt=2, act=1, ptr=P16, cu=P16, stride=256, outs=None):
+          cu_dt=2, act=1, ptr=P16, cu=P16, stride=256, outs=None, eps=1e-6):
     k = len(widths)
     wa, na = (ctypes.c_int32 * k)(*widths), (ctypes.c_int32 * k)(*normed)
     oa = (ctypes.c_void_p * k)(*(outs or [ptr] * k))
     if fn == "prefill":
         return lib.gdn_conv_prefill_fwd(ptr, stride, ptr, wdt, None, 0, None, cu, cu_dt, act, k,
-                                        wa, na, 1e-6, oa, ptr, T, N, C, W, None, None)
-    return lib.gdn_conv_decode_fwd(ptr, stride, ptr, wdt, None, 0, None, act, k, wa, na, 1e-6, oa,
+                                        wa, na, eps, oa, ptr, T, N, C, W, None, None)
+    return lib.gdn_conv_decode_fwd(ptr, stride, ptr, wdt, None, 0, None, act, k, wa, na, eps, oa,
                                    ptr, T, C, W, None)
 
 
@@ -37,6 +37,7 @@ def test_conv_abi_refusals(cuda_lib, fn):
     assert _conv(lib, fn, widths=tuple([32] * 9), normed=tuple([0] * 9), C=288) == -1
     assert _conv(lib, fn, wdt=2) == -3
     assert _conv(lib, fn, act=2) == -1
+    assert _conv(lib, fn, eps=-1.0) == -1 and _conv(lib, fn, eps=float("nan")) == -1
     assert _conv(lib, fn, ptr=None) == -1
     assert _conv(lib, fn, outs=[P16, None]) == -1
     assert _conv(lib, fn, stride=-1) == -1
@@ -153,6 +154,8 @@ CU = torch.tensor([0, 4], dtype=torch.int32)
     (dict(split=(64, 128, 64), l2norm=(False, True, False)), ValueError),
     (dict(split=(128, 128), l2norm=(True,)), ValueError),
     (dict(activation="gelu"), ValueError),
+    (dict(eps=-1e-6), ValueError),
+    (dict(eps=float("nan")), ValueError),
 ])
 def test_conv_prefill_refusals(any_device, change, error):
     args = dict(x=_bf(4, 256), weight=torch.zeros(256, 4), bias=None, state=None, cu_seqlens=CU)

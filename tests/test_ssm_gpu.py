@@ -250,6 +250,22 @@ def test_empty_calls():
     assert out.shape == (0, 1, 4, 64) and ns.shape == (0, 4, 64, 64)
 
 
+@pytest.mark.parametrize("ptype", [torch.bfloat16, torch.float16, torch.float64])
+def test_parameter_types(ptype):
+    """A_log, D and dt_bias of other types: bf16 as they are, others through fp32."""
+    a = make([200, 3], seed=28)
+    a = [t.to(ptype) if i in (2, 5, 6) else t for i, t in enumerate(a)]
+    exact = [t.float() if i in (2, 5, 6) else t for i, t in enumerate(a)]
+    check_prompt(ssm.prefill(*dev(a), check=True), exact, True)
+    check_prompt(ssm.prefill_recurrent(*dev(a), check=True), exact, False)
+    tok = [t[:2, None] if i in (0, 1, 3, 4) else t for i, t in enumerate(a[:8])]
+    out, ns = ssm.decode(*dev(tok))
+    one = [t[:2] if i in (0, 1, 3, 4) else t for i, t in enumerate(exact[:8])]
+    y, ye, fin, fe = scan(*one, [0, 1, 2])
+    assert_within(out[:, 0], y, ye, "output", rounding=BF16)
+    assert_within(ns, fin, fe, "state")
+
+
 def test_tokens_without_sequences():
     """Rows that no sequence covers, as all are where there is none: nothing runs."""
     a = dev(make([700], seed=27))
