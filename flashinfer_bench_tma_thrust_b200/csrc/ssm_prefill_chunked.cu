@@ -25,8 +25,8 @@
 //
 // Segments. With few (sequence, column block) chains the sequences are cut into segments of a
 // multiple of 128 tokens. A first kernel (the same code, second product only) computes what
-// each segment adds to the state and what it leaves of it; each block of the second kernel
-// then folds those of the segments before its own into its first state.
+// each segment, or each part of one, adds to the state and what it leaves of it; each block of
+// the second kernel then folds those of the segments before its own into its first state.
 //
 // Warps: 0-7 the output (M, the scaling of Y, y, and a chunk's first quarter of f x), 8-15 the
 // state (the other quarters, S), which run at their own pace and so cover each other's waits; 16
@@ -39,7 +39,7 @@
 // stores 2400) in 6300 cycles, half of them with work for the tensor cores. With heads of 128
 // and states of 128, at the 1.7 to 1.9 GHz that the power limit leaves: 4 x 32768 tokens of 32
 // heads 945 to 1090 us (3.0 to 3.4 TB/s of the bytes that have to move), one sequence of 32768
-// of 64 heads of 64 410 us, of which the segments' states take 129, and one chunk, mostly
+// of 64 heads of 64 400 us, of which the segments' states take 99, and one chunk, mostly
 // latency, 10.4 us. Two chunks per SM at a time would need twice the shared memory.
 #include <algorithm>
 #include <cmath>
@@ -154,8 +154,9 @@ struct Maps {
 struct Segments {
   int64_t slots;                    // grid: slots x column blocks
   int len;                          // tokens per segment; 0: one per sequence
-  float* add;                       // [slots, H, P, Ns] (through the maps)
-  float* left;                      // [slots, H]
+  int parts, part;                  // the states kernel: blocks per segment, tokens of each
+  float* add;                       // [slots, parts, H, P, Ns] (through the maps)
+  float* left;                      // [slots, parts, H]
 };
 
 template <int P, int NS, bool kStates>
@@ -388,8 +389,9 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
   constexpr int kMisc = kOutWarps + K::kStateWarps;
   uint64_t* const bars = reinterpret_cast<uint64_t*>(sm + K::kBars);
 
-  const int64_t slot = blockIdx.x / col_blocks;
-  const int cb = static_cast<int>(blockIdx.x - slot * col_blocks);
+  const int64_t piece = blockIdx.x / col_blocks;  // a slot, or one of its parts
+  const int cb = static_cast<int>(blockIdx.x - piece * col_blocks);
+  const int64_t slot = kStates ? piece / sg.parts : piece;
   if (warp == 0) {
     int64_t n, seg, lo, hi;
     find_segment(p, sg, slot, n, seg, lo, hi);
@@ -432,13 +434,16 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
   __syncthreads();
   tc_fence_after();
   const int64_t n = s_where[0], seg = s_where[1], s_begin = s_where[2], s_end = s_where[3];
-  const int64_t t_begin = sg.len ? s_begin + seg * sg.len : s_begin;
-  const int64_t t_end = sg.len ? min(t_begin + sg.len, s_end) : s_end;
-  const bool last = t_end >= s_end;
+  const int64_t seg_begin = sg.len ? s_begin + seg * sg.len : s_begin;
+  const int64_t seg_end = sg.len ? min(seg_begin + sg.len, s_end) : s_end;
+  const bool last = seg_end >= s_end;
   if (n >= p.N || (kStates && last)) {  // (the second kernel computes a sequence's last state)
     if (warp == kMisc) tmem_dealloc(s_tmem, 512);
     return;
   }
+
+  const int64_t t_begin = kStates ? seg_begin + (piece - slot * sg.parts) * sg.part : seg_begin;
+  const int64_t t_end = kStates ? min(t_begin + sg.part, seg_end) : seg_end;
 
   const int rep = p.H / p.G;                                  // heads of a group
   const int per_group = (rep + kHeads - 1) / kHeads;
@@ -706,10 +711,11 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       return base + (at >> 5) * (P * 128) + (s_tile ^ (16 * ((at >> 2) & 7)));
     };
     if (!kStates) {
-      const int items = (p.state ? 1 : 0) + static_cast<int>(seg);
+      const int items = (p.state ? 1 : 0) + static_cast<int>(seg) * sg.parts;
+      const int64_t r0 = slot * sg.parts - items;
       for (int k = 0; k < items; ++k) {
-        // the sequence's first state, then its segments before this one
-        const int64_t r = slot - items + k;
+        // the sequence's first state, then the parts of its segments before this one
+        const int64_t r = r0 + k;
         const float g = p.state && k == 0 ? 0.f : (mine ? sg.left[r * p.H + h0 + row_head] : 0.f);
         wait(bars_u + 8 * (kFullState), k & 1);
         if (mine) {
@@ -815,7 +821,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         }
       }
     }
-    if (kStates && mine && sp == 0 && row % P == 0) sg.left[slot * p.H + h0 + row_head] = left;
+    if (kStates && mine && sp == 0 && row % P == 0) sg.left[piece * p.H + h0 + row_head] = left;
     if (kStates || last) {
       // over B and the state's operand: the last dS is done, and with it all that reads them
 #pragma unroll
@@ -824,7 +830,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       fence_async_smem();
       named_bar_sync(2, K::kStateWarps * 32);
       if (warp == kOutWarps && lane == 0) {
-        const int64_t to = ((kStates ? slot : n) * p.H + h0) * static_cast<int64_t>(P);
+        const int64_t to = ((kStates ? piece : n) * p.H + h0) * static_cast<int64_t>(P);
         for (int hh = 0; hh < heads; ++hh)
           tma_store_3d(&maps.last, sm + K::kB + hh * (P * NS * 4), 0, static_cast<int>(to) + hh * P,
                        0);
@@ -974,12 +980,12 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
           load_x(0);
         }
         if (!kStates) {  // states, one after the other in the other stages of x
-          const int items = (p.state ? 1 : 0) + static_cast<int>(seg);
+          const int items = (p.state ? 1 : 0) + static_cast<int>(seg) * sg.parts;
           for (int k = 0; k < items; ++k) {
             if (k > 0) wait(bars_u + 8 * (kStateRead), (k - 1) & 1);
             const bool first = p.state && k == 0;
             const int64_t from =
-                ((first ? n : slot - items + k) * p.H + h0) * static_cast<int64_t>(P);
+                ((first ? n : slot * sg.parts - items + k) * p.H + h0) * static_cast<int64_t>(P);
             mbar_arrive_expect_tx(bars + kFullState, heads * P * NS * 4);
             for (int hh = 0; hh < heads; ++hh)
               tma_load_3d(sm + K::kX + K::kXBytes + hh * (P * NS * 4),
@@ -1106,41 +1112,62 @@ int column_blocks(int H, int G, int P) {
   return G * ((H / G + heads - 1) / heads);
 }
 
-// Tokens per segment (0: whole sequences) and the number of slots that covers any lengths.
+// How the sequences are cut, with slots that cover any lengths. Without segments: one slot each.
 // In us, with heads and states of 128: a chunk takes 3.4, one of the states' kernel 2.0, that
 // kernel's start 9 and each segment that is folded into a first state 1.1. The host does not know
 // the lengths: the longest sequence of several is taken as half as long again as their mean.
 // 32 heads, whole / in segments: 1000 tokens 34.0 / 28.7, 1900 58 / 39, 3000 88 / 53, 8192 218 /
 // 103; one head, in segments of 1024 / by this rule: 2000 tokens 59 / 31, 8192 59 / 48, 131072
 // 209 / 165. (Four sequences of 300, 400, 2000 and 900 with 16 heads lose: 59 / 62.)
-void plan(int64_t T, int64_t N, int H, int G, int P, int& len, int64_t& slots) {
+Segments plan(int64_t T, int64_t N, int H, int G, int P) {
   constexpr int kSms = 148;
-  len = 0;
-  slots = N;
-  const int64_t fit = kSms / column_blocks(H, G, P);  // segments that run at the same time
-  if (N == 0 || fit <= N) return;
+  constexpr double kChunk = 3.4, kState = 2.0, kStart = 9, kFold = 1.1;
+  Segments sg{};
+  sg.slots = N;
+  sg.parts = 1;
+  const int cols = column_blocks(H, G, P);
+  const int64_t fit = kSms / cols;  // segments that run at the same time
+  if (N == 0 || fit <= N) return sg;
   const double longest = static_cast<double>(N == 1 ? T : 3 * T / (2 * N)) / kL;  // in chunks
   // as many as fit, but not so many that the folding takes longer than it saves
   double l = static_cast<double>((T + fit - N) / (fit - N + 1)) / kL;
-  l = std::ceil(std::max({l, 2.0, std::sqrt(longest * 1.1 / (3.4 + 2.0))}));
-  if (3.4 * longest <= (3.4 + 2.0) * l + 9 + 1.1 * longest / l) return;
-  len = static_cast<int>(l) * kL;
-  slots = T / len + N;
+  l = std::ceil(std::max({l, 2.0, std::sqrt(longest * kFold / (kChunk + kState))}));
+  if (kChunk * longest <= (kChunk + kState) * l + kStart + kFold * longest / l) return sg;
+  sg.len = static_cast<int>(l) * kL;
+  sg.slots = T / sg.len + N;
+  // A sequence's last segment has no part in the states kernel, and a part takes less than half
+  // of a segment's time: several to a segment may fill the SMs better (32 column blocks: 32768
+  // tokens, 3 segments with states, 437 us in all, in 3 parts each 424; 12000 and 3000 tokens 219
+  // and 188).
+  const double busy = std::max(1.0, static_cast<double>((T - 1) / sg.len - (N - 1) / 2)) * cols;
+  double best = 0;
+  for (int parts = 1; parts <= 4; ++parts) {
+    const double part = std::ceil(l / parts);
+    if (part * (parts - 1) >= l) break;
+    const double time = std::ceil(busy * parts / kSms) * (kStart + kState * part) +
+                        kFold * parts * longest / l;
+    if (parts == 1 || time < best) {
+      best = time;
+      sg.parts = parts;
+      sg.part = static_cast<int>(part) * kL;
+    }
+  }
+  return sg;
 }
 
 template <int P, int NS>
 int launch_as(const SsmParams& p, cudaStream_t stream) {
-  Segments sg{};
-  plan(p.T, p.N, p.H, p.G, p.P, sg.len, sg.slots);
+  Segments sg = plan(p.T, p.N, p.H, p.G, p.P);
+  const int64_t pieces = sg.slots * sg.parts;
   const int cols = column_blocks(p.H, p.G, p.P);
-  if (sg.slots * cols > 0x7fffffffLL) return GDN_ERR_UNSUPPORTED_SHAPE;
+  if (pieces * cols > 0x7fffffffLL) return GDN_ERR_UNSUPPORTED_SHAPE;
   Maps maps;
   const int64_t hp = static_cast<int64_t>(p.H) * P, gn = static_cast<int64_t>(p.G) * NS;
   if (!encode(&maps.x, p.x, p.T, hp, 2) || !encode(&maps.b, p.B, p.T, gn, 1) ||
       !encode(&maps.c, p.C, p.T, gn, NS / 64) || !encode(&maps.out, p.out, p.T, hp, 1))
     return GDN_ERR_CUDA;
   // (row coordinates are 32-bit)
-  if (p.N * hp > 0x7fffffffLL || sg.slots * hp > 0x7fffffffLL) return GDN_ERR_UNSUPPORTED_SHAPE;
+  if (p.N * hp > 0x7fffffffLL || pieces * hp > 0x7fffffffLL) return GDN_ERR_UNSUPPORTED_SHAPE;
   const void* const first = p.state ? p.state : p.new_state;
   if (!encode_state(&maps.first, first, p.N * hp, P, NS)) return GDN_ERR_CUDA;
   maps.add = maps.last = maps.first;
@@ -1148,15 +1175,15 @@ int launch_as(const SsmParams& p, cudaStream_t stream) {
   if (sg.len) {
     if (!p.workspace) return GDN_ERR_WORKSPACE;
     sg.add = p.workspace;
-    sg.left = p.workspace + sg.slots * hp * NS;
-    if (!encode_state(&maps.add, sg.add, sg.slots * hp, P, NS)) return GDN_ERR_CUDA;
+    sg.left = p.workspace + pieces * hp * NS;
+    if (!encode_state(&maps.add, sg.add, pieces * hp, P, NS)) return GDN_ERR_CUDA;
     maps.last = maps.add;
     using K = Cfg<P, NS, true>;
     auto fn = ssm_chunk_kernel<P, NS, true>;
     if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, K::kBytes) !=
         cudaSuccess)
       return GDN_ERR_CUDA;
-    fn<<<grid, K::kThreads, K::kBytes, stream>>>(p, maps, sg, cols);
+    fn<<<grid * sg.parts, K::kThreads, K::kBytes, stream>>>(p, maps, sg, cols);
     if (cudaGetLastError() != cudaSuccess) return GDN_ERR_CUDA;
   }
   if (!encode_state(&maps.last, p.new_state, p.N * hp, P, NS)) return GDN_ERR_CUDA;
@@ -1185,11 +1212,10 @@ bool ssm_chunked_takes(int P, int Ns, int64_t T, int64_t N) {
 }
 
 size_t ssm_chunked_workspace(int64_t T, int64_t N, int H, int G, int P, int Ns) {
-  int len;
-  int64_t slots;
-  plan(T, N, H, G, P, len, slots);
-  return len ? static_cast<size_t>(slots) * H * (static_cast<size_t>(P) * Ns + 1) * sizeof(float)
-             : 0;
+  const Segments sg = plan(T, N, H, G, P);
+  return sg.len ? static_cast<size_t>(sg.slots * sg.parts) * H *
+                      (static_cast<size_t>(P) * Ns + 1) * sizeof(float)
+                : 0;
 }
 
 int launch_ssm_chunked(const SsmParams& p, cudaStream_t stream) {
