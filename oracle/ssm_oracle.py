@@ -73,8 +73,8 @@ def gates(dt, dt_bias, A_log):
 def scan(x, dt, A_log, B, C, D, dt_bias, state, bounds, chunk_products=False):
     """x [T, H, P]. Returns (y, y's bound, state, state's bound) in fp64; rows of no sequence
     are NaN. ``chunk_products``: the bounds of the chunked tensor-core form, whose state terms
-    are bf16 pairs (each off by at most 2^-16 of a term) summed in fp32 by a unit that may
-    truncate, and whose output terms are products with one operand rounded to bf16."""
+    (fp32 products, exactly split) are summed in fp32 by a unit that may truncate, and whose
+    output terms are products with one operand rounded to bf16."""
     t, h, p = x.shape
     g_, ns = B.shape[1], B.shape[2]
     rep = h // g_
@@ -87,7 +87,7 @@ def scan(x, dt, A_log, B, C, D, dt_bias, state, bounds, chunk_products=False):
     ye = torch.zeros(t, h, p, dtype=torch.float64)
     fin = torch.zeros(n_seq, h, p, ns, dtype=torch.float64)
     fe = torch.zeros(n_seq, h, p, ns, dtype=torch.float64)
-    term = 2.0 ** -16 + 64 * 2.0 ** -23 if chunk_products else 0.0
+    term = 64 * 2.0 ** -23 if chunk_products else 0.0
     for n in range(n_seq):
         s = torch.zeros(h, p, ns, dtype=torch.float64) if state is None else state[n].double().cpu()
         s_abs, e = s.abs(), torch.zeros_like(s)

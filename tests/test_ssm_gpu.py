@@ -89,6 +89,18 @@ def test_chunked_segments(lengths, P, Ns):
     check_prompt(ssm.prefill(*dev(a), check=True), a, True)
 
 
+@pytest.mark.parametrize("H,lengths,length,parts", [
+    (24, [1400, 600], 512, 2), (17, [1500, 900, 700], 640, 2), (32, [1000, 2000], 1024, 2)])
+def test_chunked_segments_in_parts(H, lengths, length, parts):
+    """More heads: the segments' states in parts, also of unequal sizes (2 and 3 chunks of 5)."""
+    a = make(lengths, H=H, G=H, seed=H)
+    T, N = sum(lengths), len(lengths)
+    from flashinfer_bench_tma_thrust_b200 import _lib
+    assert _lib.load().gdn_ssm_prefill_workspace_size(T, N, H, H, 64, 64) == \
+        (T // length + N) * parts * H * (64 * 64 + 1) * 4
+    check_prompt(ssm.prefill(*dev(a), check=True), a, True)
+
+
 def test_chunked_uncovered_rows_and_neighbours():
     """Rows in front of, between and behind the sequences hold NaN: they reach nothing, and
     their outputs are not written."""
@@ -144,12 +156,12 @@ def test_chunked_many_sequences():
 
 def test_chunked_matches_recurrent_on_long_prompts():
     """The two kernels at sizes beyond the oracle: outputs within two bf16 roundings and the
-    chunked form's bf16 operands, states within its 2^-16 terms (relative to the whole)."""
+    chunked form's bf16 operands, states within fp32's terms of both (relative to the whole)."""
     a = dev(make([3000, 0, 5000, 129], H=32, G=16, P=128, Ns=128, seed=34))
     o1, s1 = ssm.prefill(*a, check=True)
     o2, s2 = ssm.prefill_recurrent(*a)
     assert ((o1.double() - o2.double()).norm() / o2.double().norm()) < 2 ** -8
-    assert ((s1 - s2).norm() / s2.norm()) < 2 ** -16
+    assert ((s1 - s2).norm() / s2.norm()) < 64 * 2 ** -23
 
 
 SIZES = [(1, 16), (8, 16), (40, 32), (64, 64), (80, 128), (128, 128), (100, 256), (256, 256), (3, 64)]
