@@ -199,8 +199,8 @@ enum Bar {
   kYFree = kState + 2,                 // Y read out
   kStaged = kYFree + 1,                // y in shared memory [3]
   kZeroed = kStaged + 3,
-  kXRead = kZeroed + 1,                // x read by the state's warps, so that y may replace it
-  kFullState = kXRead + 1,             // a state in the second and third stage of x
+  kXRead = kZeroed + 1,                // x read by the state's warps, so that y may replace it [2]
+  kFullState = kXRead + 2,             // a state in the second and third stage of x
   kStateRead = kFullState + 1,
   kBarCount = kStateRead + 1,
 };
@@ -415,7 +415,10 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       mbar_init(bars + kGatesFull + i, kHeads);
       mbar_init(bars + kGatesFree + i, kOutWarps + K::kStateWarps);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(bars + kState + i, K::kStateWarps);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bars + kState + i, K::kStateWarps);
+      mbar_init(bars + kXRead + i, K::kStateWarps);
+    }
     for (int i = 0; i < 4; ++i) {
       mbar_init(bars + kFx + i, K::kFxWarps);
       mbar_init(bars + kFxFree + i, 1);
@@ -423,7 +426,6 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     for (int i : {kCB, kYM}) mbar_init(bars + i, 1);
     for (int i : {kMy, kYFree}) mbar_init(bars + i, 8);
     mbar_init(bars + kZeroed, K::kStateWarps);
-    mbar_init(bars + kXRead, K::kStateWarps);
     mbar_init(bars + kFullState, 1);
     mbar_init(bars + kStateRead, K::kStateWarps);
     fence_mbar_init();
@@ -510,7 +512,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     tmem_st_wait();
     tc_fence_before();
     arrive(kFx + place);
-    if (!kStates && t == 3) arrive(kXRead);
+    if (!kStates && t == 3) arrive(kXRead + (c & 1));
   };
 
   if (warp < kOutWarps) {
@@ -652,7 +654,9 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
           tmem_ld_wait();
           tc_fence_before();
           arrive(kYFree);  // the next chunk's first product may start
-          wait(bars_u + 8 * (kXRead), c & 1);
+          // Two barriers: the state's warps may be done with chunk c + 1 by now (its dS waits for
+          // nothing of this role behind first_fx), but not with c + 2, whose first_fx comes later.
+          wait(bars_u + 8 * (kXRead + (c & 1)), (c >> 1) & 1);
   #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const uint32_t at = xrow ^ (16 * k);
