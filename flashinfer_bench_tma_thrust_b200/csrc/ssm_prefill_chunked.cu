@@ -193,7 +193,7 @@ enum Bar {
   kDS = kCB + 1,                       //   dS [3, by stage of B]
   kYM = kDS + 3,                       //   M x
   kFx = kYM + 1,                       // f x written [4, by place]
-  kFxFree = kFx + 4,                   // f x read by its products [4]
+  kFxFree = kFx + 4,                   // f x read by its products [4, by quarter of a chunk]
   kMy = kFxFree + 4,                   // M and the scaled Y written
   kState = kMy + 1,                    // S written, dS read [2]
   kYFree = kState + 2,                 // Y read out
@@ -485,7 +485,12 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     uint32_t u[2][4];  // [columns 0-15, 16-31]: tokens 0-7 of columns 0-7, 8-15; tokens 8-15
     ldmatrix_x4_trans(xa, u[0]);
     ldmatrix_x4_trans(xa ^ 32, u[1]);
-    if (k >= K::kPlaces) wait(bars_u + 8 * (kFxFree + place), (k / K::kPlaces - 1) & 1);
+    // The place's last use, `last`, was another quarter. A barrier per quarter, not per place: each
+    // role has waited for its quarter's earlier phases itself, and its own f x comes before the next.
+    // (A place has two phases per chunk here, of which a role would look at every other: it could
+    // take the end of the phase before the last for that of the last.)
+    if (const int last = k - K::kPlaces; last >= 0)
+      wait(bars_u + 8 * (kFxFree + last % 4), (last / 4) & 1);
     const uint32_t at = lanes + (kStates ? 0 : kTF) + 16 * kTerms * place + 8 * part;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -883,7 +888,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
               mma_bf16_ts_w(td, tf + 16 * r + 8 * s, desc(d_b, b0, s * 2048), kIdDS,
                             t > 0 || r > 0 || s > 0);
           }
-          mma_commit_w(bars + kFxFree + place);
+          mma_commit_w(bars + kFxFree + t);
           if (t == 3) mma_commit_w(bars + kDS + st);
         };
         auto fx_bar = [&](int t) { return bars_u + 8 * (kFx + (4 * c + t) % K::kPlaces); };

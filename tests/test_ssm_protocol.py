@@ -34,15 +34,16 @@ class Bar:
 
 
 class Model:
-    def __init__(self, chunks, ragged, xread_slots=2):
+    def __init__(self, chunks, ragged, xread_slots=2, free_by_quarter=True):
         self.n, self.ragged, self.slots = chunks, ragged, xread_slots
+        self.by_quarter = free_by_quarter
         b = lambda name, count, k=None: (  # noqa: E731
             Bar(name, count) if k is None else [Bar(f"{name}[{i}]", count) for i in range(k)])
         self.full_x, self.full_b, self.full_c = b("full_x", 1, X_STAGES), b("full_b", 1), b("full_c", 1)
         self.gates_full, self.gates_free = b("gates_full", 1, GATE_STAGES), \
             b("gates_free", 2 * WARPS, GATE_STAGES)
         self.cb, self.ds, self.ym = b("cb", 1), b("ds", 1), b("ym", 1)
-        self.fx, self.fx_free = b("fx", WARPS, PLACES), b("fx_free", 1, PLACES)
+        self.fx, self.fx_free = b("fx", WARPS, PLACES), b("fx_free", 1, 4)
         self.my, self.state, self.y_free = b("my", WARPS), b("state", WARPS), b("y_free", WARPS)
         self.staged, self.zeroed = b("staged", WARPS, X_STAGES), b("zeroed", WARPS)
         self.x_read, self.together = b("x_read", WARPS, self.slots), b("together", WARPS)
@@ -64,19 +65,18 @@ class Model:
     # Roles: generators that yield what they wait for (None: nothing, another may go first).
 
     def write_fx(self, w, c, t):
-        place, use = (4 * c + t) % PLACES, (4 * c + t) // PLACES
+        place, last = (4 * c + t) % PLACES, 4 * c + t - PLACES
         self.expect(self.X[c % X_STAGES], ("x", c), "x read for f x")
-        if use > 0:
-            yield lambda: self.wait_place(c, t, use)
+        if last >= 0:
+            if self.by_quarter:
+                yield lambda: self.fx_free[last % 4].passed(last // 4)
+            else:
+                yield lambda: self.fx_free[place].passed(last // PLACES)
         self.F[place][w] = (c, t)
         yield None
         self.fx[place].arrive()
         if t == 3:
             self.x_read[c % self.slots].arrive()
-
-    def wait_place(self, c, t, use):
-        # (not by parity: which phase of the place's barrier this is, is another matter)
-        return self.fx_free[(4 * c + t) % PLACES].phase >= use
 
     def first_fx(self, w, c):
         yield lambda: self.full_x[c % X_STAGES].passed(c // X_STAGES)
@@ -147,7 +147,8 @@ class Model:
                         self.fx[(4 * c + t) % PLACES].passed((4 * c + t) // PLACES):
                     if not act:
                         return True
-                    self.pipe += [("ds", c, t), ("arrive", self.fx_free[(4 * c + t) % PLACES])]
+                    free = self.fx_free[t if self.by_quarter else (4 * c + t) % PLACES]
+                    self.pipe += [("ds", c, t), ("arrive", free)]
                     self.pipe += [("arrive", self.ds)] if t == 3 else []
                     has["t"], acted = t + 1, True
                 if not has["cb"]:
@@ -276,3 +277,10 @@ def test_the_model_sees_a_barrier_that_runs_ahead():
     warp that had yet to look at it: the block then stood still."""
     with pytest.raises(Unsound, match="x_read"):
         schedules(600, xread_slots=1)
+
+
+def test_the_model_sees_a_phase_that_is_skipped():
+    """One barrier per place of f x has two phases per chunk. The output's warps, which write one
+    quarter of four, looked at every other, and could write over a quarter still to be read."""
+    with pytest.raises(Unsound, match="fx_free"):
+        schedules(600, free_by_quarter=False)
