@@ -489,8 +489,10 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     // role has waited for its quarter's earlier phases itself, and its own f x comes before the next.
     // (A place has two phases per chunk here, of which a role would look at every other: it could
     // take the end of the phase before the last for that of the last.)
-    if (const int last = k - K::kPlaces; last >= 0)
+    if (const int last = k - K::kPlaces; last >= 0) {
       wait(bars_u + 8 * (kFxFree + last % 4), (last / 4) & 1);
+      tc_fence_after();
+    }
     const uint32_t at = lanes + (kStates ? 0 : kTF) + 16 * kTerms * place + 8 * part;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {

@@ -7,8 +7,13 @@ while that barrier is in the awaited phase or the one after. The model checks th
 and that every access finds the chunk that it is meant for.
 """
 import random
+import re
+from pathlib import Path
 
 import pytest
+
+SOURCE = Path(__file__).resolve().parents[1] / "flashinfer_bench_tma_thrust_b200" / "csrc" / \
+    "ssm_prefill_chunked.cu"
 
 X_STAGES, PLACES, GATE_STAGES, WARPS = 3, 2, 4, 2  # WARPS: of each role, the barriers' counts
 
@@ -284,3 +289,23 @@ def test_the_model_sees_a_phase_that_is_skipped():
     quarter of four, looked at every other, and could write over a quarter still to be read."""
     with pytest.raises(Unsound, match="fx_free"):
         schedules(600, free_by_quarter=False)
+
+
+def test_tmem_accesses_are_fenced_behind_the_products():
+    """Each wait on a barrier that a product's commit completes is followed by the fence that orders
+    this thread's tensor memory accesses behind it, before the next such access. (The issuing
+    warp's and the copies' waits precede none.)"""
+    code = re.sub(r"//[^\n]*", "", SOURCE.read_text())
+    events = re.findall(
+        r"\bwait\(bars_u \+ 8 \* \(?(kCB|kYM|kDS|kFxFree)\b|\b(tc_fence_after)\(\)"
+        r"|\b(tmem_ld|tmem_st)(?:\d+|_frag)\(", code)
+    pending, seen = None, set()
+    for bar, fence, access in events:
+        if bar:
+            pending = bar
+            seen.add(bar)
+        elif fence:
+            pending = None
+        else:
+            assert pending is None, f"{access} behind a wait for {pending} without a fence"
+    assert seen == {"kCB", "kYM", "kDS", "kFxFree"}
