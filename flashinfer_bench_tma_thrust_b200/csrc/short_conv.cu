@@ -15,8 +15,8 @@
 // rows arrive by asynchronous copies in a ring of its own in shared memory, 12 to 16 rows ahead:
 // with rows in flight in registers (4 per thread, 16 warps per SM) HBM's latency was not
 // covered. No thread waits for another. Sums are fp32; silu takes ex2.approx and a shared
-// approximate reciprocal (a few fp32 ulp, far below the bf16 rounding of the output, the only
-// other one). 65536 x 6144 take 262 us (6.2 TB/s); 19679 x 8192 115 us, and 130 with the norm of
+// approximate reciprocal (relative error below 2^-16, at the exponents of v = -92; the bf16
+// rounding of the output is the only other one). 65536 x 6144 take 262 us (6.2 TB/s); 19679 x 8192 115 us, and 130 with the norm of
 // half of the channels: besides HBM the instructions per row (130 for 8 channels) come near a
 // bound then.
 #include <cmath>
@@ -155,13 +155,11 @@ __device__ __forceinline__ Place place_of(const ConvParams& p, int c) {
   return Place{p.out[s], p.begin[s + 1] - p.begin[s], c - p.begin[s], p.normed[s]};
 }
 
-// v / (1 + e^-v) of two values with three MUFU operations instead of four: one reciprocal of
-// the product of the denominators. v is held at -43.5, where silu is -43.5 2^-62.8, nothing to
-// bf16's neighbours, so that the product stays finite (and a v of -1e38 or -infinity gives that
-// too). A NaN is kept by the factor v but not by the exponent, which both values share.
+// silu, v / (1 + e^-v), of two values with three MUFU operations instead of four: one reciprocal
+// of the product of the denominators, which fp32 holds for v from kFar up. A NaN is kept by the
+// factor v but not by the exponent, which both values share.
+constexpr float kFar = -43.5f;
 __device__ __forceinline__ float2 silu2(float2 v) {
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(-43.5f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(-43.5f));
   const float2 z = __fmul2_rn(v, make_float2(-kLog2e, -kLog2e));
   float2 e;
   float r;
@@ -170,6 +168,41 @@ __device__ __forceinline__ float2 silu2(float2 v) {
   const float2 a = __fadd2_rn(e, make_float2(1.f, 1.f));
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a.x * a.y));
   return __fmul2_rn(v, __fmul2_rn(make_float2(a.y, a.x), make_float2(r, r)));
+}
+// What silu2 makes silu(v) of where v is below kFar. There silu(v) is v e^v to the last bit, and
+// silu2 halves a value as small as 2 v e^v. Two factors, since e^v leaves the normal numbers (at
+// -87) before v e^v does (at -92). -infinity gives zero.
+__device__ __forceinline__ float from_far(float v) {
+  v = fmaxf(v, -120.f);  // (zero from -108 down)
+  float h;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h) : "f"(v * (0.5f * kLog2e)));
+  return (v + v) * h * h;
+}
+// silu of rows of eight values. Values below kFar are rare: a minimum over all rows finds them. (With
+// a branch per row the rows' instructions do not mix: 12 % more time.)
+template <int kTok>
+__device__ __forceinline__ void silu_rows(float2 (&y)[kTok][kP]) {
+  float low = 0.f;
+#pragma unroll
+  for (int t = 0; t < kTok; ++t) {
+#pragma unroll
+    for (int i = 0; i < kP; ++i) low = fminf(low, fminf(y[t][i].x, y[t][i].y));
+  }
+  if (low < kFar) {
+#pragma unroll
+    for (int t = 0; t < kTok; ++t) {
+#pragma unroll
+      for (int i = 0; i < kP; ++i) {
+        if (y[t][i].x < kFar) y[t][i].x = from_far(y[t][i].x);
+        if (y[t][i].y < kFar) y[t][i].y = from_far(y[t][i].y);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < kTok; ++t) {
+#pragma unroll
+    for (int i = 0; i < kP; ++i) y[t][i] = silu2(y[t][i]);
+  }
 }
 
 // The W-1 rows before the current one, as floats.
@@ -227,13 +260,7 @@ __device__ __forceinline__ void output_rows(const ConvParams& p, const Taps<W>& 
       win.v[W - 2][i] = cur;
     }
   }
-  if (p.silu) {
-#pragma unroll
-    for (int t = 0; t < kTok; ++t) {
-#pragma unroll
-      for (int i = 0; i < kP; ++i) y[t][i] = silu2(y[t][i]);
-    }
-  }
+  if (p.silu) silu_rows(y);
   if (pl.normed) {  // the same for the 16 lanes of a head
     float q[kTok];
 #pragma unroll

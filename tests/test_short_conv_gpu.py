@@ -100,6 +100,34 @@ def test_one_channel_leaves_its_neighbours_alone(bad):
                 assert v == pytest.approx(bad, rel=2 ** -8)  # (bf16's own rounding of it)
 
 
+FAR = 2.0 ** -14  # silu's exponent |v| log2(e) < 150 rounds by 2^-17, its exponential by 2 ulp
+
+
+def passed_through(values, C=256):
+    """Arguments of a convolution that hands each channel its input (one tap of one)."""
+    w = torch.zeros(C, 2)
+    w[:, 1] = 1
+    x = values.bfloat16()
+    return dev(x, w, None, None, torch.tensor([0, x.shape[0]], dtype=torch.int32))
+
+
+@pytest.mark.parametrize("rows", [1, 50, 1300])
+def test_silu_far_below_zero(rows):
+    """silu is v e^v where e^-v is large: relative accuracy down to the least normal number, also
+    next to ordinary channels, and zero behind it."""
+    g = torch.Generator().manual_seed(rows)
+    x = torch.randn(rows, 256, generator=g) * 3
+    far = torch.rand(rows, 256, generator=g) < 0.3
+    x = torch.where(far, -40 - 51 * torch.rand(rows, 256, generator=g), x).bfloat16()
+    x[:, 3], x[-1, 200], x[0, 77] = -200, float("-inf"), -3e38
+    got = short_conv.prefill(*passed_through(x))[0]
+    v = x.double()
+    want = torch.where(v > -700, v * torch.sigmoid(v), 0.0)
+    assert_within(got, want, FAR * want.abs(), "silu", rounding=BF16)
+    one = short_conv.decode(x[:, None].cuda(), *passed_through(x)[1:2])[0]
+    assert torch.equal(one[:, 0], got)
+
+
 def test_zero_head_norm_and_eps():
     """A head of zeros stays zero; eps enters under the root."""
     x, w, _, _, cu = make([5], 256, 4, bias=False, seed=3)
