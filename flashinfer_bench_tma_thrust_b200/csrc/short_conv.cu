@@ -19,6 +19,7 @@
 // rounding of the output is the only other one). 65536 x 6144 take 262 us (6.2 TB/s); 19679 x 8192 115 us, and 130 with the norm of
 // half of the channels: besides HBM the instructions per row (130 for 8 channels) come near a
 // bound then.
+#include <cfloat>
 #include <cmath>
 
 #include "gdn_b200.h"
@@ -235,14 +236,46 @@ __device__ __forceinline__ void head_sums(float (&q)[kTok]) {
   }
 }
 
+// A thread's part of its head's sum of squares.
+__device__ __forceinline__ float square_sum(const float2 (&y)[kP]) {
+  float2 q = __fmul2_rn(y[0], y[0]);
+#pragma unroll
+  for (int i = 1; i < kP; ++i) q = __ffma2_rn(y[i], y[i], q);
+  return q.x + q.y;
+}
+
+// The norm of a head whose sum of squares (with eps) is not between kLeastSum and FLT_MAX: squares
+// that fp32 cannot hold are missing in it or have made it infinite. The head, and eps with it, is
+// scaled by a power of two that brings its largest value (or the root of eps) next to one, and is
+// left so; returns what it is then multiplied by. Zeros without eps (0 / 0), infinities and NaN:
+// as they were.
+constexpr float kLeastSum = 0x1p-80f;  // a square below 2^-126 is nothing to it
+__device__ __forceinline__ float norm_far(float2 (&y)[kP], float eps, float r) {
+  const uint32_t lanes = 0xffffu << (threadIdx.x & 16);
+  float m = sqrtf(eps);
+#pragma unroll
+  for (int i = 0; i < kP; ++i) m = fmaxf(m, fmaxf(fabsf(y[i].x), fabsf(y[i].y)));
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor_sync(lanes, m, o));
+  if (m == 0.f || m > FLT_MAX) return r;
+  const float s = __uint_as_float((254u - min(__float_as_uint(m) >> 23, 253u)) << 23);
+#pragma unroll
+  for (int i = 0; i < kP; ++i) y[i] = __fmul2_rn(y[i], make_float2(s, s));
+  float q[1] = {square_sum(y)};
+  head_sums(q);
+  return rsqrtf(fmaf(eps * s, s, q[0]));
+}
+
 // kTok output rows from row `at` on (kWide: at `out`): the taps over the window and `rows`
 // (which enter the window one by one), activation, norm of the head (16 lanes), store. All lanes
-// of the warp call it; `live` says whether this thread's channels exist.
-template <int W, bool kWide, int kTok>
+// of the warp call it; `live` says whether this thread's channels exist. Without kCareful a
+// head whose sum of squares is out of range sets `far`, and its row is not right. (Branches to
+// norm_far between the rows cost 3 % of the time, registers included; such heads are freaks.)
+template <int W, bool kWide, bool kCareful, int kTok>
 __device__ __forceinline__ void output_rows(const ConvParams& p, const Taps<W>& taps,
                                             const Place& pl, int c, int64_t at,
                                             __nv_bfloat16* out, Window<W>& win,
-                                            const Row (&rows)[kTok], bool live) {
+                                            const Row (&rows)[kTok], bool live, bool& far) {
   float2 y[kTok][kP];
 #pragma unroll
   for (int t = 0; t < kTok; ++t) {
@@ -264,16 +297,19 @@ __device__ __forceinline__ void output_rows(const ConvParams& p, const Taps<W>& 
   if (pl.normed) {  // the same for the 16 lanes of a head
     float q[kTok];
 #pragma unroll
-    for (int t = 0; t < kTok; ++t) {
-      float2 q2 = __fmul2_rn(y[t][0], y[t][0]);
-#pragma unroll
-      for (int i = 1; i < kP; ++i) q2 = __ffma2_rn(y[t][i], y[t][i], q2);
-      q[t] = q2.x + q2.y;
-    }
+    for (int t = 0; t < kTok; ++t) q[t] = square_sum(y[t]);
     head_sums(q);
 #pragma unroll
     for (int t = 0; t < kTok; ++t) {
-      const float r = rsqrtf(q[t] + p.eps);
+      const float sum = q[t] + p.eps;
+      float r = rsqrtf(sum);
+      if (!(sum >= kLeastSum && sum <= FLT_MAX)) {
+        if (kCareful) {
+          r = norm_far(y[t], p.eps, r);
+        } else {
+          far = true;
+        }
+      }
 #pragma unroll
       for (int i = 0; i < kP; ++i) y[t][i] = __fmul2_rn(y[t][i], make_float2(r, r));
     }
@@ -331,8 +367,79 @@ __device__ __forceinline__ void copy16_async(uint4* to, const __nv_bfloat16* fro
                : "memory");
 }
 
+// A thread's way through the tokens of a tile, over the sequences' bounds.
 template <int W, bool kWide>
-__global__ void __launch_bounds__(kThreads)
+struct Walk {
+  const ConvParams& p;
+  const int c;
+  int64_t n, start, end;  // the sequence; none left (n = N): nothing is written
+  Window<W> win;
+  __device__ __forceinline__ Walk(const ConvParams& p_, int c_) : p(p_), c(c_) {}
+  __device__ __forceinline__ void bounds() {
+    start = end = p.T;
+    if (n < p.N) {
+      start = bound(p, n);
+      end = bound(p, n + 1);
+    }
+  }
+  __device__ __forceinline__ void begin(int64_t t0) {  // by the whole warp
+    n = find_sequence(p.cu_seqlens, p.cu_dtype, p.N, t0);
+    bounds();
+#pragma unroll
+    for (int r = 0; r < W - 1; ++r) win.set(r, Row{make_uint4(0u, 0u, 0u, 0u)});
+    if (n < p.N && start < t0) {  // the tile begins inside a sequence
+#pragma unroll
+      for (int r = 0; r < W - 1; ++r) {
+        const int64_t u = t0 - (W - 1) + r;
+        if (u >= start) {
+          win.set(r, load_row<kWide>(p.x + u * p.x_stride, c, p.C));
+        } else if (p.state) {
+          win.set(r, load_row<kWide>(p.state + (n * (W - 1) + (u - start) + (W - 1)) * p.C, c, p.C));
+        }
+      }
+    }
+  }
+  // Whether token t, the one behind the last that was asked for, lies in a sequence; the window is
+  // then that of t.
+  __device__ __forceinline__ bool next(int64_t t) {
+    while (t >= end && n < p.N) {  // into the next sequence that has tokens
+      ++n;
+      bounds();
+    }
+    if (n >= p.N || t < start) return false;
+    if (t == start) {
+#pragma unroll
+      for (int r = 0; r < W - 1; ++r)
+        win.set(r, p.state ? load_row<kWide>(p.state + (n * (W - 1) + r) * p.C, c, p.C)
+                           : Row{make_uint4(0u, 0u, 0u, 0u)});
+    }
+    return true;
+  }
+};
+
+// A tile's tokens with care, by the whole warp (the norms need whole heads). A function of its own:
+// in line it cost the first pass registers, and with them 9 %.
+template <int W, bool kWide>
+__device__ __noinline__ void tile_again(const ConvParams& p, int c, int64_t t0, int64_t t1) {
+  const bool live = c < p.C;
+  const int cl = live ? c : 0;
+  const Taps<W> taps = load_taps<W, kWide>(p, cl);
+  Place pl = place_of(p, cl);
+  if (!live) pl.normed = 0;
+  Walk<W, kWide> walk(p, cl);
+  walk.begin(t0);
+  bool far = false;
+#pragma unroll 1
+  for (int64_t t = t0; t < t1; ++t) {
+    if (!walk.next(t)) continue;
+    const Row row[1] = {load_row<kWide>(p.x + t * p.x_stride, cl, p.C)};
+    output_rows<W, kWide, true, 1>(p, taps, pl, cl, t, pl.out + t * pl.width + pl.at, walk.win, row,
+                                   live, far);
+  }
+}
+
+template <int W, bool kWide>
+__global__ void __launch_bounds__(kThreads, W == 2 ? 5 : 4)  // blocks per SM, as without tile_again
 conv_prefill_kernel(const __grid_constant__ ConvParams p, int64_t tiles, int run) {
   const int c = (blockIdx.x * kThreads + threadIdx.x) * kVec;
   const bool live = c < p.C;
@@ -389,65 +496,37 @@ conv_prefill_kernel(const __grid_constant__ ConvParams p, int64_t tiles, int run
   const Taps<W> taps = load_taps<W, kWide>(p, cl);
   Place pl = place_of(p, cl);
   if (!live) pl.normed = 0;  // (a normed section is whole warps)
-  int64_t n = find_sequence(p.cu_seqlens, p.cu_dtype, p.N, t0);
-  int64_t start = p.T, end = p.T;  // of sequence n; none left: nothing is written
-  if (n < p.N) {
-    start = bound(p, n);
-    end = bound(p, n + 1);
-  }
-  Window<W> win;
-  const Row zero{make_uint4(0u, 0u, 0u, 0u)};
-#pragma unroll
-  for (int r = 0; r < W - 1; ++r) win.set(r, zero);
-  if (n < p.N && start < t0) {  // the tile begins inside a sequence
-#pragma unroll
-    for (int r = 0; r < W - 1; ++r) {
-      const int64_t u = t0 - (W - 1) + r;
-      if (u >= start) {
-        win.set(r, load_row<kWide>(p.x + u * p.x_stride, cl, p.C));
-      } else if (p.state) {
-        win.set(r, load_row<kWide>(p.state + (n * (W - 1) + (u - start) + (W - 1)) * p.C, cl, p.C));
-      }
-    }
-  }
+  Walk<W, kWide> walk(p, cl);
+  walk.begin(t0);
+  bool far = false;
   __nv_bfloat16* to = pl.out + t0 * pl.width + pl.at;  // kWide: the batch's first output row
 #pragma unroll 1
   for (int b = 0; b < batches; ++b, to += kAhead * pl.width) {
     const int64_t tb = t0 + b * kAhead;
     fetch(b + kSlots - 1);  // its slot's rows are in registers or behind
     asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 1) : "memory");
-    if (n < p.N && start < tb && tb + kAhead <= min(end, t1)) {
+    if (walk.n < p.N && walk.start < tb && tb + kAhead <= min(walk.end, t1)) {
       // all of the batch and the rows before it lie in one sequence
 #pragma unroll
       for (int a = 0; a < kAhead; a += 2) {  // two rows at a time: more take too many registers
         const Row rows[2] = {fetched(b, a), fetched(b, a + 1)};
-        output_rows<W, kWide, 2>(p, taps, pl, cl, tb + a, to + a * pl.width, win, rows, live);
+        output_rows<W, kWide, false, 2>(p, taps, pl, cl, tb + a, to + a * pl.width, walk.win, rows,
+                                        live, far);
       }
       continue;
     }
 #pragma unroll 1
-    for (int a = 0; a < kAhead; ++a) {  // token by token, over the sequences' bounds
+    for (int a = 0; a < kAhead; ++a) {
       const int64_t t = tb + a;
       if (t >= t1) break;
-      while (t >= end && n < p.N) {  // into the next sequence that has tokens
-        ++n;
-        start = end = p.T;
-        if (n < p.N) {
-          start = bound(p, n);
-          end = bound(p, n + 1);
-        }
-      }
-      if (n >= p.N || t < start) continue;  // a token of no sequence
-      if (t == start) {
-#pragma unroll
-        for (int r = 0; r < W - 1; ++r)
-          win.set(r, p.state ? load_row<kWide>(p.state + (n * (W - 1) + r) * p.C, cl, p.C) : zero);
-      }
+      if (!walk.next(t)) continue;
       const Row row[1] = {fetched(b, a)};
-      output_rows<W, kWide, 1>(p, taps, pl, cl, t, to + a * pl.width, win, row, live);
+      output_rows<W, kWide, false, 1>(p, taps, pl, cl, t, to + a * pl.width, walk.win, row, live,
+                                      far);
     }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
+  if (__any_sync(0xffffffffu, far)) tile_again<W, kWide>(p, c, t0, t1);
 }
 
 // One token per sequence, bound by HBM (1024 sequences of 8192 channels with 4 taps 26.7 us,
@@ -477,6 +556,7 @@ conv_decode_kernel(const __grid_constant__ ConvParams p, int per_thread) {
   const Taps<W> taps = load_taps<W, kWide>(p, cl);
   Place pl = place_of(p, cl);
   if (!live) pl.normed = 0;
+  bool far = false;  // (with care at once: bound by memory, it costs nothing here)
   for (int64_t n = n0; n < n1; ++n) {
     Row rows[W];
 #pragma unroll
@@ -491,7 +571,8 @@ conv_decode_kernel(const __grid_constant__ ConvParams p, int per_thread) {
 #pragma unroll
     for (int r = 0; r < W - 1; ++r) win.set(r, rows[r]);
     const Row row[1] = {rows[W - 1]};
-    output_rows<W, kWide, 1>(p, taps, pl, cl, n, pl.out + n * pl.width + pl.at, win, row, live);
+    output_rows<W, kWide, true, 1>(p, taps, pl, cl, n, pl.out + n * pl.width + pl.at, win, row, live,
+                                   far);
   }
 }
 

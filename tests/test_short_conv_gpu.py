@@ -128,6 +128,31 @@ def test_silu_far_below_zero(rows):
     assert torch.equal(one[:, 0], got)
 
 
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-6])
+@pytest.mark.parametrize("rows", [3, 1300])
+@pytest.mark.parametrize("activation", ["silu", None])
+def test_norm_of_heads_whose_squares_leave_fp32(eps, rows, activation):
+    """Heads of values whose squares underflow or overflow: the norm is still that of the head."""
+    g = torch.Generator().manual_seed(rows)
+    x = torch.randn(rows, 256, generator=g)
+    if activation:
+        x[0::3] = -44 - 30 * torch.rand(x[0::3].shape, generator=g)
+    else:
+        x[0::3] *= 1e-25
+    x[1::3, :128] *= 1e30
+    x = x.bfloat16()
+    args = passed_through(x)
+    got = short_conv.prefill(*args, activation=activation, l2norm=True, eps=eps)[0]
+    v = x.double()
+    v = (v * torch.sigmoid(v) if activation else v).unflatten(1, (-1, 128))
+    e = torch.tensor(eps).double()  # (as fp32 has it)
+    want = (v / (v.pow(2).sum(-1, keepdim=True) + e).sqrt()).flatten(1)
+    # twice silu's error (value and norm) and the norm's own 140 roundings of a sum
+    assert_within(got, want, (2 * FAR + 140 * 2.0 ** -24) * want.abs(), "normed", rounding=BF16)
+    one = short_conv.decode(x[:, None].cuda(), args[1], activation=activation, l2norm=True, eps=eps)
+    assert (one[0][:, 0].double() - got.double()).abs().le(2.0 ** -7 * got.double().abs()).all()
+
+
 def test_zero_head_norm_and_eps():
     """A head of zeros stays zero; eps enters under the root."""
     x, w, _, _, cu = make([5], 256, 4, bias=False, seed=3)
