@@ -216,7 +216,8 @@ struct Window {
 };
 
 // Sums of kTok values per lane over 16 lanes, each in every lane. Two values: an exchange that
-// leaves one value per lane, three more steps on it, and two broadcasts, 6 shuffles for 8.
+// leaves one value per lane, three more steps on it, and two broadcasts, 6 shuffles for 8. The order
+// of the sums is the same for one value, so that bits do not depend on how tokens fall into rows.
 template <int kTok>
 __device__ __forceinline__ void head_sums(float (&q)[kTok]) {
   const uint32_t lanes = 0xffffu << (threadIdx.x & 16);
@@ -231,7 +232,7 @@ __device__ __forceinline__ void head_sums(float (&q)[kTok]) {
 #pragma unroll
     for (int t = 0; t < kTok; ++t) {
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) q[t] += __shfl_xor_sync(lanes, q[t], o);
+      for (int o = 1; o < 16; o <<= 1) q[t] += __shfl_xor_sync(lanes, q[t], o);
     }
   }
 }

@@ -318,3 +318,28 @@ def test_feeds_gdn_prefill():
     check((q, k, v), ns, x, w, b, s, cu.tolist(), split=split, norm=norm)
     assert ((out.float().cpu() - want.float()).abs() <= 1e-2 + 1e-2 * want.float().abs()).all()
     assert ((state.cpu() - wstate).norm() / wstate.norm()) < 1e-3
+
+
+def test_bits_do_not_depend_on_packing():
+    """A long prompt as a whole, among others, in pieces and token by token: the same bits, normed
+    heads too."""
+    C, T = 1160, 2400
+    kw = dict(split=(128, 1024, 8), l2norm=(True, True, False))
+    x, w, b, s, _ = make([T], C, 4, seed=42)
+    x, w, b, s = dev(x, w, b, s)
+    cu = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    whole, end = short_conv.prefill(x, w, b, s, cu(0, T), **kw)
+    # behind another sequence of 7 tokens: other tiles, other batches
+    both, _ = short_conv.prefill(torch.cat([x[:7], x]), w, b, torch.cat([s, s]), cu(0, 7, T + 7), **kw)
+    assert all(torch.equal(u[7:], v) for u, v in zip(both, whole))
+    parts, st = [], s
+    for lo, hi in ((0, 1201), (1201, 1204), (1204, T)):
+        o, st = short_conv.prefill(x[lo:hi], w, b, st, cu(0, hi - lo), **kw)
+        parts.append(o)
+    assert all(torch.equal(torch.cat([p[i] for p in parts]), whole[i]) for i in range(3))
+    assert torch.equal(st, end)
+    # every token with its own earlier rows as its state
+    rows = torch.cat([s[0], x])
+    before = torch.stack([rows[k:k + T] for k in range(3)], 1).contiguous()
+    tokens, _ = short_conv.decode(x[:, None], w, b, before, **kw)
+    assert all(torch.equal(u[:, 0], v) for u, v in zip(tokens, whole))
