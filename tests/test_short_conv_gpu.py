@@ -320,6 +320,53 @@ def test_feeds_gdn_prefill():
     assert ((state.cpu() - wstate).norm() / wstate.norm()) < 1e-3
 
 
+# Prompts whose tiles hold several batches of tokens: (lengths, channels, split, norm).
+LONG = [
+    # runs of 12 tokens (three batches), bounds inside batches and tiles
+    ([700, 3, 0, 1, 995, 701], 1160, (128, 1024, 8), (True, True, False)),
+    # runs of 24 (the ring of four batches comes round)
+    ([1, 2500, 18, 1481], 2304, (1024, 1024, 256), (True, False, True)),
+    # the rule for longer runs (32 here, eight batches)
+    ([29000, 5, 1500], 128, (128,), (True,)),
+    # runs of 40, odd channels (no vector access)
+    ([9001, 0, 13999], 357, (128, 229), (True, False)),
+]
+
+
+@pytest.mark.parametrize("lengths,C,split,norm", LONG)
+@pytest.mark.parametrize("W", [2, 3, 4])
+def test_long_prompts(lengths, C, split, norm, W):
+    x, w, b, s, cu = make(lengths, C, W, seed=C + W)
+    got, ns = short_conv.prefill(*dev(x, w, b, s, cu), split=split, l2norm=norm, check=True)
+    check(got, ns, x, w, b, s, cu.tolist(), split=split, norm=norm)
+
+
+def test_long_prompt_of_unaligned_rows():
+    lengths, C = [700, 3, 995, 702], 1160
+    x, w, b, s, cu = make(lengths, C, 4, seed=41)
+    wide = torch.full((2400, C + 7), float("nan"), dtype=torch.bfloat16)
+    wide[:, 3:3 + C] = x
+    kw = dict(split=(128, 1024, 8), l2norm=(True, True, False))
+    w, b, s, cu = dev(w, b, s, cu)
+    got, ns = short_conv.prefill(wide.cuda()[:, 3:3 + C], w, b, s, cu, **kw)
+    want, want_ns = short_conv.prefill(x.cuda(), w, b, s, cu, **kw)
+    assert all(torch.equal(u, v) for u, v in zip(got, want)) and torch.equal(ns, want_ns)
+
+
+@pytest.mark.parametrize("rows", [1303, 5])
+@pytest.mark.parametrize("W", [2, 3, 4])
+def test_many_tokens(rows, W):
+    """Several sequences per thread, the last thread with fewer: also in place."""
+    C, split, norm = 1160, (128, 1024, 8), (True, True, False)
+    x, w, b, s, _ = make([1] * rows, C, W, seed=rows + W)
+    xd, wd, bd, sd = dev(x[:, None], w, b, s)
+    got, ns = short_conv.decode(xd, wd, bd, sd, split=split, l2norm=norm)
+    check(tuple(v[:, 0] for v in got), ns, x, w, b, s, list(range(rows + 1)), split=split, norm=norm)
+    again, same = short_conv.decode_inplace(xd, wd, bd, sd, split=split, l2norm=norm)
+    assert same is sd and torch.equal(sd, ns)
+    assert all(torch.equal(u, v) for u, v in zip(got, again))
+
+
 def test_bits_do_not_depend_on_packing():
     """A long prompt as a whole, among others, in pieces and token by token: the same bits, normed
     heads too."""
