@@ -94,6 +94,7 @@ SIGNATURES = {
     ),
     "gdn_selftest_umma": (_int, [_p, _p, _p, _int, _int, _p, _p]),
     "gdn_selftest_wait_timeout": (_int, [_p, _p, _p]),
+    "gdn_selftest_scan_wait": (_int, [_i32, _int, _p, _p, _p]),
     "gdn_selftest_umma_ts": (_int, [_p, _p, _p, _p, _p]),
 }
 

@@ -7,6 +7,7 @@
 #include "gdn_b200.h"
 #include "gdn_common.cuh"
 #include "sm100_umma.cuh"
+#include "ssm_launch.h"
 
 namespace gdn {
 namespace {
@@ -207,5 +208,45 @@ __global__ void wait_timeout_kernel(int* status, long long* waited_ns) {
 extern "C" int gdn_selftest_wait_timeout(int* status, long long* waited_ns, void* stream) {
   if (!status || !waited_ns) return GDN_ERR_INVALID_ARG;
   gdn::wait_timeout_kernel<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>(status, waited_ns);
+  return cudaGetLastError() == cudaSuccess ? GDN_OK : GDN_ERR_CUDA;
+}
+
+namespace gdn {
+namespace {
+
+// The chunked scan's waits, with `tries` polls at most: on a barrier that `arrive` completes or
+// that nothing does, then once more on a phase that nothing completes. Reported as there.
+__global__ void scan_wait_kernel(uint32_t tries, int arrive, int* status, long long* waited_ns) {
+  __shared__ uint64_t bar;
+  if (threadIdx.x == 0) {
+    sm100::mbar_init(&bar, 1);
+    sm100::fence_mbar_init();
+    if (arrive) sm100::mbar_arrive(&bar);
+  }
+  __syncthreads();
+  sm100::Waiter wait;
+  wait.left = tries;
+  const uint64_t t0 = sm100::globaltimer_ns();
+  wait(sm100::smem_u32(&bar), 0);
+  const uint64_t t1 = sm100::globaltimer_ns();
+  if (!wait.ok()) report_wait(status);
+  wait(sm100::smem_u32(&bar), arrive ? 1 : 0);
+  const uint64_t t2 = sm100::globaltimer_ns();
+  if (threadIdx.x == 0) {
+    waited_ns[0] = static_cast<long long>(t1 - t0);
+    waited_ns[1] = static_cast<long long>(t2 - t1);
+  }
+}
+
+}  // namespace
+}  // namespace gdn
+
+extern "C" int gdn_selftest_scan_wait(int32_t tries, int arrive, int* status,
+                                      long long* waited_ns, void* stream) {
+  if (!status || !waited_ns || tries < 1 ||
+      tries > static_cast<int32_t>(gdn::sm100::Waiter::kTries))
+    return GDN_ERR_INVALID_ARG;
+  gdn::scan_wait_kernel<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>(tries, arrive, status,
+                                                                         waited_ns);
   return cudaGetLastError() == cudaSuccess ? GDN_OK : GDN_ERR_CUDA;
 }

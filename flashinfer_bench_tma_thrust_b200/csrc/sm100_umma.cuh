@@ -167,6 +167,30 @@ __device__ __forceinline__ bool mbar_wait_spin(uint64_t* bar, uint32_t parity) {
   }
 }
 
+// A thread's bounded waits in few instructions, for kernels whose roles' code together has to stay
+// in the instruction cache. A wait gives up after kTries polls of at most kPollNs each, a second or
+// two; later waits of the thread do not wait at all.
+struct Waiter {
+  static constexpr uint32_t kTries = 1u << 20, kPollNs = 2000;
+  uint32_t left = kTries;
+  __device__ __forceinline__ void operator()(uint32_t bar, uint32_t parity) {
+    uint32_t i = left;
+    for (; i; --i) {
+      uint32_t done;
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(done)
+          : "r"(bar), "r"(parity), "r"(kPollNs)
+          : "memory");
+      if (done) return;
+    }
+    left = 0;
+  }
+  __device__ __forceinline__ bool ok() const { return left != 0; }
+};
+
 // ---------------------------------------------------------------- fences
 __device__ __forceinline__ void fence_async_smem() {
   // make generic-proxy writes to shared memory visible to the async proxy (MMA / TMA)

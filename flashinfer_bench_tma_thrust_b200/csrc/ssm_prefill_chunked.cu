@@ -206,30 +206,6 @@ enum Bar {
 };
 static_assert(kBarCount <= kMaxBars, "");
 
-// Bounded waits in few instructions (all roles' code together has to stay in the instruction
-// cache, or they wait for instructions more than for each other). A wait gives up after kTries
-// polls of at most kPollNs each, a second or two; later waits of the thread do not wait at all.
-struct Waiter {
-  static constexpr uint32_t kTries = 1u << 20, kPollNs = 2000;
-  uint32_t left = kTries;
-  __device__ __forceinline__ void operator()(uint32_t bar, uint32_t parity) {
-    uint32_t i = left;
-    for (; i; --i) {
-      uint32_t done;
-      asm volatile(
-          "{\n\t.reg .pred p;\n\t"
-          "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-          "selp.u32 %0, 1, 0, p;\n\t}"
-          : "=r"(done)
-          : "r"(bar), "r"(parity), "r"(kPollNs)
-          : "memory");
-      if (done) return;
-    }
-    left = 0;
-  }
-  __device__ __forceinline__ bool ok() const { return left != 0; }
-};
-
 __device__ __forceinline__ int64_t clamp_to(int64_t v, int64_t T) {
   return v < 0 ? 0 : (v > T ? T : v);
 }

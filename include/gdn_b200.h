@@ -364,6 +364,16 @@ GDN_API int gdn_selftest_umma_ts(const void* A, const void* B, float* D, int* st
  */
 GDN_API int gdn_selftest_wait_timeout(int* status, long long* waited_ns, void* stream);
 
+/*
+ * Diagnostics. The bounded wait of the chunked scan, with at most `tries` polls (1 to 2^20)
+ * of 2 us: on a barrier that is complete (`arrive` non-zero) or that nothing completes, then
+ * on a phase that nothing completes. status: two int32 words as for gdn_ssm_prefill_fwd, [0]
+ * becomes 1 where the first wait gave up; waited_ns: device int64 [2], the time of each (a
+ * thread that gave up once does not wait again).
+ */
+GDN_API int gdn_selftest_scan_wait(int32_t tries, int arrive, int* status, long long* waited_ns,
+                                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

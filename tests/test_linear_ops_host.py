@@ -106,6 +106,12 @@ def test_ssm_chunked_workspace_and_alignment(cuda_lib):
     assert _ssm(lib, "chunked", T=0x7fffff01) == -2
 
 
+def test_scan_wait_refusals(cuda_lib):
+    call = cuda_lib.gdn_selftest_scan_wait
+    assert call(0, 0, P16, P16, None) == -1 and call((1 << 20) + 1, 0, P16, P16, None) == -1
+    assert call(1, 0, None, P16, None) == -1 and call(1, 0, P16, None, None) == -1
+
+
 def test_cpu_tensors_are_refused():
     z = torch.zeros
     with pytest.raises(ValueError, match="CUDA"):

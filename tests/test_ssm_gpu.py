@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from flashinfer_bench_tma_thrust_b200 import GDNError, short_conv, ssm
+from flashinfer_bench_tma_thrust_b200 import GDNError, _lib, short_conv, ssm
 from oracle.ssm_oracle import BF16, assert_within, scan
 
 pytestmark = pytest.mark.gpu
@@ -362,3 +362,67 @@ def test_graph_and_other_stream():
     torch.cuda.synchronize()
     for u, v in ((want, other), (want, got), (wantd, gotd)):
         assert torch.equal(u[0], v[0]) and torch.equal(u[1], v[1])
+
+
+# bf16 states in several batches per warp: 600 sequences of 8 heads, the last batch full or not
+@pytest.mark.parametrize("P,Ns", [(64, 128), (100, 64), (128, 128), (256, 16), (250, 256)])
+def test_token_bf16_states_in_batches(P, Ns):
+    B, H, G = 600, 8, 2
+    a = make([1] * B, H=H, G=G, P=P, Ns=Ns, seed=P + Ns, state=False)
+    a[7] = torch.randn(B, H, P, Ns, generator=torch.Generator().manual_seed(P)).bfloat16()
+    tok = dev([a[0][:, None], a[1][:, None], a[2], a[3][:, None], a[4][:, None], a[5], a[6], a[7]])
+    out, ns = ssm.decode(*tok)
+    assert torch.equal(tok[7].cpu(), a[7])
+    some = [0, 1, 299, 598, 599]
+    y, ye, fin, fe = scan(*[a[i][some] if i in (0, 1, 3, 4, 7) else a[i] for i in range(8)],
+                          list(range(len(some) + 1)))
+    assert_within(out[some], y, ye, "output", rounding=BF16)
+    assert_within(ns[some], fin, fe, "state", rounding=BF16)
+    # all of them: as one sequence alone, which takes one batch per warp (the same operations)
+    for i in (7, 300, 599):
+        alone = ssm.decode(*[t[i:i + 1] if k in (0, 1, 3, 4, 7) else t for k, t in enumerate(tok)])
+        assert torch.equal(alone[0], out[i:i + 1]) and torch.equal(alone[1], ns[i:i + 1])
+    again, same = ssm.decode_inplace(*tok)
+    assert same is tok[7] and torch.equal(again, out) and torch.equal(same, ns)
+
+
+@pytest.mark.parametrize("T,segments", [(400, False), (3000, True)])
+@pytest.mark.parametrize("bad", ["beyond", "before", "decreasing", "all twice"])
+def test_bad_bounds_in_the_chunked_kernel(T, segments, bad):
+    """Bounds outside [0, T] are clamped and decreasing ones taken as empty; the call is reported,
+    and after a reset the next one is right."""
+    cu = {"beyond": [0, T // 2, T + 99], "before": [-3, T // 3, T], "decreasing": [0, T - 10, 20, T],
+          "all twice": [0, T, 0, T]}[bad]
+    a = make([T], H=2, G=1, P=64, Ns=128, state=False, seed=51)
+    n = len(cu) - 1
+    assert (_lib.load().gdn_ssm_prefill_workspace_size(T, n, 2, 1, 64, 128) > 0) == segments
+    assert T > 4 * n + 8
+    a[7] = torch.randn(n, 2, 64, 128, generator=torch.Generator().manual_seed(52))
+    good = dev(a[:7] + [a[7][:1], a[8]])
+    a[8] = torch.tensor(cu, dtype=torch.int64)
+    d = dev(a)
+    with pytest.raises(GDNError, match="cu_seqlens"):
+        ssm.prefill(*d, check=True)
+    with pytest.raises(GDNError, match="cu_seqlens"):   # sticky until cleared
+        ssm.prefill(*good)
+    ssm.reset_device_status()
+    a = a[:7] + [a[7][:1], torch.tensor([0, T], dtype=torch.int32)]
+    check_prompt(ssm.prefill(*good, check=True), a, True)
+
+
+def test_a_wait_that_nothing_ends_gives_up():
+    """The chunked kernel's bounded wait: it reports, later ones do not wait, the context lives."""
+    call = _lib.load().gdn_selftest_scan_wait
+    stream = torch.cuda.current_stream().cuda_stream
+    for arrive in (0, 1):
+        status = torch.zeros(2, dtype=torch.int32, device="cuda")
+        waited = torch.full((2,), -1, dtype=torch.int64, device="cuda")
+        _lib.check(call(5000, arrive, status.data_ptr(), waited.data_ptr(), stream), "scan_wait")
+        torch.cuda.synchronize()
+        assert status.tolist() == [1 - arrive, 0]
+        # 5000 polls of 2 us at most: 10 ms, with the timer's steps of a microsecond or so besides
+        assert (waited >= 0).all() and (waited <= 100e6).all()
+        assert waited[arrive] > 0
+        if not arrive:
+            assert waited[1] < 20e3
+    assert (torch.ones(8, device="cuda") * 2).sum().item() == 16
