@@ -42,6 +42,7 @@
 // of 64 heads of 64 400 us, of which the segments' states take 99, and one chunk, mostly
 // latency, 10.4 us. Two chunks per SM at a time would need twice the shared memory.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 #include "gdn_b200.h"
@@ -114,6 +115,14 @@ __device__ __forceinline__ uint4 lds4u(uint32_t a) {
 __device__ __forceinline__ void sts4u(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w)
                : "memory");
+}
+__device__ __forceinline__ void sts_u16(uint32_t a, unsigned short v) {
+  asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_u16(uint32_t a) {
+  unsigned short v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
+  return v;
 }
 // Offset of row `row`'s 16-byte chunk 0 in a swizzled tile; chunk k is at this XOR 16 k.
 __device__ __forceinline__ uint32_t row_base(uint32_t row) {
@@ -199,8 +208,8 @@ enum Bar {
   kYFree = kState + 2,                 // Y read out
   kStaged = kYFree + 1,                // y in shared memory [3]
   kZeroed = kStaged + 3,
-  kXRead = kZeroed + 1,                // x read by the state's warps, so that y may replace it [2]
-  kFullState = kXRead + 2,             // a state in the second and third stage of x
+  kChecked = kZeroed + 1,              // nothing in x that is not finite, or no more
+  kFullState = kChecked + 1,           // a state in the second and third stage of x
   kStateRead = kFullState + 1,
   kBarCount = kStateRead + 1,
 };
@@ -360,11 +369,17 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
   uint8_t* const sm = align_smem<1024>(raw_smem);
   __shared__ int64_t s_where[4];
   __shared__ uint32_t s_tmem;
+  // Per stage of x and column: the token of the segment from which on an infinity or NaN in x leaves
+  // y not finite (-1: none); whether there is any.
+  __shared__ int s_poison[kStates ? 1 : K::kXStages * 128];
+  __shared__ volatile int s_poisoned;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kOutWarps = K::kOutWarps;                   // first, then the state's
   constexpr int kMisc = kOutWarps + K::kStateWarps;
   uint64_t* const bars = reinterpret_cast<uint64_t*>(sm + K::kBars);
 
+  if (!kStates && threadIdx.x >= 64 && threadIdx.x < 64 + K::kXStages * 128)
+    s_poison[threadIdx.x - 64] = -1;
   const int64_t piece = blockIdx.x / col_blocks;  // a slot, or one of its parts
   const int cb = static_cast<int>(blockIdx.x - piece * col_blocks);
   const int64_t slot = kStates ? piece / sg.parts : piece;
@@ -380,6 +395,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         report_bad_bounds(p.status);
     }
   } else if (threadIdx.x == 32) {
+    s_poisoned = 0;
     for (int i = 0; i < 3; ++i) {
       mbar_init(bars + kFullX + i, 1);
       mbar_init(bars + kFullB + i, 1);
@@ -391,10 +407,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       mbar_init(bars + kGatesFull + i, kHeads);
       mbar_init(bars + kGatesFree + i, kOutWarps + K::kStateWarps);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(bars + kState + i, K::kStateWarps);
-      mbar_init(bars + kXRead + i, K::kStateWarps);
-    }
+    for (int i = 0; i < 2; ++i) mbar_init(bars + kState + i, K::kStateWarps);
     for (int i = 0; i < 4; ++i) {
       mbar_init(bars + kFx + i, K::kFxWarps);
       mbar_init(bars + kFxFree + i, 1);
@@ -402,6 +415,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     for (int i : {kCB, kYM}) mbar_init(bars + i, 1);
     for (int i : {kMy, kYFree}) mbar_init(bars + i, 8);
     mbar_init(bars + kZeroed, K::kStateWarps);
+    mbar_init(bars + kChecked, 4);  // (the state's warps with value 0 of each column)
     mbar_init(bars + kFullState, 1);
     mbar_init(bars + kStateRead, K::kStateWarps);
     fence_mbar_init();
@@ -495,7 +509,6 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
     tmem_st_wait();
     tc_fence_before();
     arrive(kFx + place);
-    if (!kStates && t == 3) arrive(kXRead + (c & 1));
   };
 
   if (warp < kOutWarps) {
@@ -629,6 +642,9 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         const int st = c % K::kXStages;
         const uint32_t xrow = sm_u + K::kX + st * K::kXBytes + half * kBlock + row_base(row);
         wait(bars_u + 8 * (kYM), c & 1);
+        // (dS, and with it all that reads x, is done too, so that y may replace it. Ahead of kYFree:
+        // without that the next chunk's dS does not end, and kChecked cannot run ahead.)
+        wait(bars_u + 8 * (kChecked), c & 1);
         tc_fence_after();
         {
           float y[2][32];
@@ -637,9 +653,6 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
           tmem_ld_wait();
           tc_fence_before();
           arrive(kYFree);  // the next chunk's first product may start
-          // Two barriers: the state's warps may be done with chunk c + 1 by now (its dS waits for
-          // nothing of this role behind first_fx), but not with c + 2, whose first_fx comes later.
-          wait(bars_u + 8 * (kXRead + (c & 1)), (c >> 1) & 1);
   #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const uint32_t at = xrow ^ (16 * k);
@@ -656,6 +669,14 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
               w[e] = pack2_rn(v.x, v.y);
             }
             sts4u(at, w[0], w[1], w[2], w[3]);
+          }
+        }
+        if (s_poisoned) {
+#pragma unroll 1
+          for (int k = 0; k < 64; ++k) {  // of this token's columns
+            const int first = s_poison[st * 128 + 64 * half + k];
+            if ((first >> 7) == c && row >= (first & 127))
+              sts_u16((xrow ^ (16 * (k >> 3))) + 2 * (k & 7), 0x7fff);
           }
         }
         if (c < chunks - 1 || tail == kL) {
@@ -768,12 +789,36 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         float v[16];
         tmem_ld16(td + i0, v);
         tmem_ld_wait();
+        const bool finite = fabsf(S[0]) <= FLT_MAX;
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
           const float2 s = fma2(g2, make_float2(S[i0 + i], S[i0 + i + 1]),
                                 make_float2(v[i], v[i + 1]));
           S[i0 + i] = s.x;
           S[i0 + i + 1] = s.y;
+        }
+        if (!kStates && i0 == 0 && sp == 0) {
+          // An infinity or NaN in x leaves none of its column's state finite, and one value shows it.
+          // In M x it would reach the tokens before it too (0 x NaN): it gives way to a zero first,
+          // and y becomes NaN from its token on. (Looking at x itself, with 8 instructions in each of
+          // its readers, took 4 % of the time of 4 x 32768 tokens, this takes 2 %.)
+          if (finite && !(fabsf(S[0]) <= FLT_MAX)) {
+            const uint32_t xt = sm_u + K::kX + (c % K::kXStages) * K::kXBytes + (q >> 1) * kBlock;
+            int first = kL;
+#pragma unroll 1
+            for (int j = kL - 1; j >= 0; --j) {
+              const uint32_t at = xt + sw128_offset(j, row & 63);
+              if ((lds_u16(at) & 0x7f80u) != 0x7f80u) continue;
+              sts_u16(at, 0);
+              first = j;
+            }
+            if (first < kL) {
+              s_poison[c % K::kXStages * 128 + row] = c * kL + first;
+              s_poisoned = 1;
+              fence_async_smem();
+            }
+          }
+          arrive(kChecked);
         }
       }
       if (kStates) left *= g;
@@ -912,7 +957,9 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
                            desc(d_k, b0, kstep(s, K::kBStep)), kIdCB, s > 0);
               mma_commit_w(bars + kCB);
             }
-          } else if (!ym && ready(kMy, c & 1)) {
+          } else if (!ym && ready(kMy, c & 1) && ready(kChecked, c & 1)) {
+            // (behind all of the chunk's f x, whose writers take infinities and NaN out of x: they
+            // are done long before M, so this waits for nothing)
             ym = true;
             tc_fence_after();
   #pragma unroll 1

@@ -22,9 +22,8 @@ before a stream capture.
 ``prefill`` takes the chunked kernel where P and Ns are 64 or 128 and T is above 4 N + 8, else
 goes token by token. Both give the state to fp32's accuracy (the chunked one: 1e-6 of its size);
 their outputs may differ by a rounding of bf16. A dt of -infinity skips a token (d = 0, g = 1).
-A NaN or infinity in x of a token reaches, in the chunked kernel, also the outputs of its channel
-at up to 127 tokens before it in the same sequence (products with zeros), and leaves NaN in the
-state where the recurrence may leave an infinity.
+A NaN or infinity of a token reaches no token before it. From it on, what it enters is not finite:
+the same values in both kernels, but NaN in the chunked one where the other may have an infinity.
 """
 from __future__ import annotations
 

@@ -321,9 +321,8 @@ GDN_API int gdn_ssm_prefill_recurrent_fwd(const void* x, const void* dt, int dt_
  *
  * With P and Ns of 64 or 128 and more than 4 N + 8 tokens the chunked tensor-core kernels run
  * (chunks of 128 tokens; one launch, two where few long sequences are cut into segments; x and
- * out 16-byte aligned, T < 2^31 - 256); other calls run the token-by-token kernel. In a chunk
- * an infinity or NaN in x also reaches the outputs of up to 127 tokens before it, of the same
- * channel.
+ * out 16-byte aligned, T < 2^31 - 256); other calls run the token-by-token kernel. An infinity
+ * or NaN of a token reaches no token before it; from it on, what it enters is not finite.
  */
 GDN_API size_t gdn_ssm_prefill_workspace_size(int64_t T, int64_t N, int32_t H, int32_t G,
                                               int32_t P, int32_t Ns);

@@ -426,3 +426,49 @@ def test_a_wait_that_nothing_ends_gives_up():
         if not arrive:
             assert waited[1] < 20e3
     assert (torch.ones(8, device="cuda") * 2).sum().item() == 16
+
+
+BAD = [float("nan"), float("inf"), -float("inf")]
+
+
+@pytest.mark.parametrize("P,Ns,H,G", [(64, 64, 3, 1), (128, 128, 2, 2), (64, 128, 4, 2)])
+@pytest.mark.parametrize("where", ["x", "B", "C", "dt"])
+def test_what_is_not_finite_reaches_no_earlier_token(P, Ns, H, G, where):
+    """A NaN or infinity of a token: the values of the tokens before it, of the other sequences and
+    of the channels that it does not enter keep their bits; the others are not finite, as in the
+    recurrence, output by output and state by state."""
+    lengths = [300, 135]
+    clean = make(lengths, H=H, G=G, P=P, Ns=Ns, seed=61)
+    index = {"x": 0, "dt": 1, "B": 3, "C": 4}[where]
+    want = ssm.prefill(*dev(clean), check=True)
+    for k, j in enumerate([0, 5, 31, 32, 63, 100, 127, 128, 140, 255, 256, 299, 301, 434]):
+        a = [t.clone() if isinstance(t, torch.Tensor) else t for t in clean]
+        spot = a[index][j].view(-1)
+        spot[(37 * k + 5) % spot.numel()] = BAD[k % 3] if where != "dt" else BAD[k % 2]
+        d = dev(a)
+        out, ns = ssm.prefill(*d, check=True)
+        out_r, ns_r = ssm.prefill_recurrent(*d)
+        ok, ok_s = torch.isfinite(out), torch.isfinite(ns)
+        assert torch.equal(ok, torch.isfinite(out_r)) and torch.equal(ok_s, torch.isfinite(ns_r))
+        assert not ok.all() and (where == "C" or not ok_s.all())
+        lo = 0 if j < 300 else 300
+        assert ok[lo:j].all() and ok[:lo].all() and (j >= 300 or ok[300:].all())
+        assert torch.equal(out[ok], want[0][ok]) and torch.equal(ns[ok_s], want[1][ok_s])
+
+
+@pytest.mark.parametrize("value", BAD)
+def test_what_is_not_finite_in_segments_and_many_places(value):
+    """The same over segments of one sequence, with many such values, several to a chunk and column."""
+    clean = make([3000], H=2, G=1, P=64, Ns=128, seed=62)
+    g = torch.Generator().manual_seed(63)
+    a = [t.clone() if isinstance(t, torch.Tensor) else t for t in clean]
+    first = torch.full((2, 64), 3000)
+    for _ in range(60):
+        t, h, p = (int(torch.randint(n, (1,), generator=g)) for n in (3000, 2, 64))
+        a[0][t, h, p] = value
+        first[h, p] = min(int(first[h, p]), t)
+    want, got = ssm.prefill(*dev(clean), check=True), ssm.prefill(*dev(a), check=True)
+    ok = torch.arange(3000)[:, None, None] < first
+    assert torch.equal(torch.isfinite(got[0]).cpu(), ok)
+    assert torch.equal(torch.isfinite(got[1]).cpu(), (first == 3000)[None, :, :, None].expand(1, 2, 64, 128))
+    assert torch.equal(got[0].cpu()[ok], want[0].cpu()[ok])

@@ -39,9 +39,11 @@ class Bar:
 
 
 class Model:
-    def __init__(self, chunks, ragged, xread_slots=2, free_by_quarter=True):
-        self.n, self.ragged, self.slots = chunks, ragged, xread_slots
-        self.by_quarter = free_by_quarter
+    def __init__(self, chunks, ragged, x_read=0, free_by_quarter=True, checked_late=False):
+        """As the kernel has it; or with "x read" as barriers of its own (``x_read`` of them), with
+        one barrier per place of f x, or with "checked" waited for behind the hand-over of Y."""
+        self.n, self.ragged, self.slots = chunks, ragged, x_read
+        self.by_quarter, self.late = free_by_quarter, checked_late
         b = lambda name, count, k=None: (  # noqa: E731
             Bar(name, count) if k is None else [Bar(f"{name}[{i}]", count) for i in range(k)])
         self.full_x, self.full_b, self.full_c = b("full_x", 1, X_STAGES), b("full_b", 1), b("full_c", 1)
@@ -51,12 +53,14 @@ class Model:
         self.fx, self.fx_free = b("fx", WARPS, PLACES), b("fx_free", 1, 4)
         self.my, self.state, self.y_free = b("my", WARPS), b("state", WARPS), b("y_free", WARPS)
         self.staged, self.zeroed = b("staged", WARPS, X_STAGES), b("zeroed", WARPS)
-        self.x_read, self.together = b("x_read", WARPS, self.slots), b("together", WARPS)
+        self.checked, self.together = b("checked", WARPS), b("together", WARPS)
+        self.x_read = b("x_read", WARPS, self.slots)
         # what each place holds, by the warp whose part it is
         self.X = [[None] * WARPS for _ in range(X_STAGES)]
         self.F = [[None] * WARPS for _ in range(PLACES)]
         self.G, self.Y, self.S = [None] * WARPS, [None] * WARPS, [None] * WARPS
         self.B = self.C = self.D = None
+        self.clean = [0] * chunks  # warps that have taken what is not finite out of x
         self.pipe, self.loads = [], []  # products and commits, bulk loads: each in order
         self.done = False
 
@@ -80,7 +84,7 @@ class Model:
         self.F[place][w] = (c, t)
         yield None
         self.fx[place].arrive()
-        if t == 3:
+        if t == 3 and self.slots:
             self.x_read[c % self.slots].arrive()
 
     def first_fx(self, w, c):
@@ -104,10 +108,15 @@ class Model:
             if c + 1 < self.n:
                 yield from self.first_fx(w, c + 1)
             yield lambda: self.ym.passed(c)
+            if not self.late:
+                yield lambda: self.checked.passed(c)
             self.expect(self.Y[w], ("y", c), "Y read out")
             yield None
             self.y_free.arrive()
-            yield lambda: self.x_read[c % self.slots].passed(c // self.slots)
+            if self.late:
+                yield lambda: self.checked.passed(c)
+            if self.slots:
+                yield lambda: self.x_read[c % self.slots].passed(c // self.slots)
             self.X[c % X_STAGES][w] = ("out", c)
             yield None
             if not self.is_ragged(c):
@@ -132,6 +141,10 @@ class Model:
             if c > 0:
                 yield lambda: self.ds.passed(c - 1)
                 self.expect(self.D, (c - 1, 3), "dS")
+                self.expect(self.X[(c - 1) % X_STAGES], ("x", c - 1), "x to be checked")
+                yield None
+                self.clean[c - 1] += 1
+                self.checked.arrive()
                 yield None
                 self.gates_free[(c - 1) % GATE_STAGES].arrive()
                 if c < self.n:
@@ -164,7 +177,7 @@ class Model:
                             return True
                         self.pipe += [("cb", c), ("arrive", self.cb)]
                         has["cb"] = acted = True
-                elif not has["ym"] and self.my.passed(c):
+                elif not has["ym"] and self.my.passed(c) and self.checked.passed(c):
                     if not act:
                         return True
                     self.pipe += [("ym", c), ("arrive", self.ym)]
@@ -194,6 +207,7 @@ class Model:
                 else:
                     self.expect(self.G, ("m", c), "M")
                     self.expect(self.X[c % X_STAGES], ("x", c), "x of M x")
+                    self.expect(self.clean[c], WARPS, "x without what is not finite")
 
             inputs()
             yield None
@@ -279,9 +293,13 @@ def test_every_wait_meets_its_phase():
 
 def test_the_model_sees_a_barrier_that_runs_ahead():
     """One barrier for all chunks' "x read" let the state's warps go two chunks ahead of an output
-    warp that had yet to look at it: the block then stood still."""
+    warp that had yet to look at it: the block then stood still. So would one for "checked" that is
+    looked at behind the hand-over of Y. Two, by the chunk's parity, do not."""
     with pytest.raises(Unsound, match="x_read"):
-        schedules(600, xread_slots=1)
+        schedules(600, x_read=1)
+    with pytest.raises(Unsound, match="checked"):
+        schedules(600, checked_late=True)
+    schedules(200, x_read=2)
 
 
 def test_the_model_sees_a_phase_that_is_skipped():
