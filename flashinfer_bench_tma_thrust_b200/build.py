@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import hashlib
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -32,6 +33,12 @@ NVCC_FLAGS = [
     # full-precision math: gates use expf/log1pf and must match the fp32 reference
 ]
 
+# Kernels that hand their registers from some warps to others: what they have to be compiled to, per
+# thread at launch, since the shares add up to that (their launchers check it too, call by call).
+LAUNCH_REGISTERS = {
+    "ssm_prefill_chunked": (r"ssm_chunk_kernelILi\d+ELi\d+ELb0E", 96, 4),  # name, count, kernels
+}
+
 SOURCES = sorted(CSRC.glob("*.cu"))
 HEADERS = sorted(list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + list(INCLUDE.glob("*.h")))
 
@@ -51,6 +58,23 @@ def _digest(paths, extra: str = "") -> str:
     return h.hexdigest()[:16]
 
 
+def check_registers(stem: str, ptxas: str) -> None:
+    """Raise unless ptxas' report on source `stem` gives its kernels the registers they rely on."""
+    if stem not in LAUNCH_REGISTERS:
+        return
+    pattern, want, kernels = LAUNCH_REGISTERS[stem]
+    found = {}
+    for name, report in re.findall(
+            r"Compiling entry function '(\S+)'(.*?)(?=Compiling entry function|\Z)", ptxas, re.S):
+        used = re.search(r"Used (\d+) registers", report)
+        if re.search(pattern, name) and used:
+            found[name] = int(used.group(1))
+    if len(found) != kernels or any(n != want for n in found.values()):
+        raise RuntimeError(
+            f"{stem}.cu: {kernels} kernels have to use {want} registers each, or the shares of their "
+            f"warps do not add up and every launch is refused; this compiler gives {found}")
+
+
 def build(verbose: bool = False, force: bool = False, ptxas_verbose: bool = False) -> Path:
     """Compile every ``csrc/*.cu`` for sm_100a and link ``libgdn_b200.so``."""
     nvcc = _nvcc()
@@ -67,11 +91,21 @@ def build(verbose: bool = False, force: bool = False, ptxas_verbose: bool = Fals
             stale.unlink()
         cmd = [nvcc, *ARCH_FLAGS, *NVCC_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", "-c", str(src),
                "-o", str(obj)]
-        if ptxas_verbose:
+        checked = src.stem in LAUNCH_REGISTERS
+        if ptxas_verbose or checked:
             cmd[1:1] = ["-Xptxas", "-v"]
         if verbose:
             print(" ".join(cmd), file=sys.stderr)
-        subprocess.run(cmd, check=True)
+        if checked:
+            cmd[cmd.index("-o") + 1] = str(obj) + ".tmp"
+            report = subprocess.run(cmd, stderr=subprocess.PIPE, text=True)
+            if ptxas_verbose or report.returncode:
+                print(report.stderr, file=sys.stderr)
+            report.check_returncode()
+            check_registers(src.stem, report.stderr)
+            os.replace(str(obj) + ".tmp", obj)
+        else:
+            subprocess.run(cmd, check=True)
     link_key = _digest(objs)
     stamp = BUILD_DIR / "link.stamp"
     if LIB_PATH.exists() and stamp.exists() and stamp.read_text() == link_key and not force:

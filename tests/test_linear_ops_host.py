@@ -235,3 +235,24 @@ def test_status_words_raise_and_name_the_cause(monkeypatch):
     words[:] = torch.tensor([1, 0])
     with pytest.raises(_lib.GDNError, match="wait"):
         _status.address(99)
+
+
+def _report(counts, name="ssm_chunk_kernelILi{}ELi64ELb0EEEv"):
+    return "".join(f"ptxas info    : Compiling entry function '_ZN3gdn{name.format(64 + i)}' for "
+                   "'sm_100a'\nptxas info    : Function properties\n    0 bytes stack frame\n"
+                   f"ptxas info    : Used {n} registers, used 3 barriers\n"
+                   for i, n in enumerate(counts))
+
+
+def test_the_build_checks_the_registers_that_a_kernel_hands_out():
+    from flashinfer_bench_tma_thrust_b200 import build
+
+    stem = "ssm_prefill_chunked"
+    other = _report([90], "ssm_chunk_kernelILi{}ELi64ELb1EEEv")  # (not one of them)
+    build.check_registers(stem, _report([96] * 4) + other)
+    for bad in (_report([96, 96, 88, 96]), _report([96] * 3), other, ""):
+        with pytest.raises(RuntimeError, match="96 registers"):
+            build.check_registers(stem, bad)
+    build.check_registers("short_conv", "")
+    source = (build.CSRC / f"{stem}.cu").read_text()
+    assert f"kLaunchRegs = {build.LAUNCH_REGISTERS[stem][1]}," in source
