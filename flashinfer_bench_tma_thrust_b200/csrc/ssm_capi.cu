@@ -16,7 +16,9 @@ int fill_conv(gdn::ConvParams* p, const void* x, int64_t x_row_stride, const voi
               const int32_t* normed, float eps, void* const* outs, int64_t T, int64_t N,
               int32_t C, int32_t W) {
   if (T < 0 || N < 0) return GDN_ERR_INVALID_ARG;
-  if (C <= 0 || W < 2 || W > gdn::kMaxTaps) return GDN_ERR_UNSUPPORTED_SHAPE;
+  // (channel numbers are 32-bit, and the last block's go on for up to 1024 behind C)
+  if (C <= 0 || C > INT32_MAX - 2048 || W < 2 || W > gdn::kMaxTaps)
+    return GDN_ERR_UNSUPPORTED_SHAPE;
   if (sections < 1 || sections > gdn::kMaxSections || !widths || !normed || !outs)
     return GDN_ERR_INVALID_ARG;
   if (!real_ok(weight_dtype) || (bias && !real_ok(bias_dtype))) return GDN_ERR_UNSUPPORTED_DTYPE;

@@ -106,6 +106,13 @@ def test_ssm_chunked_workspace_and_alignment(cuda_lib):
     assert _ssm(lib, "chunked", T=0x7fffff01) == -2
 
 
+@pytest.mark.parametrize("fn", ["prefill", "decode"])
+def test_conv_channels_that_leave_32_bits(cuda_lib, fn):
+    """Channel numbers are 32-bit and a block's last thread lies up to 1024 behind C."""
+    for C in (0x7fffffff - 2047, 0x7fffffff - 1000, 0x7fffffff):
+        assert _conv(cuda_lib, fn, C=C, widths=(C,), normed=(0,), stride=C) == -2
+
+
 def test_scan_wait_refusals(cuda_lib):
     call = cuda_lib.gdn_selftest_scan_wait
     assert call(0, 0, P16, P16, None) == -1 and call((1 << 20) + 1, 0, P16, P16, None) == -1
