@@ -48,6 +48,13 @@ def require_all(device: torch.device, names: tuple, tensors: tuple) -> None:
             require_cuda(name, t, device)
 
 
+def require_given(names: tuple, tensors: tuple) -> None:
+    """TypeError for the first argument that is None (the others' kinds are `require_all`'s)."""
+    for name, t in zip(names, tensors):
+        if t is None:
+            raise TypeError(f"{name} must be a torch.Tensor, got NoneType")
+
+
 def as_bf16(name: str, t: torch.Tensor) -> torch.Tensor:
     if t.dtype != torch.bfloat16:
         raise TypeError(f"{name} must be bfloat16, got {t.dtype}")

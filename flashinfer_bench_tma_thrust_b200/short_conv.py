@@ -47,6 +47,8 @@ _BF16, _empty, _empty_like = torch.bfloat16, torch.empty, torch.empty_like
 
 def _taps(x, weight, bias):
     """(weight, code, bias, code, W), checked."""
+    if weight is None:
+        C.require_given(("weight",), (weight,))
     ch, shape = x.shape[-1], weight.shape
     if len(shape) == 3 and shape[1] == 1:
         weight = weight[:, 0]

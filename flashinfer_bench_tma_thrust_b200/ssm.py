@@ -70,6 +70,8 @@ def _args(x, dt, A_log, B, C, D, dt_bias, state, cu, lead: int):
     if len(shape) != lead + 2 or (lead == 2 and shape[1] != 1):
         raise ValueError("x must be a %s tensor" % ("[T, H, P]" if lead == 1 else "[B, 1, H, P]"))
     K.require_all(x.device, _NAMES, (x, dt, A_log, B, C, D, dt_bias, state, cu))
+    if dt is None or A_log is None or B is None or C is None or dt_bias is None:
+        K.require_given(("dt", "A_log", "B", "C", "dt_bias"), (dt, A_log, B, C, dt_bias))
     of_b, head = B.shape, shape[:lead]
     T, H, P = shape[0], shape[-2], shape[-1]
     if len(of_b) != lead + 2 or of_b[:lead] != head or C.shape != of_b:

@@ -231,6 +231,22 @@ def test_ssm_decode_refusals(any_device):
             ssm.decode_inplace(**{**args, "state": state})
 
 
+def test_required_tensors_that_are_none(any_device):
+    z = torch.zeros
+    prompt = dict(x=_bf(4, 4, 64), dt=z(4, 4), A_log=z(4), B=_bf(4, 2, 128), C=_bf(4, 2, 128), D=None,
+                  dt_bias=z(4), state=None, cu_seqlens=CU)
+    token = dict(x=_bf(4, 1, 4, 64), dt=z(4, 1, 4), A_log=z(4), B=_bf(4, 1, 2, 64),
+                 C=_bf(4, 1, 2, 64), D=None, dt_bias=z(4), state=None)
+    for name in ("dt", "A_log", "B", "C", "dt_bias"):
+        for fn, args in ((ssm.prefill, prompt), (ssm.prefill_recurrent, prompt), (ssm.decode, token)):
+            with pytest.raises(TypeError, match=f"^{name} must be a torch.Tensor"):
+                fn(**{**args, name: None})
+    with pytest.raises(TypeError, match="^weight must be a torch.Tensor"):
+        short_conv.prefill(_bf(4, 256), None, None, None, CU)
+    with pytest.raises(TypeError, match="^weight must be a torch.Tensor"):
+        short_conv.decode(_bf(4, 1, 256), None)
+
+
 def test_status_words_raise_and_name_the_cause(monkeypatch):
     words = torch.zeros(2, dtype=torch.int32)
     monkeypatch.setitem(_status._words, 99, (words, ctypes.c_int64.from_address(words.data_ptr()),
