@@ -16,9 +16,10 @@
 // with rows in flight in registers (4 per thread, 16 warps per SM) HBM's latency was not
 // covered. No thread waits for another. Sums are fp32; silu takes ex2.approx and a shared
 // approximate reciprocal (relative error below 2^-16, at the exponents of v = -92; the bf16
-// rounding of the output is the only other one). 65536 x 6144 take 262 us (6.2 TB/s); 19679 x 8192 115 us, and 130 with the norm of
-// half of the channels: besides HBM the instructions per row (130 for 8 channels) come near a
-// bound then.
+// rounding of the output is the only other one). 65536 x 6144 take 259 to 271 us in short runs
+// (6.2 to 5.9 TB/s) and 299 where the power limit holds the clocks down; 19679 x 8192, half of the
+// channels normed, 131 and 138 us: besides HBM (55 % busy) the instructions per row (130 for 8
+// channels, 59 % of the issue slots) come near a bound then.
 #include <cfloat>
 #include <cmath>
 
@@ -179,8 +180,9 @@ __device__ __forceinline__ float from_far(float v) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h) : "f"(v * (0.5f * kLog2e)));
   return (v + v) * h * h;
 }
-// silu of rows of eight values. Values below kFar are rare: a minimum over all rows finds them. (With
-// a branch per row the rows' instructions do not mix: 12 % more time.)
+// silu of rows of eight values. Values below kFar are rare: a minimum over all rows finds them.
+// (With a branch per row the rows' instructions do not mix: 12 % more time. The minimum costs
+// 0.6 %, and the pass over such values up to a quarter where most rows have one.)
 template <int kTok>
 __device__ __forceinline__ void silu_rows(float2 (&y)[kTok][kP]) {
   float low = 0.f;
@@ -216,8 +218,8 @@ struct Window {
 };
 
 // Sums of kTok values per lane over 16 lanes, each in every lane. Two values: an exchange that
-// leaves one value per lane, three more steps on it, and two broadcasts, 6 shuffles for 8. The order
-// of the sums is the same for one value, so that bits do not depend on how tokens fall into rows.
+// leaves one value per lane, three more steps on it, and two broadcasts, 6 shuffles for 8. The
+// order of the sums is the same for one value: bits do not depend on how tokens fall into rows.
 template <int kTok>
 __device__ __forceinline__ void head_sums(float (&q)[kTok]) {
   const uint32_t lanes = 0xffffu << (threadIdx.x & 16);
@@ -395,7 +397,8 @@ struct Walk {
         if (u >= start) {
           win.set(r, load_row<kWide>(p.x + u * p.x_stride, c, p.C));
         } else if (p.state) {
-          win.set(r, load_row<kWide>(p.state + (n * (W - 1) + (u - start) + (W - 1)) * p.C, c, p.C));
+          win.set(r,
+                  load_row<kWide>(p.state + (n * (W - 1) + (u - start) + (W - 1)) * p.C, c, p.C));
         }
       }
     }
@@ -530,9 +533,10 @@ conv_prefill_kernel(const __grid_constant__ ConvParams p, int64_t tiles, int run
   if (__any_sync(0xffffffffu, far)) tile_again<W, kWide>(p, c, t0, t1);
 }
 
-// One token per sequence, bound by HBM (1024 sequences of 8192 channels with 4 taps 26.7 us,
-// 5.0 TB/s with the launch): each thread reads its 8 channels of the W-1 state rows and of x,
-// and writes the rows moved up by one, so the new state may be the old one's memory.
+// One token per sequence, bound by HBM (1024 sequences of 8192 channels with 4 taps 26.7 us, in
+// short and long runs, 5.0 TB/s with the launch): each thread reads its 8 channels of the W-1
+// state rows and of x, and writes the rows moved up by one, so the new state may be the old one's
+// memory.
 template <int W>
 constexpr int kDecodeBlocks = W == 4 ? 4 : (W == 3 ? 5 : 7);  // per SM, by the registers
 
@@ -572,8 +576,8 @@ conv_decode_kernel(const __grid_constant__ ConvParams p, int per_thread) {
 #pragma unroll
     for (int r = 0; r < W - 1; ++r) win.set(r, rows[r]);
     const Row row[1] = {rows[W - 1]};
-    output_rows<W, kWide, true, 1>(p, taps, pl, cl, n, pl.out + n * pl.width + pl.at, win, row, live,
-                                   far);
+    output_rows<W, kWide, true, 1>(p, taps, pl, cl, n, pl.out + n * pl.width + pl.at, win, row,
+                                   live, far);
   }
 }
 
@@ -597,12 +601,12 @@ template <int W>
 int prefill_w(const ConvParams& p, cudaStream_t stream) {
   const unsigned bx = (p.C + kThreads * kVec - 1) / (kThreads * kVec);
   // Four blocks per SM run at a time. While one round of them covers the tokens in runs of 48 or
-  // less, it does: 8192 channels, 7 tokens 3.4 us in runs of 1 and 5.5 of 8; 1000 11.1 in runs of
-  // 16, 12.1 of 8; 3000 28.3 of 48, 31.7 of 8. Beyond, a run costs its rows and as long as 10 more
-  // (bounds, taps, W-1 rows again), and the last round is half empty: with `round` tokens to a
-  // round of runs of one, (round / run + 1/2) (run + 10) is least at sqrt(20 round). 5000 tokens
-  // 42.1 us in runs of 32, 43.9 of 48, 45.6 of 64; 19679 129.5 of 64, 135 of 32, 136 of 128; 65536
-  // x 6144 261 of 128, 267 of 72 or 144.
+  // less, it does: 8192 channels, in a graph, 7 tokens 3.6 us in runs of 1 and 5.7 of 8; 1000 11.0
+  // in runs of 16, 12.3 of 8; 3000 26.9 of 44, 28.7 of 48, 32.1 of 8. Beyond, a run costs its rows
+  // and as long as 10 more (bounds, taps, W-1 rows again), and the last round is half empty: with
+  // `round` tokens to a round of runs of one, (round / run + 1/2) (run + 10) is least at
+  // sqrt(20 round). 5000 tokens 43.0 us in runs of 32, 44.7 of 48, 47.0 of 64; 19679 130.3 of 64,
+  // 135 of 32 or 128; 65536 x 6144 259 of 112 (the rule's), 266 of 72, 265 of 128, 264 of 144.
   const int64_t round = (bx * p.T + 148 * 4 - 1) / (148 * 4);
   const int run = round <= 2    ? static_cast<int>(round < 1 ? 1 : round)
                   : round <= 48 ? static_cast<int>(round + 3) / 4 * 4

@@ -21,7 +21,10 @@
 //
 // Roundings: x, B and C are exact bf16 operands, and so are the three terms of f x, whose sum
 // is the fp32 product (the state, an fp32 result, is off by 3e-7; two terms left 2e-6). S and M
-// are rounded once to bf16 as operands: they reach only y, which is rounded to bf16 itself.
+// are rounded once to bf16 as operands (a second term of S has no room in shared memory, one of M
+// would double its product): they reach only y, which is rounded to bf16 itself. Relative to 64
+// bits y is off by 0.0017 to 0.0022, of which its own rounding is 0.0017; most where a first state
+// makes up most of y.
 //
 // Segments. With few (sequence, column block) chains the sequences are cut into segments of a
 // multiple of 128 tokens. A first kernel (the same code, second product only) computes what
@@ -34,13 +37,16 @@
 // the gates (one head each, up to four chunks ahead). Every wait is bounded; a block that gives
 // up reports it and runs on without waiting, so no barrier is left short of its threads.
 //
-// What bounds it: shared memory. Per chunk of 128 x 128 with Ns = 128 a block moves about 5400
-// of its 128-byte lines (products' operands 1800, bulk copies 1000, the roles' own loads and
-// stores 2400) in 6300 cycles, half of them with work for the tensor cores. With heads of 128
-// and states of 128, at the 1.7 to 1.9 GHz that the power limit leaves: 4 x 32768 tokens of 32
-// heads 945 to 1090 us (3.0 to 3.4 TB/s of the bytes that have to move), one sequence of 32768
-// of 64 heads of 64 400 us, of which the segments' states take 99, and one chunk, mostly
-// latency, 10.4 us. Two chunks per SM at a time would need twice the shared memory.
+// What bounds it: the chain of one chunk (product, M, M x, y, the next product) through single
+// buffers of C B^T and Y, some 6400 cycles of which the tensor cores work half. No unit is at its
+// limit: with heads and states of 128 the busy SMs issue in 62 % of the cycles, the tensor pipe is
+// at 47 %, shared memory's banks move 3900 lines of 128 bytes per chunk (1800 of them for the
+// roles' own loads and stores), HBM is at 35 %; the longest stall is for loads from TMEM, then
+// fixed latencies. In long runs the power limit holds the clocks down besides. 4 x 32768 tokens of
+// 32 heads take 1030 us in short runs and 1110 in long ones (3.1 and 2.9 TB/s of the bytes that
+// have to move), one sequence of 32768 of 64 heads of 64 367 us in a graph and 430 in long runs, of
+// which the segments' states take a quarter, and one chunk, mostly latency, 10.4 us. Two chunks per
+// SM at a time would need twice the shared memory.
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -536,7 +542,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         // ---- M over C B^T, 16 columns at a time: those of head h go to 8 columns of the same
         // 16, so a warp overwrites nothing that another has yet to read. The two warps of a
         // quarter take every other 16 (each has one piece on the diagonal).
-  #pragma unroll 1
+#pragma unroll 1
         for (int k = 0; k < 4; ++k) {  // piece k: columns 32 k + 16 half on, in block k of 32
           float g[16];
           const int j0 = 32 * k + 16 * half;
@@ -552,20 +558,20 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
               // between j and i: both exponents are at most 0, and one exponential per row is left
               float ex[kHeads];
               float4 u[kHeads][4];
-  #pragma unroll
+#pragma unroll
               for (int hh = 0; hh < kHeads; ++hh) {  // all loads before the first use
                 const uint32_t gh = ga + hh * kGatesBytes;
                 ex[hh] = lds(gh + kCum + 4 * row);
                 if (k + 1 < q) ex[hh] += lds(gh + kTot + 4 * (k + 1));
                 if (k + 2 < q) ex[hh] += lds(gh + kTot + 4 * (k + 2));
-  #pragma unroll
+#pragma unroll
                 for (int j = 0; j < 4; ++j) u[hh][j] = lds4(gh + kU + 4 * (j0 + 4 * j));
               }
-  #pragma unroll
+#pragma unroll
               for (int hh = 0; hh < kHeads; ++hh) {
                 const float e = ex2(ex[hh]);
                 const float2 a = make_float2(e, e);
-  #pragma unroll
+#pragma unroll
                 for (int j = 0; j < 4; ++j) {
                   const float4 v = u[hh][j];
                   const float2 v0 = mul2(mul2(make_float2(v.x, v.y), a),
@@ -580,16 +586,16 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
               const int i = row - j0;  // columns j <= i are on or below the diagonal
               float own[kHeads];
               float4 x[kHeads][4];
-  #pragma unroll
+#pragma unroll
               for (int hh = 0; hh < kHeads; ++hh) {
                 const uint32_t gh = ga + hh * kGatesBytes;
                 own[hh] = lds(gh + kCum + 4 * row);
-  #pragma unroll
+#pragma unroll
                 for (int j = 0; j < 4; ++j) x[hh][j] = lds4(gh + kH + 4 * (j0 + 4 * j));
               }
-  #pragma unroll
+#pragma unroll
               for (int hh = 0; hh < kHeads; ++hh) {
-  #pragma unroll
+#pragma unroll
                 for (int j = 0; j < 4; ++j) {
                   const float4 v = x[hh][j];
                   const float* const gj = g + 4 * j;
@@ -602,13 +608,13 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
                 }
               }
             } else {
-  #pragma unroll
+#pragma unroll
               for (int hh = 0; hh < kHeads; ++hh) {
-  #pragma unroll
+#pragma unroll
                 for (int j = 0; j < 8; ++j) m[hh][j] = 0u;
               }
             }
-  #pragma unroll
+#pragma unroll
             for (int hh = 0; hh < kHeads; ++hh) tmem_st8(at + 8 * hh, m[hh]);
           }
         }
@@ -616,13 +622,13 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         {
           const float e = lds(ga + col_head * kGatesBytes + kDec + 4 * row);
           const float2 e2 = make_float2(e, e);
-  #pragma unroll 1
+#pragma unroll 1
           for (int k = 0; k < 2; ++k) {
             const uint32_t ty = lanes + kTY + 64 * half + 32 * k;
             float y[32];
             tmem_ld32(ty, y);
             tmem_ld_wait();
-  #pragma unroll
+#pragma unroll
             for (int i = 0; i < 32; i += 2) {
               const float2 v = mul2(make_float2(y[i], y[i + 1]), e2);
               y[i] = v.x;
@@ -653,13 +659,13 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
           tmem_ld_wait();
           tc_fence_before();
           arrive(kYFree);  // the next chunk's first product may start
-  #pragma unroll
+#pragma unroll
           for (int k = 0; k < 8; ++k) {
             const uint32_t at = xrow ^ (16 * k);
             const uint4 xv = p.D ? lds4u(at) : make_uint4(0u, 0u, 0u, 0u);
             const uint32_t u[4] = {xv.x, xv.y, xv.z, xv.w};
             uint32_t w[4];
-  #pragma unroll
+#pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float2 v = fma2(make_float2(skip, skip),
                                     make_float2(__uint_as_float(u[e] << 16),
@@ -904,9 +910,9 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
           const uint32_t tf = tm + (kStates ? 0 : kTF) + 16 * kTerms * place;
           const uint32_t b0 = fresh(bb + t * 4096);
           tc_fence_after();
-  #pragma unroll
+#pragma unroll
           for (int r = 0; r < kTerms; ++r) {
-  #pragma unroll
+#pragma unroll
             for (int s = 0; s < 2; ++s)
               mma_bf16_ts_w(td, tf + 16 * r + 8 * s, desc(d_b, b0, s * 2048), kIdDS,
                             t > 0 || r > 0 || s > 0);
@@ -919,7 +925,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         if (kStates) {
           wait(bars_u + 8 * (kFullB + st), par);
           if (c >= 2) wait(bars_u + 8 * (kState + (c & 1)), ((c >> 1) - 1) & 1);
-  #pragma unroll 1
+#pragma unroll 1
           for (int t = 0; t < 4; ++t) {
             wait(fx_bar(t), fx_par(t));
             issue_ds(tm + kTD + 128 * (c & 1), t);
@@ -936,7 +942,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
         auto ready = [&](int bar, uint32_t parity) {
           return force || mbar_test_wait(bars_u + 8 * bar, parity);
         };
-  #pragma unroll 1
+#pragma unroll 1
         while (!ym || t < 4) {
           b_in = b_in || ready(kFullB + st, par);
           state_in = state_in || ready(kState, c & 1);
@@ -951,7 +957,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
               cb = true;
               tc_fence_after();
               const uint32_t b0 = fresh(bb), c0 = fresh(sm_u + K::kC);
-  #pragma unroll 4
+#pragma unroll 4
               for (int s = 0; s < NS / 16; ++s)
                 mma_bf16_w(tm + kTG, desc(d_k, c0, kstep(s, kBlock)),
                            desc(d_k, b0, kstep(s, K::kBStep)), kIdCB, s > 0);
@@ -962,10 +968,10 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
             // are done long before M, so this waits for nothing)
             ym = true;
             tc_fence_after();
-  #pragma unroll 1
+#pragma unroll 1
             for (int hh = 0; hh < kHeads; ++hh) {
               const uint32_t x0 = fresh(xb + hh * kBlock);
-  #pragma unroll 4
+#pragma unroll 4
               for (int s = 0; s < 8; ++s)
                 mma_bf16_ts_w(tm + kTY + hh * 64, tm + kTG + 16 * s + 8 * hh,
                               desc(d_x, x0, s * 2048), kIdYM, 1);
@@ -1084,7 +1090,7 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       // (a conversion here would wait for each of the four in turn, 800 cycles each)
       const bool half = p.dt_dtype == kBF16;
       auto load = [&](int c, uint32_t (&raw)[4]) {
-  #pragma unroll
+#pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int t = min(c * kL + 4 * lane + k, tokens - 1);
           const int64_t at = (static_cast<int64_t>(tok0) + t) * p.H + h;
@@ -1094,11 +1100,11 @@ ssm_chunk_kernel(const __grid_constant__ SsmParams p, const __grid_constant__ Ma
       };
       uint32_t raw[4];
       if (chunks > 0) load(0, raw);
-  #pragma unroll 1
+#pragma unroll 1
       for (int c = 0; c < chunks; ++c) {
         const int gs = c % kGateStages;
         float dt[4];
-  #pragma unroll
+#pragma unroll
         for (int k = 0; k < 4; ++k) dt[k] = __uint_as_float(half ? raw[k] << 16 : raw[k]);
         if (c + 1 < chunks) load(c + 1, raw);
         if (c >= kGateStages)
@@ -1150,9 +1156,9 @@ int column_blocks(int H, int G, int P) {
 // In us, with heads and states of 128: a chunk takes 3.4, one of the states' kernel 2.0, that
 // kernel's start 9 and each segment that is folded into a first state 1.1. The host does not know
 // the lengths: the longest sequence of several is taken as half as long again as their mean.
-// 32 heads, whole / in segments: 1000 tokens 34.0 / 28.7, 1900 58 / 39, 3000 88 / 53, 8192 218 /
-// 103; one head, in segments of 1024 / by this rule: 2000 tokens 59 / 31, 8192 59 / 48, 131072
-// 209 / 165. (Four sequences of 300, 400, 2000 and 900 with 16 heads lose: 59 / 62.)
+// 32 heads, whole / in segments, in a graph: 1000 tokens 34.9 / 28.6, 1900 60 / 40, 3000 91 / 53,
+// 8192 226 / 105; one head, in segments of 1024 / by this rule: 2000 tokens 55 / 31, 8192 60 / 49,
+// 131072 210 / 165. (Four sequences of 300, 400, 2000 and 900 with 16 heads gain nothing: 63.5.)
 Segments plan(int64_t T, int64_t N, int H, int G, int P) {
   constexpr int kSms = 148;
   constexpr double kChunk = 3.4, kState = 2.0, kStart = 9, kFold = 1.1;
@@ -1171,8 +1177,7 @@ Segments plan(int64_t T, int64_t N, int H, int G, int P) {
   sg.slots = T / sg.len + N;
   // A sequence's last segment has no part in the states kernel, and a part takes less than half
   // of a segment's time: several to a segment may fill the SMs better (32 column blocks: 32768
-  // tokens, 3 segments with states, 437 us in all, in 3 parts each 424; 12000 and 3000 tokens 219
-  // and 188).
+  // tokens, 3 segments with states, 418 us in all in a graph, in 3 parts each 367).
   const double busy = std::max(1.0, static_cast<double>((T - 1) / sg.len - (N - 1) / 2)) * cols;
   double best = 0;
   for (int parts = 1; parts <= 4; ++parts) {

@@ -111,8 +111,9 @@ __device__ __forceinline__ float bf16_at(const __nv_bfloat16* p) {
 
 // ---------------------------------------------------------------- one token per sequence
 // HBM bounds it: the state goes through once (5 flop per 8 bytes): 256 sequences of 32 heads of
-// 128 x 128 in fp32 take 161 us, 6.7 TB/s; 300 of 80 heads of 64 x 128 in bf16, with twice the
-// rows per byte, 134 us, 5.9 TB/s, near the issue limit. A warp takes batches of
+// 128 x 128 in fp32 take 162 us in short runs, 6.7 TB/s, and 177 where the power limit holds the
+// clocks down; 300 of 80 heads of 64 x 128 in bf16, with twice the rows per byte, 136 us, 5.8 TB/s,
+// and 143, near the issue limit. A warp takes batches of
 // kRows * kPer rows, of which each lane holds x and y of one; a batch's loads are all in
 // flight, and the next batch's too, before it is used. Blocks of 4 warps share a head's rows.
 template <typename S, int kLanes, int kPieces, int kRows, bool kLoop>

@@ -23,10 +23,10 @@ wants its q and k:
     returns    (output or tuple of sections, new_state)
 
 Sums are fp32, outputs bf16, rounded once; how tokens are packed or cut into calls changes no bit
-of them. An empty sequence passes its state through; outputs
-of tokens that no sequence covers are not written. Inputs are never modified (except by
-``decode_inplace``). Every call is one launch on the current stream of x's device. The first
-call on a device allocates its status words: make it before a stream capture.
+of them. A head of zeros with eps = 0 gives NaN (0 / 0). An empty sequence passes its state
+through; outputs of tokens that no sequence covers are not written. Inputs are never modified
+(except by ``decode_inplace``). Every call is one launch on the current stream of x's device. The
+first ``prefill`` on a device allocates its status words: make it before a stream capture.
 """
 from __future__ import annotations
 
