@@ -99,8 +99,9 @@ def build(verbose: bool = False, force: bool = False, ptxas_verbose: bool = Fals
         if checked:
             cmd[cmd.index("-o") + 1] = str(obj) + ".tmp"
             report = subprocess.run(cmd, stderr=subprocess.PIPE, text=True)
-            if ptxas_verbose or report.returncode:
-                print(report.stderr, file=sys.stderr)
+            for line in report.stderr.splitlines():
+                if ptxas_verbose or report.returncode or not re.match(r"ptxas info|    \d+ bytes", line):
+                    print(line, file=sys.stderr)
             report.check_returncode()
             check_registers(src.stem, report.stderr)
             os.replace(str(obj) + ".tmp", obj)

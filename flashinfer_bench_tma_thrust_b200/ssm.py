@@ -23,9 +23,10 @@ before a stream capture.
 goes token by token. Both give the state to fp32's accuracy (the chunked one: 1e-6 of its size).
 The chunked kernel multiplies the state, and the decayed products of C and B, rounded to bf16: its
 outputs are off by up to 2^-8 of the sum of their terms' sizes, which is more than their own
-rounding where terms cancel. ``prefill_recurrent`` has fp32 there. A dt of -infinity skips a token (d = 0, g = 1).
-A NaN or infinity of a token reaches no token before it. From it on, what it enters is not finite:
-the same values in both kernels, but NaN in the chunked one where the other may have an infinity.
+rounding where terms cancel. ``prefill_recurrent`` has fp32 there. A dt of -infinity skips a token
+(d = 0, g = 1). A NaN or infinity of a token reaches no token before it. From it on, what it enters
+is not finite: the same values in both kernels, but NaN in the chunked one where the other may have
+an infinity.
 """
 from __future__ import annotations
 

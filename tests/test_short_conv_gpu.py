@@ -390,3 +390,16 @@ def test_bits_do_not_depend_on_packing():
     before = torch.stack([rows[k:k + T] for k in range(3)], 1).contiguous()
     tokens, _ = short_conv.decode(x[:, None], w, b, before, **kw)
     assert all(torch.equal(u[:, 0], v) for u, v in zip(tokens, whole))
+
+
+def test_prompts_past_2_31_elements():
+    """x and its sections of more than 2^31 elements: the last sequence as it is alone."""
+    T, C, last = 270000, 8192, 2000
+    g = torch.Generator("cuda").manual_seed(43)
+    x = torch.randn(T, C, generator=g, device="cuda", dtype=torch.bfloat16)
+    w = torch.randn(C, 4, generator=g, device="cuda") / 2
+    assert (T - last) * C > 2 ** 31
+    cu = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    got, ns = short_conv.prefill(x, w, None, None, cu(0, T - last, T), l2norm=True, check=True)
+    want, end = short_conv.prefill(x[T - last:], w, None, None, cu(0, last), l2norm=True, check=True)
+    assert torch.equal(got[T - last:], want) and torch.equal(ns[1], end[0])

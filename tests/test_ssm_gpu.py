@@ -472,3 +472,39 @@ def test_what_is_not_finite_in_segments_and_many_places(value):
     assert torch.equal(torch.isfinite(got[0]).cpu(), ok)
     assert torch.equal(torch.isfinite(got[1]).cpu(), (first == 3000)[None, :, :, None].expand(1, 2, 64, 128))
     assert torch.equal(got[0].cpu()[ok], want[0].cpu()[ok])
+
+
+def test_graphs_with_segments_beside_each_other():
+    """Two captured calls with workspaces, replayed at once on two streams, and eager calls between."""
+    a, b = (dev(make(L, H=2, G=1, P=64, Ns=128, seed=71)) for L in ([2500], [1500, 0, 1100]))
+    want = [ssm.prefill(*v, check=True) for v in (a, b)]
+    graphs, got = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for g, v in zip(graphs, (a, b)):
+        with torch.cuda.graph(g):
+            got.append(ssm.prefill(*v))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        again = ssm.prefill(*a)
+    torch.cuda.synchronize()
+    for u, v in ((got[0], want[0]), (got[1], want[1]), (again, want[0])):
+        assert torch.equal(u[0], v[0]) and torch.equal(u[1], v[1])
+
+
+def test_prompts_past_2_31_elements():
+    """x and y of more than 2^31 elements: the last sequence as it is alone."""
+    T, H, P, Ns, last = 140000, 128, 128, 64, 900
+    g = torch.Generator("cuda").manual_seed(72)
+    new = lambda *s: torch.randn(*s, generator=g, device="cuda", dtype=torch.bfloat16)  # noqa: E731
+    x, B, C, dt = new(T, H, P), new(T, 1, Ns), new(T, 1, Ns), new(T, H)
+    A_log, dtb = torch.zeros(H, device="cuda"), torch.full((H,), -3.0, device="cuda")
+    assert x.numel() > 2 ** 31 and (T - last) * H * P > 2 ** 31
+    cu = torch.tensor([0, 100, T - last, T], dtype=torch.int32, device="cuda")
+    out, ns = ssm.prefill(x, dt, A_log, B, C, None, dtb, None, cu, check=True)
+    tail = slice(T - last, T)
+    one = torch.tensor([0, last], dtype=torch.int32, device="cuda")
+    want, end = ssm.prefill(x[tail], dt[tail], A_log, B[tail], C[tail], None, dtb, None, one, check=True)
+    assert torch.equal(out[tail], want) and torch.equal(ns[2], end[0])
